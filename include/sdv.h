@@ -38,6 +38,7 @@
  *                           sequence's start)
  *   sdv_attention_workspace_size  <- no counterpart (the reference allocates its score,
  *                           softmax and kv_repeat temporaries inside torch)
+ *   sdv_kv8_*             <- no counterpart: the 8-bit KV cache
  *   sdv_fp8_encode       <- the tensor.to(torch.float8_e4m3fn) cast (model_self.py:312)
  *   sdv_status_string    <- TORCH_CHECK messages (attention.cu:245-262)
  */
@@ -307,6 +308,74 @@ int sdv_paged_attention_noalloc(const void* q, const void* k_pages, const void* 
 int sdv_pack_contiguous(const void* k, const void* v_codes, const float* v_scales, int32_t batch,
                         int32_t kv_heads, int32_t seq_len, int32_t head_dim, void* k_pages, void* v_pages,
                         float* page_scales, int32_t* block_table, void* stream);
+
+/* ------------------------------------------------------------------ the 8-bit KV cache (kv8)
+ *
+ * K and V both in one byte a value, with an fp32 scale per (token, KV head) each: 2 (head_dim + 4) bytes
+ * per token and KV head.  No counterpart in the reference, whose caches keep K in BF16 (v_fp8) or
+ * scale groups of 32 dimensions (fp8).  One layer per call; blocks of 16 tokens:
+ *   k_pages  [num_blocks][kv_heads][4][head_dim/16][4][16]  code of token 4p + r, dim 16c + j at [p][c][r][j]
+ *   v_pages  [num_blocks][kv_heads][head_dim][16]           dimension-major in a block
+ *   scales   [num_blocks][kv_heads][2][16] fp32             K's 16 tokens, then V's
+ * format: SDV_KV8_FP8 (E4M3FN codes, Q = 448) or SDV_KV8_INT8 (two's complement, Q = 127), K and V
+ * alike.  A row (one token's head_dim values of one KV head) has s = max|x| / Q (IEEE fp32 division; 0
+ * -> 1) and codes RNE(x / s); a row that holds an infinity or a NaN has scale NaN and codes 0.
+ *
+ * Ragged rows: cu_rows int32 [batch + 1] on the device, sequence b's rows being cu_rows[b] ..
+ * cu_rows[b+1] - 1 of the packed tensors (entries are clamped to [0, total_rows]; a sequence may have
+ * none).  Rows behind cu_rows[batch] are neither read nor written.  Packed tensors are BF16
+ * [total_rows][heads][head_dim] whose tokens lie `*_stride` elements apart (a multiple of 8, at
+ * least heads * head_dim), so that the q, k and v parts of one projection's output can be passed
+ * as they lie.  block_table int32 [batch][max_blocks_per_seq]; an entry outside [0, num_blocks), or a
+ * position past the table, is never dereferenced.
+ * Alignment: packed tensors, pages and scales 16 B, int32 arrays 4 B, tree_mask 8 B, workspace 256 B. */
+#define SDV_KV8_FP8 0
+#define SDV_KV8_INT8 1
+
+/*
+ * Quantize the rows and write them into the cache: row i of sequence b is position
+ * seq_lens[b] - n_b + i, n_b its row count, seq_lens[b] its length with the new tokens (NULL: max_seq_len,
+ * for every sequence; a call that a HIP graph records then needs no lengths in device memory).  Rows at negative
+ * positions (a length below the row count) or in blocks that the table does not name are skipped.
+ */
+int sdv_kv8_append(const void* k_new, const void* v_new, int64_t k_stride, int64_t v_stride, int32_t total_rows,
+                   void* k_pages, void* v_pages, float* scales, int32_t num_blocks, int32_t format,
+                   const int32_t* block_table, int32_t max_blocks_per_seq, const int32_t* cu_rows,
+                   const int32_t* seq_lens, int32_t max_seq_len, int32_t batch, int32_t kv_heads, int32_t head_dim,
+                   void* stream);
+
+/*
+ * Read the cache back: row i of sequence b is position starts[b] + i, bf16(code * scale) in k_out and
+ * v_out (tokens k_stride and v_stride elements apart).  Positions in no block read as zeros.
+ */
+int sdv_kv8_gather(const void* k_pages, const void* v_pages, const float* scales, int32_t num_blocks, int32_t format,
+                   const int32_t* block_table, int32_t max_blocks_per_seq, const int32_t* cu_rows,
+                   const int32_t* starts, int32_t batch, int32_t total_rows, int32_t kv_heads, int32_t head_dim,
+                   void* k_out, void* v_out, int64_t k_stride, int64_t v_stride, void* stream);
+
+/* Bytes of workspace sdv_kv8_attention needs for these sizes (0 on invalid sizes).  It carries nothing
+ * from call to call and needs no initialisation; calls that may overlap need one each. */
+size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
+                                        int32_t head_dim, int32_t max_q_len, int32_t max_seq_len);
+
+/*
+ * Attention of every sequence's new tokens over its cached context, which ends with them: single
+ * tokens, verify blocks, prompt chunks, or all in one batch.  Row i of sequence b (n_b rows, T_b =
+ * seq_lens[b] clamped to [0, max_seq_len], or max_seq_len where seq_lens is NULL) is position T_b - n_b + i and sees keys up to its own;
+ * with tree_mask (uint64 [total_rows]; max_q_len <= 64) it sees the context T_b - n_b and, of the new
+ * tokens, those j whose bit j of its mask is set: a tree of drafted tokens.  q head h reads KV head
+ * h / (q_heads / kv_heads).  max_q_len is the largest n_b.  Softmax of scale * q.k in fp32, probabilities
+ * times V's scale rounded to BF16 for the product with V, fp32 sums, BF16 output.  A row that sees
+ * nothing is 0; what a row does not see, infinities and NaN among it, does not reach it.
+ * Size limits: (max_seq_len + total_rows) * q_heads / kv_heads <= 2^30 and, with tiles of 16 rows (32 where
+ * max_q_len * q_heads / kv_heads > 16), tiles * steps of 64 keys * kv_heads < 2^31.
+ */
+int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
+                      int32_t num_blocks, int32_t format, const int32_t* block_table, int32_t max_blocks_per_seq,
+                      const int32_t* cu_rows, const int32_t* seq_lens, const uint64_t* tree_mask, int32_t batch,
+                      int32_t total_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
+                      int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes, void* out,
+                      int64_t out_stride, void* stream);
 
 /* Elementwise fp32 -> E4M3FN (RNE, NaN beyond 464 / for Inf and NaN), device buffers. */
 int sdv_fp8_encode(const float* in, uint8_t* out, int64_t n, void* stream);

@@ -28,6 +28,9 @@ SDV_ERR_HIP = -6
 SCALE_DIV = 0
 SCALE_RCP = 1
 
+KV8_FP8 = 0
+KV8_INT8 = 1
+
 PHASE_QK = 1
 PHASE_PV = 2
 PHASE_REDUCE = 4
@@ -67,6 +70,13 @@ SIGNATURES = {
     "sdv_paged_attention_noalloc": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _I32, _P,
                                                    _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P]),
     "sdv_pack_contiguous": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P]),
+    "sdv_kv8_append": (ctypes.c_int, [_P, _P, _I64, _I64, _I32, _P, _P, _P, _I32, _I32, _P, _I32, _P, _P, _I32,
+                                      _I32, _I32, _I32, _P]),
+    "sdv_kv8_gather": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _P, _P,
+                                      _I64, _I64, _P]),
+    "sdv_kv8_attention_workspace_size": (_SZ, [_I32] * 7),
+    "sdv_kv8_attention": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I32, _I32,
+                                         _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ, _P, _I64, _P]),
     "sdv_fp8_encode": (ctypes.c_int, [_P, _P, _I64, _P]),
     "sdv_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "sdv_abi_version": (ctypes.c_int, []),

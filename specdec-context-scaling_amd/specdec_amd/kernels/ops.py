@@ -15,6 +15,10 @@ Operators
                       (ops.py:67-76) over a contiguous v_fp8 cache: k BF16 (B,KV,T,D) and
                       v given as the (payload, scale) pair the engine stores.
                       One kernel packs the cache into pages first.
+``kv8_append``        the 8-bit cache: new tokens' K and V quantized (fp8 or int8) into pages.
+``kv8_gather``        the 8-bit cache read back into packed BF16 rows.
+``kv8_attention``     ragged query rows (single tokens, verify blocks or trees, prompt chunks,
+                      or all in one batch) over the 8-bit cache.
 ``fp8_encode``        elementwise fp32 -> E4M3FN on the device.
 """
 from __future__ import annotations
@@ -580,6 +584,210 @@ def fp8_encode(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# ---------------------------------------------------------------------------- the 8-bit KV cache
+_KV8_FORMATS = {torch.float8_e4m3fn: _native.KV8_FP8, torch.int8: _native.KV8_INT8}
+_KV8_SCRATCH: dict = {}  # (device, stream) -> kv8_attention's workspace of eager calls
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _kv8_call(fn, what: str, dev: torch.device, *args) -> None:
+    """fn(*args, stream) on dev's current stream, with dev the current device."""
+    if dev.index is not None and dev.index != _get_device():
+        with torch.cuda.device(dev):
+            st = fn(*args, _stream(dev))
+    else:
+        st = fn(*args, _stream(dev))
+    if st:
+        _native.check(st, what)
+
+
+def _kv8_pages(k_pages, v_pages, scales, block_table, dev):
+    """(blocks, KV heads, head_dim, format) of a layer's kv8 pages, checked."""
+    try:
+        nb, kv, four, dc, r, j = k_pages.shape
+        shapes = (four, r, j) == (4, 4, 16) and v_pages.shape == (nb, kv, dc * 16, BLOCK) and scales.shape == (nb, kv, 2, BLOCK)
+        fmt = _KV8_FORMATS.get(k_pages.dtype)
+        if (shapes and fmt is not None and v_pages.dtype is k_pages.dtype and scales.dtype is torch.float32
+                and block_table.dtype is torch.int32 and block_table.dim() == 2 and dev.type == "cuda" and k_pages.device == dev
+                and v_pages.device == dev and scales.device == dev and block_table.device == dev and k_pages.is_contiguous()
+                and v_pages.is_contiguous() and scales.is_contiguous() and block_table.is_contiguous()):
+            return nb, kv, dc * 16, fmt
+    except (AttributeError, ValueError):  # not a tensor, or of another rank
+        pass
+    types = tuple(_KV8_FORMATS)
+    _need(k_pages, "k_pages", types, dev, (6,))
+    _need(v_pages, "v_pages", (k_pages.dtype,), dev, (4,))
+    _need(scales, "scales", (torch.float32,), dev, (4,))
+    _need(block_table, "block_table", (torch.int32,), dev, (2,))
+    _fail(f"kv8 pages must be (num_blocks, KV, 4, D/16, 4, 16) / (num_blocks, KV, D, 16) / (num_blocks, KV, 2, 16); got "
+          f"{tuple(k_pages.shape)}, {tuple(v_pages.shape)}, {tuple(scales.shape)}")
+
+
+def _kv8_rows(t, name, dev, heads=None, dim=None, write=False):
+    """(tensor, elements between tokens) of packed BF16 rows (total, heads, D).  Rows may lie any
+    multiple of 8 elements apart; what else the kernels cannot take as it lies is copied (an output:
+    refused)."""
+    if not isinstance(t, torch.Tensor):
+        _fail(f"{name} must be a tensor")
+    if t.dtype is not torch.bfloat16 or t.device != dev or t.dim() != 3:
+        _fail(f"{name} must be (rows, heads, D) bfloat16 on {dev} (got {tuple(t.shape)} {t.dtype} on {t.device})")
+    n, h, d = t.shape
+    if (heads is not None and h != heads) or (dim is not None and d != dim):
+        _fail(f"{name} {tuple(t.shape)} does not match {heads} heads of {dim}")
+    row, head, one = t.stride()
+    if n <= 1:
+        row = h * d
+    if one == 1 and (head == d or h == 1) and row >= h * d and row % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, row
+    if write:
+        _fail(f"{name} must have contiguous heads and tokens a multiple of 8 elements apart, 16-byte aligned (strides {t.stride()})")
+    return t.clone(memory_format=torch.contiguous_format), h * d
+
+
+def _kv8_ints(t, name, dev, n, dtype=torch.int32):
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == dev and t.shape == (n,) and t.is_contiguous()):
+        _need(t, name, (dtype,), dev, (1,))
+        _fail(f"{name} {tuple(t.shape)} needs {n} entries")
+    return t.data_ptr()
+
+
+def kv8_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
+               block_table: torch.Tensor, cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_seq_len: int = 0) -> None:
+    """Quantize new tokens' K and V and write them into the 8-bit cache, in place.
+
+    k_new/v_new: BF16 (total, KV, D), the sequences' rows one after another; parts of a wider
+    projection output may be passed as they lie.  Pages of one layer: k (num_blocks, KV, 4, D/16, 4,
+    16) and v (num_blocks, KV, D, 16), both float8_e4m3fn or int8, scales (num_blocks, KV, 2, 16)
+    fp32 (K's, then V's).  block_table int32 (B, max_blocks).  cu_rows int32 (B + 1,): sequence b's
+    rows are cu_rows[b] .. cu_rows[b+1] - 1; they are its last positions, seq_lens int32 (B,) being
+    the lengths with them, or None: every sequence has max_seq_len tokens.  Rows behind cu_rows[B]
+    are not touched; rows whose position the block table does not hold are skipped.
+    """
+    dev = k_pages.device
+    nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
+    k_new, ks = _kv8_rows(k_new, "k_new", dev, kv, d)
+    v_new, vs = _kv8_rows(v_new, "v_new", dev, kv, d)
+    if k_new.shape[0] != v_new.shape[0]:
+        _fail(f"k_new {tuple(k_new.shape)} != v_new {tuple(v_new.shape)}")
+    B, mb = block_table.shape
+    if seq_lens is None and max_seq_len <= 0:
+        _fail("seq_lens None needs max_seq_len")
+    cu = _kv8_ints(cu_rows, "cu_rows", dev, B + 1)
+    lens = None if seq_lens is None else _kv8_ints(seq_lens, "seq_lens", dev, B)
+    if k_new.shape[0] == 0:
+        return
+    _kv8_call(_native.load().sdv_kv8_append, "sdv_kv8_append", dev, k_new.data_ptr(), v_new.data_ptr(), ks, vs, k_new.shape[0],
+              k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), nb, fmt, block_table.data_ptr(), mb,
+              cu, lens, int(max_seq_len), B, kv, d)
+
+
+def kv8_gather(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+               cu_rows: torch.Tensor, starts: torch.Tensor, total_rows: int, *, k_out: torch.Tensor | None = None,
+               v_out: torch.Tensor | None = None):
+    """Read the 8-bit cache back: (k, v) BF16 (total_rows, KV, D), each value bf16(code * scale).
+
+    Rows cu_rows[b] .. cu_rows[b+1] - 1 (int32 (B + 1,)) are positions starts[b], starts[b] + 1, ...
+    (int32 (B,)) of sequence b; positions that the block table does not hold read as zeros, rows
+    behind cu_rows[B] are not written.  k_out/v_out: write there instead (tokens may lie any
+    multiple of 8 elements apart).  The other arguments as for kv8_append.
+    """
+    dev = k_pages.device
+    nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
+    total_rows = int(total_rows)
+    if total_rows < 0:
+        _fail(f"total_rows {total_rows} is negative")
+    B, mb = block_table.shape
+    outs = []
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        if t is None:
+            t = torch.empty((total_rows, kv, d), dtype=torch.bfloat16, device=dev)
+        outs.append((*_kv8_rows(t, name, dev, kv, d, write=True), name))
+        if t.shape[0] != total_rows:
+            _fail(f"{name} {tuple(t.shape)} needs {total_rows} rows")
+    (k, ks, _), (v, vs, _) = outs
+    cu, first = _kv8_ints(cu_rows, "cu_rows", dev, B + 1), _kv8_ints(starts, "starts", dev, B)
+    if total_rows == 0:
+        return k, v
+    _kv8_call(_native.load().sdv_kv8_gather, "sdv_kv8_gather", dev, k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), nb,
+              fmt, block_table.data_ptr(), mb, cu, first, B, total_rows, kv, d, k.data_ptr(), v.data_ptr(), ks, vs)
+    return k, v
+
+
+@functools.lru_cache(maxsize=256)
+def kv8_attention_workspace_bytes(batch: int, total_rows: int, q_heads: int, kv_heads: int, head_dim: int, max_q_len: int,
+                                  max_seq_len: int) -> int:
+    n = _native.load().sdv_kv8_attention_workspace_size(batch, total_rows, q_heads, kv_heads, head_dim, max_q_len, max_seq_len)
+    if n == 0:
+        _fail(f"unsupported kv8 attention sizes B={batch} rows={total_rows} H={q_heads} KV={kv_heads} D={head_dim} "
+              f"max_q_len={max_q_len} max_seq_len={max_seq_len}")
+    return int(n)
+
+
+def _kv8_scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
+    """kv8_attention's workspace: one per (device, stream), whose calls are ordered.  A call that a
+    HIP graph records gets its own, from the graph's memory, so that no two graphs share one."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    key = (dev, _stream(dev))
+    ws = _KV8_SCRATCH.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _KV8_SCRATCH[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws
+
+
+def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                  cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_q_len: int, max_seq_len: int, *,
+                  scale: float | None = None, tree_mask: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  workspace_tensor: torch.Tensor | None = None) -> torch.Tensor:
+    """GQA attention of ragged query rows over the 8-bit cache; returns BF16 (total, H, D).
+
+    q BF16 (total, H, D): sequence b's rows are cu_rows[b] .. cu_rows[b+1] - 1, its last positions
+    (seq_lens[b] tokens in all, <= max_seq_len; None: max_seq_len for every sequence).  Any row counts
+    may stand in one batch; max_q_len is the largest.  A row sees the keys up to its own position;
+    with tree_mask (int64 or uint64 (total,), max_q_len <= 64) the context before the new tokens and
+    the new tokens j whose bit j of its mask is set.  scale: default 1 / sqrt(D).  A row that sees
+    nothing is 0; rows behind cu_rows[B] are not written.  out (like q; tokens may lie any multiple of
+    8 elements apart) and workspace_tensor (uint8, kv8_attention_workspace_bytes; not shared by calls
+    that may overlap) are the caller's own.  The pages as for kv8_append.
+    """
+    dev = k_pages.device
+    nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
+    q, q_row = _kv8_rows(q, "q", dev, None, d)
+    total, H = q.shape[:2]
+    if H == 0 or H % kv:
+        _fail(f"q {tuple(q.shape)} does not match pages (KV={kv}, D={d})")
+    B, mb = block_table.shape
+    max_q_len, max_seq_len = int(max_q_len), int(max_seq_len)
+    cu = _kv8_ints(cu_rows, "cu_rows", dev, B + 1)
+    lens = None if seq_lens is None else _kv8_ints(seq_lens, "seq_lens", dev, B)
+    tree = None
+    if tree_mask is not None:
+        if max_q_len > 64:
+            _fail(f"a tree mask holds 64 tokens (max_q_len {max_q_len})")
+        tree = _kv8_ints(tree_mask, "tree_mask", dev, total, torch.uint64 if tree_mask.dtype is torch.uint64 else torch.int64)
+    if out is None:
+        out = torch.empty((total, H, d), dtype=torch.bfloat16, device=dev)
+        out_row = H * d
+    else:
+        out, out_row = _kv8_rows(out, "out", dev, H, d, write=True)
+        if out.shape[0] != total:
+            _fail(f"out {tuple(out.shape)} != q {tuple(q.shape)}")
+    nbytes = kv8_attention_workspace_bytes(B, total, H, kv, d, max_q_len, max_seq_len)
+    if workspace_tensor is None:
+        workspace_tensor = _kv8_scratch(dev, nbytes)
+    else:
+        _need(workspace_tensor, "workspace_tensor", (torch.uint8,), dev)
+        if workspace_tensor.numel() < nbytes:
+            _fail(f"workspace_tensor holds {workspace_tensor.numel()} bytes, {nbytes} needed")
+    if total == 0:
+        return out
+    _kv8_call(_native.load().sdv_kv8_attention, "sdv_kv8_attention", dev, q.data_ptr(), q_row, k_pages.data_ptr(),
+              v_pages.data_ptr(), scales.data_ptr(), nb, fmt, block_table.data_ptr(), mb, cu, lens, tree, B, total, H, kv, d,
+              max_q_len, max_seq_len, d ** -0.5 if scale is None else float(scale), workspace_tensor.data_ptr(),
+              workspace_tensor.numel(), out.data_ptr(), out_row)
+    return out
+
+
 # ---------------------------------------------------------------------------- torch.library
 # The ops as torch custom operators (namespace "sdv"), so torch.compile and fake-tensor tracing
 # see them: the real implementations are the functions above (the C ABI through ctypes); the
@@ -633,3 +841,39 @@ def _lib_quant_append(v_new: torch.Tensor, slot_mapping: torch.Tensor, k_pages: 
 @_lib_quant_append.register_fake
 def _(v_new, slot_mapping, k_pages, v_pages, v_scales, k_new=None, scale_mode="div"):
     return None
+
+
+@torch.library.custom_op("sdv::kv8_append", mutates_args=("k_pages", "v_pages", "scales"))
+def _lib_kv8_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
+                    block_table: torch.Tensor, cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_seq_len: int = 0) -> None:
+    kv8_append(k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len)
+
+
+@_lib_kv8_append.register_fake
+def _(k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len=0):
+    return None
+
+
+@torch.library.custom_op("sdv::kv8_gather", mutates_args=())
+def _lib_kv8_gather(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                    cu_rows: torch.Tensor, starts: torch.Tensor, total_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return kv8_gather(k_pages, v_pages, scales, block_table, cu_rows, starts, total_rows)
+
+
+@_lib_kv8_gather.register_fake
+def _(k_pages, v_pages, scales, block_table, cu_rows, starts, total_rows):
+    shape = (total_rows, v_pages.shape[1], v_pages.shape[2])
+    return tuple(v_pages.new_empty(shape, dtype=torch.bfloat16) for _ in range(2))
+
+
+@torch.library.custom_op("sdv::kv8_attention", mutates_args=())
+def _lib_kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
+                       block_table: torch.Tensor, cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_q_len: int,
+                       max_seq_len: int, scale: float | None = None, tree_mask: torch.Tensor | None = None) -> torch.Tensor:
+    return kv8_attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale=scale,
+                         tree_mask=tree_mask)
+
+
+@_lib_kv8_attention.register_fake
+def _(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale=None, tree_mask=None):
+    return q.new_empty(q.shape)
