@@ -353,8 +353,10 @@ int sdv_kv8_gather(const void* k_pages, const void* v_pages, const float* scales
                    const int32_t* starts, int32_t batch, int32_t total_rows, int32_t kv_heads, int32_t head_dim,
                    void* k_out, void* v_out, int64_t k_stride, int64_t v_stride, void* stream);
 
-/* Bytes of workspace sdv_kv8_attention needs for these sizes (0 on invalid sizes).  It carries nothing
- * from call to call and needs no initialisation; calls that may overlap need one each. */
+/* Bytes of workspace sdv_kv8_attention needs for these sizes (0 on invalid sizes).  Its first
+ * SDV_KV8_SYNC_BYTES bytes must be zero before the first call that uses it; every call leaves them
+ * zero again, and nothing else carries over.  Calls that may overlap need a workspace each. */
+#define SDV_KV8_SYNC_BYTES 4096
 size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
                                         int32_t head_dim, int32_t max_q_len, int32_t max_seq_len);
 

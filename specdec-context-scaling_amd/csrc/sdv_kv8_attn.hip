@@ -36,6 +36,119 @@ __device__ __forceinline__ uint32_t kv8_keep(int n, int w) {
 // probabilities are at most 2^8, and BF16 and fp32 hold them as exactly as they hold those below 1.
 constexpr float kKv8Slack = 8.0f;
 
+// ---------------------------------------------------------------------------- shared tiles
+// The parts of a tile that several ranges share: each workgroup leaves its sums in a slot of the
+// workspace and counts itself in done[first range]; the one that finds all others counted adds the
+// parts up in range order (so the result does not depend on which one it is) and clears the count.
+// Nothing waits.  Parts are written and read with device scope (sc1: through to the memory that all
+// XCDs see), 16 bytes at a time, and every wavefront waits for its stores before the barrier before
+// the count.  Fences that write back or drop an XCD's L2 instead cost its other workgroups more (a
+// batch of 32 sequences 56 -> 59 us with an acquire fence per merge).
+typedef unsigned int kv8_u32x4 __attribute__((ext_vector_type(4)));
+constexpr int kDeviceScope = 16;  // sc1
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv8_parts(float* part, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(part, 0, bytes, 0x00027000);
+}
+__device__ __forceinline__ void kv8_put(__amdgpu_buffer_rsrc_t r, int at, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(kv8_u32x4, v), r, at, 0, kDeviceScope);
+}
+__device__ __forceinline__ f32x4 kv8_get(__amdgpu_buffer_rsrc_t r, int at) {
+  return __builtin_bit_cast(f32x4, (kv8_u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kDeviceScope));
+}
+
+// True in the workgroup that finishes last of `parts`.  All its threads call it.
+__device__ __forceinline__ bool kv8_last(uint32_t* done, int parts, int* lds_flag) {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t before = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *lds_flag = before + 1 == (uint32_t)parts;
+    if (before + 1 == (uint32_t)parts) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  asm volatile("" ::: "memory");
+  return *lds_flag != 0;
+}
+
+// A tile's rows: row0 .. row0 + rows - 1 of the sequence whose packed rows begin at `first`.
+struct Kv8TileRows {
+  int row0, rows, first, kvh;
+};
+
+// Four dimensions of row r of a tile: the sum over the keys divided by that of the exponentials.
+template <int D>
+__device__ __forceinline__ void kv8_write(const Kv8AttnArgs& a, const Kv8TileRows& t, int r, int d, f32x4 acc, float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing: 0
+  const int tok = (t.row0 + r) / a.G, head = t.row0 + r - tok * a.G;
+  *reinterpret_cast<uint2*>(a.out + (int64_t)(t.first + tok) * a.out_stride + (int64_t)(t.kvh * a.G + head) * D + d) =
+      make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+}
+
+// Adds up a tile's parts: slot 2 w0 + skip, then 2 (w0 + 1), 2 (w0 + 2), ...  A batch of them at a time:
+// their maxima and sums by way of LDS, 16 pieces of 16 bytes a thread in flight beside them (a load that
+// goes past the caches takes about a microsecond).
+template <int D, int TR>
+__device__ __forceinline__ void kv8_merge(const Kv8AttnArgs& a, __amdgpu_buffer_rsrc_t mem, int w0, int skip, int parts,
+                                          Kv8TileRows t, float2* lds) {
+  constexpr int kItems = TR * D / 4 / kKv8Threads;  // four-dimension pieces of the tile per thread
+  constexpr int kPart = TR * (D + 4), kBatch = 16 / kItems;
+  constexpr int kStats = (kBatch * TR + kKv8Threads - 1) / kKv8Threads;
+  const int tid = threadIdx.x;
+  const auto part_of = [&](int k) { return (2 * w0 + (k == 0 ? skip : 2 * k)) * kPart * 4; };
+  float mm[kItems], ll[kItems];
+  f32x4 acc[kItems];
+  int piece[kItems], row[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    piece[i] = min(tid + i * kKv8Threads, t.rows * (D / 4) - 1);
+    row[i] = piece[i] / (D / 4);
+    mm[i] = -INFINITY;
+    ll[i] = 0.0f;
+    acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  for (int k0 = 0; k0 < parts; k0 += kBatch) {
+    f32x4 st[kStats], x[kBatch][kItems];
+#pragma unroll
+    for (int j = 0; j < kStats; ++j) {  // past the last part its own again, not counted
+      const int e = tid + j * kKv8Threads;
+      st[j] = kv8_get(mem, part_of(min(k0 + e / TR, parts - 1)) + (TR * D + 4 * (e % TR)) * 4);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) x[k][i] = kv8_get(mem, part_of(min(k0 + k, parts - 1)) + 16 * piece[i]);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kStats; ++j) {
+      const int e = tid + j * kKv8Threads;
+      if (e < kBatch * TR) lds[e] = k0 + e / TR < parts ? make_float2(st[j][0], st[j][1]) : make_float2(-INFINITY, 0.0f);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      float mx = mm[i];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) mx = fmaxf(mx, lds[k * TR + row[i]].x);
+      const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mm[i] - mx);
+      acc[i] *= f;
+      ll[i] *= f;
+      mm[i] = mx;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float2 s = lds[k * TR + row[i]];
+        const float w = k0 + k >= parts ? 0.0f : mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.x - mx);
+        ll[i] += s.y * w;
+        acc[i] += x[k][i] * w;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kItems; ++i)
+    if (tid + i * kKv8Threads < t.rows * (D / 4)) kv8_write<D>(a, t, row[i], 4 * (piece[i] % (D / 4)), acc[i], ll[i]);
+}
+
 // ---------------------------------------------------------------------------- few rows
 // Tiles of 16 or 32 rows: single tokens and verify blocks.  Each of a workgroup's four wavefronts
 // streams every fourth step of the tile with all of its rows; their sums meet in LDS at its end.
@@ -44,34 +157,48 @@ constexpr float kKv8Slack = 8.0f;
 // the four blocks as its 16 key rows, so that lane (n, g) of its result holds row n and tokens 4p + r
 // of block g, and after all four MFMAs every token of block g: with the 16 tokens as its k-slots that
 // is the B operand of O^T = V^T P^T as it stands (A: lane (d, g) the 16 codes of dimension d in block g,
-// one 16-byte load).
+// one 16-byte load).  The matrix cores have time to spare here, so P goes in as two BF16 operands, the
+// rounded value and what the rounding left (16 bits in all), over BF16's whole range of scales.
 template <int D, int FMT, int RT>
-__global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_rows_kernel(Kv8AttnArgs a) {
+__global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a) {
   constexpr int TR = 16 * RT, KI = D / 64, KS = D / 32, DT = D / 16;
-  constexpr int kWaves = kKv8Threads / kWave, kRow = D + 4;
+  constexpr int kWaves = kKv8Threads / kWave, kRow = D + 4, kPart = TR * (D + 4);
   __shared__ __align__(16) float lds_o[kWaves][TR][kRow];
   __shared__ float lds_m[kWaves][TR], lds_l[kWaves][TR];
+  __shared__ __align__(16) uint16_t lds_q[RT == 1 ? 8 : TR * D];
   __shared__ Kv8PlanLds lds_plan;
+  __shared__ int lds_flag;
 
-  Kv8Cut cut = {};
   Kv8Place<TR> at;
-  if (!at.begin(a, lds_plan, (int)blockIdx.x, (int)gridDim.x)) {
-    if (threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
-    return;
-  }
+  if (!at.begin(a, lds_plan, (int)blockIdx.x, (int)gridDim.x)) return;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int n = lane & 15, g = lane >> 4;
   const int64_t page_bytes = (int64_t)kBlock * D;
+  constexpr bool kLate = RT == 2 && D == 128;  // registers are short: the order below is held
   bool first_part = true;
 
   for (;;) {
     const Kv8Seq seq = at.seq;
     const int b = at.b, kvh = at.kvh;
-    const int s0 = (int)(at.u - at.tile0), s1 = (int)min(at.steps, at.end - at.tile0);
+    const uint32_t first_unit = at.u - at.tile0, last_unit = min(at.units_of, at.end - at.tile0);
+    const int steps = kv8_steps<TR>(seq, a.G, at.i, 1);
+    const int s0 = (int)first_unit * a.unit, s1 = min((int)last_unit * a.unit, steps);
     const int row0 = at.i * TR, rows = min(seq.n * a.G - row0, TR);
 
-    // query operand: lane (n, g), k-step 2i + h: dimensions (4i + g)*16 + 8h .. +7
-    bf16x8 qop[RT][KS];
+    const int32_t* table = a.r.table + (int64_t)b * a.r.max_blocks;
+    // block id of this lane's K and V block in a step; -1: none
+    const auto block_id = [&](int step, int k) {
+      const int j = step * 4 + k;
+      const int id = table[min(j, a.r.max_blocks - 1)];
+      return j < a.r.max_blocks && id >= 0 && id < a.r.num_blocks ? id : -1;
+    };
+    int step = s0 + wave;
+    int idk = block_id(step, n >> 2), idv = block_id(step, g);
+    int idk_next = block_id(step + kWaves, n >> 2), idv_next = block_id(step + kWaves, g);
+
+    // query operand: lane (n, g), k-step 2i + h: dimensions (4i + g)*16 + 8h .. +7.  One row tile of it
+    // stays in registers; of two tiles it would not leave two wavefronts a SIMD, and lies in LDS.
+    bf16x8 qreg[RT == 1 ? KS : 1];
     int lim[RT];          // last key that the row sees; with a tree, the context's last
     uint64_t bits[RT];    // new tokens that it sees (tree)
 #pragma unroll
@@ -79,9 +206,14 @@ __global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_
       const int r = row0 + 16 * rt + n, tok = r / a.G, head = r - tok * a.G;
       const bool live = 16 * rt + n < rows;
       const uint16_t* src = a.q + (int64_t)(seq.first + (live ? tok : 0)) * a.q_stride + (int64_t)(kvh * a.G + (live ? head : 0)) * D;
+      if constexpr (RT == 1) {
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk)
-        qop[rt][kk] = *reinterpret_cast<const bf16x8*>(src + (4 * (kk >> 1) + g) * 16 + 8 * (kk & 1));
+        for (int kk = 0; kk < KS; ++kk) qreg[kk] = *reinterpret_cast<const bf16x8*>(src + (4 * (kk >> 1) + g) * 16 + 8 * (kk & 1));
+      } else {
+        for (int kk = wave; kk < KS; kk += kWaves)
+          *reinterpret_cast<uint4*>(&lds_q[(rt * KS + kk) * 512 + lane * 8]) =
+              *reinterpret_cast<const uint4*>(src + (4 * (kk >> 1) + g) * 16 + 8 * (kk & 1));
+      }
       lim[rt] = seq.tree ? seq.ctx - 1 : seq.ctx + (live ? tok : 0);
       bits[rt] = seq.tree && live ? a.tree[seq.first + tok] : 0;
     }
@@ -98,13 +230,6 @@ __global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_
       for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int32_t* table = a.r.table + (int64_t)b * a.r.max_blocks;
-    // block id of this lane's K and V block in a step; -1: none
-    const auto block_id = [&](int step, int k) {
-      const int j = step * 4 + k;
-      const int id = table[min(j, a.r.max_blocks - 1)];
-      return j < a.r.max_blocks && id >= 0 && id < a.r.num_blocks ? id : -1;
-    };
     uint4 kw[4][KI], vw[DT];
     float4 sk, sv, sk_next, sv_next;
     const auto load_k = [&](int id) {
@@ -124,18 +249,12 @@ __global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) vw[dt] = load_stream16(src + dt * (16 * kBlock));
     };
-
-    int step = s0 + wave;
-    int idk = -1, idv = -1, idk_next = -1, idv_next = -1;
     if (step < s1) {
-      idk = block_id(step, n >> 2);
-      idv = block_id(step, g);
-      idk_next = block_id(step + kWaves, n >> 2);
-      idv_next = block_id(step + kWaves, g);
       load_k(idk);
       load_s(idv);
       load_v(idv);
     }
+    if constexpr (RT > 1) __syncthreads();  // lds_q
     for (; step < s1; step += kWaves) {
       sk = sk_next;
       sv = sv_next;
@@ -144,39 +263,76 @@ __global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int p = 0; p < 4; ++p) s[rt][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (RT > 1) asm volatile("" ::: "memory");  // the operand is read again each step
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
+      for (int kk = 0; kk < KS; ++kk) {
+        if constexpr (kLate) __builtin_amdgcn_sched_barrier(0);
+        bf16x8 qop[RT];
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
+        for (int rt = 0; rt < RT; ++rt) {
+          if constexpr (RT == 1)
+            qop[rt] = qreg[kk];
+          else
+            qop[rt] = *reinterpret_cast<const bf16x8*>(&lds_q[(rt * KS + kk) * 512 + lane * 8]);
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
           const uint4 w = kw[p][kk >> 1];
           const bf16x8 kop = (kk & 1) ? kv8_bf16x8<FMT>(w.z, w.w) : kv8_bf16x8<FMT>(w.x, w.y);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qop[rt][kk], s[rt][p], 0, 0, 0);
+          for (int rt = 0; rt < RT; ++rt) s[rt][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qop[rt], s[rt][p], 0, 0, 0);
         }
-      // the next step's K goes into the registers that are free now; the one after's block ids first,
-      // so that waiting for them later does not wait for the data in between
+      }
+      // The next step's K goes into the registers that are free now (with two row tiles of head_dim 128
+      // after the scores, which need them); the one after's block ids first, so that waiting for them
+      // later does not wait for the data in between.
       const int idv_now = idv;
       const bool more = step + kWaves < s1;
-      if (more) {
+      const auto load_next = [&]() {
         idk = idk_next;
         idv = idv_next;
         idk_next = block_id(step + 2 * kWaves, n >> 2);
         idv_next = block_id(step + 2 * kWaves, g);
         load_k(idk);
         load_s(idv);
-      }
+      };
+      if (!kLate && more) load_next();
 
       const bool masked = step * kKv8Step + kKv8Step - 1 > all || __any(idv_now < 0);
       const int key0 = step * kKv8Step + g * kBlock;  // this lane's first token
-      const auto seen = [&](int rt, int t) {
-        const int key = key0 + t;
-        if (key <= lim[rt]) return idv_now >= 0;
-        const int j = key - seq.ctx;
-        return idv_now >= 0 && key < seq.T && j < 64 && ((bits[rt] >> j) & 1);
+      // which of this lane's 16 tokens each of its rows sees
+      uint32_t vis[RT];
+      if (masked) {
+        const auto first = [](int k) { return (1u << min(max(k, 0), 16)) - 1u; };
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          vis[rt] = first(lim[rt] + 1 - key0);
+          const int sh = key0 - seq.ctx;  // the token behind bit 0 of the mask, from this lane's first
+          if (seq.tree && sh > -16 && sh < 64) vis[rt] |= (uint32_t)(sh >= 0 ? bits[rt] >> sh : bits[rt] << -sh) & first(seq.T - key0);
+          if (idv_now < 0) vis[rt] = 0;
+        }
+      }
+      const auto seen = [&](int rt, int t) { return ((vis[rt] >> t) & 1) != 0; };
+      if (masked) {  // codes behind the sequence's end, or of no block, may decode to NaN
+        const int valid = idv_now < 0 ? 0 : seq.T - key0;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          vw[dt].x &= kv8_keep(valid, 0);
+          vw[dt].y &= kv8_keep(valid, 1);
+          vw[dt].z &= kv8_keep(valid, 2);
+          vw[dt].w &= kv8_keep(valid, 3);
+        }
+      }
+      bf16x8 hi[RT][2], lo[RT][2];
+      const auto add_v = [&](int rt, int dt, bf16x8 v0, bf16x8 v1) {
+        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, hi[rt][0], o[rt][dt], 0, 0, 0);
+        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, hi[rt][1], o[rt][dt], 0, 0, 0);
+        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, lo[rt][0], o[rt][dt], 0, 0, 0);
+        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, lo[rt][1], o[rt][dt], 0, 0, 0);
       };
-      bf16x8 pop[RT][2];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
+        if constexpr (kLate) __builtin_amdgcn_sched_barrier(0);
         float y[16];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -203,7 +359,7 @@ __global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_
           m[rt] = mx;
         }
         const float ms = m[rt] == -INFINITY ? 0.0f : m[rt];
-        uint32_t w[8];
+        uint32_t wh[8], wl[8];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           const float4 v4 = quad_lane4(sv, p);
@@ -216,30 +372,26 @@ __global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_
             // the scale of a token that the row does not see may be anything
             if (masked) e[r] = seen(rt, 4 * p + r) ? e[r] : 0.0f;
           }
-          w[2 * p] = pack_bf16x2(e[0], e[1]);
-          w[2 * p + 1] = pack_bf16x2(e[2], e[3]);
-        }
-        pop[rt][0] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
-        pop[rt][1] = __builtin_bit_cast(bf16x8, make_uint4(w[4], w[5], w[6], w[7]));
-      }
-      if (masked) {  // codes behind the sequence's end, or of no block, may decode to NaN
-        const int valid = idv_now < 0 ? 0 : seq.T - key0;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          vw[dt].x &= kv8_keep(valid, 0);
-          vw[dt].y &= kv8_keep(valid, 1);
-          vw[dt].z &= kv8_keep(valid, 2);
-          vw[dt].w &= kv8_keep(valid, 3);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w = pack_bf16x2(e[2 * h], e[2 * h + 1]);
+            wh[2 * p + h] = w;
+            wl[2 * p + h] = pack_bf16x2(e[2 * h] - bf16_lo(w), e[2 * h + 1] - bf16_hi(w));
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          hi[rt][h] = __builtin_bit_cast(bf16x8, make_uint4(wh[4 * h], wh[4 * h + 1], wh[4 * h + 2], wh[4 * h + 3]));
+          lo[rt][h] = __builtin_bit_cast(bf16x8, make_uint4(wl[4 * h], wl[4 * h + 1], wl[4 * h + 2], wl[4 * h + 3]));
         }
       }
+      if (kLate && more) load_next();
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
+        if constexpr (kLate) __builtin_amdgcn_sched_barrier(0);
         const bf16x8 v0 = kv8_bf16x8<FMT>(vw[dt].x, vw[dt].y), v1 = kv8_bf16x8<FMT>(vw[dt].z, vw[dt].w);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pop[rt][0], o[rt][dt], 0, 0, 0);
-          o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pop[rt][1], o[rt][dt], 0, 0, 0);
-        }
+        for (int rt = 0; rt < RT; ++rt) add_v(rt, dt, v0, v1);
       }
       if (more) load_v(idv);
     }
@@ -257,9 +409,10 @@ __global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(&lds_o[wave][16 * rt + n][16 * dt + 4 * g]) = o[rt][dt];
     }
     __syncthreads();
-    const bool whole = s0 == 0 && s1 == (int)at.steps;
+    const bool whole = s0 == 0 && s1 == steps;
     const int slot = 2 * at.w + (first_part ? 0 : 1);
-    float* part = a.part + (int64_t)slot * (TR * (D + 2));
+    const __amdgpu_buffer_rsrc_t parts_mem = kv8_parts(a.part, 2 * at.ranges * kPart * 4);
+    const int part = slot * kPart * 4;  // byte offsets: at most 1024 parts of 32 rows
     for (int e = tid; e < rows * (D / 4); e += kKv8Threads) {
       const int r = e / (D / 4), d = 4 * (e % (D / 4));
       float mm = lds_m[0][r];
@@ -274,62 +427,26 @@ __global__ __launch_bounds__(kKv8Threads, D == 128 && RT == 2 ? 1 : 2) void kv8_
         acc += *reinterpret_cast<const f32x4*>(&lds_o[k][r][d]) * f;
       }
       if (whole) {
-        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;  // a row that sees nothing: 0
-        const int t = (row0 + r) / a.G, head = row0 + r - t * a.G;
-        uint2 w = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-        *reinterpret_cast<uint2*>(a.out + (int64_t)(seq.first + t) * a.out_stride + (int64_t)(kvh * a.G + head) * D + d) = w;
+        kv8_write<D>(a, {row0, rows, seq.first, kvh}, r, d, acc, ll);
       } else {
-        *reinterpret_cast<f32x4*>(part + r * D + d) = acc;
-        if (d == 0) {
-          part[TR * D + r] = mm;
-          part[TR * D + TR + r] = ll;
-        }
+        kv8_put(parts_mem, part + (r * D + d) * 4, acc);
+        if (d == 0) kv8_put(parts_mem, part + (TR * D + 4 * r) * 4, f32x4{mm, ll, 0.0f, 0.0f});
       }
     }
-    if (!whole && s0 == 0) {
-      cut.parts = at.owner(at.tile0 + at.steps - 1) - at.w + 1;
-      cut.slot = slot;
-      cut.first = seq.first;
-      cut.n = seq.n;
-      cut.kvh = kvh;
-      cut.i = at.i;
+    if (!whole) {
+      // the tile's parts: slot 2x of every range x, but for the first range, which may have begun with
+      // another tile's end
+      const int w0 = at.owner(at.tile0), parts = at.owner(at.tile0 + at.units_of - 1) - w0 + 1;
+      if (kv8_last(a.done + w0, parts, &lds_flag)) {
+        kv8_merge<D, TR>(a, parts_mem, w0, at.start(w0) == at.tile0 ? 0 : 1, parts, {row0, rows, seq.first, kvh},
+                         reinterpret_cast<float2*>(&lds_o[0][0][0]));
+      }
     }
     first_part = false;
-    at.u = at.tile0 + (uint32_t)s1;
+    at.u = at.tile0 + last_unit;
     if (at.u >= at.end || !at.next(a)) break;
     __syncthreads();
   }
-  if (tid == 0) a.cuts[blockIdx.x] = cut;
-}
-
-// ---------------------------------------------------------------------------- shared tiles
-// The parts of the tile that workgroup x's range cuts, summed in their order: a thread per four
-// dimensions of a row.
-template <int D, int TR>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a) {
-  const Kv8Cut cut = a.cuts[blockIdx.x];
-  const int e = (int)(blockIdx.y * 256 + threadIdx.x), r = e / (D / 4), d = 4 * (e % (D / 4));
-  const int row = cut.i * TR + r;
-  if (cut.parts == 0 || row >= cut.n * a.G) return;
-  constexpr int kPart = TR * (D + 2);
-  const float* first = a.part + (int64_t)cut.slot * kPart;
-  const float* rest = a.part + (int64_t)(cut.slot & ~1) * kPart;  // part k >= 1: + 2k slots
-  const auto part = [&](int k) { return k == 0 ? first : rest + (int64_t)2 * k * kPart; };
-  float mm = -INFINITY;
-  for (int k = 0; k < cut.parts; ++k) mm = fmaxf(mm, part(k)[TR * D + r]);
-  float ll = 0.0f;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int k = 0; k < cut.parts; ++k) {
-    const float* p = part(k);
-    const float f = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(p[TR * D + r] - mm);
-    ll += p[TR * D + TR + r] * f;
-    acc += *reinterpret_cast<const f32x4*>(p + r * D + d) * f;
-  }
-  const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-  const int t = row / a.G, head = row - t * a.G;
-  uint2 w = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-  *reinterpret_cast<uint2*>(a.out + (int64_t)(cut.first + t) * a.out_stride + (int64_t)(cut.kvh * a.G + head) * D + d) = w;
 }
 
 }  // namespace sdv
@@ -341,17 +458,22 @@ static int kv8_tile_rows(int32_t G, int32_t max_q_len) { return (int64_t)G * max
 
 constexpr int kKv8Grid = 512;  // two workgroups per CU
 
-// Most units of a call, or -1 where they or the row and key counts pass what the plan's 32-bit sums hold.
-static int64_t kv8_units(int32_t batch, int32_t total, int32_t G, int32_t kv_heads, int32_t max_len, int tile) {
+// Most tiles of one KV head, and most units of a call, or -1 where they or the row and key counts pass
+// what the plan's 32-bit sums hold.
+static int64_t kv8_tiles(int32_t batch, int32_t total, int32_t G, int tile) {
+  const int64_t cut = (int64_t)total * G / tile + batch;
+  return cut < (int64_t)total * G ? cut : (int64_t)total * G;
+}
+static int64_t kv8_units(int32_t batch, int32_t total, int32_t G, int32_t kv_heads, int32_t max_len, int tile, int unit) {
   if (((int64_t)max_len + total) * G > (1 << 30)) return -1;
-  const int64_t tiles = (int64_t)total * G / tile + batch;
-  const int64_t units = tiles * (((int64_t)max_len + total) / kKv8Step + 1) * kv_heads;
+  const int64_t units = kv8_tiles(batch, total, G, tile) * (((int64_t)max_len + total) / (kKv8Step * unit) + 1) * kv_heads;
   return units > INT32_MAX ? -1 : units;
 }
 
 static size_t kv8_workspace(int tile, int32_t head_dim) {
-  return kKv8Grid * sizeof(Kv8Cut) + (size_t)kKv8Grid * 2 * tile * (head_dim + 2) * sizeof(float);
+  return SDV_KV8_SYNC_BYTES + (size_t)kKv8Grid * 2 * tile * (head_dim + 4) * sizeof(float);
 }
+static_assert(kKv8Grid * sizeof(uint32_t) <= SDV_KV8_SYNC_BYTES, "a count per range");
 
 static int kv8_attn_sizes(int32_t batch, int32_t total, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
                           int32_t max_len) {
@@ -360,7 +482,7 @@ static int kv8_attn_sizes(int32_t batch, int32_t total, int32_t q_heads, int32_t
   if (head_dim != 64 && head_dim != 128) return SDV_ERR_UNSUPPORTED;
   if (batch > INT32_MAX / 4 || total > INT32_MAX / 2) return SDV_ERR_SHAPE;
   const int32_t G = q_heads / kv_heads;
-  return kv8_units(batch, total, G, kv_heads, max_len, kv8_tile_rows(G, max_q_len)) < 0 ? SDV_ERR_SHAPE : SDV_OK;
+  return kv8_units(batch, total, G, kv_heads, max_len, kv8_tile_rows(G, max_q_len), 1) < 0 ? SDV_ERR_SHAPE : SDV_OK;
 }
 
 extern "C" size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
@@ -372,7 +494,6 @@ extern "C" size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_
 template <int D, int FMT, int RT>
 static void kv8_launch(const Kv8AttnArgs& a, int grid, hipStream_t st) {
   hipLaunchKernelGGL((kv8_rows_kernel<D, FMT, RT>), dim3((unsigned)grid), dim3(kKv8Threads), 0, st, a);
-  hipLaunchKernelGGL((kv8_merge_kernel<D, 16 * RT>), dim3((unsigned)grid, 16 * RT * D / 1024), dim3(256), 0, st, a);
 }
 
 extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
@@ -411,11 +532,17 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   a.kv_heads = kv_heads;
   a.max_len = max_seq_len;
   a.c = (float)((double)scale * 1.4426950408889634);
-  a.min_units = kKv8Threads / kWave;
-  a.cuts = static_cast<Kv8Cut*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kKv8Grid * sizeof(Kv8Cut));
-  const int64_t most = kv8_units(batch, total_rows, G, kv_heads, max_seq_len, tile) / a.min_units;
-  const int grid = (int)(most < 1 ? 1 : most < kKv8Grid ? most : kKv8Grid);
+  a.done = static_cast<uint32_t*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + SDV_KV8_SYNC_BYTES);
+  // Where the device holds a workgroup for every four steps of every tile (one a wavefront), each takes
+  // four steps of one tile: the call is as long as its latencies, and a second tile would double them
+  // (eight sequences of 1000 to 4096 keys, five rows each: 29 us in equal ranges, 24 so; one of 2048
+  // keys 11.2 and 9.1).  Else equal
+  // ranges of single steps.
+  const int64_t tiles = kv8_tiles(batch, total_rows, G, tile) * kv_heads;
+  a.unit = tiles * ((max_seq_len + 4 * kKv8Step - 1) / (4 * kKv8Step)) <= kKv8Grid ? 4 : 1;
+  const int64_t most = kv8_units(batch, total_rows, G, kv_heads, max_seq_len, tile, a.unit);
+  const int grid = (int)(most < kKv8Grid ? most : kKv8Grid);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool fp8 = format == SDV_KV8_FP8;
   if (head_dim == 128 && tile == 16)

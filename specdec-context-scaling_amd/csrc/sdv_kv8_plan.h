@@ -2,31 +2,23 @@
 //
 // A sequence's query rows (token-major: row r is token r / G, head r % G of the KV head's group) are
 // cut into tiles of TR rows; a tile streams the keys its last row sees in steps of 64.  The steps of
-// all tiles, in the order (KV head, sequence, tile), are one sequence of units that is cut into
-// equal contiguous ranges, one per workgroup: single tokens over long contexts, prompt chunks and
+// all tiles, in the order (KV head, sequence, tile), are one sequence that is cut into equal
+// contiguous ranges, one per workgroup: single tokens over long contexts, prompt chunks and
 // batches of both are then equally long for every workgroup, and a workgroup crosses at most two
-// tiles that it shares.  Lengths are read on the device; every workgroup works out its own range.
+// tiles that it shares.  Where there are fewer steps than that takes, a tile's steps are counted in
+// units of several, each one workgroup's.  Lengths are read on the device; every workgroup works out
+// its own range.
 //
-// The steps of a sequence's tiles up to the i-th sum in closed form: tile j has
-// ceil((ctx G + TR (j + 1)) / (64 G)) steps (the last one ceil(T / 64)), a sum of floors of a linear
-// function, which takes as many turns as Euclid's algorithm on (64 G, TR).
+// The units of a sequence's tiles up to the i-th sum in closed form: of u keys each, tile j has
+// ceil((ctx G + TR (j + 1)) / (u G)) (the last one ceil(T / u)), a sum of floors of a linear
+// function, which takes as many turns as Euclid's algorithm on (u G, TR).
 #pragma once
 
 #include "sdv_kv8.h"
 
 namespace sdv {
 
-constexpr int kKv8Step = 64;  // keys per unit: four page blocks
-
-// A tile that begins in a workgroup's range and is cut by its end.  Its first part lies in `slot`
-// (2w or 2w + 1), the later ones in the first slots of the ranges that follow: 2(w + 1), 2(w + 2), ...
-struct Kv8Cut {
-  int parts;     // 0: none
-  int slot;
-  int first, n;  // the sequence's packed rows
-  int kvh, i;    // KV head and tile
-  int pad[2];
-};
+constexpr int kKv8Step = 64;  // keys per step: four page blocks
 
 struct Kv8AttnArgs {
   Kv8Rows r;
@@ -40,9 +32,9 @@ struct Kv8AttnArgs {
   const float* scales;
   int G, kv_heads, max_len;
   float c;         // softmax scale times log2 e
-  int min_units;   // fewest units of a workgroup's range
-  Kv8Cut* cuts;    // per workgroup
-  float* part;     // two slots per workgroup: [TR][D] sums, [TR] maxima, [TR] sums of exponentials
+  int unit;        // steps per unit
+  uint32_t* done;  // per range: finished parts of the shared tile that begins in it; 0 between calls
+  float* part;     // two slots per range: [TR][D] sums, then [TR][4]: maximum, sum of exponentials, -, -
 };
 
 // Sum of floor((a i + b) / m) over i < n.
@@ -81,30 +73,34 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int b) {
   s.T = a.lens ? min(max(a.lens[b], 0), a.max_len) : a.max_len;
   s.ctx = s.T - s.n;
   s.tiles = (s.n * a.G + TR - 1) / TR;
-  s.tree = a.tree != nullptr;
+  int tree = a.tree != nullptr;
+  asm("" : "+v"(tree));  // else the compiler writes the kernels out twice, with and without
+  s.tree = __builtin_amdgcn_readfirstlane(tree);
   return s;
 }
 
-// Steps of the tiles before the i-th, i < tiles.
+// Units of `unit` steps of the tiles before the i-th (i < tiles), of the i-th, and of all.
 template <int TR>
-__device__ __forceinline__ uint32_t kv8_before(const Kv8Seq& s, int G, int i) {
-  if (s.tree) return (uint32_t)i * (uint32_t)((max(s.T, 1) + kKv8Step - 1) / kKv8Step);
-  const uint32_t m = kKv8Step * G;
+__device__ __forceinline__ uint32_t kv8_before(const Kv8Seq& s, int G, int i, int unit) {
+  const uint32_t keys = kKv8Step * unit;
+  if (s.tree) return (uint32_t)i * (((uint32_t)max(s.T, 1) + keys - 1) / keys);
+  const uint32_t m = keys * G;
   return floor_sum((uint32_t)i, m, TR, (uint32_t)(max(s.ctx, 0) * G + TR) + m - 1);
 }
 
 template <int TR>
-__device__ __forceinline__ uint32_t kv8_steps(const Kv8Seq& s, int G, int i) {
-  if (s.tree) return (uint32_t)(max(s.T, 1) + kKv8Step - 1) / kKv8Step;
+__device__ __forceinline__ uint32_t kv8_steps(const Kv8Seq& s, int G, int i, int unit) {
+  const uint32_t keys = kKv8Step * unit;
+  if (s.tree) return ((uint32_t)max(s.T, 1) + keys - 1) / keys;
   const int ctx = max(s.ctx, 0);
-  if (i == s.tiles - 1) return (uint32_t)(ctx + s.n + kKv8Step - 1) / kKv8Step;
-  const uint32_t m = kKv8Step * G;
+  if (i == s.tiles - 1) return ((uint32_t)(ctx + s.n) + keys - 1) / keys;
+  const uint32_t m = keys * G;
   return ((uint32_t)(ctx * G + TR * (i + 1)) + m - 1) / m;
 }
 
 template <int TR>
-__device__ __forceinline__ uint32_t kv8_seq_units(const Kv8Seq& s, int G) {
-  return s.tiles == 0 ? 0 : kv8_before<TR>(s, G, s.tiles - 1) + kv8_steps<TR>(s, G, s.tiles - 1);
+__device__ __forceinline__ uint32_t kv8_seq_units(const Kv8Seq& s, int G, int unit) {
+  return s.tiles == 0 ? 0 : kv8_before<TR>(s, G, s.tiles - 1, unit) + kv8_steps<TR>(s, G, s.tiles - 1, unit);
 }
 
 // Inclusive sum over a wavefront's lanes (DPP row shifts, then row broadcasts).
@@ -137,7 +133,7 @@ struct Kv8Place {
   uint32_t u, end;     // next unit, end of the range
   int kvh, b, i;       // the tile that holds u
   Kv8Seq seq;
-  uint32_t tile0, steps;  // its first unit and its steps
+  uint32_t tile0, units_of;  // its first unit and its units
 
   __device__ __forceinline__ uint32_t start(int x) const { return (uint32_t)x * share + min((uint32_t)x, rest); }
   __device__ __forceinline__ int owner(uint32_t x) const {
@@ -150,12 +146,12 @@ struct Kv8Place {
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
     const int per_run = (a.r.batch + kKv8Threads - 1) / kKv8Threads;
     if (a.r.batch == 1) {
-      per_head = kv8_seq_units<TR>(kv8_seq<TR>(a, 0), a.G);
+      per_head = kv8_seq_units<TR>(kv8_seq<TR>(a, 0), a.G, a.unit);
     } else {
       uint32_t mine = 0;
       for (int k = 0; k < per_run; ++k) {
         const int x = tid * per_run + k;
-        if (x < a.r.batch) mine += kv8_seq_units<TR>(kv8_seq<TR>(a, x), a.G);
+        if (x < a.r.batch) mine += kv8_seq_units<TR>(kv8_seq<TR>(a, x), a.G, a.unit);
       }
       const uint32_t scan = kv8_lane_scan(mine);
       if (lane == kWave - 1) lds.wave[tid / kWave] = scan;
@@ -175,7 +171,7 @@ struct Kv8Place {
     per_head = __builtin_amdgcn_readfirstlane(per_head);
     units = per_head * (uint32_t)a.kv_heads;
     if (units == 0) return false;
-    ranges = (int)min((uint32_t)grid, max(units / (uint32_t)a.min_units, 1u));
+    ranges = (int)min((uint32_t)grid, units);
     w = index;
     if (w >= ranges) return false;
     share = units / (uint32_t)ranges;
@@ -204,7 +200,7 @@ struct Kv8Place {
       for (;; ++b) {
         if (b >= a.r.batch) return false;  // not reached: the runs hold the unit
         seq = kv8_seq<TR>(a, b);
-        const uint32_t n = kv8_seq_units<TR>(seq, a.G);
+        const uint32_t n = kv8_seq_units<TR>(seq, a.G, a.unit);
         if (rem < n) break;
         rem -= n;
         tile0 += n;
@@ -216,20 +212,20 @@ struct Kv8Place {
     i = 0;
     for (int count = seq.tiles; count > 1;) {
       const int stride = (count + kWave - 1) / kWave;
-      const bool at = lane * stride < count && kv8_before<TR>(seq, a.G, i + min(lane * stride, count - 1)) <= rem;
+      const bool at = lane * stride < count && kv8_before<TR>(seq, a.G, i + min(lane * stride, count - 1), a.unit) <= rem;
       const int k = __popcll(__ballot(at)) - 1;
       i += k * stride;
       count = min(stride, count - k * stride);
     }
     i = __builtin_amdgcn_readfirstlane(i);
-    tile0 += __builtin_amdgcn_readfirstlane(kv8_before<TR>(seq, a.G, i));
-    steps = kv8_steps<TR>(seq, a.G, i);
+    tile0 += __builtin_amdgcn_readfirstlane(kv8_before<TR>(seq, a.G, i, a.unit));
+    units_of = kv8_steps<TR>(seq, a.G, i, a.unit);
     return true;
   }
 
   // The tile after this one; false past the last (not reached while u < end).
   __device__ __forceinline__ bool next(const Kv8AttnArgs& a) {
-    tile0 += steps;
+    tile0 += units_of;
     if (++i >= seq.tiles) {
       i = 0;
       do {
@@ -240,7 +236,7 @@ struct Kv8Place {
         seq = kv8_seq<TR>(a, b);
       } while (seq.tiles == 0);
     }
-    steps = kv8_steps<TR>(seq, a.G, i);
+    units_of = kv8_steps<TR>(seq, a.G, i, a.unit);
     return true;
   }
 };

@@ -30,6 +30,7 @@ SCALE_RCP = 1
 
 KV8_FP8 = 0
 KV8_INT8 = 1
+KV8_SYNC_BYTES = 4096        # SDV_KV8_SYNC_BYTES: workspace prefix that is zero between kv8 attention calls
 
 PHASE_QK = 1
 PHASE_PV = 2

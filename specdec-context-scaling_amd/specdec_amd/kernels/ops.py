@@ -723,15 +723,22 @@ def kv8_attention_workspace_bytes(batch: int, total_rows: int, q_heads: int, kv_
     return int(n)
 
 
+def kv8_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """A fresh workspace for kv8_attention of at least nbytes, its count area zeroed."""
+    ws = torch.empty(max(int(nbytes), _native.KV8_SYNC_BYTES), dtype=torch.uint8, device=device)
+    ws[:_native.KV8_SYNC_BYTES].zero_()
+    return ws
+
+
 def _kv8_scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
     """kv8_attention's workspace: one per (device, stream), whose calls are ordered.  A call that a
     HIP graph records gets its own, from the graph's memory, so that no two graphs share one."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        return kv8_workspace(dev, nbytes)
     key = (dev, _stream(dev))
     ws = _KV8_SCRATCH.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _KV8_SCRATCH[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = _KV8_SCRATCH[key] = kv8_workspace(dev, nbytes)
     return ws
 
 
@@ -747,8 +754,8 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     with tree_mask (int64 or uint64 (total,), max_q_len <= 64) the context before the new tokens and
     the new tokens j whose bit j of its mask is set.  scale: default 1 / sqrt(D).  A row that sees
     nothing is 0; rows behind cu_rows[B] are not written.  out (like q; tokens may lie any multiple of
-    8 elements apart) and workspace_tensor (uint8, kv8_attention_workspace_bytes; not shared by calls
-    that may overlap) are the caller's own.  The pages as for kv8_append.
+    8 elements apart) and workspace_tensor (kv8_workspace of kv8_attention_workspace_bytes; not shared
+    by calls that may overlap) are the caller's own.  The pages as for kv8_append.
     """
     dev = k_pages.device
     nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)

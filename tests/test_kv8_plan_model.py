@@ -1,4 +1,4 @@
-"""The shares of sdv_kv8_plan.h, modelled: every step of every tile lies in one range, the closed
+"""The shares of sdv_kv8_plan.h, modelled: every unit of every tile lies in one range, the closed
 form counts what it should, parts lie in slots of their own, and no 32-bit sum overflows."""
 from __future__ import annotations
 
@@ -33,20 +33,21 @@ def tiles(n, G, TR):
     return (n * G + TR - 1) // TR
 
 
-def before(n, T, G, TR, i, tree):
+def before(n, T, G, TR, i, tree, unit=1):
     if tree:
-        return i * ((max(T, 1) + STEP - 1) // STEP)
-    m = STEP * G
+        return i * -(-max(T, 1) // (STEP * unit))
+    m = STEP * unit * G
     return floor_sum(i, m, TR, max(T - n, 0) * G + TR + m - 1)
 
 
-def steps(n, T, G, TR, i, tree):
+def units_of(n, T, G, TR, i, tree, unit=1):
+    """Units of `unit` steps of tile i."""
     if tree:
-        return (max(T, 1) + STEP - 1) // STEP
+        return -(-max(T, 1) // (STEP * unit))
     ctx = max(T - n, 0)
     if i == tiles(n, G, TR) - 1:
-        return (ctx + n + STEP - 1) // STEP
-    m = STEP * G
+        return -(-(ctx + n) // (STEP * unit))
+    m = STEP * unit * G
     return (ctx * G + TR * (i + 1) + m - 1) // m
 
 
@@ -56,19 +57,23 @@ def keys(n, T, G, TR, i):
     return max(T - n, 0) + last // G + 1
 
 
+@pytest.mark.parametrize("unit", [1, 4])
 @pytest.mark.parametrize("G", [1, 2, 3, 6, 7, 20])
 @pytest.mark.parametrize("TR", [16, 32, 128, 256])
-def test_steps_cover_the_keys(G, TR):
+def test_units_cover_the_keys(G, TR, unit):
     rng = random.Random(G * TR)
     for _ in range(60):
         n = rng.choice([1, 2, 5, rng.randint(1, 70), rng.randint(1, 3000)])
         T = rng.choice([0, n - 1, n, n + rng.randint(0, 40), n + rng.randint(0, 40000)])
         total = 0
         for i in range(tiles(n, G, TR)):
-            s = steps(n, T, G, TR, i, False)
-            assert total == before(n, T, G, TR, i, False)
-            need = keys(n, T, G, TR, i)
-            assert s * STEP >= need and (s - 1) * STEP < need + (0 if i == tiles(n, G, TR) - 1 else 1)
+            s = units_of(n, T, G, TR, i, False, unit)
+            assert total == before(n, T, G, TR, i, False, unit)
+            need, step = keys(n, T, G, TR, i), STEP * unit
+            assert s * step >= need and (s - 1) * step < need + (0 if i == tiles(n, G, TR) - 1 else 1)
+            # the tile's steps, of which the last unit may hold fewer
+            steps = units_of(n, T, G, TR, i, False)
+            assert (s - 1) * unit < steps <= s * unit
             total += s
 
 
@@ -81,12 +86,13 @@ def test_ranges(seed):
     for _ in range(rng.choice([1, 2, 9, 40])):
         n = rng.choice([0, 1, 1, 5, rng.randint(1, 64 if tree else 600)])
         seqs.append((n, n + rng.randint(0, 5000)))
-    order = [(h, b, i, steps(n, T, G, TR, i, tree)) for h in range(KV) for b, (n, T) in enumerate(seqs) for i in range(tiles(n, G, TR))]
+    grid, unit = rng.choice([1, 8, 256, 512]), rng.choice([1, 4])
+    order = [(h, b, i, units_of(n, T, G, TR, i, tree, unit)) for h in range(KV) for b, (n, T) in enumerate(seqs)
+             for i in range(tiles(n, G, TR))]
     units = sum(x[3] for x in order)
     if units == 0:
         return
-    grid, least = rng.choice([1, 8, 256, 512]), rng.choice([1, 4])
-    ranges = min(grid, max(units // least, 1))
+    ranges = min(grid, units)
     share, rest = units // ranges, units % ranges
     start = lambda w: w * share + min(w, rest)  # noqa: E731
     split = rest * (share + 1)
