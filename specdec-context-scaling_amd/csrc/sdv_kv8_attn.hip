@@ -36,6 +36,8 @@ __device__ __forceinline__ uint32_t kv8_keep(int n, int w) {
 // probabilities are at most 2^8, and BF16 and fp32 hold them as exactly as they hold those below 1.
 constexpr float kKv8Slack = 8.0f;
 
+constexpr int kKv8Threads = 256;  // of the kernel for few rows
+
 // ---------------------------------------------------------------------------- shared tiles
 // The parts of a tile that several ranges share: each workgroup leaves its sums in a slot of the
 // workspace and counts itself in done[first range]; the one that finds all others counted adds the
@@ -166,10 +168,10 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
   __shared__ __align__(16) float lds_o[kWaves][TR][kRow];
   __shared__ float lds_m[kWaves][TR], lds_l[kWaves][TR];
   __shared__ __align__(16) uint16_t lds_q[RT == 1 ? 8 : TR * D];
-  __shared__ Kv8PlanLds lds_plan;
+  __shared__ Kv8PlanLds<kKv8Threads> lds_plan;
   __shared__ int lds_flag;
 
-  Kv8Place<TR> at;
+  Kv8Place<TR, kKv8Threads> at;
   if (!at.begin(a, lds_plan, (int)blockIdx.x, (int)gridDim.x)) return;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int n = lane & 15, g = lane >> 4;
@@ -180,9 +182,9 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
   for (;;) {
     const Kv8Seq seq = at.seq;
     const int b = at.b, kvh = at.kvh;
-    const uint32_t first_unit = at.u - at.tile0, last_unit = min(at.units_of, at.end - at.tile0);
-    const int steps = kv8_steps<TR>(seq, a.G, at.i, 1);
-    const int s0 = (int)first_unit * a.unit, s1 = min((int)last_unit * a.unit, steps);
+    const uint32_t last_unit = min(at.units_of, at.end - at.tile0);
+    int s0, s1, steps;
+    if (!at.part(a, s0, s1, steps)) break;  // the range ends within the tile's start
     const int row0 = at.i * TR, rows = min(seq.n * a.G - row0, TR);
 
     const int32_t* table = a.r.table + (int64_t)b * a.r.max_blocks;
@@ -434,11 +436,9 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
       }
     }
     if (!whole) {
-      // the tile's parts: slot 2x of every range x, but for the first range, which may have begun with
-      // another tile's end
-      const int w0 = at.owner(at.tile0), parts = at.owner(at.tile0 + at.units_of - 1) - w0 + 1;
+      const int w0 = at.first_range(a), parts = at.parts(a);
       if (kv8_last(a.done + w0, parts, &lds_flag)) {
-        kv8_merge<D, TR>(a, parts_mem, w0, at.start(w0) == at.tile0 ? 0 : 1, parts, {row0, rows, seq.first, kvh},
+        kv8_merge<D, TR>(a, parts_mem, w0, at.second_part(a), parts, {row0, rows, seq.first, kvh},
                          reinterpret_cast<float2*>(&lds_o[0][0][0]));
       }
     }
@@ -451,12 +451,19 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
 
 }  // namespace sdv
 
+#include "sdv_kv8_chunk.h"
+
 using namespace sdv;
 
-// Rows per tile: 16 where a sequence's rows fit one tile of 16, else 32.
-static int kv8_tile_rows(int32_t G, int32_t max_q_len) { return (int64_t)G * max_q_len <= 16 ? 16 : 32; }
+// Rows per tile: 16 or 32 where a sequence's rows fit that, else 256.
+static int kv8_tile_rows(int32_t G, int32_t max_q_len) {
+  const int64_t rows = (int64_t)G * max_q_len;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : kChunkRows;
+}
 
 constexpr int kKv8Grid = 512;  // two workgroups per CU
+
+constexpr int kKv8Start = 5;  // steps that starting a tile costs, about
 
 // Most tiles of one KV head, and most units of a call, or -1 where they or the row and key counts pass
 // what the plan's 32-bit sums hold.
@@ -464,13 +471,15 @@ static int64_t kv8_tiles(int32_t batch, int32_t total, int32_t G, int tile) {
   const int64_t cut = (int64_t)total * G / tile + batch;
   return cut < (int64_t)total * G ? cut : (int64_t)total * G;
 }
-static int64_t kv8_units(int32_t batch, int32_t total, int32_t G, int32_t kv_heads, int32_t max_len, int tile, int unit) {
+static int64_t kv8_units(int32_t batch, int32_t total, int32_t G, int32_t kv_heads, int32_t max_len, int tile, int unit, int start) {
   if (((int64_t)max_len + total) * G > (1 << 30)) return -1;
-  const int64_t units = kv8_tiles(batch, total, G, tile) * (((int64_t)max_len + total) / (kKv8Step * unit) + 1) * kv_heads;
+  const int64_t units = kv8_tiles(batch, total, G, tile) * (((int64_t)max_len + total) / (kKv8Step * unit) + 1 + start) * kv_heads;
   return units > INT32_MAX ? -1 : units;
 }
 
 static size_t kv8_workspace(int tile, int32_t head_dim) {
+  if (tile == kChunkRows)
+    return SDV_KV8_SYNC_BYTES + kChunkGrid * (sizeof(Kv8Cut) + 2 * sizeof(float) * (head_dim == 128 ? chunk_part<128>() : chunk_part<64>()));
   return SDV_KV8_SYNC_BYTES + (size_t)kKv8Grid * 2 * tile * (head_dim + 4) * sizeof(float);
 }
 static_assert(kKv8Grid * sizeof(uint32_t) <= SDV_KV8_SYNC_BYTES, "a count per range");
@@ -482,7 +491,7 @@ static int kv8_attn_sizes(int32_t batch, int32_t total, int32_t q_heads, int32_t
   if (head_dim != 64 && head_dim != 128) return SDV_ERR_UNSUPPORTED;
   if (batch > INT32_MAX / 4 || total > INT32_MAX / 2) return SDV_ERR_SHAPE;
   const int32_t G = q_heads / kv_heads;
-  return kv8_units(batch, total, G, kv_heads, max_len, kv8_tile_rows(G, max_q_len), 1) < 0 ? SDV_ERR_SHAPE : SDV_OK;
+  return kv8_units(batch, total, G, kv_heads, max_len, kv8_tile_rows(G, max_q_len), 1, kKv8Start) < 0 ? SDV_ERR_SHAPE : SDV_OK;
 }
 
 extern "C" size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
@@ -494,6 +503,15 @@ extern "C" size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_
 template <int D, int FMT, int RT>
 static void kv8_launch(const Kv8AttnArgs& a, int grid, hipStream_t st) {
   hipLaunchKernelGGL((kv8_rows_kernel<D, FMT, RT>), dim3((unsigned)grid), dim3(kKv8Threads), 0, st, a);
+}
+
+template <int D, int FMT>
+static void kv8_launch_chunk(Kv8AttnArgs a, int grid, int64_t tiles, hipStream_t st) {
+  a.cuts = reinterpret_cast<Kv8Cut*>(a.part);
+  a.part += kChunkGrid * sizeof(Kv8Cut) / sizeof(float);
+  hipLaunchKernelGGL((kv8_chunk_kernel<D, FMT>), dim3((unsigned)grid), dim3(kChunkThreads), 0, st, a);
+  const unsigned cuts = (unsigned)(tiles < grid ? tiles : grid);  // at most
+  hipLaunchKernelGGL((kv8_chunk_merge_kernel<D>), dim3(cuts, kChunkWaves * D / 32), dim3(256), 0, st, a, grid);
 }
 
 extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
@@ -533,6 +551,7 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   a.max_len = max_seq_len;
   a.c = (float)((double)scale * 1.4426950408889634);
   a.done = static_cast<uint32_t*>(workspace);
+  a.cuts = nullptr;
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + SDV_KV8_SYNC_BYTES);
   // Where the device holds a workgroup for every four steps of every tile (one a wavefront), each takes
   // four steps of one tile: the call is as long as its latencies, and a second tile would double them
@@ -540,12 +559,18 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   // keys 11.2 and 9.1).  Else equal
   // ranges of single steps.
   const int64_t tiles = kv8_tiles(batch, total_rows, G, tile) * kv_heads;
-  a.unit = tiles * ((max_seq_len + 4 * kKv8Step - 1) / (4 * kKv8Step)) <= kKv8Grid ? 4 : 1;
-  const int64_t most = kv8_units(batch, total_rows, G, kv_heads, max_seq_len, tile, a.unit);
-  const int grid = (int)(most < kKv8Grid ? most : kKv8Grid);
+  const int most_grid = tile == kChunkRows ? kChunkGrid : kKv8Grid;
+  a.unit = tiles * ((max_seq_len + 4 * kKv8Step - 1) / (4 * kKv8Step)) <= most_grid ? 4 : 1;
+  a.start = a.unit == 1 ? kKv8Start : 0;
+  const int64_t most = kv8_units(batch, total_rows, G, kv_heads, max_seq_len, tile, a.unit, a.start);
+  const int grid = (int)(most < most_grid ? most : most_grid);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool fp8 = format == SDV_KV8_FP8;
-  if (head_dim == 128 && tile == 16)
+  if (tile == kChunkRows && head_dim == 128)
+    fp8 ? kv8_launch_chunk<128, kFp8>(a, grid, tiles, st) : kv8_launch_chunk<128, kInt8>(a, grid, tiles, st);
+  else if (tile == kChunkRows)
+    fp8 ? kv8_launch_chunk<64, kFp8>(a, grid, tiles, st) : kv8_launch_chunk<64, kInt8>(a, grid, tiles, st);
+  else if (head_dim == 128 && tile == 16)
     fp8 ? kv8_launch<128, kFp8, 1>(a, grid, st) : kv8_launch<128, kInt8, 1>(a, grid, st);
   else if (head_dim == 128)
     fp8 ? kv8_launch<128, kFp8, 2>(a, grid, st) : kv8_launch<128, kInt8, 2>(a, grid, st);

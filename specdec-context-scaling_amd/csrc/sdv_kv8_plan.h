@@ -5,8 +5,9 @@
 // all tiles, in the order (KV head, sequence, tile), are one sequence that is cut into equal
 // contiguous ranges, one per workgroup: single tokens over long contexts, prompt chunks and
 // batches of both are then equally long for every workgroup, and a workgroup crosses at most two
-// tiles that it shares.  Where there are fewer steps than that takes, a tile's steps are counted in
-// units of several, each one workgroup's.  Lengths are read on the device; every workgroup works out
+// tiles that it shares.  A tile's steps are preceded by a few that stand for what starting it costs.
+// Where there are fewer steps than that takes, a tile's steps are counted in units of several, each
+// one workgroup's.  Lengths are read on the device; every workgroup works out
 // its own range.
 //
 // The units of a sequence's tiles up to the i-th sum in closed form: of u keys each, tile j has
@@ -19,6 +20,8 @@
 namespace sdv {
 
 constexpr int kKv8Step = 64;  // keys per step: four page blocks
+
+struct Kv8Cut;
 
 struct Kv8AttnArgs {
   Kv8Rows r;
@@ -33,7 +36,9 @@ struct Kv8AttnArgs {
   int G, kv_heads, max_len;
   float c;         // softmax scale times log2 e
   int unit;        // steps per unit
+  int start;       // units that stand for a tile's start
   uint32_t* done;  // per range: finished parts of the shared tile that begins in it; 0 between calls
+  Kv8Cut* cuts;    // per workgroup, of the kernels whose parts a second launch adds up
   float* part;     // two slots per range: [TR][D] sums, then [TR][4]: maximum, sum of exponentials, -, -
 };
 
@@ -79,9 +84,10 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int b) {
   return s;
 }
 
-// Units of `unit` steps of the tiles before the i-th (i < tiles), of the i-th, and of all.
+// Units of `unit` steps of the tiles before the i-th (i < tiles), of the i-th, and of all; `start` are
+// added to each tile.
 template <int TR>
-__device__ __forceinline__ uint32_t kv8_before(const Kv8Seq& s, int G, int i, int unit) {
+__device__ __forceinline__ uint32_t kv8_steps_before(const Kv8Seq& s, int G, int i, int unit) {
   const uint32_t keys = kKv8Step * unit;
   if (s.tree) return (uint32_t)i * (((uint32_t)max(s.T, 1) + keys - 1) / keys);
   const uint32_t m = keys * G;
@@ -99,8 +105,18 @@ __device__ __forceinline__ uint32_t kv8_steps(const Kv8Seq& s, int G, int i, int
 }
 
 template <int TR>
-__device__ __forceinline__ uint32_t kv8_seq_units(const Kv8Seq& s, int G, int unit) {
-  return s.tiles == 0 ? 0 : kv8_before<TR>(s, G, s.tiles - 1, unit) + kv8_steps<TR>(s, G, s.tiles - 1, unit);
+__device__ __forceinline__ uint32_t kv8_before(const Kv8Seq& s, const Kv8AttnArgs& a, int i) {
+  return kv8_steps_before<TR>(s, a.G, i, a.unit) + (uint32_t)(i * a.start);
+}
+
+template <int TR>
+__device__ __forceinline__ uint32_t kv8_units_of(const Kv8Seq& s, const Kv8AttnArgs& a, int i) {
+  return kv8_steps<TR>(s, a.G, i, a.unit) + (uint32_t)a.start;
+}
+
+template <int TR>
+__device__ __forceinline__ uint32_t kv8_seq_units(const Kv8Seq& s, const Kv8AttnArgs& a) {
+  return s.tiles == 0 ? 0 : kv8_before<TR>(s, a, s.tiles - 1) + kv8_units_of<TR>(s, a, s.tiles - 1);
 }
 
 // Inclusive sum over a wavefront's lanes (DPP row shifts, then row broadcasts).
@@ -115,15 +131,15 @@ __device__ __forceinline__ uint32_t kv8_lane_scan(uint32_t x) {
   return (uint32_t)v;
 }
 
-constexpr int kKv8Threads = 256;
-
+// NT: threads of a workgroup.
+template <int NT>
 struct Kv8PlanLds {
-  uint32_t run[kKv8Threads + 1];  // units before each run of sequences (a run per thread)
-  uint32_t wave[kKv8Threads / kWave];
+  uint32_t run[NT + 1];  // units before each run of sequences (a run per thread)
+  uint32_t wave[NT / kWave];
 };
 
 // A workgroup's place among the units.
-template <int TR>
+template <int TR, int NT>
 struct Kv8Place {
   uint32_t per_head;   // units of one KV head
   uint32_t units;      // of all
@@ -133,7 +149,7 @@ struct Kv8Place {
   uint32_t u, end;     // next unit, end of the range
   int kvh, b, i;       // the tile that holds u
   Kv8Seq seq;
-  uint32_t tile0, units_of;  // its first unit and its units
+  uint32_t tile0, units_of;  // its first unit and its units, those of its start among them
 
   __device__ __forceinline__ uint32_t start(int x) const { return (uint32_t)x * share + min((uint32_t)x, rest); }
   __device__ __forceinline__ int owner(uint32_t x) const {
@@ -141,17 +157,34 @@ struct Kv8Place {
     return (int)(x < split ? x / (share + 1) : rest + (x - split) / share);
   }
 
+  // Up to 64 tiles of a sequence are counted in the lanes of a wavefront and added up there (one
+  // division, where the closed form takes ten, one after the other: 3 us of a chunk's start).
+  uint32_t lane_units, lane_sum;
+  __device__ __forceinline__ void scan_tiles(const Kv8AttnArgs& a) {
+    const int lane = threadIdx.x & (kWave - 1);
+    lane_units = lane < seq.tiles ? kv8_units_of<TR>(seq, a, lane) : 0;
+    lane_sum = kv8_lane_scan(lane_units);
+  }
+
   // False: no range for this workgroup.  `grid` workgroups, this one `index`.
-  __device__ __forceinline__ bool begin(const Kv8AttnArgs& a, Kv8PlanLds& lds, int index, int grid) {
+  __device__ __forceinline__ bool begin(const Kv8AttnArgs& a, Kv8PlanLds<NT>& lds, int index, int grid) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
-    const int per_run = (a.r.batch + kKv8Threads - 1) / kKv8Threads;
+    const int per_run = (a.r.batch + NT - 1) / NT;
+    bool scanned = false;
     if (a.r.batch == 1) {
-      per_head = kv8_seq_units<TR>(kv8_seq<TR>(a, 0), a.G, a.unit);
+      seq = kv8_seq<TR>(a, 0);
+      if (seq.tiles <= kWave) {
+        scan_tiles(a);
+        scanned = true;
+        per_head = __builtin_amdgcn_readlane(lane_sum, kWave - 1);
+      } else {
+        per_head = kv8_seq_units<TR>(seq, a);
+      }
     } else {
       uint32_t mine = 0;
       for (int k = 0; k < per_run; ++k) {
         const int x = tid * per_run + k;
-        if (x < a.r.batch) mine += kv8_seq_units<TR>(kv8_seq<TR>(a, x), a.G, a.unit);
+        if (x < a.r.batch) mine += kv8_seq_units<TR>(kv8_seq<TR>(a, x), a);
       }
       const uint32_t scan = kv8_lane_scan(mine);
       if (lane == kWave - 1) lds.wave[tid / kWave] = scan;
@@ -159,13 +192,13 @@ struct Kv8Place {
       uint32_t before = 0;
       per_head = 0;
 #pragma unroll
-      for (int k = 0; k < kKv8Threads / kWave; ++k) {
+      for (int k = 0; k < NT / kWave; ++k) {
         const uint32_t v = lds.wave[k];
         before += k < tid / kWave ? v : 0;
         per_head += v;
       }
       lds.run[tid] = before + scan - mine;
-      if (tid == 0) lds.run[kKv8Threads] = per_head;
+      if (tid == 0) lds.run[NT] = per_head;
       __syncthreads();
     }
     per_head = __builtin_amdgcn_readfirstlane(per_head);
@@ -184,15 +217,10 @@ struct Kv8Place {
     b = 0;
     if (a.r.batch > 1) {
       // the last run that begins at or before rem; runs of no units share their start with the next
-      int lo = 0, hi = kKv8Threads;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (lds.run[mid] <= rem)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      lo = __builtin_amdgcn_readfirstlane(lo);
+      constexpr int kSkip = NT / kWave;
+      const int outer = __popcll(__ballot(lds.run[lane * kSkip] <= rem)) - 1;
+      const int inner = __popcll(__ballot(lane < kSkip && lds.run[outer * kSkip + min(lane, kSkip - 1)] <= rem)) - 1;
+      const int lo = __builtin_amdgcn_readfirstlane(outer * kSkip + inner);
       b = lo * per_run;
       const uint32_t base = __builtin_amdgcn_readfirstlane(lds.run[lo]);
       rem -= base;
@@ -200,28 +228,50 @@ struct Kv8Place {
       for (;; ++b) {
         if (b >= a.r.batch) return false;  // not reached: the runs hold the unit
         seq = kv8_seq<TR>(a, b);
-        const uint32_t n = kv8_seq_units<TR>(seq, a.G, a.unit);
+        if (per_run == 1) break;
+        const uint32_t n = kv8_seq_units<TR>(seq, a);
         if (rem < n) break;
         rem -= n;
         tile0 += n;
       }
-    } else {
-      seq = kv8_seq<TR>(a, 0);
     }
-    // the tile: the lanes test 64 of them at a time
     i = 0;
-    for (int count = seq.tiles; count > 1;) {
-      const int stride = (count + kWave - 1) / kWave;
-      const bool at = lane * stride < count && kv8_before<TR>(seq, a.G, i + min(lane * stride, count - 1), a.unit) <= rem;
-      const int k = __popcll(__ballot(at)) - 1;
-      i += k * stride;
-      count = min(stride, count - k * stride);
+    if (seq.tiles > 1) {
+      uint32_t before;
+      if (seq.tiles <= kWave) {
+        if (!scanned) scan_tiles(a);
+        i = __popcll(__ballot(lane < seq.tiles && lane_sum <= rem));
+        before = __builtin_amdgcn_readlane(lane_sum - lane_units, i);
+      } else {  // the lanes test 64 tiles at a time
+        for (int count = seq.tiles; count > 1;) {
+          const int stride = (count + kWave - 1) / kWave;
+          const bool at = lane * stride < count && kv8_before<TR>(seq, a, i + min(lane * stride, count - 1)) <= rem;
+          const int k = __popcll(__ballot(at)) - 1;
+          i += k * stride;
+          count = min(stride, count - k * stride);
+        }
+        before = __builtin_amdgcn_readfirstlane(kv8_before<TR>(seq, a, i));
+      }
+      i = __builtin_amdgcn_readfirstlane(i);
+      tile0 += before;
     }
-    i = __builtin_amdgcn_readfirstlane(i);
-    tile0 += __builtin_amdgcn_readfirstlane(kv8_before<TR>(seq, a.G, i, a.unit));
-    units_of = kv8_steps<TR>(seq, a.G, i, a.unit);
+    units_of = kv8_units_of<TR>(seq, a, i);
     return true;
   }
+
+  // Steps s0 .. s1 - 1 of the tile's `steps` are this range's; false: none, the range ends in its start.
+  __device__ __forceinline__ bool part(const Kv8AttnArgs& a, int& s0, int& s1, int& steps) const {
+    steps = (int)kv8_steps<TR>(seq, a.G, i, 1);
+    const int lo = max((int)(u - tile0) - a.start, 0), hi = (int)min(end - tile0, units_of) - a.start;
+    s0 = lo * a.unit;
+    s1 = min(hi * a.unit, steps);
+    return lo < hi;
+  }
+  // The range with the tile's first step, how many ranges have steps of it, and whether the first one's
+  // part is its second (it began with the end of another tile).
+  __device__ __forceinline__ int first_range(const Kv8AttnArgs& a) const { return owner(tile0 + (uint32_t)a.start); }
+  __device__ __forceinline__ int parts(const Kv8AttnArgs& a) const { return owner(tile0 + units_of - 1) - first_range(a) + 1; }
+  __device__ __forceinline__ int second_part(const Kv8AttnArgs& a) const { return start(first_range(a)) < tile0 ? 1 : 0; }
 
   // The tile after this one; false past the last (not reached while u < end).
   __device__ __forceinline__ bool next(const Kv8AttnArgs& a) {
@@ -236,7 +286,7 @@ struct Kv8Place {
         seq = kv8_seq<TR>(a, b);
       } while (seq.tiles == 0);
     }
-    units_of = kv8_steps<TR>(seq, a.G, i, a.unit);
+    units_of = kv8_units_of<TR>(seq, a, i);
     return true;
   }
 };

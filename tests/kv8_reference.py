@@ -88,7 +88,12 @@ def attention(q, pages, bt, new, lens, scale=None, tree=None):
     * forms q.c in fp32 from exact products (D + 4 roundings of values up to sum |q c|, the scales' and
       the exponent's own among them), which moves a score by dx and its exponential by as much,
       relatively, in the numerator and in the sum;
-    * rounds each exponential times V's scale to BF16 once (U, of sum p |v|), sums in fp32;
+    * rounds each exponential times V's scale to BF16 once (U, of sum p |v|), sums in fp32; or, in the
+      kernel for many rows, the exponentials p (1 for the largest, so that their sum l is at least 1)
+      as 2^7 p and V as 2^b v / 2^E to FP16, 2^E at most the largest V scale s of the keys and b at
+      least 5.  Where FP16 is normal that is 2^-11 each of a term, less than U; where it is not,
+      half of its smallest step, 2^-25: 2^-32 of p, which makes 2^-32 sum |v| / l, and 2^-30 s of v,
+      which makes 2^-30 s, since the p / l sum to 1;
     * rounds the output to BF16 (U, of the output).
 
     Blocks that the table does not name, and rows that see nothing, as the operator has them.  NaN
@@ -139,7 +144,9 @@ def attention(q, pages, bt, new, lens, scale=None, tree=None):
                 size = ((x[:, h].abs() @ c.nan_to_num().abs().t()) * sk.abs()).nan_to_num()
                 dx = (D + 4) * 2.0 ** -24 * torch.where(seen, size, torch.zeros_like(size)).amax(-1, keepdim=True) + 2.0 ** -20
                 out[at:at + n, h] = o
-                bound[at:at + n, h] = U * o.abs() + (U + 2 * dx) * (1 + U) * (p @ v0.abs()) / l
+                tiny = seen.double() @ v0.abs() * 2.0 ** -32 / l
+                largest = torch.where(named & ~bad, vs[:, h // G], torch.zeros_like(vs[:, 0])).nan_to_num().max()
+                bound[at:at + n, h] = U * o.abs() + (1 + U) * ((U + 2 * dx) * (p @ v0.abs()) / l + tiny + 2.0 ** -30 * largest)
         at += n
     return out, bound
 

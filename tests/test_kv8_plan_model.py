@@ -77,7 +77,7 @@ def test_units_cover_the_keys(G, TR, unit):
             total += s
 
 
-@pytest.mark.parametrize("seed", range(8))
+@pytest.mark.parametrize("seed", range(24))
 def test_ranges(seed):
     rng = random.Random(seed)
     G, TR, KV = rng.choice([1, 3, 6, 7]), rng.choice([16, 32, 256]), rng.choice([1, 2, 4])
@@ -87,7 +87,8 @@ def test_ranges(seed):
         n = rng.choice([0, 1, 1, 5, rng.randint(1, 64 if tree else 600)])
         seqs.append((n, n + rng.randint(0, 5000)))
     grid, unit = rng.choice([1, 8, 256, 512]), rng.choice([1, 4])
-    order = [(h, b, i, units_of(n, T, G, TR, i, tree, unit)) for h in range(KV) for b, (n, T) in enumerate(seqs)
+    head = 0 if unit > 1 else rng.choice([0, 5])  # units that stand for a tile's start
+    order = [(h, b, i, head + units_of(n, T, G, TR, i, tree, unit)) for h in range(KV) for b, (n, T) in enumerate(seqs)
              for i in range(tiles(n, G, TR))]
     units = sum(x[3] for x in order)
     if units == 0:
@@ -101,12 +102,12 @@ def test_ranges(seed):
     for w in range(ranges):
         assert start(w) < start(w + 1)
         assert owner(start(w)) == w and owner(start(w + 1) - 1) == w
-    # walk the ranges as the kernel does
+    # walk the ranges as the kernels do
     tile0, at = [], 0
     for x in order:
         tile0.append(at)
         at += x[3]
-    parts, cuts, used = {}, {}, set()
+    parts, whole, used = {}, set(), set()
     t = 0
     for w in range(ranges):
         u, end, first = start(w), start(w + 1), True
@@ -114,22 +115,25 @@ def test_ranges(seed):
             t += 1
         k = t
         while u < end:
-            s0, s1 = u - tile0[k], min(order[k][3], end - tile0[k])
-            assert 0 <= s0 < s1
-            if not (s0 == 0 and s1 == order[k][3]):
+            lo, hi = max(u - tile0[k] - head, 0), min(order[k][3], end - tile0[k]) - head
+            if lo >= hi:
+                break  # the range ends in the tile's start
+            if lo == 0 and hi == order[k][3] - head:
+                whole.add(k)
+            else:
                 slot = 2 * w + (0 if first else 1)
                 assert slot not in used and slot < 2 * grid
                 used.add(slot)
-                parts.setdefault(k, []).append((slot, s0, s1))
-                if s0 == 0:
-                    assert w not in cuts
-                    cuts[w] = (k, slot, owner(tile0[k] + order[k][3] - 1) - w + 1)
+                parts.setdefault(k, []).append((w, slot, lo, hi))
             first = False
-            u = tile0[k] + s1
+            u = min(tile0[k] + order[k][3], end)
             k += 1
-    # every cut tile is merged once, from all of its parts in their order
-    assert sorted(c[0] for c in cuts.values()) == sorted(parts)
-    for w, (k, slot, count) in cuts.items():
-        want = [slot] + [2 * (w + j) for j in range(1, count)]
-        assert [p[0] for p in parts[k]] == want and [(slot & ~1) + 2 * j for j in range(1, count)] == want[1:]
-        assert [p[1] for p in parts[k]] == [0] + [p[2] for p in parts[k]][:-1] and parts[k][-1][2] == order[k][3]
+    # every tile is whole in one range, or its parts cover it in order and lie where the merge looks
+    assert whole.isdisjoint(parts) and len(whole) + len(parts) == len(order)
+    for k, own in parts.items():
+        w0 = owner(tile0[k] + head)
+        count = owner(tile0[k] + order[k][3] - 1) - w0 + 1
+        second = 1 if start(w0) < tile0[k] else 0
+        assert [p[0] for p in own] == list(range(w0, w0 + count))
+        assert [p[1] for p in own] == [2 * w0 + second] + [2 * (w0 + j) for j in range(1, count)]
+        assert [p[2] for p in own] == [0] + [p[3] for p in own][:-1] and own[-1][3] == order[k][3] - head
