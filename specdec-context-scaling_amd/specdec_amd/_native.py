@@ -119,6 +119,30 @@ def load(path: os.PathLike | str | None = None, make_default: bool = False) -> c
     return lib
 
 
+_BINDING = _BOUND = None
+
+
+def binding():
+    """The kv8 operators' extension module (csrc/kv8_binding.cpp), bound to the library that every op
+    of this process calls.  Raises SdvError when it is absent."""
+    global _BINDING, _BOUND
+    lib = _LIB if _LIB is not None else load()
+    if _BOUND is not lib:
+        if _BINDING is None:
+            try:
+                import torch  # noqa: F401  (the module links against its libraries)
+
+                from . import _kv8_binding
+            except ImportError as e:
+                raise SdvError(f"{LIB_PATH.parent / '_kv8_binding.so'} is not built ({e}); run `python -m specdec_amd.build` "
+                               f"(or __graft_entry__.build()) on a machine with hipcc") from e
+            _BINDING = _kv8_binding
+        _BINDING.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
+                        ("sdv_kv8_append", "sdv_kv8_gather", "sdv_kv8_attention", "sdv_kv8_attention_workspace_size")))
+        _BOUND = lib
+    return _BINDING
+
+
 def status_string(status: int) -> str:
     return load().sdv_status_string(int(status)).decode()
 

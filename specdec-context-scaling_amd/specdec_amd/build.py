@@ -5,7 +5,7 @@ Here the native code is a plain C-ABI shared library compiled ahead of time, in-
 ``hipcc --offload-arch=gfx950`` (it cross-compiles without a GPU), and loaded with ctypes;
 ``load()`` keeps the reference's name and its "build once, cache the module" behaviour.
 
-    python -m specdec_amd.build          # compile specdec_amd/libsdv.so
+    python -m specdec_amd.build          # compile specdec_amd/libsdv.so and specdec_amd/_kv8_binding.so
     python -m specdec_amd.build --trace  # compile specdec_amd/libsdv_trace.so (phase stamps)
 """
 from __future__ import annotations
@@ -74,6 +74,33 @@ def build(verbose: bool = False, trace: bool = False) -> Path:
     return out
 
 
+BINDING_PATH = PKG_DIR / "_kv8_binding.so"
+
+
+def build_binding(verbose: bool = False) -> Path:
+    """Compile csrc/kv8_binding.cpp (host code against the installed torch) into
+    specdec_amd/_kv8_binding.so (always recompiles)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    libs = cpp_extension.library_paths("cuda")
+    cmd = [_hipcc(), "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           *(f"-isystem{p}" for p in cpp_extension.include_paths("cuda")), f"-isystem{sysconfig.get_paths()['include']}",
+           "-o", str(tmp), str(CSRC / "kv8_binding.cpp"), *(f"-L{p}" for p in libs), f"-Wl,-rpath,{libs[0]}",
+           "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise _native.SdvError(f"hipcc failed ({res.returncode}):\n{res.stdout}{res.stderr}")
+    if verbose and res.stderr.strip():
+        print(res.stderr, file=sys.stderr)
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
+
+
 def load():
     """The loaded native library (ctypes.CDLL); raises SdvError if it has not been built."""
     return _native.load()
@@ -81,3 +108,5 @@ def load():
 
 if __name__ == "__main__":
     print(build(verbose=True, trace="--trace" in sys.argv))
+    if "--trace" not in sys.argv:
+        print(build_binding(verbose=True))

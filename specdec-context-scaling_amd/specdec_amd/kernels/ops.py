@@ -601,6 +601,12 @@ def _kv8_call(fn, what: str, dev: torch.device, *args) -> None:
         _native.check(st, what)
 
 
+def _kv8_device(k_pages) -> torch.device:
+    if not isinstance(k_pages, torch.Tensor):
+        _fail("k_pages must be a tensor")
+    return k_pages.device
+
+
 def _kv8_pages(k_pages, v_pages, scales, block_table, dev):
     """(blocks, KV heads, head_dim, format) of a layer's kv8 pages, checked."""
     try:
@@ -663,7 +669,13 @@ def kv8_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, 
     the lengths with them, or None: every sequence has max_seq_len tokens.  Rows behind cu_rows[B]
     are not touched; rows whose position the block table does not hold are skipped.
     """
-    dev = k_pages.device
+    st = _native.binding().append(k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len)
+    if st is not None:
+        if st:
+            _native.check(st, "sdv_kv8_append")
+        return
+    # something unusual, or wrong: copied where it may be, else named
+    dev = _kv8_device(k_pages)
     nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
     k_new, ks = _kv8_rows(k_new, "k_new", dev, kv, d)
     v_new, vs = _kv8_rows(v_new, "v_new", dev, kv, d)
@@ -691,7 +703,13 @@ def kv8_gather(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tenso
     behind cu_rows[B] are not written.  k_out/v_out: write there instead (tokens may lie any
     multiple of 8 elements apart).  The other arguments as for kv8_append.
     """
-    dev = k_pages.device
+    if k_out is None and v_out is None:
+        got = _native.binding().gather(k_pages, v_pages, scales, block_table, cu_rows, starts, total_rows)
+        if got is not None:
+            if got.__class__ is int:
+                _native.check(got, "sdv_kv8_gather")
+            return got
+    dev = _kv8_device(k_pages)
     nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
     total_rows = int(total_rows)
     if total_rows < 0:
@@ -757,7 +775,14 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     8 elements apart) and workspace_tensor (kv8_workspace of kv8_attention_workspace_bytes; not shared
     by calls that may overlap) are the caller's own.  The pages as for kv8_append.
     """
-    dev = k_pages.device
+    if out is None and workspace_tensor is None:
+        got = _native.binding().attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale,
+                                          tree_mask)
+        if got is not None:
+            if got.__class__ is int:
+                _native.check(got, "sdv_kv8_attention")
+            return got
+    dev = _kv8_device(k_pages)
     nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
     q, q_row = _kv8_rows(q, "q", dev, None, d)
     total, H = q.shape[:2]
