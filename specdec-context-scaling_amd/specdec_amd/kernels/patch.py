@@ -17,7 +17,11 @@ Packs here:
   replaces the dequantize + cat + kv_repeat + eager attention of :715-776 and the cat-based
   append of :778-800.  Appending first is exact: eager attends over dequant(quant(v_cur))
   for the current tokens (:703-704), which is what the kernel reads back.  Other cache
-  formats ("fp16", "fp8") fall through to the engine's original forward.
+  formats ("fp16", "fp8") fall through to the engine's original forward;
+* ``"kv8"``   -- the same switch (``set_kv_format("v_fp8")``) selects a cache that holds K in 8
+  bits as well (:class:`KV8Cache`, ``kv_format`` "fp8" or "int8"): the new tokens go through
+  ``ops.kv8_append``, attention through ``ops.kv8_attention``, softmax in fp32 without the eager
+  path's rounding points.
 
 The layer cache keeps the reference's dict contract ``{"fmt": "v_fp8", "k", "v", "v_scale"}``
 (docs/design_g4_cache_api.md:7-11) with zero-storage shape carriers for the three tensors
@@ -36,13 +40,15 @@ import torch
 
 from .._native import SdvError
 from ..engine import accounting
+from ..engine.kv8_cache import FORMATS as KV8_FORMATS
+from ..engine.kv8_cache import KV8Cache, KV8LayerPages
 from ..engine.paged_cache import LayerPages, PagedKVCache
 
-_PACKS = ("torch", "fp8v")
+_PACKS = ("torch", "fp8v", "kv8")
 _ORIG: dict = {}
 _PACK = "torch"
 _TARGET = None
-_OPTS = {"scale_mode": "rcp", "capacity_tokens": 256, "seed": None}
+_OPTS = {"scale_mode": "rcp", "capacity_tokens": 256, "seed": None, "kv_format": "fp8"}
 
 
 def _default_module():
@@ -50,19 +56,22 @@ def _default_module():
 
 
 def install(pack: str, model_module=None, *, scale_mode: str = "rcp", capacity_tokens: int = 256,
-            seed: int | None = None) -> str:
+            seed: int | None = None, kv_format: str = "fp8") -> str:
     """Activate a pack on `model_module` (default: the reference's specdec.engine.model_self).
 
     scale_mode: how max|v| / 448 is evaluated -- "rcp" (max * RN(1/448): what torch's device
     kernels compute, i.e. the reference engine running on a GPU) or "div" (IEEE division:
     torch on the CPU).  capacity_tokens: initial page capacity per layer (pools grow by
-    doubling).  seed: shuffle the free block list (fragmented placement) when set.
+    doubling).  seed: shuffle the free block list (fragmented placement) when set.  kv_format:
+    the "kv8" pack's codes, "fp8" or "int8".
     """
     global _PACK, _TARGET
     if pack not in _PACKS:
         raise ValueError(f"unknown pack {pack!r}; choose from {sorted(_PACKS)}")
     if scale_mode not in ("rcp", "div"):
         raise ValueError("scale_mode must be 'rcp' or 'div'")
+    if kv_format not in KV8_FORMATS:
+        raise ValueError(f"kv_format must be one of {sorted(KV8_FORMATS)}")
     m = model_module if model_module is not None else (_TARGET or _default_module())
     if _TARGET is not None and m is not _TARGET:
         restore()
@@ -71,9 +80,11 @@ def install(pack: str, model_module=None, *, scale_mode: str = "rcp", capacity_t
     if not _ORIG:
         _ORIG["attn"] = m.SelfAttention.forward
     restore()
-    _OPTS.update(scale_mode=scale_mode, capacity_tokens=int(capacity_tokens), seed=seed)
+    _OPTS.update(scale_mode=scale_mode, capacity_tokens=int(capacity_tokens), seed=seed, kv_format=kv_format)
     if pack == "fp8v":
         m.SelfAttention.forward = _fp8v_forward
+    elif pack == "kv8":
+        m.SelfAttention.forward = _kv8_forward
     _PACK = pack
     return pack
 
@@ -125,14 +136,29 @@ def _accounting(m):
 
 
 def _fp8v_forward(self, x, cos, sin, cache=None):
+    return _paged_forward(self, x, cos, sin, cache, "fp8v")
+
+
+def _kv8_forward(self, x, cos, sin, cache=None):
+    return _paged_forward(self, x, cos, sin, cache, "kv8")
+
+
+def _new_pool(pack: str, KV: int, D: int, batch: int, tokens: int, device):
+    opts = dict(batch=batch, capacity_tokens=max(_OPTS["capacity_tokens"], tokens), device=device, seed=_OPTS["seed"])
+    if pack == "kv8":
+        return KV8LayerPages(KV8Cache(KV, D, kv_format=_OPTS["kv_format"], **opts))
+    return LayerPages(PagedKVCache(KV, D, scale_mode=_OPTS["scale_mode"], **opts))
+
+
+def _paged_forward(self, x, cos, sin, cache, pack: str):
     m = _TARGET
     fmt = cache.get("fmt", self.kv_format) if cache is not None else self.kv_format
     if fmt != "v_fp8" or (cache is not None and "pages" not in cache):
         return _ORIG["attn"](self, x, cos, sin, cache)
     if x.device.type != "cuda":
-        raise SdvError("the fp8v pack runs on a HIP device; move the model there or install('torch')")
+        raise SdvError(f"the {pack} pack runs on a HIP device; move the model there or install('torch')")
     if x.dtype != torch.bfloat16:
-        raise SdvError(f"the fp8v pack computes in bfloat16 (the model runs in {x.dtype})")
+        raise SdvError(f"the {pack} pack computes in bfloat16 (the model runs in {x.dtype})")
     b, s, _ = x.shape
     H, KV, D = self.heads, self.kv_heads, self.head_dim
     q = self.q_proj(x).view(b, s, H, D).transpose(1, 2)
@@ -144,13 +170,14 @@ def _fp8v_forward(self, x, cos, sin, cache=None):
     if cache is None:
         if torch.cuda.is_current_stream_capturing():
             raise SdvError("a prefill from an empty cache creates the page pool; run it before recording a graph")
-        pool = PagedKVCache(KV, D, batch=b, capacity_tokens=max(_OPTS["capacity_tokens"], s), device=x.device,
-                            seed=_OPTS["seed"], scale_mode=_OPTS["scale_mode"])
-        pages = LayerPages(pool)
+        pages = _new_pool(pack, KV, D, b, s, x.device)
+        pool = pages.pool
         t0 = 0
     else:
         pages = cache["pages"]
         pool = pages.pool
+        if isinstance(pool, KV8Cache) != (pack == "kv8"):
+            raise SdvError(f"the {pack} pack cannot go on with a cache that another pack has made")
         t0 = int(cache["k"].shape[2])          # logical length (a trim may have shortened it)
         for i in range(b):
             pool.set_length(i, t0)
@@ -161,7 +188,7 @@ def _fp8v_forward(self, x, cos, sin, cache=None):
     path, reason = decide(phase, s)
     record(path, phase, s, T, reason, H, KV, D)
 
-    # append the s new tokens (quantized V, BF16 K) and attend over the context, one call
+    # append the s new tokens and attend over the context that includes them
     out = pool.append_attend(0, q.transpose(1, 2).contiguous(), k.transpose(1, 2), v.transpose(1, 2),
                              starts=[t0] * b, q_token_major=True)   # (b, s, H, D)
     out = out.view(b, s, H * D)
