@@ -142,7 +142,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   Pages p;
   int64_t ks, vs, max_len;
   const int32_t *cu, *lens;
-  if (n != 9 || !pages(o + 2, p) || !whole(o[8], max_len)) Py_RETURN_NONE;
+  if (!g_append || n != 9 || !pages(o + 2, p) || !whole(o[8], max_len)) Py_RETURN_NONE;
   const at::Tensor *k = rows(o[0], p, p.kv, ks), *v = rows(o[1], p, p.kv, vs);
   if (!k || !v || k->size(0) != v->size(0) || !ints(o[6], p, p.batch + 1, cu) || !lengths(o[7], p, lens) || (!lens && max_len == 0))
     Py_RETURN_NONE;
@@ -158,7 +158,7 @@ PyObject* gather(PyObject*, PyObject* const* o, Py_ssize_t n) {
   Pages p;
   int64_t total;
   const int32_t *cu, *starts;
-  if (n != 7 || !pages(o, p) || !whole(o[6], total) || total == 0 || !ints(o[4], p, p.batch + 1, cu) || !ints(o[5], p, p.batch, starts))
+  if (!g_gather || n != 7 || !pages(o, p) || !whole(o[6], total) || total == 0 || !ints(o[4], p, p.batch + 1, cu) || !ints(o[5], p, p.batch, starts))
     Py_RETURN_NONE;
   Launch on(p);
   const auto options = at::TensorOptions().dtype(at::kBFloat16).device(p.device);
@@ -182,7 +182,7 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   Pages p;
   int64_t q_row, max_q, max_len;
   const int32_t *cu, *lens;
-  if (n != 11 || !pages(o + 1, p) || !whole(o[7], max_q) || !whole(o[8], max_len)) Py_RETURN_NONE;
+  if (!g_attention || n != 11 || !pages(o + 1, p) || !whole(o[7], max_q) || !whole(o[8], max_len)) Py_RETURN_NONE;
   const at::Tensor* q = rows(o[0], p, 0, q_row);
   if (!q || !ints(o[5], p, p.batch + 1, cu) || !lengths(o[6], p, lens)) Py_RETURN_NONE;
   const int64_t total = q->size(0), heads = q->size(1);

@@ -110,6 +110,42 @@ def test_tensors_on_the_cpu_are_refused():
         ops.kv8_attention(x, kp, vp, sc, bt, cu, ln, 1, 16)
 
 
+def test_extension_module_leaves_cpu_tensors_to_the_general_path():
+    b = _native.binding()
+    kp, vp, sc = torch.zeros((2, 2, 4, 8, 4, 16), dtype=torch.int8), torch.zeros((2, 2, 128, 16), dtype=torch.int8), torch.ones((2, 2, 2, 16))
+    bt, cu, ln = torch.zeros((1, 2), dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    x = torch.zeros((1, 2, 128), dtype=torch.bfloat16)
+    assert b.append(x, x, kp, vp, sc, bt, cu, ln, 0) is None
+    assert b.gather(kp, vp, sc, bt, cu, ln, 1) is None
+    assert b.attention(x, kp, vp, sc, bt, cu, ln, 1, 16, None, None) is None
+    for bad in ((), (None,) * 11, (1, "x", None, 2.0, [], {}, (), 0, 0, 0, 0)):
+        assert b.attention(*bad) is None and b.append(*bad) is None and b.gather(*bad) is None
+    with pytest.raises(TypeError):
+        b.bind(1)
+    with pytest.raises(ValueError):
+        b.bind(0, 0, 0, 0)
+    with pytest.raises(TypeError):
+        b.bind("a", "b", "c", "d")
+
+
+def test_fake_tensors_propagate_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        kp = torch.empty((9, 2, 4, 8, 4, 16), dtype=torch.float8_e4m3fn, device="cuda")
+        vp, sc = torch.empty((9, 2, 128, 16), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((9, 2, 2, 16), device="cuda")
+        bt, cu, ln = (torch.empty(n, dtype=torch.int32, device="cuda") for n in ((3, 4), (4,), (3,)))
+        q, x = (torch.empty((7, h, 128), dtype=torch.bfloat16, device="cuda") for h in (12, 2))
+        out = torch.ops.sdv.kv8_attention(q, kp, vp, sc, bt, cu, ln, 3, 60)
+        assert out.shape == q.shape and out.dtype is torch.bfloat16
+        k, v = torch.ops.sdv.kv8_gather(kp, vp, sc, bt, cu, ln, 11)
+        assert k.shape == v.shape == (11, 2, 128) and k.dtype is torch.bfloat16
+        assert torch.ops.sdv.kv8_append(x, x, kp, vp, sc, bt, cu, None, 60) is None
+    schema = str(torch.ops.sdv.kv8_append.default._schema)
+    assert all(re.search(r"Tensor\(a\d+!\) " + name, schema) for name in ("k_pages", "v_pages", "scales"))
+    assert "!" not in str(torch.ops.sdv.kv8_attention.default._schema)
+
+
 def test_int8_quotient_gives_the_ieee_codes(tmp_path):
     cc = shutil.which("gcc")
     if cc is None:
