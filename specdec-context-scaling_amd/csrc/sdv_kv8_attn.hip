@@ -59,7 +59,7 @@ __device__ __forceinline__ f32x4 kv8_get(__amdgpu_buffer_rsrc_t r, int at) {
   return __builtin_bit_cast(f32x4, (kv8_u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kDeviceScope));
 }
 
-// True in the workgroup that finishes last of `parts`.  All its threads call it.
+// True in the workgroup that finishes last of `parts`.  All its threads call it; *lds_flag is theirs.
 __device__ __forceinline__ bool kv8_last(uint32_t* done, int parts, int* lds_flag) {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -155,28 +155,35 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttnArgs& a, __amdgpu_buffer_
 // Tiles of 16 or 32 rows: single tokens and verify blocks.  Each of a workgroup's four wavefronts
 // streams every fourth step of the tile with all of its rows; their sums meet in LDS at its end.
 //
-// A step is four page blocks.  S^T = K Q^T on v_mfma_f32_16x16x32_bf16: MFMA p takes tokens 4p..4p+3 of
-// the four blocks as its 16 key rows, so that lane (n, g) of its result holds row n and tokens 4p + r
-// of block g, and after all four MFMAs every token of block g: with the 16 tokens as its k-slots that
-// is the B operand of O^T = V^T P^T as it stands (A: lane (d, g) the 16 codes of dimension d in block g,
-// one 16-byte load).  The matrix cores have time to spare here, so P goes in as two BF16 operands, the
-// rounded value and what the rounding left (16 bits in all), over BF16's whole range of scales.
+// A wavefront's step is four page blocks, or two where it has two row tiles (with four their registers
+// do not leave two wavefronts a SIMD: 32 sequences of 2048 to 32768 keys, five rows each, 95 us, so 77).  S^T = K Q^T on
+// v_mfma_f32_16x16x32_bf16: of four blocks, MFMA p takes tokens 4p..4p+3 of each as its 16 key rows, so
+// that lane (n, g) of its result holds row n and tokens 4p + r of block g, and after all four MFMAs every
+// token of block g: with the 16 tokens as its k-slots that is the B operand of O^T = V^T P^T as it stands
+// (A: lane (d, g) the 16 codes of dimension d in block g, one 16-byte load).  Of two blocks, lane group
+// g has tokens 8 (g % 2) + 4p + r of block g / 2.  The matrix cores have time to spare here, so P goes
+// in as two BF16 operands, the rounded value and what the rounding left (16 bits in all), over BF16's
+// whole range of scales.
 template <int D, int FMT, int RT>
 __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a) {
   constexpr int TR = 16 * RT, KI = D / 64, KS = D / 32, DT = D / 16;
   constexpr int kWaves = kKv8Threads / kWave, kRow = D + 4, kPart = TR * (D + 4);
+  constexpr int PG = RT == 1 ? 4 : 2;  // page blocks of a wavefront's step, and MFMAs of its q.k^T
+  constexpr int NT = 4 * PG;           // a lane's tokens of them
   __shared__ __align__(16) float lds_o[kWaves][TR][kRow];
   __shared__ float lds_m[kWaves][TR], lds_l[kWaves][TR];
   __shared__ __align__(16) uint16_t lds_q[RT == 1 ? 8 : TR * D];
   __shared__ Kv8PlanLds<kKv8Threads> lds_plan;
-  __shared__ int lds_flag;
+  static_assert(sizeof(lds_o) + sizeof(lds_m) + sizeof(lds_l) + sizeof(lds_q) + sizeof(lds_plan) <= 80 * 1024, "two workgroups per CU");
 
   Kv8Place<TR, kKv8Threads> at;
   if (!at.begin(a, lds_plan, (int)blockIdx.x, (int)gridDim.x)) return;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int n = lane & 15, g = lane >> 4;
   const int64_t page_bytes = (int64_t)kBlock * D;
-  constexpr bool kLate = RT == 2 && D == 128;  // registers are short: the order below is held
+  // the lane's place in a step: block and token of the key row that it loads, of the tokens that it holds
+  const int kblk = PG == 4 ? n >> 2 : n >> 3, vblk = PG == 4 ? g : g >> 1;
+  const int kpart = PG == 4 ? 0 : 2 * (n >> 2 & 1), vtok = PG == 4 ? 0 : 8 * (g & 1);
   bool first_part = true;
 
   for (;;) {
@@ -190,13 +197,14 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
     const int32_t* table = a.r.table + (int64_t)b * a.r.max_blocks;
     // block id of this lane's K and V block in a step; -1: none
     const auto block_id = [&](int step, int k) {
-      const int j = step * 4 + k;
+      const int j = step * PG + k;
       const int id = table[min(j, a.r.max_blocks - 1)];
       return j < a.r.max_blocks && id >= 0 && id < a.r.num_blocks ? id : -1;
     };
-    int step = s0 + wave;
-    int idk = block_id(step, n >> 2), idv = block_id(step, g);
-    int idk_next = block_id(step + kWaves, n >> 2), idv_next = block_id(step + kWaves, g);
+    int step = s0 * (4 / PG) + wave;
+    const int last = s1 * (4 / PG);
+    int idk = block_id(step, kblk), idv = block_id(step, vblk);
+    int idk_next = block_id(step + kWaves, kblk), idv_next = block_id(step + kWaves, vblk);
 
     // query operand: lane (n, g), k-step 2i + h: dimensions (4i + g)*16 + 8h .. +7.  One row tile of it
     // stays in registers; of two tiles it would not leave two wavefronts a SIMD, and lies in LDS.
@@ -232,43 +240,55 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
       for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    uint4 kw[4][KI], vw[DT];
+    uint4 kw[PG][KI];
+    uint32_t vw[DT][PG];
     float4 sk, sv, sk_next, sv_next;
     const auto load_k = [&](int id) {
-      const uint8_t* src = a.k_pages + ((int64_t)max(id, 0) * a.kv_heads + kvh) * page_bytes + g * 64 + (n & 3) * 16;
+      const uint8_t* src = a.k_pages + ((int64_t)max(id, 0) * a.kv_heads + kvh) * page_bytes + kpart * (4 * D) + g * 64 + (n & 3) * 16;
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
+      for (int p = 0; p < PG; ++p)
 #pragma unroll
         for (int i = 0; i < KI; ++i) kw[p][i] = load_stream16(src + p * (4 * D) + i * 256);
     };
     const auto load_s = [&](int id) {
-      const float* src = a.scales + ((int64_t)max(id, 0) * a.kv_heads + kvh) * (2 * kBlock) + 4 * (n & 3);
+      const float* src = a.scales + ((int64_t)max(id, 0) * a.kv_heads + kvh) * (2 * kBlock) + vtok + 4 * (n & (PG - 1));
       sk_next = *reinterpret_cast<const float4*>(src);
       sv_next = *reinterpret_cast<const float4*>(src + kBlock);
     };
     const auto load_v = [&](int id) {
-      const uint8_t* src = a.v_pages + ((int64_t)max(id, 0) * a.kv_heads + kvh) * page_bytes + n * kBlock;
+      const uint8_t* src = a.v_pages + ((int64_t)max(id, 0) * a.kv_heads + kvh) * page_bytes + n * kBlock + vtok;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) vw[dt] = load_stream16(src + dt * (16 * kBlock));
+      for (int dt = 0; dt < DT; ++dt) {
+        if constexpr (PG == 4) {
+          const uint4 w = load_stream16(src + dt * (16 * kBlock));
+          vw[dt][0] = w.x;
+          vw[dt][1] = w.y;
+          vw[dt][2] = w.z;
+          vw[dt][3] = w.w;
+        } else {
+          const uint64_t w = __builtin_nontemporal_load(reinterpret_cast<const uint64_t*>(src + dt * (16 * kBlock)));
+          vw[dt][0] = (uint32_t)w;
+          vw[dt][1] = (uint32_t)(w >> 32);
+        }
+      }
     };
-    if (step < s1) {
+    if (step < last) {
       load_k(idk);
       load_s(idv);
       load_v(idv);
     }
     if constexpr (RT > 1) __syncthreads();  // lds_q
-    for (; step < s1; step += kWaves) {
+    for (; step < last; step += kWaves) {
       sk = sk_next;
       sv = sv_next;
-      f32x4 s[RT][4];
+      f32x4 s[RT][PG];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) s[rt][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int p = 0; p < PG; ++p) s[rt][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if constexpr (RT > 1) asm volatile("" ::: "memory");  // the operand is read again each step
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
-        if constexpr (kLate) __builtin_amdgcn_sched_barrier(0);
         bf16x8 qop[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -278,39 +298,37 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
             qop[rt] = *reinterpret_cast<const bf16x8*>(&lds_q[(rt * KS + kk) * 512 + lane * 8]);
         }
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < PG; ++p) {
           const uint4 w = kw[p][kk >> 1];
           const bf16x8 kop = (kk & 1) ? kv8_bf16x8<FMT>(w.z, w.w) : kv8_bf16x8<FMT>(w.x, w.y);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) s[rt][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qop[rt], s[rt][p], 0, 0, 0);
         }
       }
-      // The next step's K goes into the registers that are free now (with two row tiles of head_dim 128
-      // after the scores, which need them); the one after's block ids first, so that waiting for them
-      // later does not wait for the data in between.
+      // The next step's K goes into the registers that are free now; the one after's block ids first, so
+      // that waiting for them later does not wait for the data in between.
       const int idv_now = idv;
-      const bool more = step + kWaves < s1;
-      const auto load_next = [&]() {
+      const bool more = step + kWaves < last;
+      if (more) {
         idk = idk_next;
         idv = idv_next;
-        idk_next = block_id(step + 2 * kWaves, n >> 2);
-        idv_next = block_id(step + 2 * kWaves, g);
+        idk_next = block_id(step + 2 * kWaves, kblk);
+        idv_next = block_id(step + 2 * kWaves, vblk);
         load_k(idk);
         load_s(idv);
-      };
-      if (!kLate && more) load_next();
+      }
 
-      const bool masked = step * kKv8Step + kKv8Step - 1 > all || __any(idv_now < 0);
-      const int key0 = step * kKv8Step + g * kBlock;  // this lane's first token
-      // which of this lane's 16 tokens each of its rows sees
+      const bool masked = (step + 1) * (PG * kBlock) - 1 > all || __any(idv_now < 0);
+      const int key0 = step * (PG * kBlock) + vblk * kBlock + vtok;  // this lane's first token
+      // which of this lane's tokens each of its rows sees
       uint32_t vis[RT];
       if (masked) {
-        const auto first = [](int k) { return (1u << min(max(k, 0), 16)) - 1u; };
+        const auto first = [](int k) { return (1u << min(max(k, 0), NT)) - 1u; };
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           vis[rt] = first(lim[rt] + 1 - key0);
           const int sh = key0 - seq.ctx;  // the token behind bit 0 of the mask, from this lane's first
-          if (seq.tree && sh > -16 && sh < 64) vis[rt] |= (uint32_t)(sh >= 0 ? bits[rt] >> sh : bits[rt] << -sh) & first(seq.T - key0);
+          if (seq.tree && sh > -NT && sh < 64) vis[rt] |= (uint32_t)(sh >= 0 ? bits[rt] >> sh : bits[rt] << -sh) & first(seq.T - key0);
           if (idv_now < 0) vis[rt] = 0;
         }
       }
@@ -319,36 +337,28 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
         const int valid = idv_now < 0 ? 0 : seq.T - key0;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          vw[dt].x &= kv8_keep(valid, 0);
-          vw[dt].y &= kv8_keep(valid, 1);
-          vw[dt].z &= kv8_keep(valid, 2);
-          vw[dt].w &= kv8_keep(valid, 3);
+#pragma unroll
+          for (int p = 0; p < PG; ++p) vw[dt][p] &= kv8_keep(valid, p);
         }
       }
-      bf16x8 hi[RT][2], lo[RT][2];
-      const auto add_v = [&](int rt, int dt, bf16x8 v0, bf16x8 v1) {
-        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, hi[rt][0], o[rt][dt], 0, 0, 0);
-        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, hi[rt][1], o[rt][dt], 0, 0, 0);
-        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, lo[rt][0], o[rt][dt], 0, 0, 0);
-        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, lo[rt][1], o[rt][dt], 0, 0, 0);
-      };
+      constexpr int NH = PG / 2;  // p.V products per dimension tile, 32 tokens each
+      bf16x8 hi[RT][NH], lo[RT][NH];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        if constexpr (kLate) __builtin_amdgcn_sched_barrier(0);
-        float y[16];
+        float y[NT];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < PG; ++p) {
           const float4 k4 = quad_lane4(sk, p);
 #pragma unroll
           for (int r = 0; r < 4; ++r) y[4 * p + r] = s[rt][p][r] * ((&k4.x)[r] * a.c);
         }
         if (masked) {
 #pragma unroll
-          for (int t = 0; t < 16; ++t) y[t] = seen(rt, t) ? y[t] : -INFINITY;
+          for (int t = 0; t < NT; ++t) y[t] = seen(rt, t) ? y[t] : -INFINITY;
         }
         float mx = y[0];
 #pragma unroll
-        for (int t = 1; t < 16; ++t) mx = fmaxf(mx, y[t]);
+        for (int t = 1; t < NT; ++t) mx = fmaxf(mx, y[t]);
         if (__any(mx > m[rt] + kKv8Slack)) {
           float2 pr = lane_pair<16>(mx);
           mx = fmaxf(pr.x, pr.y);
@@ -361,9 +371,9 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
           m[rt] = mx;
         }
         const float ms = m[rt] == -INFINITY ? 0.0f : m[rt];
-        uint32_t wh[8], wl[8];
+        uint32_t wh[2 * PG], wl[2 * PG];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < PG; ++p) {
           const float4 v4 = quad_lane4(sv, p);
           float e[4];
 #pragma unroll
@@ -382,19 +392,22 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
           }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < NH; ++h) {
           hi[rt][h] = __builtin_bit_cast(bf16x8, make_uint4(wh[4 * h], wh[4 * h + 1], wh[4 * h + 2], wh[4 * h + 3]));
           lo[rt][h] = __builtin_bit_cast(bf16x8, make_uint4(wl[4 * h], wl[4 * h + 1], wl[4 * h + 2], wl[4 * h + 3]));
         }
       }
-      if (kLate && more) load_next();
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        if constexpr (kLate) __builtin_amdgcn_sched_barrier(0);
-        const bf16x8 v0 = kv8_bf16x8<FMT>(vw[dt].x, vw[dt].y), v1 = kv8_bf16x8<FMT>(vw[dt].z, vw[dt].w);
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) add_v(rt, dt, v0, v1);
-      }
+        for (int h = 0; h < NH; ++h) {
+          const bf16x8 v = kv8_bf16x8<FMT>(vw[dt][2 * h], vw[dt][2 * h + 1]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi[rt][h], o[rt][dt], 0, 0, 0);
+            o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo[rt][h], o[rt][dt], 0, 0, 0);
+          }
+        }
       if (more) load_v(idv);
     }
 
@@ -437,7 +450,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
     }
     if (!whole) {
       const int w0 = at.first_range(a), parts = at.parts(a);
-      if (kv8_last(a.done + w0, parts, &lds_flag)) {
+      if (kv8_last(a.done + w0, parts, lds_plan.T)) {
         kv8_merge<D, TR>(a, parts_mem, w0, at.second_part(a), parts, {row0, rows, seq.first, kvh},
                          reinterpret_cast<float2*>(&lds_o[0][0][0]));
       }
@@ -473,7 +486,7 @@ static int64_t kv8_tiles(int32_t batch, int32_t total, int32_t G, int tile) {
 }
 static int64_t kv8_units(int32_t batch, int32_t total, int32_t G, int32_t kv_heads, int32_t max_len, int tile, int unit, int start) {
   if (((int64_t)max_len + total) * G > (1 << 30)) return -1;
-  const int64_t units = kv8_tiles(batch, total, G, tile) * (((int64_t)max_len + total) / (kKv8Step * unit) + 1 + start) * kv_heads;
+  const int64_t units = kv8_tiles(batch, total, G, tile) * (((int64_t)max_len + total) / (kKv8Step << unit) + 1 + start) * kv_heads;
   return units > INT32_MAX ? -1 : units;
 }
 
@@ -491,7 +504,7 @@ static int kv8_attn_sizes(int32_t batch, int32_t total, int32_t q_heads, int32_t
   if (head_dim != 64 && head_dim != 128) return SDV_ERR_UNSUPPORTED;
   if (batch > INT32_MAX / 4 || total > INT32_MAX / 2) return SDV_ERR_SHAPE;
   const int32_t G = q_heads / kv_heads;
-  return kv8_units(batch, total, G, kv_heads, max_len, kv8_tile_rows(G, max_q_len), 1, kKv8Start) < 0 ? SDV_ERR_SHAPE : SDV_OK;
+  return kv8_units(batch, total, G, kv_heads, max_len, kv8_tile_rows(G, max_q_len), 0, kKv8Start) < 0 ? SDV_ERR_SHAPE : SDV_OK;
 }
 
 extern "C" size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
@@ -553,15 +566,26 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   a.done = static_cast<uint32_t*>(workspace);
   a.cuts = nullptr;
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + SDV_KV8_SYNC_BYTES);
-  // Where the device holds a workgroup for every four steps of every tile (one a wavefront), each takes
-  // four steps of one tile: the call is as long as its latencies, and a second tile would double them
-  // (eight sequences of 1000 to 4096 keys, five rows each: 29 us in equal ranges, 24 so; one of 2048
-  // keys 11.2 and 9.1).  Else equal
-  // ranges of single steps.
+  // Units.  Where the device holds a workgroup for every unit of every tile, each takes one: the call is
+  // as long as its latencies, and a second tile would double them (GPU time, 2 KV heads: eight sequences
+  // of 1000 to 4096 keys, five rows each, 31 us in equal ranges of single steps and 19 so; one of 2048
+  // keys 12 and 9).  A unit is four steps, one per wavefront; of a tile's S steps longer ones make less
+  // to add up, and the shortest calls have units of about the root of S / 8 of them (16 rows; 2S / 8, 32:
+  // their parts are larger).  One row in us, at 4, 8 and 16 steps: 8192 keys 12.3 11.8 16.3, 32768 keys
+  // 26 20 20, 131072 keys 51 52 35; five rows: 8192 keys 21 19 26, 32768 keys 50 35 34.  Units of eight
+  // also where ones of four would not fit: eight sequences of 8192 keys, one row each, 14 us, in ranges 19; with
+  // 16 steps the two are even (sixteen sequences 19.9 and 21.8, of mixed lengths 18.4 and 18.1).
   const int64_t tiles = kv8_tiles(batch, total_rows, G, tile) * kv_heads;
+  const int64_t steps = ((int64_t)max_seq_len + kKv8Step - 1) / kKv8Step;
   const int most_grid = tile == kChunkRows ? kChunkGrid : kKv8Grid;
-  a.unit = tiles * ((max_seq_len + 4 * kKv8Step - 1) / (4 * kKv8Step)) <= most_grid ? 4 : 1;
-  a.start = a.unit == 1 ? kKv8Start : 0;
+  const auto fits = [&](int unit) { return tiles * (((steps - 1) >> unit) + 1) <= most_grid; };
+  int unit = 2;
+  if (tile != kChunkRows) {
+    while ((int64_t)128 << (2 * unit) < steps * tile) ++unit;
+    if (unit == 2 && !fits(2)) unit = 3;
+  }
+  a.unit = fits(unit) ? unit : 0;
+  a.start = a.unit == 0 ? kKv8Start : 0;
   const int64_t most = kv8_units(batch, total_rows, G, kv_heads, max_seq_len, tile, a.unit, a.start);
   const int grid = (int)(most < most_grid ? most : most_grid);
   hipStream_t st = static_cast<hipStream_t>(stream);

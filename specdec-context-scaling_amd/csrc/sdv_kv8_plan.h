@@ -19,7 +19,7 @@
 
 namespace sdv {
 
-constexpr int kKv8Step = 64;  // keys per step: four page blocks
+constexpr int kKv8StepBits = 6, kKv8Step = 1 << kKv8StepBits;  // keys per step: four page blocks
 
 struct Kv8Cut;
 
@@ -35,7 +35,7 @@ struct Kv8AttnArgs {
   const float* scales;
   int G, kv_heads, max_len;
   float c;         // softmax scale times log2 e
-  int unit;        // steps per unit
+  int unit;        // steps per unit, as a power of two
   int start;       // units that stand for a tile's start
   uint32_t* done;  // per range: finished parts of the shared tile that begins in it; 0 between calls
   Kv8Cut* cuts;    // per workgroup, of the kernels whose parts a second launch adds up
@@ -72,34 +72,43 @@ struct Kv8Seq {
 };
 
 template <int TR>
-__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int b) {
+__device__ __forceinline__ Kv8Seq kv8_seq_of(const Kv8AttnArgs& a, int first, int n, int T) {
   Kv8Seq s;
-  kv8_rows(a.r, b, s.first, s.n);
-  s.T = a.lens ? min(max(a.lens[b], 0), a.max_len) : a.max_len;
-  s.ctx = s.T - s.n;
-  s.tiles = (s.n * a.G + TR - 1) / TR;
+  s.first = first;
+  s.n = n;
+  s.T = T;
+  s.ctx = T - n;
+  s.tiles = (n * a.G + TR - 1) / TR;
   int tree = a.tree != nullptr;
   asm("" : "+v"(tree));  // else the compiler writes the kernels out twice, with and without
   s.tree = __builtin_amdgcn_readfirstlane(tree);
   return s;
 }
 
-// Units of `unit` steps of the tiles before the i-th (i < tiles), of the i-th, and of all; `start` are
+template <int TR>
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int b) {
+  int first, n;
+  kv8_rows(a.r, b, first, n);
+  return kv8_seq_of<TR>(a, first, n, a.lens ? min(max(a.lens[b], 0), a.max_len) : a.max_len);
+}
+
+// Units of 2^unit steps of the tiles before the i-th (i < tiles), of the i-th, and of all; `start` are
 // added to each tile.
 template <int TR>
 __device__ __forceinline__ uint32_t kv8_steps_before(const Kv8Seq& s, int G, int i, int unit) {
-  const uint32_t keys = kKv8Step * unit;
-  if (s.tree) return (uint32_t)i * (((uint32_t)max(s.T, 1) + keys - 1) / keys);
+  const uint32_t keys = (uint32_t)kKv8Step << unit;
+  if (s.tree) return (uint32_t)i * (((uint32_t)max(s.T, 1) + keys - 1) >> (kKv8StepBits + unit));
+  if (i == 0) return 0;
   const uint32_t m = keys * G;
   return floor_sum((uint32_t)i, m, TR, (uint32_t)(max(s.ctx, 0) * G + TR) + m - 1);
 }
 
 template <int TR>
 __device__ __forceinline__ uint32_t kv8_steps(const Kv8Seq& s, int G, int i, int unit) {
-  const uint32_t keys = kKv8Step * unit;
-  if (s.tree) return ((uint32_t)max(s.T, 1) + keys - 1) / keys;
+  const uint32_t keys = (uint32_t)kKv8Step << unit;
+  if (s.tree) return ((uint32_t)max(s.T, 1) + keys - 1) >> (kKv8StepBits + unit);
   const int ctx = max(s.ctx, 0);
-  if (i == s.tiles - 1) return ((uint32_t)(ctx + s.n) + keys - 1) / keys;
+  if (i == s.tiles - 1) return ((uint32_t)(ctx + s.n) + keys - 1) >> (kKv8StepBits + unit);
   const uint32_t m = keys * G;
   return ((uint32_t)(ctx * G + TR * (i + 1)) + m - 1) / m;
 }
@@ -131,11 +140,11 @@ __device__ __forceinline__ uint32_t kv8_lane_scan(uint32_t x) {
   return (uint32_t)v;
 }
 
-// NT: threads of a workgroup.
+// NT: threads of a workgroup, a run of sequences each.
 template <int NT>
 struct Kv8PlanLds {
-  uint32_t run[NT + 1];  // units before each run of sequences (a run per thread)
-  uint32_t wave[NT / kWave];
+  uint4 run[NT];  // units of the wavefront's runs up to and with this one, units of this one; its one sequence's first, n
+  int T[NT];      //   and T
 };
 
 // A workgroup's place among the units.
@@ -182,24 +191,20 @@ struct Kv8Place {
       }
     } else {
       uint32_t mine = 0;
+      Kv8Seq last = {};
       for (int k = 0; k < per_run; ++k) {
         const int x = tid * per_run + k;
-        if (x < a.r.batch) mine += kv8_seq_units<TR>(kv8_seq<TR>(a, x), a);
+        if (x >= a.r.batch) break;
+        last = kv8_seq<TR>(a, x);
+        mine += kv8_seq_units<TR>(last, a);
       }
       const uint32_t scan = kv8_lane_scan(mine);
-      if (lane == kWave - 1) lds.wave[tid / kWave] = scan;
+      lds.run[tid] = make_uint4(scan, mine, (uint32_t)last.first, (uint32_t)last.n);
+      lds.T[tid] = last.T;
       __syncthreads();
-      uint32_t before = 0;
       per_head = 0;
 #pragma unroll
-      for (int k = 0; k < NT / kWave; ++k) {
-        const uint32_t v = lds.wave[k];
-        before += k < tid / kWave ? v : 0;
-        per_head += v;
-      }
-      lds.run[tid] = before + scan - mine;
-      if (tid == 0) lds.run[NT] = per_head;
-      __syncthreads();
+      for (int k = 0; k < NT / kWave; ++k) per_head += lds.run[k * kWave + kWave - 1].x;
     }
     per_head = __builtin_amdgcn_readfirstlane(per_head);
     units = per_head * (uint32_t)a.kv_heads;
@@ -216,19 +221,32 @@ struct Kv8Place {
     tile0 = (uint32_t)kvh * per_head;
     b = 0;
     if (a.r.batch > 1) {
-      // the last run that begins at or before rem; runs of no units share their start with the next
-      constexpr int kSkip = NT / kWave;
-      const int outer = __popcll(__ballot(lds.run[lane * kSkip] <= rem)) - 1;
-      const int inner = __popcll(__ballot(lane < kSkip && lds.run[outer * kSkip + min(lane, kSkip - 1)] <= rem)) - 1;
-      const int lo = __builtin_amdgcn_readfirstlane(outer * kSkip + inner);
-      b = lo * per_run;
-      const uint32_t base = __builtin_amdgcn_readfirstlane(lds.run[lo]);
-      rem -= base;
-      tile0 += base;
+      // the wavefront whose runs hold the unit, then the run: the first that ends behind it
+      int wv = 0;
+#pragma unroll
+      for (int k = 0; k < NT / kWave - 1; ++k) {
+        const uint32_t n = lds.run[k * kWave + kWave - 1].x;
+        if (wv == k && rem >= n) {
+          rem -= n;
+          tile0 += n;
+          wv = k + 1;
+        }
+      }
+      wv = __builtin_amdgcn_readfirstlane(wv);
+      rem = __builtin_amdgcn_readfirstlane(rem);
+      const uint4 run = lds.run[wv * kWave + lane];
+      const int T = lds.T[wv * kWave + lane];
+      const int at = min(__popcll(__ballot(run.x <= rem)), kWave - 1);
+      const uint32_t before = __builtin_amdgcn_readlane(run.x, at) - __builtin_amdgcn_readlane(run.y, at);
+      rem -= before;
+      tile0 += before;
+      b = (wv * kWave + at) * per_run;
+      if (per_run == 1) {
+        seq = kv8_seq_of<TR>(a, __builtin_amdgcn_readlane(run.z, at), __builtin_amdgcn_readlane(run.w, at), __builtin_amdgcn_readlane(T, at));
+      } else
       for (;; ++b) {
         if (b >= a.r.batch) return false;  // not reached: the runs hold the unit
         seq = kv8_seq<TR>(a, b);
-        if (per_run == 1) break;
         const uint32_t n = kv8_seq_units<TR>(seq, a);
         if (rem < n) break;
         rem -= n;
@@ -261,10 +279,10 @@ struct Kv8Place {
 
   // Steps s0 .. s1 - 1 of the tile's `steps` are this range's; false: none, the range ends in its start.
   __device__ __forceinline__ bool part(const Kv8AttnArgs& a, int& s0, int& s1, int& steps) const {
-    steps = (int)kv8_steps<TR>(seq, a.G, i, 1);
+    steps = (int)kv8_steps<TR>(seq, a.G, i, 0);
     const int lo = max((int)(u - tile0) - a.start, 0), hi = (int)min(end - tile0, units_of) - a.start;
-    s0 = lo * a.unit;
-    s1 = min(hi * a.unit, steps);
+    s0 = lo << a.unit;
+    s1 = min(hi << a.unit, steps);
     return lo < hi;
   }
   // The range with the tile's first step, how many ranges have steps of it, and whether the first one's
