@@ -587,7 +587,6 @@ def fp8_encode(x: torch.Tensor) -> torch.Tensor:
 # ---------------------------------------------------------------------------- the 8-bit KV cache
 _KV8_FORMATS = {torch.float8_e4m3fn: _native.KV8_FP8, torch.int8: _native.KV8_INT8}
 _KV8_SCRATCH: dict = {}  # (device, stream) -> kv8_attention's workspace of eager calls
-_KV8_READY: dict = {}    # id(tensor) -> weakref of workspaces whose count area is known to be zero
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -745,20 +744,8 @@ def kv8_attention_workspace_bytes(batch: int, total_rows: int, q_heads: int, kv_
 def kv8_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """A fresh workspace for kv8_attention of at least nbytes, its count area zeroed."""
     ws = torch.empty(max(int(nbytes), _native.KV8_SYNC_BYTES), dtype=torch.uint8, device=device)
-    _kv8_zero(ws)
-    return ws
-
-
-def _kv8_zero(ws: torch.Tensor) -> None:
-    """Zero a workspace's count area, once: calls leave it zero (a recorded fill has not run yet, and
-    does not count)."""
-    ref = _KV8_READY.get(id(ws))
-    if ref is not None and ref() is ws:
-        return
     ws[:_native.KV8_SYNC_BYTES].zero_()
-    if not torch.cuda.is_current_stream_capturing():
-        key = id(ws)
-        _KV8_READY[key] = weakref.ref(ws, lambda _r, key=key: _KV8_READY.pop(key, None))
+    return ws
 
 
 def _kv8_scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
@@ -785,8 +772,12 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     with tree_mask (int64 or uint64 (total,), max_q_len <= 64) the context before the new tokens and
     the new tokens j whose bit j of its mask is set.  scale: default 1 / sqrt(D).  A row that sees
     nothing is 0; rows behind cu_rows[B] are not written.  out (like q; tokens may lie any multiple of
-    8 elements apart) and workspace_tensor (kv8_workspace of kv8_attention_workspace_bytes, for this
-    operator alone and not for calls that may overlap) are the caller's own.  The pages as for kv8_append.
+    8 elements apart) and workspace_tensor (uint8, of kv8_attention_workspace_bytes, not for calls that
+    may overlap) are the caller's own.  The pages as for kv8_append.
+
+    A sequence with more than 32 rows per KV head (or a batch with one by max_q_len) holds V relative to
+    the largest V scale of a row tile's keys, those that a row does not see among them: of V, 2^-29 of that
+    largest and less loses bits below BF16's.
     """
     if out is None and workspace_tensor is None:
         got = _native.binding().attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale,
@@ -826,7 +817,8 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
             _fail(f"workspace_tensor holds {workspace_tensor.numel()} bytes, {nbytes} needed")
         if workspace_tensor.data_ptr() % 256:
             _fail("workspace_tensor must be 256-byte aligned")
-        _kv8_zero(workspace_tensor)
+        if total:  # it may have held anything since the last call
+            workspace_tensor[:_native.KV8_SYNC_BYTES].zero_()
     if total == 0:
         return out
     _kv8_call(_native.load().sdv_kv8_attention, "sdv_kv8_attention", dev, q.data_ptr(), q_row, k_pages.data_ptr(),
