@@ -363,14 +363,18 @@ size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32
 /*
  * Attention of every sequence's new tokens over its cached context, which ends with them: single
  * tokens, verify blocks, prompt chunks, or all in one batch.  Row i of sequence b (n_b rows, T_b =
- * seq_lens[b] clamped to [0, max_seq_len], or max_seq_len where seq_lens is NULL) is position T_b - n_b + i and sees keys up to its own;
- * with tree_mask (uint64 [total_rows]; max_q_len <= 64) it sees the context T_b - n_b and, of the new
- * tokens, those j whose bit j of its mask is set: a tree of drafted tokens.  q head h reads KV head
- * h / (q_heads / kv_heads).  max_q_len is the largest n_b.  Softmax of scale * q.k in fp32, probabilities
- * times V's scale rounded to BF16 for the product with V, fp32 sums, BF16 output.  A row that sees
- * nothing is 0; what a row does not see, infinities and NaN among it, does not reach it.
+ * seq_lens[b] clamped to [0, max_seq_len], or max_seq_len where seq_lens is NULL) is position T_b - n_b + i
+ * and sees keys up to its own; with tree_mask (uint64 [total_rows]; max_q_len <= 64) it sees the context
+ * T_b - n_b and, of the new tokens, those j whose bit j of its mask is set: a tree of drafted tokens.  q head h reads KV head
+ * h / (q_heads / kv_heads).  max_q_len is the largest n_b (it chooses the kernel; a sequence with more
+ * rows is computed all the same).  Softmax of scale * q.k in fp32, sums in fp32, BF16 output.  A row that
+ * sees nothing is 0; what a row does not see, infinities and NaN among it, does not reach it.
+ * Operands of the product with V: with max_q_len * q_heads / kv_heads <= 32 the probability times V's scale
+ * to 16 bits; with more, probability and V to FP16's 11 bits, V relative to the largest V scale of the keys
+ * of a tile of 256 rows (seen by a row or not), so that V of 2^-29 of that largest and less is held to fewer bits
+ * than BF16's.
  * Size limits: (max_seq_len + total_rows) * q_heads / kv_heads <= 2^30 and, with tiles of 16 rows (32 where
- * max_q_len * q_heads / kv_heads > 16), tiles * steps of 64 keys * kv_heads < 2^31.
+ * max_q_len * q_heads / kv_heads > 16, 256 where it is > 32), tiles * (steps of 64 keys + 5) * kv_heads < 2^31.
  */
 int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
                       int32_t num_blocks, int32_t format, const int32_t* block_table, int32_t max_blocks_per_seq,

@@ -73,4 +73,16 @@ __device__ __forceinline__ float kv8_decode(uint32_t w, int sel) {
   return (float)(int8_t)(w >> (8 * sel));
 }
 
+// Inclusive sum over a wavefront's lanes (DPP row shifts, then row broadcasts).
+__device__ __forceinline__ uint32_t kv8_lane_scan(uint32_t x) {
+  int v = (int)x;
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return (uint32_t)v;
+}
+
 }  // namespace sdv

@@ -3,10 +3,11 @@
 //   x_j = scale * s^K_j * (q . c^K_j),   out = sum_j e^(x_j - M) s^V_j c^V_j / sum_j e^(x_j - M)
 //
 // over the keys j that the row sees, in one pass over them with a running maximum and sum.  The
-// codes c are exact in BF16, so q.c is exact products summed in fp32 on the matrix cores, and the
-// scales multiply the fp32 scores and probabilities.  The one rounding before the output's is
-// e^(..) s^V to BF16, the operand of its product (half a step, 2^-9 of each term; the terms' errors
-// are independent).
+// codes c are exact in BF16, so q.c is exact products summed in fp32 on the matrix cores, and K's
+// scales multiply the fp32 scores.  The one rounding before the output's is that of the operands of
+// the second product: e^(..) s^V to 16 bits here, e^(..) and s^V c^V to FP16 in the kernel for many
+// rows.  (With e^(..) s^V as one BF16 operand, 2^-9 of each term, the outputs' error against 64 bits
+// was 2.7e-3, of which BF16 outputs alone make 1.6e-3.)
 #include "sdv_kv8_plan.h"
 
 namespace sdv {
@@ -164,6 +165,11 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttnArgs& a, __amdgpu_buffer_
 // g has tokens 8 (g % 2) + 4p + r of block g / 2.  The matrix cores have time to spare here, so P goes
 // in as two BF16 operands, the rounded value and what the rounding left (16 bits in all), over BF16's
 // whole range of scales.
+//
+// Long batches are bound by memory: single tokens of 32 sequences of 2048 to 32768 keys (293 MB of pages,
+// 2 KV heads of 128) take 55 to 57 us, 5.2 TB/s, a large copy's rate; the matrix cores are busy a tenth of
+// it.  Short calls are bound by latencies, each a microsecond or more: lengths, page ids, the pages,
+// the merge's count, and the parts.  One token over 2048 keys takes 7.3 us eager, over 32768 20.
 template <int D, int FMT, int RT>
 __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a) {
   constexpr int TR = 16 * RT, KI = D / 64, KS = D / 32, DT = D / 16;
@@ -468,12 +474,6 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
 
 using namespace sdv;
 
-// Rows per tile: 16 or 32 where a sequence's rows fit that, else 256.
-static int kv8_tile_rows(int32_t G, int32_t max_q_len) {
-  const int64_t rows = (int64_t)G * max_q_len;
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : kChunkRows;
-}
-
 constexpr int kKv8Grid = 512;  // two workgroups per CU
 
 constexpr int kKv8Start = 5;  // steps that starting a tile costs, about
@@ -490,6 +490,18 @@ static int64_t kv8_units(int32_t batch, int32_t total, int32_t G, int32_t kv_hea
   return units > INT32_MAX ? -1 : units;
 }
 
+// Rows per tile: 16 or 32 where a sequence's rows fit that.  With more rows 256, whose stages serve more of
+// them (1800 over 32768 keys 82 us, in tiles of 32 195), or 32 where all tiles of those together have at
+// most eight steps for each workgroup of the device: the many small ones start sooner and their parts need
+// no second launch.  2 KV heads of 128, tiles of 32 and of 256, in us: 300 tokens' 1800 rows 12 and 25, 288 rows over 2048 keys 14 and 23, 144 over 8192
+// (1280 steps) 20 and 25, 1200 over 2048 (2432) 21 and 28; of four sequences of 8192 48 rows each (2560) 24
+// and 24, 144 each (5632) 33 and 32, 288 each (10240) 42 and 37; 1200 over 8192 (9728) 44 and 36.
+static int kv8_tile_rows(int32_t batch, int32_t total, int32_t G, int32_t kv_heads, int32_t max_q_len, int32_t max_len) {
+  const int64_t rows = (int64_t)G * max_q_len, steps = ((int64_t)max_len + kKv8Step - 1) / kKv8Step;
+  if (rows <= 32) return rows <= 16 ? 16 : 32;
+  return kv8_tiles(batch, total, G, 32) * kv_heads <= 8 * kKv8Grid / steps ? 32 : kChunkRows;
+}
+
 static size_t kv8_workspace(int tile, int32_t head_dim) {
   if (tile == kChunkRows)
     return SDV_KV8_SYNC_BYTES + kChunkGrid * (sizeof(Kv8Cut) + 2 * sizeof(float) * (head_dim == 128 ? chunk_part<128>() : chunk_part<64>()));
@@ -504,13 +516,13 @@ static int kv8_attn_sizes(int32_t batch, int32_t total, int32_t q_heads, int32_t
   if (head_dim != 64 && head_dim != 128) return SDV_ERR_UNSUPPORTED;
   if (batch > INT32_MAX / 4 || total > INT32_MAX / 2) return SDV_ERR_SHAPE;
   const int32_t G = q_heads / kv_heads;
-  return kv8_units(batch, total, G, kv_heads, max_len, kv8_tile_rows(G, max_q_len), 0, kKv8Start) < 0 ? SDV_ERR_SHAPE : SDV_OK;
+  return kv8_units(batch, total, G, kv_heads, max_len, kv8_tile_rows(batch, total, G, kv_heads, max_q_len, max_len), 0, kKv8Start) < 0 ? SDV_ERR_SHAPE : SDV_OK;
 }
 
 extern "C" size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
                                                    int32_t head_dim, int32_t max_q_len, int32_t max_seq_len) {
   if (kv8_attn_sizes(batch, total_rows, q_heads, kv_heads, head_dim, max_q_len, max_seq_len) != SDV_OK) return 0;
-  return kv8_workspace(kv8_tile_rows(q_heads / kv_heads, max_q_len), head_dim);
+  return kv8_workspace(kv8_tile_rows(batch, total_rows, q_heads / kv_heads, kv_heads, max_q_len, max_seq_len), head_dim);
 }
 
 template <int D, int FMT, int RT>
@@ -544,7 +556,7 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   if (!aligned(q, 16) || !aligned(out, 16) || q_stride % 8 || out_stride % 8 || !aligned(k_pages, 16) || !aligned(v_pages, 16) ||
       !aligned(scales, 16) || !aligned(block_table, 4) || !aligned(cu_rows, 4) || !aligned(seq_lens, 4) || !aligned(tree_mask, 8))
     return SDV_ERR_ALIGN;
-  const int G = q_heads / kv_heads, tile = kv8_tile_rows(G, max_q_len);
+  const int G = q_heads / kv_heads, tile = kv8_tile_rows(batch, total_rows, G, kv_heads, max_q_len, max_seq_len);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < kv8_workspace(tile, head_dim)) return SDV_ERR_WORKSPACE;
   if (total_rows == 0) return SDV_OK;
 
@@ -573,18 +585,19 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   // to add up, and the shortest calls have units of about the root of S / 8 of them (16 rows; 2S / 8, 32:
   // their parts are larger).  One row in us, at 4, 8 and 16 steps: 8192 keys 12.3 11.8 16.3, 32768 keys
   // 26 20 20, 131072 keys 51 52 35; five rows: 8192 keys 21 19 26, 32768 keys 50 35 34.  Units of eight
-  // also where ones of four would not fit: eight sequences of 8192 keys, one row each, 14 us, in ranges 19; with
-  // 16 steps the two are even (sixteen sequences 19.9 and 21.8, of mixed lengths 18.4 and 18.1).
+  // also where ones of four would not fit (eight sequences of 8192 keys, one row each, 14 us, in ranges
+  // 19) and where tiles of 32 rows would then stand two a CU (576 rows over 2048 keys 16 us, with four 19);
+  // with 16 steps the two are even (sixteen sequences 19.9 and 21.8, of mixed lengths 18.4 and 18.1).
   const int64_t tiles = kv8_tiles(batch, total_rows, G, tile) * kv_heads;
   const int64_t steps = ((int64_t)max_seq_len + kKv8Step - 1) / kKv8Step;
   const int most_grid = tile == kChunkRows ? kChunkGrid : kKv8Grid;
-  const auto fits = [&](int unit) { return tiles * (((steps - 1) >> unit) + 1) <= most_grid; };
+  const auto fits = [&](int unit, int grid) { return tiles * (((steps - 1) >> unit) + 1) <= grid; };
   int unit = 2;
   if (tile != kChunkRows) {
     while ((int64_t)128 << (2 * unit) < steps * tile) ++unit;
-    if (unit == 2 && !fits(2)) unit = 3;
+    if (unit == 2 && !fits(2, tile == 32 ? kKv8Grid / 2 : kKv8Grid)) unit = 3;
   }
-  a.unit = fits(unit) ? unit : 0;
+  a.unit = fits(unit, most_grid) ? unit : 0;
   a.start = a.unit == 0 ? kKv8Start : 0;
   const int64_t most = kv8_units(batch, total_rows, G, kv_heads, max_seq_len, tile, a.unit, a.start);
   const int grid = (int)(most < most_grid ? most : most_grid);

@@ -17,6 +17,14 @@
 // A token whose V scale is NaN has its V taken as 0 and its scores as NaN: that makes NaN of the rows
 // that see it, and of no others.
 //
+// Bound by the matrix cores and what keeps them waiting: 2048 rows of 12 heads over 8192 keys (90 GFLOP,
+// head_dim 128) take 109 us, 0.83 PFLOP/s, where a large product of the library reaches 1.27 at the
+// clocks that such work runs at (1.7 to 1.8 GHz).  A stage takes 3400 cycles for 2080 of MFMA on each SIMD
+// (without the scores 2600, without them and the conversions 2200); starts take 7 to 9 us (the plan 1.4,
+// then page ids, scales and codes, one after another) and the parts' launch 8 to 12 (45 MB of them).
+// 256 rows: a stage's conversion and its reads from LDS serve all of them; with 128 (four wavefronts)
+// both would double.  Wave priorities move nothing.
+//
 // Softmax in one pass: units that all rows see take exp2(s - m) against the maximum so far; one that
 // would bring a lane's sum over it to 2^8 (a score 8 above m in base 2, or more than one near that) is
 // done again with a new maximum, from products that are still in registers.  Units that need a mask,

@@ -6,9 +6,9 @@
 // contiguous ranges, one per workgroup: single tokens over long contexts, prompt chunks and
 // batches of both are then equally long for every workgroup, and a workgroup crosses at most two
 // tiles that it shares.  A tile's steps are preceded by a few that stand for what starting it costs.
-// Where there are fewer steps than that takes, a tile's steps are counted in units of several, each
-// one workgroup's.  Lengths are read on the device; every workgroup works out
-// its own range.
+// Where the device has a workgroup for each, steps are counted in units of several, each one
+// workgroup's.  Lengths are read on the device, so that a recorded call follows them; every workgroup
+// works out its own range, in 1 to 1.5 us.
 //
 // The units of a sequence's tiles up to the i-th sum in closed form: of u keys each, tile j has
 // ceil((ctx G + TR (j + 1)) / (u G)) (the last one ceil(T / u)), a sum of floors of a linear
@@ -128,18 +128,6 @@ __device__ __forceinline__ uint32_t kv8_seq_units(const Kv8Seq& s, const Kv8Attn
   return s.tiles == 0 ? 0 : kv8_before<TR>(s, a, s.tiles - 1) + kv8_units_of<TR>(s, a, s.tiles - 1);
 }
 
-// Inclusive sum over a wavefront's lanes (DPP row shifts, then row broadcasts).
-__device__ __forceinline__ uint32_t kv8_lane_scan(uint32_t x) {
-  int v = (int)x;
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-  return (uint32_t)v;
-}
-
 // NT: threads of a workgroup, a run of sequences each.
 template <int NT>
 struct Kv8PlanLds {
@@ -243,14 +231,15 @@ struct Kv8Place {
       b = (wv * kWave + at) * per_run;
       if (per_run == 1) {
         seq = kv8_seq_of<TR>(a, __builtin_amdgcn_readlane(run.z, at), __builtin_amdgcn_readlane(run.w, at), __builtin_amdgcn_readlane(T, at));
-      } else
-      for (;; ++b) {
-        if (b >= a.r.batch) return false;  // not reached: the runs hold the unit
-        seq = kv8_seq<TR>(a, b);
-        const uint32_t n = kv8_seq_units<TR>(seq, a);
-        if (rem < n) break;
-        rem -= n;
-        tile0 += n;
+      } else {
+        for (;; ++b) {
+          if (b >= a.r.batch) return false;  // not reached: the runs hold the unit
+          seq = kv8_seq<TR>(a, b);
+          const uint32_t n = kv8_seq_units<TR>(seq, a);
+          if (rem < n) break;
+          rem -= n;
+          tile0 += n;
+        }
       }
     }
     i = 0;
