@@ -586,7 +586,8 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   // their parts are larger).  One row in us, at 4, 8 and 16 steps: 8192 keys 12.3 11.8 16.3, 32768 keys
   // 26 20 20, 131072 keys 51 52 35; five rows: 8192 keys 21 19 26, 32768 keys 50 35 34.  Units of eight
   // also where ones of four would not fit (eight sequences of 8192 keys, one row each, 14 us, in ranges
-  // 19) and where tiles of 32 rows would then stand two a CU (576 rows over 2048 keys 16 us, with four 19);
+  // 19) and where a sequence's several tiles would then stand two a CU (576 rows over 2048 keys 16 us, with
+  // four 19);
   // with 16 steps the two are even (sixteen sequences 19.9 and 21.8, of mixed lengths 18.4 and 18.1).
   const int64_t tiles = kv8_tiles(batch, total_rows, G, tile) * kv_heads;
   const int64_t steps = ((int64_t)max_seq_len + kKv8Step - 1) / kKv8Step;
@@ -595,7 +596,7 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   int unit = 2;
   if (tile != kChunkRows) {
     while ((int64_t)128 << (2 * unit) < steps * tile) ++unit;
-    if (unit == 2 && !fits(2, tile == 32 ? kKv8Grid / 2 : kKv8Grid)) unit = 3;
+    if (unit == 2 && !fits(2, (int64_t)G * max_q_len > 32 ? kKv8Grid / 2 : kKv8Grid)) unit = 3;
   }
   a.unit = fits(unit, most_grid) ? unit : 0;
   a.start = a.unit == 0 ? kKv8Start : 0;
