@@ -10,7 +10,7 @@
 // packed tensor; only a sequence's first and last block are written in bytes.  A wavefront finds its
 // block by a scan over the sequences' block counts.
 //
-// Bound by memory where there is enough to move: reading 37,000 positions of 16 sequences back (174 MB
+// Bound by memory where there is enough to move: reading 112,000 positions of 16 sequences back (174 MB
 // read and written, 2 x 128) takes 35 us, 4.9 TB/s, 0.94 of a large copy's rate.  Small calls are three
 // loads one after another (lengths, block id, rows) between the ends of a launch: 32 tokens 4.8 us, a
 // chunk of 2048 5.3, of which a kernel that does nothing but a small fill is 1.8 (GPU time in a graph;
