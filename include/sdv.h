@@ -336,7 +336,8 @@ int sdv_pack_contiguous(const void* k, const void* v_codes, const float* v_scale
  * Quantize the rows and write them into the cache: row i of sequence b is position
  * seq_lens[b] - n_b + i, n_b its row count, seq_lens[b] its length with the new tokens (NULL: max_seq_len,
  * for every sequence; a call that a HIP graph records then needs no lengths in device memory).  Rows at negative
- * positions (a length below the row count) or in blocks that the table does not name are skipped.
+ * positions (a length below the row count) or in blocks that the table does not name are skipped.  No two
+ * rows of a call may have the same slot (which of them it then holds, in parts, is not defined).
  */
 int sdv_kv8_append(const void* k_new, const void* v_new, int64_t k_stride, int64_t v_stride, int32_t total_rows,
                    void* k_pages, void* v_pages, float* scales, int32_t num_blocks, int32_t format,
@@ -353,8 +354,8 @@ int sdv_kv8_gather(const void* k_pages, const void* v_pages, const float* scales
                    const int32_t* starts, int32_t batch, int32_t total_rows, int32_t kv_heads, int32_t head_dim,
                    void* k_out, void* v_out, int64_t k_stride, int64_t v_stride, void* stream);
 
-/* Bytes of workspace sdv_kv8_attention needs for these sizes (0 on invalid sizes).  Its first
- * SDV_KV8_SYNC_BYTES bytes must be zero before the first call that uses it; every call leaves them
+/* Bytes of workspace sdv_kv8_attention needs for these sizes (0 on invalid sizes); with the same heads more
+ * sequences, rows, max_q_len or max_seq_len never need less.  Its first SDV_KV8_SYNC_BYTES bytes must be zero before the first call that uses it; every call leaves them
  * zero again, and nothing else carries over.  Calls that may overlap need a workspace each. */
 #define SDV_KV8_SYNC_BYTES 4096
 size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32_t q_heads, int32_t kv_heads,

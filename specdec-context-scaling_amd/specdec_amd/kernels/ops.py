@@ -667,7 +667,8 @@ def kv8_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, 
     fp32 (K's, then V's).  block_table int32 (B, max_blocks).  cu_rows int32 (B + 1,): sequence b's
     rows are cu_rows[b] .. cu_rows[b+1] - 1; they are its last positions, seq_lens int32 (B,) being
     the lengths with them, or None: every sequence has max_seq_len tokens.  Rows behind cu_rows[B]
-    are not touched; rows whose position the block table does not hold are skipped.
+    are not touched; rows whose position the block table does not hold are skipped.  No two rows of a
+    call may have the same slot.
     """
     st = _native.binding().append(k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len)
     if st is not None:

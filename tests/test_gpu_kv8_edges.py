@@ -3,6 +3,8 @@ of more sequences than threads, V of very different sizes, one row count announc
 calls side by side on two streams, and a workspace that comes dirty."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -145,3 +147,30 @@ def test_a_workspace_that_others_wrote(cuda_device, new):
     for byte in (0xFF, 0x01, 0x7F):
         ws.fill_(byte)
         assert torch.equal(ops.kv8_attention(*args, workspace_tensor=ws).view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("new,lens,length", [([1, 1, 1], [700, 90, 300], 700), ([5, 4, 5], [700, 90, 300], 700), ([40, 7, 50], [700, 90, 300], 700),
+                                             ([40, 7, 50], [700, 90, 300], 131072)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_query_rows_that_are_not_finite(cuda_device, new, lens, length, bad):
+    """A query row with an infinity or a NaN is NaN in its own output (its head's) and reaches no other."""
+    dev = cuda_device
+    h, kv, d = HEADS["target"]
+    pages, bt = _filled(kv, d, "fp8", lens, 14)
+    q = torch.randn((sum(new), h, d), generator=_gen(5)).to(torch.bfloat16)
+    want, bound = ref.attention(q, pages, bt, new, lens)
+    row = new[0]  # the second sequence's first
+    q[row, 3, 17] = bad
+    want[row, 3] = math.nan
+    announce(f"kv8 attention, a query of {bad} {new} {length}")
+    got = ops.kv8_attention(q.to(dev), *pages.to(dev), bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), length)
+    torch.cuda.synchronize()
+    ref.within(got, want, bound)
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1], [800, 70]), ([4, 5], [800, 70]), ([60, 3], [800, 70])])
+def test_a_scale_of_zero_and_a_negative_one(cuda_device, new, lens):
+    for scale in (0.0, -0.2):
+        announce(f"kv8 attention, scale {scale} {new}")
+        got, want, bound = _attend(cuda_device, HEADS["target"], "int8", lens, new, scale=scale)
+        ref.within(got, want, bound)

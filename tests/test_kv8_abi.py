@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import random
 import re
 import shutil
 import subprocess
@@ -95,6 +96,16 @@ def test_attention_checks(lib):
     assert need > 0 and _attend(lib, wsb=need - 1) == _native.SDV_ERR_WORKSPACE
     assert lib.sdv_kv8_attention_workspace_size(1, 4, 12, 2, 96, 4, 64) == 0
     assert lib.sdv_kv8_attention_workspace_size(1, 4, 12, 5, 128, 4, 64) == 0
+
+
+def test_a_workspace_for_the_largest_call_serves_the_smaller(lib):
+    rng = random.Random(4)
+    for _ in range(3000):
+        G, kv, d = rng.choice([1, 6, 7]), rng.choice([1, 2, 8]), rng.choice([64, 128])
+        big = [rng.randint(1, 64), rng.randint(1, 4096), rng.randint(1, 600), 1 << rng.randint(4, 17)]
+        small = [rng.randint(1, x) for x in big]
+        a, b = [lib.sdv_kv8_attention_workspace_size(c[0], c[1], G * kv, kv, d, c[2], c[3]) for c in (small, big)]
+        assert 0 < a <= b, (G, kv, d, small, big)
 
 
 def test_tensors_on_the_cpu_are_refused():
