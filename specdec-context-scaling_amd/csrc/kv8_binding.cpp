@@ -116,10 +116,11 @@ at::Tensor fresh_workspace(const Pages& p, size_t bytes) {
   return ws;
 }
 
-// kv8_attention's workspace: one per device and stream, whose calls are ordered.  A call that a HIP
-// graph records gets its own, from the graph's memory, so that no two graphs share one.
+// kv8_attention's workspace: one per device and stream, whose calls are ordered.  The calls that a HIP
+// graph records on one stream share one of the graph's memory (so that no two graphs share one, and the
+// calls of one, in the order of their stream, clear its count area once a replay: a fill is 1.8 us of GPU
+// time, a short call 7).  The recording's is kept until the stream records another graph.
 at::Tensor workspace(const Pages& p, hipStream_t stream, size_t bytes) {
-  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return fresh_workspace(p, bytes);
   struct Key {
     int device;
     hipStream_t stream;
@@ -128,8 +129,23 @@ at::Tensor workspace(const Pages& p, hipStream_t stream, size_t bytes) {
   struct Hash {
     size_t operator()(const Key& k) const { return std::hash<void*>()(k.stream) * 31 + k.device; }
   };
-  static auto* cache = new std::unordered_map<Key, at::Tensor, Hash>();  // never freed: the runtime may end before it
-  at::Tensor& ws = (*cache)[{p.device.index(), stream}];
+  struct Recorded {
+    unsigned long long id = 0;
+    at::Tensor ws;
+  };
+  const Key key = {p.device.index(), stream};
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+    hipStreamCaptureStatus capture;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(stream, &capture, &id) != hipSuccess || capture != hipStreamCaptureStatusActive)
+      return fresh_workspace(p, bytes);
+    static auto* recorded = new std::unordered_map<Key, Recorded, Hash>();  // never freed: the runtime may end before it
+    Recorded& r = (*recorded)[key];
+    if (r.id != id || !r.ws.defined() || (size_t)r.ws.numel() < bytes) r = {id, fresh_workspace(p, bytes)};
+    return r.ws;
+  }
+  static auto* cache = new std::unordered_map<Key, at::Tensor, Hash>();
+  at::Tensor& ws = (*cache)[key];
   if (!ws.defined() || (size_t)ws.numel() < bytes) ws = fresh_workspace(p, bytes);
   return ws;
 }

@@ -169,7 +169,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttnArgs& a, __amdgpu_buffer_
 // Long batches are bound by memory: single tokens of 32 sequences of 2048 to 32768 keys (293 MB of pages,
 // 2 KV heads of 128) take 55 to 57 us, 5.2 TB/s, a large copy's rate; the matrix cores are busy a tenth of
 // it.  Short calls are bound by latencies, each a microsecond or more: lengths, page ids, the pages,
-// the merge's count, and the parts.  One token over 2048 keys takes 7.3 us eager, over 32768 20.
+// the merge's count, and the parts.  One token over 2048 keys takes 7.3 us, over 32768 18.
 template <int D, int FMT, int RT>
 __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a) {
   constexpr int TR = 16 * RT, KI = D / 64, KS = D / 32, DT = D / 16;
@@ -493,9 +493,10 @@ static int64_t kv8_units(int32_t batch, int32_t total, int32_t G, int32_t kv_hea
 // Rows per tile: 16 or 32 where a sequence's rows fit that.  With more rows 256, whose stages serve more of
 // them (1800 over 32768 keys 82 us, in tiles of 32 195), or 32 where all tiles of those together have at
 // most eight steps for each workgroup of the device: the many small ones start sooner and their parts need
-// no second launch.  2 KV heads of 128, tiles of 32 and of 256, in us: 300 tokens' 1800 rows 12 and 25, 288 rows over 2048 keys 14 and 23, 144 over 8192
-// (1280 steps) 20 and 25, 1200 over 2048 (2432) 21 and 28; of four sequences of 8192 48 rows each (2560) 24
-// and 24, 144 each (5632) 33 and 32, 288 each (10240) 42 and 37; 1200 over 8192 (9728) 44 and 36.
+// no second launch.  2 KV heads of 128, tiles of 32 and of 256, in us (with a fill of 1.8): 300 tokens' 1800
+// rows 12 and 25, 288 rows over 2048 keys 14 and 23, 144 over 8192 (1280 steps) 20 and 25, 1200 over 2048
+// (2432) 21 and 28; of four sequences of 8192 48 rows each (2560) 24 and 24, 144 each (5632) 33 and 32, 288
+// each (10240) 42 and 37; 1200 over 8192 (9728) 44 and 36.
 static int kv8_tile_rows(int32_t batch, int32_t total, int32_t G, int32_t kv_heads, int32_t max_q_len, int32_t max_len) {
   const int64_t rows = (int64_t)G * max_q_len, steps = ((int64_t)max_len + kKv8Step - 1) / kKv8Step;
   if (rows <= 32) return rows <= 16 ? 16 : 32;
@@ -579,7 +580,8 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   a.cuts = nullptr;
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + SDV_KV8_SYNC_BYTES);
   // Units.  Where the device holds a workgroup for every unit of every tile, each takes one: the call is
-  // as long as its latencies, and a second tile would double them (GPU time, 2 KV heads: eight sequences
+  // as long as its latencies, and a second tile would double them (GPU time, 2 KV heads, with a fill of
+  // 1.8 us before each call: eight sequences
   // of 1000 to 4096 keys, five rows each, 31 us in equal ranges of single steps and 19 so; one of 2048
   // keys 12 and 9).  A unit is four steps, one per wavefront; of a tile's S steps longer ones make less
   // to add up, and the shortest calls have units of about the root of S / 8 of them (16 rows; 2S / 8, 32:
@@ -587,8 +589,8 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   // 26 20 20, 131072 keys 51 52 35; five rows: 8192 keys 21 19 26, 32768 keys 50 35 34.  Units of eight
   // also where ones of four would not fit (eight sequences of 8192 keys, one row each, 14 us, in ranges
   // 19) and where a sequence's several tiles would then stand two a CU (576 rows over 2048 keys 16 us, with
-  // four 19);
-  // with 16 steps the two are even (sixteen sequences 19.9 and 21.8, of mixed lengths 18.4 and 18.1).
+  // four 19).  At 16 steps units and ranges are even (sixteen sequences 19.9 and 21.8, of mixed lengths 18.4
+  // and 18.1).
   const int64_t tiles = kv8_tiles(batch, total_rows, G, tile) * kv_heads;
   const int64_t steps = ((int64_t)max_seq_len + kKv8Step - 1) / kKv8Step;
   const int most_grid = tile == kChunkRows ? kChunkGrid : kKv8Grid;

@@ -60,7 +60,7 @@ class KV8Cache(PagedKVCache):
 
     def reserve_all(self, n_tokens: int, q_heads: int | None = None, q_len: int | None = None) -> None:
         """Page blocks and the device block table for the first n_tokens positions of every sequence,
-        before recording a step up to them (a recorded call brings its own workspace)."""
+        before recording a step up to them (a recording brings its own workspace)."""
         for b in range(self.batch):
             self.reserve(b, n_tokens)
         self.block_table()

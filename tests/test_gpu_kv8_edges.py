@@ -174,3 +174,49 @@ def test_a_scale_of_zero_and_a_negative_one(cuda_device, new, lens):
         announce(f"kv8 attention, scale {scale} {new}")
         got, want, bound = _attend(cuda_device, HEADS["target"], "int8", lens, new, scale=scale)
         ref.within(got, want, bound)
+
+
+def test_recorded_calls_of_one_graph(cuda_device):
+    """Calls of one recording share a workspace where their stream orders them: small and large ones after
+    each other and on a forked stream; two graphs from the same stream replayed side by side."""
+    dev = cuda_device
+    h, kv, d = HEADS["target"]
+    cases = []
+    for i, (new, lens, length) in enumerate((([1, 1], [3000, 2500], 3000), ([40, 3], [900, 2000], 131072), ([5, 5], [4000, 70], 4000),
+                                             ([1], [6000], 6000))):
+        pages, bt = _filled(kv, d, "fp8", lens, 60 + i)
+        q = torch.randn((sum(new), h, d), generator=_gen(i)).to(torch.bfloat16).to(dev)
+        cases.append((q, *pages.to(dev), bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), length))
+    want = [ops.kv8_attention(*c) for c in cases]
+    torch.cuda.synchronize()
+    main, fork = torch.cuda.Stream(), torch.cuda.Stream()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph, got = torch.cuda.CUDAGraph(), []
+        with torch.cuda.graph(graph, stream=main):
+            for c in cases:
+                got.append(ops.kv8_attention(*c))
+            fork.wait_stream(main)
+            with torch.cuda.stream(fork):
+                aside = [ops.kv8_attention(*c) for c in cases]
+            for c in cases[::-1]:
+                got.append(ops.kv8_attention(*c))
+            main.wait_stream(fork)
+        graphs.append(graph)
+        outs.append(got[:4] + got[4:][::-1] + aside)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(4):
+        announce(f"kv8 attention, two graphs of several calls, replay {turn}")
+        for got in outs:
+            for o in got:
+                o.zero_()
+        torch.cuda.synchronize()
+        for st, graph in zip(sides, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        again = ops.kv8_attention(*cases[turn])
+        torch.cuda.synchronize()
+        assert torch.equal(again.view(torch.int16), want[turn].view(torch.int16))
+        for got in outs:
+            for k, o in enumerate(got):
+                assert torch.equal(o.view(torch.int16), want[k % 4].view(torch.int16)), k
