@@ -372,8 +372,8 @@ size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32
  * sees nothing is 0; what a row does not see, infinities and NaN among it, does not reach it.
  * Operands of the product with V: with max_q_len * q_heads / kv_heads <= 32 the probability times V's scale
  * to 16 bits; with more, probability and V to FP16's 11 bits, V relative to the largest V scale of the keys
- * of a tile of 256 rows (seen by a row or not), so that V of 2^-29 of that largest and less is held to fewer bits
- * than BF16's.
+ * of a tile of 256 rows (seen by a row or not, and that of rows of zeros, 1, among them), so that an output is
+ * off by up to 2^-30 of that scale, whatever its own size.
  * Size limits: (max_seq_len + total_rows) * q_heads / kv_heads <= 2^30 and, with tiles of 16 rows (32 where
  * max_q_len * q_heads / kv_heads > 16, 256 where it is > 32), tiles * (steps of 64 keys + 5) * kv_heads < 2^31.
  */

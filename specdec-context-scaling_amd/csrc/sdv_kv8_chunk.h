@@ -10,9 +10,13 @@
 // Each stage's codes are converted once per workgroup on their way to LDS: K to BF16, V to
 // fp16(code) * fp16(scale * 2^(b - E)), E the exponent of the largest V scale of the tile's keys so
 // far (the sums are rescaled where it grows) and b such that the largest code stays under 2^15.  FP16
-// then holds rows of V down to 2^-29 of the largest with BF16's error or less.  K's scale times the
-// softmax's multiplies the scores.  p is held as 2^7 p, so that FP16 holds it to 11 bits down to 2^-21.
-// The scales of a window of 64 stages are worked out before its loop and lie in LDS.
+// then holds rows of V down to 2^-29 of the largest with BF16's error or less (a row of zeros has scale 1
+// and counts as 448 or 127: beside one an output is off by up to 2^-30, 1e-9).  Windows whose scales lie
+// farther apart could keep V's codes as they are and put its scale into two operands of p, as the kernel
+// for few rows does; a second loop for them here took the registers of the first (2048 rows over 8192
+// keys 720 us instead of 113).  K's scale times the softmax's multiplies the scores.  p is held as 2^7 p,
+// so that FP16 holds it to 11 bits down to 2^-21.  The scales of a window of 64 stages are worked out
+// before its loop and lie in LDS.
 //
 // A token whose V scale is NaN has its V taken as 0 and its scores as NaN: that makes NaN of the rows
 // that see it, and of no others.

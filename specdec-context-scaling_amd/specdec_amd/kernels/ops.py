@@ -777,8 +777,8 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     may overlap) are the caller's own.  The pages as for kv8_append.
 
     A sequence with more than 32 rows per KV head (or a batch with one by max_q_len) holds V relative to
-    the largest V scale of a row tile's keys, those that a row does not see among them: of V, 2^-29 of that
-    largest and less loses bits below BF16's.
+    the largest V scale of a row tile's keys, those that a row does not see and rows of zeros (scale 1) among
+    them: an output is off by up to 2^-30 of that scale, whatever its own size.
     """
     if out is None and workspace_tensor is None:
         got = _native.binding().attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale,
