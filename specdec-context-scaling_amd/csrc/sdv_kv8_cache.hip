@@ -11,7 +11,7 @@
 // block by a scan over the sequences' block counts.
 //
 // Bound by memory where there is enough to move: reading 112,000 positions of 16 sequences back (174 MB
-// read and written, 2 x 128) takes 35 us, 4.9 TB/s, 0.94 of a large copy's rate.  Small calls are three
+// read and written, 2 x 128) takes 30 to 34 us, 5.1 to 5.8 TB/s, a large copy's rate.  Small calls are three
 // loads one after another (lengths, block id, rows) between the ends of a launch: 32 tokens 4.8 us, a
 // chunk of 2048 5.3, of which a kernel that does nothing but a small fill is 1.8 (GPU time in a graph;
 // eager calls 4.7 and 5.1).  A workgroup is one wavefront, so that a chunk of 2048 rows is 256 of them.
@@ -219,6 +219,12 @@ __global__ __launch_bounds__(64) void kv8_append_kernel(Kv8CacheArgs a) {
 }
 
 // ---------------------------------------------------------------------------- read-back
+// The rows are written past the caches' reused lines: what is read back is mostly more than they hold
+// (112,000 positions 35.6 -> 32.2 us, 8192 4.8 -> 4.3; with K's codes read that way too 33.9 and 4.4).
+__device__ __forceinline__ void kv8_store_stream(uint16_t* p, uint4 v) {
+  __builtin_nontemporal_store(u32x4_t{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_t*>(p));
+}
+
 template <int D, int FMT>
 __global__ __launch_bounds__(64) void kv8_gather_kernel(Kv8CacheArgs a) {
   constexpr int LPR = D / 8, RPW = kWave / LPR, J = kBlock / RPW;
@@ -267,7 +273,7 @@ __global__ __launch_bounds__(64) void kv8_gather_kernel(Kv8CacheArgs a) {
       const uint32_t w = (&kw[j].x)[k >> 2];
       (&o.x)[k >> 1] = pack_bf16x2(kv8_decode<FMT>(w, k & 3) * ks[j], kv8_decode<FMT>(w, (k & 3) + 1) * ks[j]);
     }
-    if (tok >= t.t0 && tok < t.t1) *reinterpret_cast<uint4*>(kout + (int64_t)(t.row + tok) * a.k_stride) = o;
+    if (tok >= t.t0 && tok < t.t1) kv8_store_stream(kout + (int64_t)(t.row + tok) * a.k_stride, o);
   }
   uint32_t packed[8];
 #pragma unroll
@@ -282,7 +288,7 @@ __global__ __launch_bounds__(64) void kv8_gather_kernel(Kv8CacheArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; k += 2)
       (&o.x)[k >> 1] = pack_bf16x2(kv8_decode<FMT>(packed[k], j) * vs[j], kv8_decode<FMT>(packed[k + 1], j) * vs[j]);
-    if (tok >= t.t0 && tok < t.t1) *reinterpret_cast<uint4*>(vout + (int64_t)(t.row + tok) * a.v_stride) = o;
+    if (tok >= t.t0 && tok < t.t1) kv8_store_stream(vout + (int64_t)(t.row + tok) * a.v_stride, o);
   }
 }
 
