@@ -369,7 +369,8 @@ size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32
  * T_b - n_b and, of the new tokens, those j whose bit j of its mask is set: a tree of drafted tokens.  q head h reads KV head
  * h / (q_heads / kv_heads).  max_q_len is the largest n_b (it chooses the kernel; a sequence with more
  * rows is computed all the same).  Softmax of scale * q.k in fp32, sums in fp32, BF16 output.  A row that
- * sees nothing is 0; what a row does not see, infinities and NaN among it, does not reach it.
+ * sees nothing is 0 (one whose scores are all -inf, which an infinite q makes, is NaN); what a row does not
+ * see, infinities and NaN among it, does not reach it.
  * Operands of the product with V: with max_q_len * q_heads / kv_heads <= 32 the probability times V's scale
  * to 16 bits; with more, probability and V to FP16's 11 bits, V relative to the largest V scale of the keys
  * of a tile of 256 rows (seen by a row or not, and that of rows of zeros, 1, among them), so that an output is

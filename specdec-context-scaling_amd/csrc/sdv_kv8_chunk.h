@@ -515,9 +515,10 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2
     const float unit = __builtin_amdgcn_ldexpf(1.0f, e_acc - (FMT == kFp8 ? 5 : 7));
     const float2 pr = lane_pair<32>(l);
     l = pr.x + pr.y;
+    if (__builtin_expect(rv && m == -INFINITY, 0)) m = kv8_lowest(a, b, seq, tok, slo * kKv8Step, shi * kKv8Step);
     if (slo == 0 && shi == steps) {
       if (rv) {
-        const float inv = l == 0.0f ? 0.0f : unit / l;  // a row that sees nothing: 0
+        const float inv = m == -INFINITY ? 0.0f : unit / l;  // a row that sees nothing: 0
         uint16_t* dst = a.out + (int64_t)(seq.first + tok) * a.out_stride + (int64_t)head * D + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -613,7 +614,7 @@ __global__ __launch_bounds__(256) void kv8_chunk_merge_kernel(Kv8AttnArgs a, int
   } else {
     for (int k0 = 0; k0 < cut.parts; k0 += 16) add(std::integral_constant<int, 16>(), k0);
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
   const int tok = row / a.G, head = cut.kvh * a.G + row - tok * a.G;
   *reinterpret_cast<uint2*>(a.out + (int64_t)(cut.first + tok) * a.out_stride + (int64_t)head * D + 32 * dt + 8 * j + 4 * (lane >> 5)) =
       make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));

@@ -772,7 +772,7 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     may stand in one batch; max_q_len is the largest.  A row sees the keys up to its own position;
     with tree_mask (int64 or uint64 (total,), max_q_len <= 64) the context before the new tokens and
     the new tokens j whose bit j of its mask is set.  scale: default 1 / sqrt(D).  A row that sees
-    nothing is 0; rows behind cu_rows[B] are not written.  out (like q; tokens may lie any multiple of
+    nothing is 0, one whose scores are all -inf (an infinite q) NaN; rows behind cu_rows[B] are not written.  out (like q; tokens may lie any multiple of
     8 elements apart) and workspace_tensor (uint8, of kv8_attention_workspace_bytes, not for calls that
     may overlap) are the caller's own.  The pages as for kv8_append.
 

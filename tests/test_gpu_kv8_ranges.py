@@ -1,0 +1,75 @@
+"""kv8 attention at the ends of its types' ranges: infinite queries."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import kv8_reference as ref
+from conftest import announce
+from specdec_amd.kernels import ops
+from test_gpu_kv8 import HEADS, _cu, _filled, _gen, _ints, _rows
+
+pytestmark = pytest.mark.gpu
+
+# (new rows, lengths, announced length): a tile of 16 rows in one workgroup and in several, of 32, of 256 in one
+# and in several (an announced length far above the sequences' sends many rows to the kernel for many)
+SHAPES = [([1], [1], 1), ([1, 1], [3000, 40], 3000), ([5], [900], 900), ([5, 4], [4000, 4], 4000), ([40], [40], 131072),
+          ([40, 9], [6000, 300], 131072), ([300], [300], 300)]
+
+
+def _one_sign(kv, d, fmt, lens, channel, seed):
+    """(pages, table) of random tokens whose K is positive throughout in one channel of the even KV heads and
+    negative in the odd ones'."""
+    g = _gen(seed)
+    counts = [-(-t // 16) for t in lens]
+    nb = sum(counts) + 2
+    bt = ref.table(counts, nb, seed)
+    pages = ref.Pages(nb, kv, d, fmt)
+    sign = torch.tensor([1.0 if i % 2 == 0 else -1.0 for i in range(kv)])
+    for b, t in enumerate(lens):
+        k, v = _rows((t, kv, d), g), _rows((t, kv, d), g)
+        k[..., channel] = ((k[..., channel].float().abs() + 0.5) * sign).to(torch.bfloat16)
+        pages.write(*ref.slots(bt[b], torch.arange(t)), k, v)
+    return pages, bt
+
+
+@pytest.mark.parametrize("new,lens,length", SHAPES)
+@pytest.mark.parametrize("fmt,heads", [("fp8", "target"), ("int8", "draft")])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+def test_rows_whose_scores_are_all_infinite(cuda_device, fmt, heads, new, lens, length, bad):
+    """A query of +inf or -inf in a channel of one sign: every score it makes is +inf, or every one -inf, and
+    the softmax is NaN either way; no other row has any of it."""
+    dev, (h, kv, d) = cuda_device, HEADS[heads]
+    pages, bt = _one_sign(kv, d, fmt, lens, 17, 8)
+    q = torch.randn((sum(new), h, d), generator=_gen(5)).to(torch.bfloat16)
+    for head in (0, h - 1):  # one of an even KV head, one of an odd
+        q[0, head, 17] = q[-1, head, 17] = bad
+    want, bound = ref.attention(q, pages, bt, new, lens)
+    assert bool(torch.isnan(want[0, 0]).all()) and bool(torch.isnan(want[-1, h - 1]).all()) and not bool(torch.isnan(want[0, 1]).any())
+    announce(f"kv8 attention, infinite scores {fmt} {new} {length} {bad}")
+    got = ops.kv8_attention(q.to(dev), *pages.to(dev), bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), length)
+    torch.cuda.synchronize()
+    ref.within(got, want, bound)
+
+
+@pytest.mark.parametrize("length", [64, 131072])
+@pytest.mark.parametrize("new,lens", [([3, 2], [1, 0]), ([40, 7], [30, 7])])
+def test_infinite_queries_that_see_nothing(cuda_device, new, lens, length):
+    """Rows before position 0, rows over blocks that the table does not name and rows whose mask is empty are
+    0 whatever their query holds."""
+    dev, (h, kv, d) = cuda_device, HEADS["target"]
+    pages, bt = _filled(kv, d, "fp8", lens, 3)
+    q = torch.full((sum(new), h, d), -math.inf, dtype=torch.bfloat16, device=dev)
+    announce(f"kv8 attention, infinite queries that see nothing {new} {length}")
+    args = (q, *pages.to(dev))
+    got = ops.kv8_attention(*args, bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), length)
+    before = new[0] - lens[0]
+    assert bool((got[:before] == 0).all()) and bool(torch.isnan(got[before:new[0]]).all())
+    got = ops.kv8_attention(*args, torch.full_like(bt, -1).to(dev), _cu(new, dev), _ints(lens, dev), max(new), length)
+    assert bool((got == 0).all())
+    masks = torch.zeros(sum(new), dtype=torch.int64, device=dev)
+    masks[new[0] - 1] = 1 << (new[0] - 1)  # itself alone
+    got = ops.kv8_attention(*args, bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), length, tree_mask=masks)
+    assert bool(torch.isnan(got[new[0] - 1]).all()) and bool((got[:new[0] - 1] == 0).all()) and bool((got[new[0]:] == 0).all())
