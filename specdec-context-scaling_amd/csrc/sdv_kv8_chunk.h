@@ -96,6 +96,7 @@ struct Kv8Cut {
 };
 
 // A part: [wavefront][32-dimension tile][4][lane] pieces of 16 bytes, then [wavefront][lane] (maximum, sum).
+// The pieces are divided by the part's sum of exponentials: before that those of a large V pass fp32's range.
 template <int D>
 constexpr int chunk_part() {
   return kChunkRows * D + kChunkThreads * 2;
@@ -516,9 +517,11 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2
     const float2 pr = lane_pair<32>(l);
     l = pr.x + pr.y;
     if (__builtin_expect(rv && m == -INFINITY, 0)) m = kv8_lowest(a, b, seq, tok, slo * kKv8Step, shi * kKv8Step);
-    if (slo == 0 && shi == steps) {
+    const bool whole = slo == 0 && shi == steps;
+    // a row that sees nothing: 0; a part without exponentials has no weight
+    const float inv = m == -INFINITY || (!whole && l == 0.0f) ? 0.0f : unit / l;
+    if (whole) {
       if (rv) {
-        const float inv = m == -INFINITY ? 0.0f : unit / l;  // a row that sees nothing: 0
         uint16_t* dst = a.out + (int64_t)(seq.first + tok) * a.out_stride + (int64_t)head * D + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -536,7 +539,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            p4[(dt * 4 + j) * 64] = make_float4(acc[dt][4 * j] * unit, acc[dt][4 * j + 1] * unit, acc[dt][4 * j + 2] * unit, acc[dt][4 * j + 3] * unit);
+            p4[(dt * 4 + j) * 64] = make_float4(acc[dt][4 * j] * inv, acc[dt][4 * j + 1] * inv, acc[dt][4 * j + 2] * inv, acc[dt][4 * j + 3] * inv);
         reinterpret_cast<float2*>(part + kChunkRows * D)[tid] = make_float2(m, l);
       }
       if (slo == 0) {
@@ -598,15 +601,22 @@ __global__ __launch_bounds__(256) void kv8_chunk_merge_kernel(Kv8AttnArgs a, int
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
       if (k0 + k < cut.parts) mx = fmaxf(mx, st[k].x);
-    const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
-    l *= f;
-    sum = make_float4(sum.x * f, sum.y * f, sum.z * f, sum.w * f);
-    m = mx;
+    // the mean so far and the parts' means, weighted by their sums of exponentials
+    float w[kBatch], before = mx == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - mx);
+    l = before;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const float w = k0 + k >= cut.parts ? 0.0f : mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st[k].x - mx);
-      l += st[k].y * w;
-      sum = make_float4(sum.x + v[k].x * w, sum.y + v[k].y * w, sum.z + v[k].z * w, sum.w + v[k].w * w);
+      w[k] = k0 + k >= cut.parts ? 0.0f : mx == -INFINITY ? st[k].y : st[k].y * __builtin_amdgcn_exp2f(st[k].x - mx);
+      l += w[k];
+    }
+    m = mx;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    before *= inv;
+    sum = make_float4(sum.x * before, sum.y * before, sum.z * before, sum.w * before);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float x = w[k] * inv;
+      sum = make_float4(sum.x + v[k].x * x, sum.y + v[k].y * x, sum.z + v[k].z * x, sum.w + v[k].w * x);
     }
   };
   if (cut.parts <= 4) {
@@ -614,10 +624,10 @@ __global__ __launch_bounds__(256) void kv8_chunk_merge_kernel(Kv8AttnArgs a, int
   } else {
     for (int k0 = 0; k0 < cut.parts; k0 += 16) add(std::integral_constant<int, 16>(), k0);
   }
-  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  if (m != -INFINITY && l == 0.0f) sum = make_float4(NAN, NAN, NAN, NAN);  // scores of -inf alone
   const int tok = row / a.G, head = cut.kvh * a.G + row - tok * a.G;
   *reinterpret_cast<uint2*>(a.out + (int64_t)(cut.first + tok) * a.out_stride + (int64_t)head * D + 32 * dt + 8 * j + 4 * (lane >> 5)) =
-      make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+      make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
 }
 
 }  // namespace sdv

@@ -1,4 +1,4 @@
-"""kv8 attention at the ends of its types' ranges: infinite queries."""
+"""kv8 attention at the ends of its types' ranges: infinite queries, V near the largest BF16."""
 from __future__ import annotations
 
 import math
@@ -73,3 +73,37 @@ def test_infinite_queries_that_see_nothing(cuda_device, new, lens, length):
     masks[new[0] - 1] = 1 << (new[0] - 1)  # itself alone
     got = ops.kv8_attention(*args, bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), length, tree_mask=masks)
     assert bool(torch.isnan(got[new[0] - 1]).all()) and bool((got[:new[0] - 1] == 0).all()) and bool((got[new[0]:] == 0).all())
+
+
+def _large(kv, d, fmt, lens, top, seed):
+    """(pages, table) of V up to `top`, some rows of it alike and some zero."""
+    g = _gen(seed)
+    counts = [-(-t // 16) for t in lens]
+    nb = sum(counts) + 2
+    bt = ref.table(counts, nb, seed)
+    pages = ref.Pages(nb, kv, d, fmt)
+    for b, t in enumerate(lens):
+        v = torch.randn((t, kv, d), generator=g).clamp(-3, 3) / 3 * top
+        v[::5] = top
+        v[3::41] = 0.0
+        pages.write(*ref.slots(bt[b], torch.arange(t)), _rows((t, kv, d), g), v.to(torch.bfloat16))
+    return pages, bt
+
+
+def _finite(dev, heads, fmt, new, lens, length, top):
+    h, kv, d = heads
+    pages, bt = _large(kv, d, fmt, lens, top, 4)
+    q = torch.randn((sum(new), h, d), generator=_gen(6)).to(torch.bfloat16)
+    announce(f"kv8 attention, V up to {top} {fmt} {new} {length}")
+    got = ops.kv8_attention(q.to(dev), *pages.to(dev), bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), length)
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(got).all())
+    ref.within(got, *ref.attention(q, pages, bt, new, lens))
+
+
+@pytest.mark.parametrize("top", [1e33, 2.0 ** 121, 3.3e38])
+@pytest.mark.parametrize("fmt,heads", [("fp8", "target"), ("int8", "draft"), ("int8", "target")])
+@pytest.mark.parametrize("new,lens,length", [([40], [40], 131072), ([40, 9], [6000, 300], 131072), ([700, 1], [3000, 2500], 3000)])
+def test_many_rows_over_large_v(cuda_device, fmt, heads, new, lens, length, top):
+    """Finite V gives finite outputs, in tiles that one workgroup takes and in tiles whose parts are added up."""
+    _finite(cuda_device, HEADS[heads], fmt, new, lens, length, top)
