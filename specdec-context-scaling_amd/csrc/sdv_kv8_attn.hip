@@ -37,6 +37,12 @@ __device__ __forceinline__ uint32_t kv8_keep(int n, int w) {
 // probabilities are at most 2^8, and BF16 and fp32 hold them as exactly as they hold those below 1.
 constexpr float kKv8Slack = 8.0f;
 
+// Sums of up to 2^30 terms of 2^8 |V| pass fp32's range where V's scales are above 2^81.  From the first
+// scale of 2^64 on a wavefront takes its maxima to be 2^48 times as large: its sums are that much smaller
+// then, and the least probability that counts is 2^-78 (2^-126 otherwise).  Looking for one costs a call
+// over 2048 keys 0.1 us of 7.8.
+constexpr float kKv8LargeScale = 18446744073709551616.0f, kKv8Raise = 48.0f;
+
 constexpr int kKv8Threads = 256;  // of the kernel for few rows
 
 // The maximum that stands for a row none of whose scores of keys lo .. hi - 1 is above -inf: -inf where
@@ -255,7 +261,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
     const int all = seq.tree ? seq.ctx - 1 : seq.ctx + row0 / a.G;
 
     f32x4 o[RT][DT];
-    float m[RT], l[RT];
+    float m[RT], l[RT], raise = 0.0f;  // raise: wave-uniform
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       m[rt] = -INFINITY;
@@ -365,6 +371,8 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
           for (int p = 0; p < PG; ++p) vw[dt][p] &= kv8_keep(valid, p);
         }
       }
+      const float raised = raise;
+      if (__any(fmaxf(fmaxf(sv.x, sv.y), fmaxf(sv.z, sv.w)) >= kKv8LargeScale)) raise = kKv8Raise;
       constexpr int NH = PG / 2;  // p.V products per dimension tile, 32 tokens each
       bf16x8 hi[RT][NH], lo[RT][NH];
 #pragma unroll
@@ -383,18 +391,18 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
         float mx = y[0];
 #pragma unroll
         for (int t = 1; t < NT; ++t) mx = fmaxf(mx, y[t]);
-        if (__any(mx > m[rt] + kKv8Slack)) {
+        if (__any(mx > m[rt] + kKv8Slack) || raise != raised) {
           float2 pr = lane_pair<16>(mx);
           mx = fmaxf(pr.x, pr.y);
           pr = lane_pair<32>(mx);
           mx = fmaxf(fmaxf(pr.x, pr.y), m[rt]);
-          const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mx);
+          const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mx + (raised - raise));
           l[rt] *= f;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
           m[rt] = mx;
         }
-        const float ms = m[rt] == -INFINITY ? 0.0f : m[rt];
+        const float ms = m[rt] == -INFINITY ? 0.0f : m[rt] + raise;
         uint32_t wh[2 * PG], wl[2 * PG];
 #pragma unroll
         for (int p = 0; p < PG; ++p) {
@@ -441,7 +449,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
       float2 pr = lane_pair<16>(l[rt]);
       pr = lane_pair<32>(pr.x + pr.y);
       if (g == 0) {
-        lds_m[wave][16 * rt + n] = m[rt];
+        lds_m[wave][16 * rt + n] = m[rt] + raise;
         lds_l[wave][16 * rt + n] = pr.x + pr.y;
       }
 #pragma unroll

@@ -107,3 +107,38 @@ def _finite(dev, heads, fmt, new, lens, length, top):
 def test_many_rows_over_large_v(cuda_device, fmt, heads, new, lens, length, top):
     """Finite V gives finite outputs, in tiles that one workgroup takes and in tiles whose parts are added up."""
     _finite(cuda_device, HEADS[heads], fmt, new, lens, length, top)
+
+
+@pytest.mark.parametrize("top", [1e33, 2.0 ** 121, 3.3e38])
+@pytest.mark.parametrize("fmt,heads", [("fp8", "target"), ("int8", "draft"), ("int8", "target")])
+@pytest.mark.parametrize("new,lens,length", [([1], [1], 1), ([1, 1], [3000, 40], 3000), ([1], [20000], 20000), ([5], [90], 90),
+                                             ([5, 4], [4000, 4], 4000), ([1] * 40, [700 + 31 * i for i in range(40)], 2000), ([300], [300], 300)])
+def test_few_rows_over_large_v(cuda_device, fmt, heads, new, lens, length, top):
+    _finite(cuda_device, HEADS[heads], fmt, new, lens, length, top)
+
+
+@pytest.mark.parametrize("new,lens", [([1], [5000]), ([5], [900]), ([60], [900])])
+def test_large_v_that_comes_late(cuda_device, new, lens):
+    """V of 1 for most of the context, then a few tokens of 1e37, of which some rows see none: theirs are as
+    near to the result as ever."""
+    dev, (h, kv, d) = cuda_device, HEADS["target"]
+    t = lens[0]
+    g = _gen(9)
+    bt = ref.table([-(-t // 16)], -(-t // 16) + 2, 5)
+    pages = ref.Pages(-(-t // 16) + 2, kv, d, "fp8")
+    k, v = _rows((t, kv, d), g), _rows((t, kv, d), g)
+    v[t - 2:] = (v[t - 2:].float() * 1e37).to(torch.bfloat16)
+    pages.write(*ref.slots(bt[0], torch.arange(t)), k, v)
+    q = torch.randn((sum(new), h, d), generator=g).to(torch.bfloat16)
+    want, bound = ref.attention(q, pages, bt, new, lens)
+    early = new[0] - 2  # the rows that see none of it
+    if early > 0 and new[0] * h // kv <= 32:
+        # in the kernel for few rows the large scale takes no part in these: the bound of the context without it
+        small = ref.Pages(-(-t // 16) + 2, kv, d, "fp8")
+        small.write(*ref.slots(bt[0], torch.arange(t - 2)), k[:t - 2], v[:t - 2])
+        near, tight = ref.attention(q[:early], small, bt, [early], [t - 2])
+        want[:early], bound[:early] = near, tight
+    announce(f"kv8 attention, large V among small {new}")
+    got = ops.kv8_attention(q.to(dev), *pages.to(dev), bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), max(lens))
+    torch.cuda.synchronize()
+    ref.within(got, want, bound)
