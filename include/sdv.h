@@ -371,12 +371,15 @@ size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32
  * rows is computed all the same).  Softmax of scale * q.k in fp32, sums in fp32, BF16 output.  A row that
  * sees nothing is 0 (one whose scores are all -inf, which an infinite q makes, is NaN); what a row does not
  * see, infinities and NaN among it, does not reach it.
- * Operands of the product with V: with max_q_len * q_heads / kv_heads <= 32 the probability times V's scale
- * to 16 bits; with more, probability and V to FP16's 11 bits, V relative to the largest V scale of the keys
- * of a tile of 256 rows (seen by a row or not, and that of rows of zeros, 1, among them), so that an output is
- * off by up to 2^-30 of that scale, whatever its own size.
- * Size limits: (max_seq_len + total_rows) * q_heads / kv_heads <= 2^30 and, with tiles of 16 rows (32 where
- * max_q_len * q_heads / kv_heads > 16, 256 where it is > 32), tiles * (steps of 64 keys + 5) * kv_heads < 2^31.
+ * Operands of the product with V: the probability times V's scale to 16 bits in tiles of 16 or 32 rows.  In
+ * tiles of 256 the probability and V to FP16's 11 bits, V relative to the largest V scale s of the keys of the
+ * tile (seen by a row or not, and that of rows of zeros, 1, among them): beside those roundings an output is off
+ * by up to 2^-30 s, whatever its own size, and by up to 2^-32 of the sum of |V| over the keys that the row sees,
+ * divided by that of their exponentials.
+ * Tiles have 16 rows where max_q_len * q_heads / kv_heads <= 16, 32 where it is <= 32 and where it is more but
+ * tiles of 32 with the call's longest context make at most 4096 steps of 64 keys, else 256.
+ * Size limits: (max_seq_len + total_rows) * q_heads / kv_heads <= 2^30 and tiles * (steps of 64 keys + 5) *
+ * kv_heads < 2^31.
  */
 int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
                       int32_t num_blocks, int32_t format, const int32_t* block_table, int32_t max_blocks_per_seq,

@@ -9,14 +9,19 @@
 //
 // Each stage's codes are converted once per workgroup on their way to LDS: K to BF16, V to
 // fp16(code) * fp16(scale * 2^(b - E)), E the exponent of the largest V scale of the tile's keys so
-// far (the sums are rescaled where it grows) and b such that the largest code stays under 2^15.  FP16
-// then holds rows of V down to 2^-29 of the largest with BF16's error or less (a row of zeros has scale 1
-// and counts as 448 or 127: beside one an output is off by up to 2^-30, 1e-9).  Windows whose scales lie
-// farther apart could keep V's codes as they are and put its scale into two operands of p, as the kernel
-// for few rows does; a second loop for them here took the registers of the first (2048 rows over 8192
-// keys 720 us instead of 113).  K's scale times the softmax's multiplies the scores.  p is held as 2^7 p,
-// so that FP16 holds it to 11 bits down to 2^-21.  The scales of a window of 64 stages are worked out
-// before its loop and lie in LDS.
+// far (the sums are rescaled where it grows) and b such that the largest code stays under 2^15.  K's scale
+// times the softmax's multiplies the scores.  p is held as 2^7 p.  The scales of a window of 64 stages are
+// worked out before its loop and lie in LDS.
+//
+// How far that is off: each of V's two roundings is 2^-12 of a value, or 2^-25 where the product is below
+// FP16's normal numbers, which is 2^(E - 30) or less.  The scale must be a normal number itself, or its
+// rounding would be multiplied by the code.  So a window with scales below 2^(E - 18), as small V beside a row
+// of zeros (scale 1) has them, is gone over twice, the second time for those alone, in units 2^18 times
+// as small, and with no part in the sum of exponentials.  (Sums may lie 2^36 below the largest E so far; scales
+// smaller still are off by up to 2^(E - 39).)  p is off by 2^-12 of it, or by 2^-32 where it is below 2^-21.
+// Noticing such windows takes 1.3 us of a chunk's 45 to 115; a second loop that keeps V's codes as they are and
+// puts its scale into two operands of p took the registers of the first (2048 rows over 8192 keys 720 us
+// instead of 113).
 //
 // A token whose V scale is NaN has its V taken as 0 and its scores as NaN: that makes NaN of the rows
 // that see it, and of no others.
@@ -48,6 +53,7 @@ constexpr int kChunkThreads = kWave * kChunkWaves;
 constexpr int kChunkGrid = 256;      // workgroups, one per CU
 constexpr int kChunkStages = 64;     // of a window, whose page ids and scales are held in LDS
 constexpr int kChunkTokens = kKv8Step * kChunkStages;
+constexpr int kChunkBand = 18;       // binades of V's scales that one pass over a window serves
 constexpr float kChunkBits = 7.0f;   // p is held as 2^7 p
 constexpr float kChunkBound = 32768.0f;  // of a lane's 16 of them in a unit: each stays under FP16's largest
 
@@ -114,7 +120,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2
   __shared__ __align__(16) float lds_ks[kChunkTokens + 32];  // the window's scales of the scores (one unit is read past it)
   __shared__ __align__(16) _Float16 lds_vs[kChunkTokens];    // and of V
   __shared__ int lpb[kChunkTokens / kBlock];                 // its page ids; -1: no block
-  __shared__ uint32_t s_max[W], s_bad[W];
+  __shared__ uint32_t s_max[W], s_bad[W], s_low[W];
   __shared__ Kv8PlanLds<kChunkThreads> lds_plan;
 
   Kv8Cut cut = {};
@@ -189,9 +195,10 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = (f32x16)0.0f;
     float m = -INFINITY, l = 0.0f;
-    int e_acc = -120;  // exponent that the sums are relative to
+    int e_acc = -120, e_top = -120;  // exponent that the sums are relative to, the largest it has been
 
-    for (int wlo = slo; wlo < shi; wlo += kChunkStages) {  // windows; workgroup-uniform
+    bool low = false;  // second pass over a window: its small V scales
+    for (int wlo = slo; wlo < shi;) {                      // windows; workgroup-uniform
       const int nit = min(kChunkStages, shi - wlo);        // stages
       // Units of the window (32 keys): x = 0 .. 2 nit - 1, the first at key 32 ux0.  The loop multiplies
       // q.k^T one unit ahead of the scores and p.V one unit behind them: buffer s holds K of units
@@ -292,8 +299,24 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2
         any_bad |= s_bad[i];
       }
       const bool bad = __builtin_amdgcn_readfirstlane(any_bad) != 0;
-      // the sums in units of the window's exponent
-      const int e = max(e_acc, (int)(__builtin_amdgcn_readfirstlane(largest) >> 23) - 127);
+      // the sums in units of the window's exponent, or of the small scales'
+      const int e = low ? e_acc - kChunkBand : max(e_acc, (int)(__builtin_amdgcn_readfirstlane(largest) >> 23) - 127);
+      e_top = max(e_top, e);
+      const int e_split = low ? e : e < max(e_top - kChunkBand, kChunkBand - 120) ? -127 : e - kChunkBand;
+      const uint32_t split = (uint32_t)(127 + e_split) << 23;
+      bool below = false;
+#pragma unroll
+      for (int i = 0; i < kTok; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float& v = (&vst[i].x)[c];
+          const bool small = __float_as_uint(v) < split;
+          below = below || (small && v != 0.0f);
+          if (small != low) v = 0.0f;
+        }
+      if (lane == 0) s_low[wave] = 0;
+      if (below) s_low[wave] = 1;
+      const float l_top = l, m_top = m;
       if (e != e_acc) {
         const float f = __builtin_amdgcn_ldexpf(1.0f, max(e_acc - e, -126));
 #pragma unroll
@@ -509,7 +532,16 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2
           rotate();
         }
       }
-      if (wlo + kChunkStages < shi) load_ids(wlo + kChunkStages);
+      uint32_t any_low = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) any_low |= s_low[i];
+      if (low && m_top != m)
+        l = l_top * __builtin_amdgcn_exp2f(m_top - m);  // counted in the first pass
+      else if (low)
+        l = l_top;
+      low = !low && __builtin_amdgcn_readfirstlane(any_low) != 0;
+      if (!low) wlo += kChunkStages;
+      if (wlo < shi) load_ids(wlo);
     }
 
     // the sums in units of 1

@@ -776,9 +776,10 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     8 elements apart) and workspace_tensor (uint8, of kv8_attention_workspace_bytes, not for calls that
     may overlap) are the caller's own.  The pages as for kv8_append.
 
-    A sequence with more than 32 rows per KV head (or a batch with one by max_q_len) holds V relative to
-    the largest V scale of a row tile's keys, those that a row does not see and rows of zeros (scale 1) among
-    them: an output is off by up to 2^-30 of that scale, whatever its own size.
+    A call with more than 32 rows per sequence and KV head (by max_q_len) that is not a short one holds V
+    relative to the largest V scale of a row tile's keys, those that a row does not see and rows of zeros (scale 1)
+    among them: beside the roundings to 11 bits an output is off by up to 2^-30 of that scale, whatever its own
+    size, and by up to 2^-32 of the sum of |V| over its keys, divided by that of their exponentials.
     """
     if out is None and workspace_tensor is None:
         got = _native.binding().attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale,

@@ -142,3 +142,66 @@ def test_large_v_that_comes_late(cuda_device, new, lens):
     got = ops.kv8_attention(q.to(dev), *pages.to(dev), bt.to(dev), _cu(new, dev), _ints(lens, dev), max(new), max(lens))
     torch.cuda.synchronize()
     ref.within(got, want, bound)
+
+
+@pytest.mark.parametrize("zero", [True, False])
+@pytest.mark.parametrize("below", [10, 17, 18, 19, 22, 25, 27, 29, 30, 31, 37, 60])
+@pytest.mark.parametrize("fmt,heads", [("fp8", "target"), ("int8", "draft"), ("fp8", "draft"), ("int8", "target")])
+@pytest.mark.parametrize("length", [190, 131072])
+def test_small_v_beside_a_large_scale(cuda_device, length, fmt, heads, below, zero):
+    """Rows that see only V some 2^-below of a token's that the tile holds and they do not see -- a row of
+    zeros, whose scale is 1, or one of 448 or 127 --, and rows that see both.  What the large scale takes from the
+    former is half of FP16's smallest step under it, 2^-30."""
+    dev, (h, kv, d) = cuda_device, HEADS[heads]
+    n, t = 60, 190
+    g = _gen(below)
+    k = _rows((t, kv, d), g)
+    v = (torch.rand((t, kv, d), generator=g) + 0.5) * ref.LARGEST[fmt] * 2.0 ** -below
+    v[t - 7] = 0.0 if zero else torch.where(torch.rand((kv, d), generator=g) < 0.5, -1.0, 1.0) * ref.LARGEST[fmt]
+    v = v.to(torch.bfloat16)
+    bt = ref.table([12], 14, 2)
+    pages, small = ref.Pages(14, kv, d, fmt), ref.Pages(14, kv, d, fmt)
+    pages.write(*ref.slots(bt[0], torch.arange(t)), k, v)
+    early = n - 7
+    small.write(*ref.slots(bt[0], torch.arange(t - 7)), k[:t - 7], v[:t - 7])
+    q = torch.randn((n, h, d), generator=g).to(torch.bfloat16)
+    want, bound = ref.attention(q, pages, bt, [n], [t])
+    want[:early], bound[:early] = ref.attention(q[:early], small, bt, [early], [t - 7])
+    bound[:early] += 2.0 ** -30
+    announce(f"kv8 attention, small V beside a large scale {fmt} {heads} {below} {zero} {length}")
+    got = ops.kv8_attention(q.to(dev), *pages.to(dev), bt.to(dev), _cu([n], dev), _ints([t], dev), n, length)
+    torch.cuda.synchronize()
+    ref.within(got, want, bound)
+
+
+@pytest.mark.parametrize("fmt,heads", [("fp8", "target"), ("int8", "draft")])
+@pytest.mark.parametrize("down", [True, False])
+def test_v_of_every_size(cuda_device, fmt, heads, down):
+    """V whose scales run over 2^-100 .. 2^100 within a context of several windows, in tiles that one workgroup
+    takes whole and in cut ones.  The rows of the first sequences see all, those of the last only the first
+    hundred keys (larger ones follow, or smaller)."""
+    dev, (h, kv, d) = cuda_device, HEADS[heads]
+    t, n, first = 9000, 40, 100
+    g = _gen(3)
+    k, v = _rows((t, kv, d), g), _rows((t, kv, d), g)
+    e = torch.linspace(100, -100, t) if down else torch.linspace(-100, 100, t)
+    v = (v.float() * torch.exp2(e.round())[:, None, None]).to(torch.bfloat16)
+    nb = -(-t // 16)
+    bt = ref.table([nb], nb + 2, 2)
+    pages = ref.Pages(nb + 2, kv, d, fmt)
+    pages.write(*ref.slots(bt[0], torch.arange(t)), k, v)
+    q = torch.randn((2 * n, h, d), generator=g).to(torch.bfloat16)
+    lens = [t, first]
+    announce(f"kv8 attention, V of every size {fmt} {heads} {down}")
+    table = bt.expand(2, -1).contiguous()
+    got = ops.kv8_attention(q.to(dev), *pages.to(dev), table.to(dev), _cu([n, n], dev), _ints(lens, dev), n, 131072)
+    torch.cuda.synchronize()
+    ref.within(got, *ref.attention(q, pages, table, [n, n], lens))
+    many = 100  # so many sequences that a workgroup's range holds several windows
+    rows = q[:n].repeat(many, 1, 1)
+    table = bt.expand(many, -1).contiguous()
+    again = ops.kv8_attention(rows.to(dev), *pages.to(dev), table.to(dev), _cu([n] * many, dev), None, n, t)
+    torch.cuda.synchronize()
+    want, bound = ref.attention(q[:n], pages, bt, [n], [t])
+    for i in (0, 1, many // 2, many - 1):
+        ref.within(again[i * n:(i + 1) * n], want, bound)
