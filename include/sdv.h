@@ -356,7 +356,8 @@ int sdv_kv8_gather(const void* k_pages, const void* v_pages, const float* scales
 
 /* Bytes of workspace sdv_kv8_attention needs for these sizes (0 on invalid sizes); with the same heads more
  * sequences, rows, max_q_len or max_seq_len never need less.  Its first SDV_KV8_SYNC_BYTES bytes must be zero before the first call that uses it; every call leaves them
- * zero again, and nothing else carries over.  Calls that may overlap need a workspace each. */
+ * zero again, and nothing else carries over.  Calls that may overlap need a workspace each: on the device, and in host
+ * threads, whose launches on one stream (a call makes up to two) could mix. */
 #define SDV_KV8_SYNC_BYTES 4096
 size_t sdv_kv8_attention_workspace_size(int32_t batch, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
                                         int32_t head_dim, int32_t max_q_len, int32_t max_seq_len);

@@ -192,13 +192,14 @@ PyObject* gather(PyObject*, PyObject* const* o, Py_ssize_t n) {
 }
 
 // attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale,
-//           tree_mask) -> out or status
+//           tree_mask, out = None) -> out or status.  The GIL is held from the workspace to the last launch:
+// the launches of one call stand together on their stream, whichever threads call.
 PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Pages p;
-  int64_t q_row, max_q, max_len;
+  int64_t q_row, out_row, max_q, max_len;
   const int32_t *cu, *lens;
-  if (!g_attention || n != 11 || !pages(o + 1, p) || !whole(o[7], max_q) || !whole(o[8], max_len)) Py_RETURN_NONE;
+  if (!g_attention || (n != 11 && n != 12) || !pages(o + 1, p) || !whole(o[7], max_q) || !whole(o[8], max_len)) Py_RETURN_NONE;
   const at::Tensor* q = rows(o[0], p, 0, q_row);
   if (!q || !ints(o[5], p, p.batch + 1, cu) || !lengths(o[6], p, lens)) Py_RETURN_NONE;
   const int64_t total = q->size(0), heads = q->size(1);
@@ -217,13 +218,26 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   }
   const size_t bytes = g_workspace_size(p.batch, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len);
   if (bytes == 0) Py_RETURN_NONE;  // sizes that the general path refuses
+  const at::Tensor* given = nullptr;
+  if (n == 12 && o[11] != Py_None) {
+    given = rows(o[11], p, heads, out_row);
+    if (!given || given->size(0) != total) Py_RETURN_NONE;
+  }
   Launch on(p);
-  at::Tensor out = at::empty({total, heads, p.d}, q->options());
+  at::Tensor out;
+  if (!given) {
+    out = at::empty({total, heads, p.d}, q->options());
+    out_row = heads * p.d;
+  }
   const at::Tensor ws = workspace(p, on.stream, bytes);
   const int st = g_attention(q->data_ptr(), q_row, p.k, p.v, p.s, p.blocks, p.format, p.table, p.max_blocks, cu, lens, tree, p.batch,
                              (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (float)scale, ws.data_ptr(),
-                             (size_t)ws.numel(), out.data_ptr(), heads * p.d, on.stream);
+                             (size_t)ws.numel(), given ? given->data_ptr() : out.data_ptr(), out_row, on.stream);
   if (st != SDV_OK) return status(st);
+  if (given) {
+    Py_INCREF(o[11]);
+    return o[11];
+  }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }

@@ -586,7 +586,6 @@ def fp8_encode(x: torch.Tensor) -> torch.Tensor:
 
 # ---------------------------------------------------------------------------- the 8-bit KV cache
 _KV8_FORMATS = {torch.float8_e4m3fn: _native.KV8_FP8, torch.int8: _native.KV8_INT8}
-_KV8_SCRATCH: dict = {}  # (device, stream) -> kv8_attention's workspace of eager calls
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -749,18 +748,6 @@ def kv8_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     return ws
 
 
-def _kv8_scratch(dev: torch.device, nbytes: int) -> torch.Tensor:
-    """kv8_attention's workspace: one per (device, stream), whose calls are ordered.  A call that a
-    HIP graph records gets its own, from the graph's memory, so that no two graphs share one."""
-    if torch.cuda.is_current_stream_capturing():
-        return kv8_workspace(dev, nbytes)
-    key = (dev, _stream(dev))
-    ws = _KV8_SCRATCH.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = _KV8_SCRATCH[key] = kv8_workspace(dev, nbytes)
-    return ws
-
-
 def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
                   cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_q_len: int, max_seq_len: int, *,
                   scale: float | None = None, tree_mask: torch.Tensor | None = None, out: torch.Tensor | None = None,
@@ -772,18 +759,19 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     may stand in one batch; max_q_len is the largest.  A row sees the keys up to its own position;
     with tree_mask (int64 or uint64 (total,), max_q_len <= 64) the context before the new tokens and
     the new tokens j whose bit j of its mask is set.  scale: default 1 / sqrt(D).  A row that sees
-    nothing is 0, one whose scores are all -inf (an infinite q) NaN; rows behind cu_rows[B] are not written.  out (like q; tokens may lie any multiple of
-    8 elements apart) and workspace_tensor (uint8, of kv8_attention_workspace_bytes, not for calls that
-    may overlap) are the caller's own.  The pages as for kv8_append.
+    nothing is 0, one whose scores are all -inf (an infinite q) NaN; rows behind cu_rows[B] are not
+    written.  out (like q; tokens may lie any multiple of 8 elements apart) and workspace_tensor (uint8, of
+    kv8_attention_workspace_bytes; not for calls that may overlap on the device, nor for host threads that
+    may be in a call with it at once) are the caller's own.  The pages as for kv8_append.
 
     A call with more than 32 rows per sequence and KV head (by max_q_len) that is not a short one holds V
     relative to the largest V scale of a row tile's keys, those that a row does not see and rows of zeros (scale 1)
     among them: beside the roundings to 11 bits an output is off by up to 2^-30 of that scale, whatever its own
     size, and by up to 2^-32 of the sum of |V| over its keys, divided by that of their exponentials.
     """
-    if out is None and workspace_tensor is None:
+    if workspace_tensor is None:
         got = _native.binding().attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale,
-                                          tree_mask)
+                                          tree_mask, out)
         if got is not None:
             if got.__class__ is int:
                 _native.check(got, "sdv_kv8_attention")
@@ -811,9 +799,7 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         if out.shape[0] != total:
             _fail(f"out {tuple(out.shape)} != q {tuple(q.shape)}")
     nbytes = kv8_attention_workspace_bytes(B, total, H, kv, d, max_q_len, max_seq_len)
-    if workspace_tensor is None:
-        workspace_tensor = _kv8_scratch(dev, nbytes)
-    else:
+    if workspace_tensor is not None:
         _need(workspace_tensor, "workspace_tensor", (torch.uint8,), dev)
         if workspace_tensor.numel() < nbytes:
             _fail(f"workspace_tensor holds {workspace_tensor.numel()} bytes, {nbytes} needed")
@@ -823,9 +809,18 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
             workspace_tensor[:_native.KV8_SYNC_BYTES].zero_()
     if total == 0:
         return out
+    scale = d ** -0.5 if scale is None else float(scale)
+    if workspace_tensor is None:  # again, as a plain case; what still is none (a tensor subclass) has a workspace to itself
+        got = _native.binding().attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale,
+                                          tree_mask, out)
+        if got is not None:
+            if got.__class__ is int:
+                _native.check(got, "sdv_kv8_attention")
+            return got
+        workspace_tensor = kv8_workspace(dev, nbytes)
     _kv8_call(_native.load().sdv_kv8_attention, "sdv_kv8_attention", dev, q.data_ptr(), q_row, k_pages.data_ptr(),
               v_pages.data_ptr(), scales.data_ptr(), nb, fmt, block_table.data_ptr(), mb, cu, lens, tree, B, total, H, kv, d,
-              max_q_len, max_seq_len, d ** -0.5 if scale is None else float(scale), workspace_tensor.data_ptr(),
+              max_q_len, max_seq_len, scale, workspace_tensor.data_ptr(),
               workspace_tensor.numel(), out.data_ptr(), out_row)
     return out
 
