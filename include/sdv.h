@@ -389,6 +389,20 @@ int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_pages, cons
                       int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes, void* out,
                       int64_t out_stride, void* stream);
 
+/*
+ * The same call with a workspace that may hold anything: what has to be zero between calls lies in the
+ * library's own memory, in one of SDV_KV8_SLOTS areas of SDV_KV8_SYNC_BYTES / 2 on each device.  Calls that may
+ * overlap on the device need a slot each, and a recorded graph keeps the slots of its calls.  slot -1: the
+ * workspace's first bytes, as above.  SDV_ERR_WORKSPACE for any other.
+ */
+#define SDV_KV8_SLOTS 2048
+int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
+                           int32_t num_blocks, int32_t format, const int32_t* block_table, int32_t max_blocks_per_seq,
+                           const int32_t* cu_rows, const int32_t* seq_lens, const uint64_t* tree_mask, int32_t batch,
+                           int32_t total_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
+                           int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes, int32_t slot,
+                           void* out, int64_t out_stride, void* stream);
+
 /* Elementwise fp32 -> E4M3FN (RNE, NaN beyond 464 / for Inf and NaN), device buffers. */
 int sdv_fp8_encode(const float* in, uint8_t* out, int64_t n, void* stream);
 

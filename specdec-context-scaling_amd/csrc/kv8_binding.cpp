@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -22,7 +23,7 @@ namespace {
 
 decltype(&sdv_kv8_append) g_append;
 decltype(&sdv_kv8_gather) g_gather;
-decltype(&sdv_kv8_attention) g_attention;
+decltype(&sdv_kv8_attention_slot) g_attention;
 decltype(&sdv_kv8_attention_workspace_size) g_workspace_size;
 
 // A tensor of no subclass (whose data might not be where it says), or nullptr.
@@ -110,17 +111,16 @@ struct Launch {
   explicit Launch(const Pages& p) : guard(p.device), stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(p.device.index()).stream()) {}
 };
 
-at::Tensor fresh_workspace(const Pages& p, size_t bytes) {
-  at::Tensor ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(p.device));
-  ws.narrow(0, 0, SDV_KV8_SYNC_BYTES).zero_();
-  return ws;
-}
+// kv8_attention's workspace lives as long as the call (its memory is used again in the order of the stream),
+// so that nothing of a graph's memory, or of another private pool that is current, outlives it.  What
+// has to be zero between calls is a slot of the library's: one per device and stream for eager calls, which
+// their stream orders, and one per recording and stream, so that no two graphs share one.  A slot that a
+// recording has had is not given out again, as the graph may be replayed at any time.  Without a slot (-1:
+// all given out, or a stream whose handle names another one in each thread) the workspace's own counts are
+// zeroed, by a fill of 1.8 us where a short call takes 8.
+constexpr int32_t kEagerSlots = 256;
 
-// kv8_attention's workspace: one per device and stream, whose calls are ordered.  The calls that a HIP
-// graph records on one stream share one of the graph's memory (so that no two graphs share one, and the
-// calls of one, in the order of their stream, clear its count area once a replay: a fill is 1.8 us of GPU
-// time, a short call 7).  The recording's is kept until the stream records another graph.
-at::Tensor workspace(const Pages& p, hipStream_t stream, size_t bytes) {
+int32_t count_slot(const Pages& p, hipStream_t stream) {
   struct Key {
     int device;
     hipStream_t stream;
@@ -129,25 +129,31 @@ at::Tensor workspace(const Pages& p, hipStream_t stream, size_t bytes) {
   struct Hash {
     size_t operator()(const Key& k) const { return std::hash<void*>()(k.stream) * 31 + k.device; }
   };
-  struct Recorded {
-    unsigned long long id = 0;
-    at::Tensor ws;
+  struct Slots {
+    int32_t eager = -1;
+    unsigned long long recording = 0;  // the last, and its slot
+    int32_t recorded = -1;
   };
-  const Key key = {p.device.index(), stream};
-  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
-    hipStreamCaptureStatus capture;
-    unsigned long long id = 0;
-    if (hipStreamGetCaptureInfo(stream, &capture, &id) != hipSuccess || capture != hipStreamCaptureStatusActive)
-      return fresh_workspace(p, bytes);
-    static auto* recorded = new std::unordered_map<Key, Recorded, Hash>();  // never freed: the runtime may end before it
-    Recorded& r = (*recorded)[key];
-    if (r.id != id || !r.ws.defined() || (size_t)r.ws.numel() < bytes) r = {id, fresh_workspace(p, bytes)};
-    return r.ws;
+  struct Given {
+    int32_t eager = 0, recorded = kEagerSlots;
+  };
+  static auto* slots = new std::unordered_map<Key, Slots, Hash>();  // never freed: the runtime may end before them
+  static auto* given = new std::unordered_map<int, Given>();        // by device
+  if (stream == hipStreamPerThread) return -1;
+  Slots& s = (*slots)[{p.device.index(), stream}];
+  Given& g = (*given)[p.device.index()];
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) {
+    if (s.eager < 0 && g.eager < kEagerSlots) s.eager = g.eager++;
+    return s.eager;
   }
-  static auto* cache = new std::unordered_map<Key, at::Tensor, Hash>();
-  at::Tensor& ws = (*cache)[key];
-  if (!ws.defined() || (size_t)ws.numel() < bytes) ws = fresh_workspace(p, bytes);
-  return ws;
+  hipStreamCaptureStatus capture;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(stream, &capture, &id) != hipSuccess || capture != hipStreamCaptureStatusActive || id == 0) return -1;
+  if (s.recording != id) {
+    s.recording = id;
+    s.recorded = g.recorded < SDV_KV8_SLOTS ? g.recorded++ : -1;
+  }
+  return s.recorded;
 }
 
 PyObject* status(int st) { return PyLong_FromLong(st); }
@@ -229,10 +235,13 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     out = at::empty({total, heads, p.d}, q->options());
     out_row = heads * p.d;
   }
-  const at::Tensor ws = workspace(p, on.stream, bytes);
+  const int32_t slot = count_slot(p, on.stream);
+  const c10::DataPtr ws = c10::hip::HIPCachingAllocator::get()->allocate(bytes);
+  if (slot < 0)
+    at::from_blob(ws.get(), {SDV_KV8_SYNC_BYTES}, at::TensorOptions().dtype(at::kByte).device(p.device)).zero_();
   const int st = g_attention(q->data_ptr(), q_row, p.k, p.v, p.s, p.blocks, p.format, p.table, p.max_blocks, cu, lens, tree, p.batch,
-                             (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (float)scale, ws.data_ptr(),
-                             (size_t)ws.numel(), given ? given->data_ptr() : out.data_ptr(), out_row, on.stream);
+                             (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (float)scale, ws.get(),
+                             bytes, slot, given ? given->data_ptr() : out.data_ptr(), out_row, on.stream);
   if (st != SDV_OK) return status(st);
   if (given) {
     Py_INCREF(o[11]);

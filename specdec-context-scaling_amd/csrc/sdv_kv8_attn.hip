@@ -44,6 +44,10 @@ constexpr float kKv8Slack = 8.0f;
 constexpr float kKv8LargeScale = 18446744073709551616.0f, kKv8Raise = 48.0f;
 
 constexpr int kKv8Threads = 256;  // of the kernel for few rows
+constexpr int kKv8Grid = 512;     // its workgroups: two per CU
+
+// Counts of finished parts, per slot and range; every call leaves its slot's zero, as the loader does.
+__device__ uint32_t kv8_counts[SDV_KV8_SLOTS][kKv8Grid];
 
 // The maximum that stands for a row none of whose scores of keys lo .. hi - 1 is above -inf: -inf where
 // it sees none of the keys, the lowest finite number where it does (scores of an infinite q, or NaN).  Both
@@ -483,7 +487,8 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
     }
     if (!whole) {
       const int w0 = at.first_range(a), parts = at.parts(a);
-      if (kv8_last(a.done + w0, parts, lds_plan.T)) {
+      uint32_t* done = a.done ? a.done : kv8_counts[a.slot];
+      if (kv8_last(done + w0, parts, lds_plan.T)) {
         kv8_merge<D, TR>(a, parts_mem, w0, at.second_part(a), parts, {row0, rows, seq.first, kvh},
                          reinterpret_cast<float2*>(&lds_o[0][0][0]));
       }
@@ -500,8 +505,6 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
 #include "sdv_kv8_chunk.h"
 
 using namespace sdv;
-
-constexpr int kKv8Grid = 512;  // two workgroups per CU
 
 constexpr int kKv8Start = 5;  // steps that starting a tile costs, about
 
@@ -535,7 +538,7 @@ static size_t kv8_workspace(int tile, int32_t head_dim) {
     return SDV_KV8_SYNC_BYTES + kChunkGrid * (sizeof(Kv8Cut) + 2 * sizeof(float) * (head_dim == 128 ? chunk_part<128>() : chunk_part<64>()));
   return SDV_KV8_SYNC_BYTES + (size_t)kKv8Grid * 2 * tile * (head_dim + 4) * sizeof(float);
 }
-static_assert(kKv8Grid * sizeof(uint32_t) <= SDV_KV8_SYNC_BYTES, "a count per range");
+static_assert(kKv8Grid * sizeof(uint32_t) == SDV_KV8_SYNC_BYTES / 2, "a count per range");
 
 static int kv8_attn_sizes(int32_t batch, int32_t total, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
                           int32_t max_len) {
@@ -567,12 +570,12 @@ static void kv8_launch_chunk(Kv8AttnArgs a, int grid, int64_t tiles, hipStream_t
   hipLaunchKernelGGL((kv8_chunk_merge_kernel<D>), dim3(cuts, kChunkWaves * D / 32), dim3(256), 0, st, a, grid);
 }
 
-extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
-                                 int32_t num_blocks, int32_t format, const int32_t* block_table, int32_t max_blocks_per_seq,
-                                 const int32_t* cu_rows, const int32_t* seq_lens, const uint64_t* tree_mask, int32_t batch,
-                                 int32_t total_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
-                                 int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes, void* out,
-                                 int64_t out_stride, void* stream) {
+extern "C" int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
+                                      int32_t num_blocks, int32_t format, const int32_t* block_table, int32_t max_blocks_per_seq,
+                                      const int32_t* cu_rows, const int32_t* seq_lens, const uint64_t* tree_mask, int32_t batch,
+                                      int32_t total_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
+                                      int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes, int32_t slot,
+                                      void* out, int64_t out_stride, void* stream) {
   if (!q || !k_pages || !v_pages || !scales || !block_table || !cu_rows || !out) return SDV_ERR_NULL;
   const int sizes = kv8_attn_sizes(batch, total_rows, q_heads, kv_heads, head_dim, max_q_len, max_seq_len);
   if (sizes != SDV_OK) return sizes;
@@ -586,6 +589,7 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
     return SDV_ERR_ALIGN;
   const int G = q_heads / kv_heads, tile = kv8_tile_rows(batch, total_rows, G, kv_heads, max_q_len, max_seq_len);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < kv8_workspace(tile, head_dim)) return SDV_ERR_WORKSPACE;
+  if (slot < -1 || slot >= SDV_KV8_SLOTS) return SDV_ERR_WORKSPACE;
   if (total_rows == 0) return SDV_OK;
 
   Kv8AttnArgs a;
@@ -603,7 +607,8 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   a.kv_heads = kv_heads;
   a.max_len = max_seq_len;
   a.c = (float)((double)scale * 1.4426950408889634);
-  a.done = static_cast<uint32_t*>(workspace);
+  a.done = slot < 0 ? static_cast<uint32_t*>(workspace) : nullptr;
+  a.slot = slot;
   a.cuts = nullptr;
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + SDV_KV8_SYNC_BYTES);
   // Units.  Where the device holds a workgroup for every unit of every tile, each takes one: the call is
@@ -646,4 +651,15 @@ extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_
   else
     fp8 ? kv8_launch<64, kFp8, 2>(a, grid, st) : kv8_launch<64, kInt8, 2>(a, grid, st);
   return hipGetLastError() == hipSuccess ? SDV_OK : SDV_ERR_HIP;
+}
+
+extern "C" int sdv_kv8_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,
+                                 int32_t num_blocks, int32_t format, const int32_t* block_table, int32_t max_blocks_per_seq,
+                                 const int32_t* cu_rows, const int32_t* seq_lens, const uint64_t* tree_mask, int32_t batch,
+                                 int32_t total_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
+                                 int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes, void* out,
+                                 int64_t out_stride, void* stream) {
+  return sdv_kv8_attention_slot(q, q_stride, k_pages, v_pages, scales, num_blocks, format, block_table, max_blocks_per_seq, cu_rows,
+                                seq_lens, tree_mask, batch, total_rows, q_heads, kv_heads, head_dim, max_q_len, max_seq_len, scale,
+                                workspace, workspace_bytes, -1, out, out_stride, stream);
 }

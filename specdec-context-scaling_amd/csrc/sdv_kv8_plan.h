@@ -37,7 +37,8 @@ struct Kv8AttnArgs {
   float c;         // softmax scale times log2 e
   int unit;        // steps per unit, as a power of two
   int start;       // units that stand for a tile's start
-  uint32_t* done;  // per range: finished parts of the shared tile that begins in it; 0 between calls
+  uint32_t* done;  // per range: finished parts of the shared tile that begins in it; 0 between calls; or nullptr:
+  int slot;        //   a slot of kv8_counts
   Kv8Cut* cuts;    // per workgroup, of the kernels whose parts a second launch adds up
   float* part;     // two slots per range: [TR][D] sums, then [TR][4]: maximum, sum of exponentials, -, -
 };

@@ -78,6 +78,8 @@ SIGNATURES = {
     "sdv_kv8_attention_workspace_size": (_SZ, [_I32] * 7),
     "sdv_kv8_attention": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I32, _I32,
                                          _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ, _P, _I64, _P]),
+    "sdv_kv8_attention_slot": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I32, _I32,
+                                              _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ, _I32, _P, _I64, _P]),
     "sdv_fp8_encode": (ctypes.c_int, [_P, _P, _I64, _P]),
     "sdv_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "sdv_abi_version": (ctypes.c_int, []),
@@ -138,7 +140,7 @@ def binding():
                                f"(or __graft_entry__.build()) on a machine with hipcc") from e
             _BINDING = _kv8_binding
         _BINDING.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
-                        ("sdv_kv8_append", "sdv_kv8_gather", "sdv_kv8_attention", "sdv_kv8_attention_workspace_size")))
+                        ("sdv_kv8_append", "sdv_kv8_gather", "sdv_kv8_attention_slot", "sdv_kv8_attention_workspace_size")))
         _BOUND = lib
     return _BINDING
 
