@@ -87,9 +87,10 @@ class KV8Cache(PagedKVCache):
         return counts, self._hold(self._cu[1])
 
     def _lengths(self, lengths):
-        """(device lengths or None, longest): None when all are equal."""
+        """(device lengths or None, longest): None where all are equal and not 0 (the operators take one
+        length for all from 1 on)."""
         longest = max(lengths)
-        if all(n == longest for n in lengths):
+        if longest > 0 and all(n == longest for n in lengths):
             return None, longest
         self._lens = self._table("sequence lengths", self._lens, tuple(lengths), lambda: list(lengths))
         return self._hold(self._lens[1]), longest
@@ -113,8 +114,8 @@ class KV8Cache(PagedKVCache):
             raise SdvError(f"k_new {tuple(k_new.shape)} does not hold {sum(counts)} rows")
         for b in range(self.batch):
             self.reserve(b, ends[b])
-        lens, longest = self._lengths(ends)
-        if longest > 0:
+        if max(ends) > 0:
+            lens, longest = self._lengths(ends)
             ops.kv8_append(k_new, v_new, *self.layer(layer), self._hold(self.block_table()), cu, lens, longest)
         self.lengths[:] = ends
 
