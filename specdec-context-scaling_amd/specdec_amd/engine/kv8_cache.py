@@ -89,6 +89,8 @@ class KV8Cache(PagedKVCache):
     def _lengths(self, lengths):
         """(device lengths or None, longest): None where all are equal and not 0 (the operators take one
         length for all from 1 on)."""
+        if len(lengths) != self.batch or min(lengths) < 0:
+            raise ValueError(f"lengths {lengths} for a batch of {self.batch}")
         longest = max(lengths)
         if longest > 0 and all(n == longest for n in lengths):
             return None, longest
