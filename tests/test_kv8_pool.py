@@ -8,6 +8,14 @@ from specdec_amd.engine import kv8_cache
 from specdec_amd.engine.kv8_cache import KV8Cache
 
 
+def test_lengths_of_another_batch_are_refused():
+    pool = KV8Cache(2, 64, batch=2, capacity_tokens=32, device="cpu")
+    q = torch.zeros((2, 4, 1, 64), dtype=torch.bfloat16)
+    for lengths in ([5], [5, 5, 5], [-1, 3]):
+        with pytest.raises(ValueError):
+            pool.attend(0, q, lengths=lengths)
+
+
 @pytest.mark.parametrize("lengths,table,longest", [([0, 0], [0, 0], 1), ([0, 3], [0, 3], 3), ([3, 3], None, 3), ([0], [0], 1)])
 def test_lengths_that_attention_is_given(monkeypatch, lengths, table, longest):
     """Equal lengths are one number, which cannot be 0."""
