@@ -45,6 +45,8 @@ class KV8Cache(PagedKVCache):
         self._cu: tuple | None = None     # ((counts, stream), device row table) of the last call
         self._lens: tuple | None = None   # ((lengths, stream), device array) of the last call
         self._held: list = []             # tables that recorded graphs read
+        self._served = (None, None)       # block table and K pages that _streams stands for
+        self._streams: set = set()        # streams that the allocator knows to use them
 
     # ------------------------------------------------------------------ storage
     def _new_pages(self, nb: int):
@@ -53,6 +55,10 @@ class KV8Cache(PagedKVCache):
         v = torch.zeros((L, nb, KV, D, BLOCK), dtype=torch.uint8, device=self.device).view(t)
         s = torch.ones((L, nb, KV, 2, BLOCK), dtype=torch.float32, device=self.device)
         return k, v, s
+
+    def _grow(self, min_blocks: int) -> None:
+        self._note_stream()  # the old pages are read on this stream, then dropped
+        super()._grow(min_blocks)
 
     @property
     def scales(self) -> torch.Tensor:
@@ -97,6 +103,28 @@ class KV8Cache(PagedKVCache):
         self._lens = self._table("sequence lengths", self._lens, tuple(lengths), lambda: list(lengths))
         return self._hold(self._lens[1]), longest
 
+    def _note_stream(self) -> None:
+        """The block table and the pages are one for all streams, and go back to the memory of the stream
+        that made them when they are replaced.  The allocator is told of every other stream that uses them,
+        whose kernels it then waits for."""
+        if self.device.type != "cuda" or _recording(self.device):
+            return
+        if self._served[0] is not self._bt or self._served[1] is not self.k_pages:
+            self._served, self._streams = (self._bt, self.k_pages), set()
+        stream = ops._stream(self.device)
+        if stream not in self._streams:
+            self._streams.add(stream)
+            on = torch.cuda.current_stream(self.device)
+            for t in (self._bt, self.k_pages, self.v_pages, self.v_scales):
+                if t is not None:
+                    t.record_stream(on)
+
+    def _operands(self, layer: int):
+        """(K pages, V pages, scales, block table) of a call on the current stream."""
+        table = self._hold(self.block_table())
+        self._note_stream()
+        return (*self.layer(layer), table)
+
     def _hold(self, t):
         if _recording(self.device) and not any(t is h for h in self._held):
             self._held.append(t)
@@ -118,7 +146,7 @@ class KV8Cache(PagedKVCache):
             self.reserve(b, ends[b])
         if max(ends) > 0:
             lens, longest = self._lengths(ends)
-            ops.kv8_append(k_new, v_new, *self.layer(layer), self._hold(self.block_table()), cu, lens, longest)
+            ops.kv8_append(k_new, v_new, *self._operands(layer), cu, lens, longest)
         self.lengths[:] = ends
 
     def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, starts: list[int] | None = None):
@@ -154,8 +182,8 @@ class KV8Cache(PagedKVCache):
             raise SdvError(f"out {tuple(out.shape)} != q {tuple(q.shape)}")
         direct = out if shape is None else None
         lens, longest = self._lengths(lengths)
-        got = ops.kv8_attention(rows, *self.layer(layer), self._hold(self.block_table()), cu, lens, max(1, *counts), max(1, longest),
-                                scale=scale, tree_mask=tree_mask, out=direct)
+        got = ops.kv8_attention(rows, *self._operands(layer), cu, lens, max(1, *counts), max(1, longest), scale=scale,
+                                tree_mask=tree_mask, out=direct)
         if shape is not None:
             got = got.view(shape)
             got = got if q_token_major else got.transpose(1, 2).contiguous()
@@ -183,7 +211,7 @@ class KV8Cache(PagedKVCache):
             raise ValueError(f"positions {starts} + {counts} outside the sequences' {self.lengths} tokens")
         _no_recording(self.device, "positions would be copied from the host")
         at = torch.tensor(starts, dtype=torch.int32).to(self.device)
-        return ops.kv8_gather(*self.layer(layer), self.block_table(), cu, at, sum(counts))
+        return ops.kv8_gather(*self._operands(layer), cu, at, sum(counts))
 
     def gather(self, layer: int, seq: int, n: int | None = None):
         """(k, v) BF16 (KV, T, D) of a sequence's first n tokens (default: all), dequantized."""

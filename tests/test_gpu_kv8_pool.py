@@ -1,4 +1,4 @@
-"""KV8Cache at the ends of its use: sequences without tokens."""
+"""KV8Cache at the ends of its use: sequences without tokens, streams that overlap."""
 from __future__ import annotations
 
 import pytest
@@ -36,3 +36,72 @@ def test_attend_without_tokens(cuda_device, batch, rows):
         assert bool((got[:rows] == 0).all()) and torch.equal(got[rows:], full[rows:])
     pool.write(0, k[:0], v[:0], [0] * batch)
     assert pool.lengths == [0] * batch and pool.attend(0, q[:0], counts=[0] * batch).shape == (0, 12, 128)
+
+
+def _busy(stream):
+    """About 100 ms of work on `stream`, and an event behind it."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)
+    done = torch.cuda.Event()
+    done.record(stream)
+    return done
+
+
+@pytest.mark.parametrize("what", ["table", "pages"])
+def test_what_a_busy_stream_reads_is_not_given_away(cuda_device, what):
+    """The block table, or the pages, are replaced on one stream while a call that reads the old ones waits on
+    another: what the first stream allocates meanwhile, and writes, is other memory."""
+    dev = cuda_device
+    pool = KV8Cache(2, 128, batch=2, num_blocks=24, device=dev, seed=3)
+    rows, q = _rows((200, 4, 128), 1).to(dev), _rows((2, 12, 128), 2).to(dev)
+    pool.write(0, rows[:, :2], rows[:, 2:], [120, 80])
+    want = pool.attend(0, q, counts=[1, 1])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        pool.attend(0, q, counts=[1, 1])  # its own row table and lengths
+    torch.cuda.synchronize()
+    old = [pool.block_table()] if what == "table" else [pool.k_pages, pool.v_pages, pool.scales]
+    addresses, sizes = [t.data_ptr() for t in old], [t.numel() * t.element_size() for t in old]
+    del old
+    announce(f"kv8 pool: {what} replaced while a stream is busy")
+    done = _busy(side)
+    with torch.cuda.stream(side):
+        late = pool.attend(0, q, counts=[1, 1])
+    pool.reserve(0, 130 if what == "table" else 600)
+    assert torch.equal(pool.attend(0, q, counts=[1, 1]), want)
+    kept = []
+    for size in sizes:
+        for _ in range(64):
+            kept.append(torch.full((size,), 1, dtype=torch.uint8, device=dev))
+            assert kept[-1].data_ptr() not in addresses
+    assert not done.query(), "the other stream was not busy for long enough to tell"
+    torch.cuda.synchronize()
+    assert torch.equal(late, want)
+
+
+def test_two_streams_without_waits_of_the_host(cuda_device):
+    """Steps that alternate between two streams, ordered by events alone, while the other allocates and writes
+    memory of the tables' sizes: the same as on one stream."""
+    dev = cuda_device
+    counts = [[120, 60], [1, 5], [40, 1], [1, 5], [3, 3], [1, 1], [64, 64], [1, 1]]
+    steps = [(_rows((sum(c), 12, 128), 10 + i).to(dev), _rows((sum(c), 2, 128), 30 + i).to(dev), _rows((sum(c), 2, 128), 50 + i).to(dev))
+             for i, c in enumerate(counts)]
+    one, two = (KV8Cache(2, 128, batch=2, num_blocks=4, device=dev, seed=3) for _ in range(2))
+    want = [one.append_attend(0, *x, counts=c) for x, c in zip(steps, counts)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    announce("kv8 pool on two streams, ordered by events")
+    got = []
+    for i, (x, c) in enumerate(zip(steps, counts)):
+        st, other = streams[i % 2], streams[1 - i % 2]
+        st.wait_stream(other)
+        with torch.cuda.stream(st):
+            torch.cuda._sleep(2_000_000)
+            got.append(two.append_attend(0, *x, counts=c))
+        with torch.cuda.stream(other):
+            for n in (3, 2, 8, 16, 40, 4096):
+                torch.full((n,), 1, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
