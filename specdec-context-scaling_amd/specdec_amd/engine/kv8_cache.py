@@ -16,8 +16,9 @@ one write and one attention per layer.
 
 Recording into a HIP graph: with equal counts and lengths a recorded ``append_attend`` reads nothing
 from the host but the row table, which an earlier call with the same counts has made; what it cannot
-do inside a recording (add blocks, grow the pool, new tables) raises.  Tables that a recording used
-stay alive as long as the pool.
+do inside a recording (add blocks, grow the pool, new tables) raises.  Pages and tables that a recording
+used stay alive as long as the pool; once the pool has grown the graph has to be recorded again,
+since what it writes does not reach the new pages.
 """
 from __future__ import annotations
 
@@ -44,7 +45,6 @@ class KV8Cache(PagedKVCache):
                          capacity_tokens=capacity_tokens, device=device, seed=seed, growable=growable)
         self._cu: tuple | None = None     # ((counts, stream), device row table) of the last call
         self._lens: tuple | None = None   # ((lengths, stream), device array) of the last call
-        self._held: list = []             # tables that recorded graphs read
         self._served = (None, None)       # block table and K pages that _streams stands for
         self._streams: set = set()        # streams that the allocator knows to use them
 
@@ -122,13 +122,9 @@ class KV8Cache(PagedKVCache):
     def _operands(self, layer: int):
         """(K pages, V pages, scales, block table) of a call on the current stream."""
         table = self._hold(self.block_table())
+        self._hold_pages()
         self._note_stream()
         return (*self.layer(layer), table)
-
-    def _hold(self, t):
-        if _recording(self.device) and not any(t is h for h in self._held):
-            self._held.append(t)
-        return t
 
     # ------------------------------------------------------------------ kernels
     def write(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, counts, starts=None) -> None:

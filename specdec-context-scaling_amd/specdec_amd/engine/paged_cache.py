@@ -20,7 +20,10 @@ table on the device and, with equal lengths, passes no length array, and the poo
 attention workspace, so a decode or verify step copies nothing from the host and allocates
 nothing.  What it cannot do inside a recording -- add blocks (a new block table is copied
 from the host), grow the pool (new page tensors), grow the workspace -- raises instead;
-``reserve_all`` and ``workspace`` before recording make room.
+``reserve_all`` and ``workspace`` before recording make room.  The pages and tables that a
+recording read stay alive as long as the pool.  A graph goes on with those it was recorded with:
+once the pool has grown, what it writes does not reach the new pages, and it has to be
+recorded again.
 
 Ownership rule (the reference's trim returns views and its appends build new tensors, so an
 untrimmed handle keeps its data; here appends write pages in place): after
@@ -104,6 +107,7 @@ class PagedKVCache:
         # tile tables that recorded graphs read, by lengths (which alone decide a table's contents):
         # kept alive as long as the pool, one for each set of lengths recorded
         self._recorded: dict[tuple, torch.Tensor] = {}
+        self._held: list = []  # pages and tables that recorded graphs read
         self._ws = None     # attention workspace owned by the pool
         # replaced workspaces, kept alive for graphs that recorded them; each replacement is at
         # least twice the size of the one before, so they hold at most the current one's bytes
@@ -202,6 +206,17 @@ class PagedKVCache:
         self.lengths[seq] = 0
         self._bt = None
 
+    def _hold(self, t):
+        """`t`, kept alive as long as the pool where the call is being recorded."""
+        if _recording(self.device) and not any(t is h for h in self._held):
+            self._held.append(t)
+        return t
+
+    def _hold_pages(self) -> None:
+        if _recording(self.device):
+            for t in (self.k_pages, self.v_pages, self.v_scales):
+                self._hold(t)
+
     def max_blocks(self) -> int:
         return max(1, max(len(b) for b in self.blocks))
 
@@ -261,6 +276,9 @@ class PagedKVCache:
         H = q.shape[2] if q_token_major else q.shape[1]
         self._q_heads, self._q_len = max(self._q_heads, H), max(self._q_len, S)
         ws = self.workspace(ops.attention_workspace_bytes(1, B, H, self.kv_heads, S, self.head_dim, tmax))
+        if _recording(self.device):
+            self._hold_pages()
+            self._hold(self.block_table())
         if uniform and out is None:
             # the engine's per-layer call: its host cost is part of every token, so what the
             # general path checks one helper call at a time is tested here in one expression, and
@@ -341,6 +359,7 @@ class PagedKVCache:
                 _no_recording(self.device, "prefill would build its tables (call it with these lengths before, and pass the "
                                            "slots that it returns)")
             table = self._recorded.setdefault(key[0], self._tiles[2])
+            self._hold_pages()
         elif on_device:
             if slots is None or stale:
                 fresh, table = self._varlen(lengths)

@@ -1,4 +1,4 @@
-"""KV8Cache at the ends of its use: sequences without tokens, streams that overlap."""
+"""KV8Cache at the ends of its use: sequences without tokens, streams that overlap, growth after a recording."""
 from __future__ import annotations
 
 import pytest
@@ -6,6 +6,7 @@ import torch
 
 from conftest import announce
 from specdec_amd.engine.kv8_cache import KV8Cache
+from specdec_amd.engine.paged_cache import PagedKVCache
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +106,39 @@ def test_two_streams_without_waits_of_the_host(cuda_device):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", [KV8Cache, PagedKVCache])
+def test_a_recorded_step_after_the_pool_has_grown(cuda_device, kind):
+    """Growth replaces the pages and the block table: a graph recorded before keeps its own, whose memory nobody
+    else is given, and repeats its results."""
+    dev = cuda_device
+    pool = kind(2, 128, batch=2, num_blocks=24, device=dev, seed=3)
+    k, v = _rows((2, 100, 2, 128), 1).to(dev), _rows((2, 100, 2, 128), 2).to(dev)
+    step = _rows((2, 1, 12, 128), 3).to(dev), _rows((2, 1, 2, 128), 4).to(dev), _rows((2, 1, 2, 128), 5).to(dev)
+    pool.append(0, k, v, [0, 0])
+
+    def run():
+        return pool.append_attend(0, *step, [100, 100], q_token_major=True)
+
+    want = run()
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        out = run()
+    old = [pool.k_pages, pool.v_pages, pool.v_scales, pool.block_table()]
+    addresses, sizes = [t.data_ptr() for t in old], [t.numel() * t.element_size() for t in old]
+    del old
+    pool.reserve_all(600)
+    assert pool.k_pages.data_ptr() not in addresses and pool.block_table().data_ptr() not in addresses
+    kept = []
+    for size in sizes:
+        for _ in range(64):
+            kept.append(torch.zeros(size, dtype=torch.uint8, device=dev))
+            assert kept[-1].data_ptr() not in addresses
+    for turn in range(3):
+        announce(f"{kind.__name__}: a graph from before the growth, replay {turn}")
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(run(), want)
