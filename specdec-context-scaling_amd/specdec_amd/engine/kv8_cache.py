@@ -66,7 +66,8 @@ class KV8Cache(PagedKVCache):
 
     def reserve_all(self, n_tokens: int, q_heads: int | None = None, q_len: int | None = None) -> None:
         """Page blocks and the device block table for the first n_tokens positions of every sequence,
-        before recording a step up to them (a recording brings its own workspace)."""
+        before recording a step up to them.  q_heads and q_len size nothing here: a call's workspace is
+        its own, and a recording's is made with it."""
         for b in range(self.batch):
             self.reserve(b, n_tokens)
         self.block_table()
@@ -151,9 +152,12 @@ class KV8Cache(PagedKVCache):
         shape = (B * S, self.kv_heads, self.head_dim)
         self.write(layer, k_new.reshape(shape), v_new.reshape(shape), (S,) * B, starts)
 
-    def prefill(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, lengths: list[int]) -> None:
-        """Whole prompts of different lengths: write() from position 0."""
+    def prefill(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, lengths: list[int],
+                slots: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Whole prompts of different lengths: write() from position 0.  Slots come from the block table on
+        the device: `slots`, which PagedKVCache's layers hand on, is returned as it came and not read."""
         self.write(layer, k_new, v_new, lengths, [0] * self.batch)
+        return slots
 
     def attend(self, layer: int, q: torch.Tensor, *, counts=None, q_token_major: bool = False, lengths=None,
                scale: float | None = None, tree_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -1,4 +1,5 @@
-"""KV8Cache at the ends of its use: sequences without tokens, streams that overlap, growth after a recording."""
+"""KV8Cache at the ends of its use: sequences without tokens, streams that overlap, growth after a recording, prompts
+layer after layer."""
 from __future__ import annotations
 
 import pytest
@@ -142,3 +143,25 @@ def test_a_recorded_step_after_the_pool_has_grown(cuda_device, kind):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(run(), want)
+
+
+@pytest.mark.parametrize("kind", [KV8Cache, PagedKVCache])
+def test_prefill_of_layer_after_layer(cuda_device, kind):
+    """A loop that hands a layer's slots on to the next, whichever the pool; each layer's tokens read back."""
+    dev = cuda_device
+    pool = kind(2, 128, num_layers=3, batch=2, capacity_tokens=64, device=dev, seed=2)
+    pool.reserve_all(70, q_heads=12, q_len=5)
+    k, v = _rows((3, 75, 2, 128), 1).to(dev), _rows((3, 75, 2, 128), 2).to(dev)
+    slots = None
+    announce(f"{kind.__name__}: prefill of three layers")
+    for layer in range(3):
+        slots = pool.prefill(layer, k[layer], v[layer], [70, 5], slots)
+    assert pool.lengths == [70, 5]
+    for layer in range(3):
+        for seq, rows in enumerate((slice(0, 70), slice(70, 75))):
+            got = pool.gather(layer, seq)[0].transpose(0, 1).float()
+            want = k[layer, rows].float()
+            # the code is off by half a step, 2^-4 of it or half of the smallest, 2^-10 (scale max / 448); what is
+            # read back then by 2^-8 (BF16; the scale's and the product's roundings of 2^-24 are within the 2^-9 more)
+            off = want.abs() * 2.0 ** -4 + want.abs().amax(-1, keepdim=True) / 448 * 2.0 ** -10
+            assert bool(((got - want).abs() <= off + (want.abs() + off) * (2.0 ** -8 + 2.0 ** -9)).all())
