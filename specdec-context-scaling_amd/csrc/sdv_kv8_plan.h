@@ -10,12 +10,12 @@
 // workgroup's.  Lengths are read on the device, so that a recorded call follows them; every workgroup
 // works out its own range, in 1 to 1.5 us.
 //
-// The units of a sequence's tiles up to the i-th sum in closed form: of u keys each, tile j has
-// ceil((ctx G + TR (j + 1)) / (u G)) (the last one ceil(T / u)), a sum of floors of a linear
-// function, which takes as many turns as Euclid's algorithm on (u G, TR).
+// The units of a sequence's tiles up to the i-th sum in closed form (sdv_kv8_sums.h): of u keys each,
+// tile j has ceil((ctx G + TR (j + 1)) / (u G)), the last one ceil(T / u).
 #pragma once
 
 #include "sdv_kv8.h"
+#include "sdv_kv8_sums.h"
 
 namespace sdv {
 
@@ -42,29 +42,6 @@ struct Kv8AttnArgs {
   Kv8Cut* cuts;    // per workgroup, of the kernels whose parts a second launch adds up
   float* part;     // two slots per range: [TR][D] sums, then [TR][4]: maximum, sum of exponentials, -, -
 };
-
-// Sum of floor((a i + b) / m) over i < n.
-__device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-  uint32_t ans = 0;
-  while (n > 0) {
-    if (a >= m) {
-      ans += (uint32_t)((uint64_t)n * (n - 1) / 2) * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      ans += n * (b / m);
-      b %= m;
-    }
-    const uint32_t y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y % m;
-    const uint32_t t = m;
-    m = a;
-    a = t;
-  }
-  return ans;
-}
 
 struct Kv8Seq {
   int first, n, T, ctx;
@@ -100,8 +77,7 @@ __device__ __forceinline__ uint32_t kv8_steps_before(const Kv8Seq& s, int G, int
   const uint32_t keys = (uint32_t)kKv8Step << unit;
   if (s.tree) return (uint32_t)i * (((uint32_t)max(s.T, 1) + keys - 1) >> (kKv8StepBits + unit));
   if (i == 0) return 0;
-  const uint32_t m = keys * G;
-  return floor_sum((uint32_t)i, m, TR, (uint32_t)(max(s.ctx, 0) * G + TR) + m - 1);
+  return kv8_floor_sum<TR>((uint32_t)i, keys, (uint32_t)G, (uint32_t)(max(s.ctx, 0) * G + TR) + keys * G - 1);
 }
 
 template <int TR>
@@ -156,7 +132,7 @@ struct Kv8Place {
   }
 
   // Up to 64 tiles of a sequence are counted in the lanes of a wavefront and added up there (one
-  // division, where the closed form takes ten, one after the other: 3 us of a chunk's start).
+  // division, where the closed form takes three, and its terms one after the other).
   uint32_t lane_units, lane_sum;
   __device__ __forceinline__ void scan_tiles(const Kv8AttnArgs& a) {
     const int lane = threadIdx.x & (kWave - 1);
