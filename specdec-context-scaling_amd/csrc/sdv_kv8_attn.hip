@@ -526,7 +526,9 @@ static int64_t kv8_units(int32_t batch, int32_t total, int32_t G, int32_t kv_hea
 // no second launch.  2 KV heads of 128, tiles of 32 and of 256, in us (with a fill of 1.8): 300 tokens' 1800
 // rows 12 and 25, 288 rows over 2048 keys 14 and 23, 144 over 8192 (1280 steps) 20 and 25, 1200 over 2048
 // (2432) 21 and 28; of four sequences of 8192 48 rows each (2560) 24 and 24, 144 each (5632) 33 and 32, 288
-// each (10240) 42 and 37; 1200 over 8192 (9728) 44 and 36.
+// each (10240) 42 and 37; 1200 over 8192 (9728) 44 and 36.  With other heads the two are even at 6400 steps
+// (14/2/64, 26 and 27), 8192 (20/1/64, 30 and 30) and 4096 to 8192 (32/8/128, 27 and 25, 31 and 31); at less than
+// 3000 tiles of 32 take 0.5 to 0.8 of the time, past 10000 1.2 to 1.8.
 static int kv8_tile_rows(int32_t batch, int32_t total, int32_t G, int32_t kv_heads, int32_t max_q_len, int32_t max_len) {
   const int64_t rows = (int64_t)G * max_q_len, steps = ((int64_t)max_len + kKv8Step - 1) / kKv8Step;
   if (rows <= 32) return rows <= 16 ? 16 : 32;
@@ -622,7 +624,9 @@ extern "C" int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const voi
   // also where ones of four would not fit (eight sequences of 8192 keys, one row each, 14 us, in ranges
   // 19) and where a sequence's several tiles would then stand two a CU (576 rows over 2048 keys 16 us, with
   // four 19).  At 16 steps units and ranges are even (sixteen sequences 19.9 and 21.8, of mixed lengths 18.4
-  // and 18.1).
+  // and 18.1).  With other heads (14/2/64, 20/1/64, 32/8/128; 27 sizes of 1 to 16 sequences, 2048 to 131072 keys) the
+  // unit is the best or within 10% of it but for the longest contexts of one sequence, where a longer one would
+  // take up to a fifth off (20/1/64, one row over 32768 keys 23 and 19; 32/8/128, four rows 28 and 22).
   const int64_t tiles = kv8_tiles(batch, total_rows, G, tile) * kv_heads;
   const int64_t steps = ((int64_t)max_seq_len + kKv8Step - 1) / kKv8Step;
   const int most_grid = tile == kChunkRows ? kChunkGrid : kKv8Grid;

@@ -57,6 +57,7 @@ class KV8Cache(PagedKVCache):
         return k, v, s
 
     def _grow(self, min_blocks: int) -> None:
+        _no_recording(self.device, "the page pool would grow")
         self._note_stream()  # the old pages are read on this stream, then dropped
         super()._grow(min_blocks)
 
@@ -108,7 +109,7 @@ class KV8Cache(PagedKVCache):
         """The block table and the pages are one for all streams, and go back to the memory of the stream
         that made them when they are replaced.  The allocator is told of every other stream that uses them,
         whose kernels it then waits for."""
-        if self.device.type != "cuda" or _recording(self.device):
+        if self.device.type != "cuda":
             return
         if self._served[0] is not self._bt or self._served[1] is not self.k_pages:
             self._served, self._streams = (self._bt, self.k_pages), set()
@@ -122,9 +123,12 @@ class KV8Cache(PagedKVCache):
 
     def _operands(self, layer: int):
         """(K pages, V pages, scales, block table) of a call on the current stream."""
-        table = self._hold(self.block_table())
-        self._hold_pages()
-        self._note_stream()
+        table = self.block_table()
+        if _recording(self.device):
+            self._hold(table)
+            self._hold_pages()
+        else:
+            self._note_stream()
         return (*self.layer(layer), table)
 
     # ------------------------------------------------------------------ kernels
