@@ -625,7 +625,7 @@ extern "C" int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const voi
   // 19) and where a sequence's several tiles would then stand two a CU (576 rows over 2048 keys 16 us, with
   // four 19).  At 16 steps units and ranges are even (sixteen sequences 19.9 and 21.8, of mixed lengths 18.4
   // and 18.1).  With other heads (14/2/64, 20/1/64, 32/8/128; 27 sizes of 1 to 16 sequences, 2048 to 131072 keys) the
-  // unit is the best or within 10% of it but for the longest contexts of one sequence, where a longer one would
+  // unit is the best or within 11% of it but for the longest contexts of one sequence, where a longer one would
   // take up to a fifth off (20/1/64, one row over 32768 keys 23 and 19; 32/8/128, four rows 28 and 22).
   const int64_t tiles = kv8_tiles(batch, total_rows, G, tile) * kv_heads;
   const int64_t steps = ((int64_t)max_seq_len + kKv8Step - 1) / kKv8Step;
