@@ -47,7 +47,7 @@ constexpr int kKv8Threads = 256;  // of the kernel for few rows
 constexpr int kKv8Grid = 512;     // its workgroups: two per CU
 
 // Counts of finished parts, per slot and range; every call leaves its slot's zero, as the loader does.
-__device__ uint32_t kv8_counts[SDV_KV8_SLOTS][kKv8Grid];
+static __device__ uint32_t kv8_counts[SDV_KV8_SLOTS][kKv8Grid];
 
 // The maximum that stands for a row none of whose scores of keys lo .. hi - 1 is above -inf: -inf where
 // it sees none of the keys, the lowest finite number where it does (scores of an infinite q, or NaN).  Both
@@ -197,7 +197,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttnArgs& a, __amdgpu_buffer_
 // Long batches are bound by memory: single tokens of 32 sequences of 2048 to 32768 keys (293 MB of pages,
 // 2 KV heads of 128) take 55 to 57 us, 5.2 TB/s, a large copy's rate; the matrix cores are busy a tenth of
 // it.  Short calls are bound by latencies, each a microsecond or more: lengths, page ids, the pages,
-// the merge's count, and the parts.  One token over 2048 keys takes 7.3 us, over 32768 18.
+// the merge's count, and the parts.  One token over 2048 keys takes 7.5 us, over 32768 18.5.
 template <int D, int FMT, int RT>
 __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a) {
   constexpr int TR = 16 * RT, KI = D / 64, KS = D / 32, DT = D / 16;

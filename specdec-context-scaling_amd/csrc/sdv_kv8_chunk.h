@@ -27,7 +27,7 @@
 // that see it, and of no others.
 //
 // Bound by the matrix cores and what keeps them waiting: 2048 rows of 12 heads over 8192 keys (90 GFLOP,
-// head_dim 128) take 109 us, 0.83 PFLOP/s, where a large product of the library reaches 1.27 at the
+// head_dim 128) take 113 to 116 us, 0.79 PFLOP/s, where a large product of the library reaches 1.27 at the
 // clocks that such work runs at (1.7 to 1.8 GHz).  A stage takes 3400 cycles for 2080 of MFMA on each SIMD
 // (without the scores 2600, without them and the conversions 2200); starts take 7 to 9 us (the plan 1.4,
 // then page ids, scales and codes, one after another) and the parts' launch 8 to 12 (45 MB of them).
