@@ -60,6 +60,7 @@ class KV8Cache(PagedKVCache):
         _no_recording(self.device, "the page pool would grow")
         self._note_stream()  # the old pages are read on this stream, then dropped
         super()._grow(min_blocks)
+        self._served = (None, None)
 
     @property
     def scales(self) -> torch.Tensor:

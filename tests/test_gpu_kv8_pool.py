@@ -165,3 +165,15 @@ def test_prefill_of_layer_after_layer(cuda_device, kind):
             # read back then by 2^-8 (BF16; the scale's and the product's roundings of 2^-24 are within the 2^-9 more)
             off = want.abs() * 2.0 ** -4 + want.abs().amax(-1, keepdim=True) / 448 * 2.0 ** -10
             assert bool(((got - want).abs() <= off + (want.abs() + off) * (2.0 ** -8 + 2.0 ** -9)).all())
+
+
+def test_growth_gives_the_old_pages_back(cuda_device):
+    """Where nothing was recorded the pool that has grown holds its new pages alone."""
+    pool = KV8Cache(2, 128, batch=1, num_blocks=1024, device=cuda_device)
+    rows = _rows((20, 4, 128), 1).to(cuda_device)
+    pool.write(0, rows[:, :2], rows[:, 2:], [20])
+    torch.cuda.synchronize()
+    old = sum(t.numel() * t.element_size() for t in (pool.k_pages, pool.v_pages, pool.scales))
+    before = torch.cuda.memory_allocated()
+    pool.reserve(0, 1025 * 16)
+    assert torch.cuda.memory_allocated() - before <= old  # twice the blocks, and the old ones free again
