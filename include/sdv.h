@@ -322,8 +322,8 @@ int sdv_pack_contiguous(const void* k, const void* v_codes, const float* v_scale
  * -> 1) and codes RNE(x / s); a row that holds an infinity or a NaN has scale NaN and codes 0.
  *
  * Ragged rows: cu_rows int32 [batch + 1] on the device, sequence b's rows being cu_rows[b] ..
- * cu_rows[b+1] - 1 of the packed tensors (entries are clamped to [0, total_rows]; a sequence may have
- * none).  Rows behind cu_rows[batch] are neither read nor written.  Packed tensors are BF16
+ * cu_rows[b+1] - 1 of the packed tensors (entries are clamped to [0, total_rows] and must not decrease; a
+ * sequence may have none).  Rows behind cu_rows[batch] are neither read nor written.  Packed tensors are BF16
  * [total_rows][heads][head_dim] whose tokens lie `*_stride` elements apart (a multiple of 8, at
  * least heads * head_dim), so that the q, k and v parts of one projection's output can be passed
  * as they lie.  block_table int32 [batch][max_blocks_per_seq]; an entry outside [0, num_blocks), or a

@@ -79,8 +79,10 @@ def test_a_recording_keeps_no_memory_but_its_outputs(cuda_device):
     recording stream and on a forked one; replays still give the same bits."""
     cases = [_call(cuda_device, *c, seed=i) for i, c in enumerate(CASES)]
     graph, main, fork = torch.cuda.CUDAGraph(), torch.cuda.Stream(), torch.cuda.Stream()
+    own = [torch.zeros_like(want) for _, want in cases]  # outputs of the caller's
     with torch.cuda.graph(graph, stream=main):
         outs = [ops.kv8_attention(*a) for a, _ in cases]
+        assert all(ops.kv8_attention(*a, out=o) is o for (a, _), o in zip(cases, own))
         fork.wait_stream(main)
         with torch.cuda.stream(fork):
             outs += [ops.kv8_attention(*a) for a, _ in cases]
@@ -88,12 +90,12 @@ def test_a_recording_keeps_no_memory_but_its_outputs(cuda_device):
     assert {a for a, _ in _live_blocks(graph.pool())} == {o.data_ptr() for o in outs}
     for turn in range(3):
         announce(f"kv8 attention, a graph's replay {turn}")
-        for o in outs:
+        for o in outs + own:
             o.zero_()
         graph.replay()
         eager = [ops.kv8_attention(*a) for a, _ in cases]
         torch.cuda.synchronize()
-        for i, o in enumerate(outs + eager):
+        for i, o in enumerate(outs + own + eager):
             assert _same(o, cases[i % len(cases)][1])
 
 
