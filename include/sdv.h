@@ -403,6 +403,64 @@ int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const void* k_pages,
                            int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes, int32_t slot,
                            void* out, int64_t out_stride, void* stream);
 
+/* ------------------------------------------------------------------ positions, page moves
+ *
+ * Rotary positions.  The first rotary_dim dimensions of a head are pairs (x, y): (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) with interleaved = 1.  At position p pair i becomes scale (x cos t - y sin t) and
+ * scale (x sin t + y cos t), t = p inv_freq[i]; the other dimensions pass.  inv_freq: fp64 [rotary_dim / 2] on the
+ * device, radians per position (its values carry whatever stretches a context); scale: 1, or what such a method
+ * multiplies cos and sin by.  Angles are reduced in 64 bits; each value is rounded once, to BF16.  rotary_dim is a
+ * multiple of 16.  With the reference's frequencies this is its apply_rope (specdec/engine/model_self.py:272-298,
+ * specdec/kernels/cuda/rope.cu:10-38), which rounds cos, sin and the products to the rows' type.
+ *
+ * sdv_rope: rows of q (BF16 [rows][q_heads][head_dim], q_stride elements apart) and, with k_heads > 0, of k, each at
+ * positions[row] (int32, any sign), to q_out and k_out, which may be q and k themselves.  inverse = 1 rotates back (the
+ * transpose: gradients).  Alignment: rows 16 B (strides a multiple of 8), positions 4 B, inv_freq 8 B.
+ */
+int sdv_rope(const void* q, int64_t q_stride, int32_t q_heads, const void* k, int64_t k_stride, int32_t k_heads,
+             const int32_t* positions, const double* inv_freq, int32_t rotary_dim, int32_t interleaved, float scale,
+             int32_t inverse, int32_t rows, int32_t head_dim, void* q_out, int64_t q_out_stride, void* k_out,
+             int64_t k_out_stride, void* stream);
+
+/*
+ * A step's rows in one launch: q rotated to q_out (q itself, or elsewhere), k rotated, quantized and written, v quantized
+ * and written, as sdv_kv8_append has them (its arguments, in its order; K's scale and codes are those of the rotated
+ * row in fp32, which is not rounded to BF16 in between; a code is RNE(x / s), at most Q).  positions: int32
+ * [total_rows], for rows whose position is not the one that they are written at (a tree's nodes), or NULL: it is.  q rows
+ * behind cu_rows[batch] are left as they were; those without a slot are rotated all the same.
+ */
+int sdv_kv8_rope_append(const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int32_t q_heads,
+                        const void* k_new, const void* v_new, int64_t k_stride, int64_t v_stride, int32_t total_rows,
+                        void* k_pages, void* v_pages, float* scales, int32_t num_blocks, int32_t format,
+                        const int32_t* block_table, int32_t max_blocks_per_seq, const int32_t* cu_rows,
+                        const int32_t* seq_lens, int32_t max_seq_len, int32_t batch, int32_t kv_heads, int32_t head_dim,
+                        const int32_t* positions, const double* inv_freq, int32_t rotary_dim, int32_t interleaved,
+                        float scale, void* stream);
+
+/*
+ * Copy whole page blocks of every layer, in one launch: block src[i] of the `from` tensors to block dst[i] of the `to`
+ * tensors (int32 [n] on the device), which may be the same.  k_bytes, v_bytes and s_bytes are those of one block of one
+ * layer (multiples of 16), so that this serves the pages of both caches; a layer is its blocks, one after another.
+ * A pair with a number outside [0, from_blocks) or [0, to_blocks) is skipped.  No block may be the destination of two pairs, or, in
+ * one pool, a destination and a source.
+ */
+int sdv_copy_blocks(const void* k_from, const void* v_from, const float* s_from, int32_t from_blocks, void* k_to,
+                    void* v_to, float* s_to, int32_t to_blocks, int64_t k_bytes, int64_t v_bytes, int64_t s_bytes,
+                    int32_t num_layers, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+
+/*
+ * Keep tokens of the 8-bit cache and close the gaps, in place and in every layer: with kept[cu_kept[b]] ..
+ * kept[cu_kept[b+1] - 1] of sequence b (int32 [total_kept], cu_kept as cu_rows above), the token at position
+ * starts[b] + kept[cu_kept[b] + i] comes to starts[b] + i.  After the verify of a drafted tree these are the accepted
+ * path's nodes, starts the contexts' lengths before it.  Up to 64 entries of a sequence are read before any is written,
+ * whatever their order; of more, entries must ascend.  A token whose source or destination is in no block stays.  Layers lie
+ * *_layer_stride elements apart (num_layers 1: any).  Sequences whose moved tokens share blocks must not be in one call.
+ */
+int sdv_kv8_keep(void* k_pages, void* v_pages, float* scales, int32_t num_blocks, int64_t k_layer_stride,
+                 int64_t v_layer_stride, int64_t s_layer_stride, int32_t num_layers, const int32_t* block_table,
+                 int32_t max_blocks_per_seq, const int32_t* cu_kept, const int32_t* kept, int32_t total_kept,
+                 const int32_t* starts, int32_t batch, int32_t kv_heads, int32_t head_dim, void* stream);
+
 /* Elementwise fp32 -> E4M3FN (RNE, NaN beyond 464 / for Inf and NaN), device buffers. */
 int sdv_fp8_encode(const float* in, uint8_t* out, int64_t n, void* stream);
 

@@ -25,6 +25,10 @@ decltype(&sdv_kv8_append) g_append;
 decltype(&sdv_kv8_gather) g_gather;
 decltype(&sdv_kv8_attention_slot) g_attention;
 decltype(&sdv_kv8_attention_workspace_size) g_workspace_size;
+decltype(&sdv_rope) g_rope;
+decltype(&sdv_kv8_rope_append) g_rope_append;
+decltype(&sdv_copy_blocks) g_copy;
+decltype(&sdv_kv8_keep) g_keep;
 
 // A tensor of no subclass (whose data might not be where it says), or nullptr.
 const at::Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -80,23 +84,46 @@ bool pages(PyObject* const* o, Pages& p) {
 }
 
 // Packed BF16 rows (total, heads, D) whose tokens lie `stride` elements apart.
-const at::Tensor* rows(PyObject* o, const Pages& p, int64_t heads, int64_t& stride) {
+const at::Tensor* rows_of(PyObject* o, c10::Device dev, int64_t d, int64_t heads, int64_t& stride) {
   const at::Tensor* t = tensor(o);
-  if (!t || t->dim() != 3 || t->scalar_type() != at::kBFloat16 || t->device() != p.device) return nullptr;
+  if (!t || t->dim() != 3 || t->scalar_type() != at::kBFloat16 || t->device() != dev) return nullptr;
   const int64_t n = t->size(0), h = t->size(1);
-  if (t->size(2) != p.d || (heads && h != heads) || n == 0 || n > INT32_MAX || h > INT32_MAX) return nullptr;
-  stride = n == 1 ? h * p.d : t->stride(0);
-  if (t->stride(2) != 1 || (t->stride(1) != p.d && h != 1) || stride < h * p.d || stride % 8 != 0 ||
+  if (t->size(2) != d || (heads && h != heads) || n == 0 || n > INT32_MAX || h > INT32_MAX) return nullptr;
+  stride = n == 1 ? h * d : t->stride(0);
+  if (t->stride(2) != 1 || (t->stride(1) != d && h != 1) || stride < h * d || stride % 8 != 0 ||
       reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 != 0)
     return nullptr;
   return t;
 }
+const at::Tensor* rows(PyObject* o, const Pages& p, int64_t heads, int64_t& stride) { return rows_of(o, p.device, p.d, heads, stride); }
 
-bool ints(PyObject* o, const Pages& p, int64_t n, const int32_t*& at) {
+bool ints_of(PyObject* o, c10::Device dev, int64_t n, const int32_t*& at) {
   const at::Tensor* t = tensor(o);
-  if (!t || t->dim() != 1 || t->size(0) != n || !fits(*t, p.device, at::kInt)) return false;
+  if (!t || t->dim() != 1 || t->size(0) != n || !fits(*t, dev, at::kInt)) return false;
   at = static_cast<const int32_t*>(t->data_ptr());
   return true;
+}
+bool ints(PyObject* o, const Pages& p, int64_t n, const int32_t*& at) { return ints_of(o, p.device, n, at); }
+
+bool real(PyObject* o, double& v) {
+  if (!PyFloat_CheckExact(o)) return false;
+  v = PyFloat_AS_DOUBLE(o);
+  return true;
+}
+
+bool truth(PyObject* o, int32_t& v) {
+  v = o == Py_True;
+  return v || o == Py_False;
+}
+
+// The rotated dimensions that fp64 frequencies stand for, or 0.
+int32_t frequencies(PyObject* o, c10::Device dev, int64_t d, const double*& at) {
+  const at::Tensor* t = tensor(o);
+  if (!t || t->dim() != 1 || !fits(*t, dev, at::kDouble)) return 0;
+  const int64_t n = 2 * t->size(0);
+  if (n <= 0 || n > d || n % 16 != 0) return 0;
+  at = static_cast<const double*>(t->data_ptr());
+  return (int32_t)n;
 }
 
 bool lengths(PyObject* o, const Pages& p, const int32_t*& at) {
@@ -108,7 +135,8 @@ bool lengths(PyObject* o, const Pages& p, const int32_t*& at) {
 struct Launch {
   c10::OptionalDeviceGuard guard;
   hipStream_t stream;
-  explicit Launch(const Pages& p) : guard(p.device), stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(p.device.index()).stream()) {}
+  explicit Launch(c10::Device dev) : guard(dev), stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream()) {}
+  explicit Launch(const Pages& p) : Launch(p.device) {}
 };
 
 // kv8_attention's workspace lives as long as the call (its memory is used again in the order of the stream),
@@ -251,6 +279,169 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// rope(q, k or None, positions, inv_freq, interleaved, scale, inverse) -> (q, k or None) or status
+PyObject* rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t qs, ks = 0, heads = 0;
+  double scale;
+  int32_t interleaved, inverse;
+  const int32_t* positions;
+  const double* inv_freq;
+  if (!g_rope || n != 7 || !truth(o[4], interleaved) || !real(o[5], scale) || !truth(o[6], inverse)) Py_RETURN_NONE;
+  const at::Tensor* first = tensor(o[0]);
+  if (!first || first->dim() != 3 || !first->is_cuda()) Py_RETURN_NONE;
+  const c10::Device dev = first->device();
+  const int64_t d = first->size(2);
+  const at::Tensor *q = rows_of(o[0], dev, d, 0, qs), *k = nullptr;
+  if (!q || (o[1] != Py_None && !(k = rows_of(o[1], dev, d, 0, ks))) || !ints_of(o[2], dev, q->size(0), positions)) Py_RETURN_NONE;
+  if (k && k->size(0) != q->size(0)) Py_RETURN_NONE;
+  const int32_t rotary = frequencies(o[3], dev, d, inv_freq);
+  if (rotary == 0) Py_RETURN_NONE;
+  Launch on(dev);
+  at::Tensor q_out = at::empty({q->size(0), q->size(1), d}, q->options()), k_out;
+  if (k) {
+    heads = k->size(1);
+    k_out = at::empty({k->size(0), heads, d}, q->options());
+  }
+  const int st = g_rope(q->data_ptr(), qs, (int32_t)q->size(1), k ? k->data_ptr() : nullptr, ks, (int32_t)heads, positions, inv_freq, rotary,
+                        interleaved, (float)scale, inverse, (int32_t)q->size(0), (int32_t)d, q_out.data_ptr(), q->size(1) * d,
+                        k ? k_out.data_ptr() : nullptr, heads * d, on.stream);
+  if (st != SDV_OK) return status(st);
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(q_out)));
+  if (!k) Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(out, 1, k ? THPVariable_Wrap(std::move(k_out)) : Py_None);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// rope_append(q, k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len, inv_freq,
+//             interleaved, scale, positions or None) -> q or status
+PyObject* rope_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages p;
+  int64_t qs, ks, vs, max_len;
+  double scale;
+  int32_t interleaved;
+  const int32_t *cu, *lens, *positions = nullptr;
+  const double* inv_freq;
+  if (!g_rope_append || n != 14 || !pages(o + 3, p) || !whole(o[9], max_len) || !truth(o[11], interleaved) || !real(o[12], scale)) Py_RETURN_NONE;
+  const at::Tensor *q = rows(o[0], p, 0, qs), *k = rows(o[1], p, p.kv, ks), *v = rows(o[2], p, p.kv, vs);
+  if (!q || !k || !v || q->size(0) != k->size(0) || v->size(0) != k->size(0) || !ints(o[7], p, p.batch + 1, cu) || !lengths(o[8], p, lens) ||
+      (!lens && max_len == 0) || (o[13] != Py_None && !ints(o[13], p, q->size(0), positions)))
+    Py_RETURN_NONE;
+  const int32_t rotary = frequencies(o[10], p.device, p.d, inv_freq);
+  if (rotary == 0) Py_RETURN_NONE;
+  Launch on(p);
+  const int64_t heads = q->size(1);
+  at::Tensor out = at::empty({q->size(0), heads, p.d}, q->options());
+  const int st = g_rope_append(q->data_ptr(), qs, out.data_ptr(), heads * p.d, (int32_t)heads, k->data_ptr(), v->data_ptr(), ks, vs,
+                               (int32_t)q->size(0), p.k, p.v, p.s, p.blocks, p.format, p.table, p.max_blocks, cu, lens, (int32_t)max_len,
+                               p.batch, p.kv, p.d, positions, inv_freq, rotary, interleaved, (float)scale, on.stream);
+  if (st != SDV_OK) return status(st);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// The blocks of a layer (or of layers): K, V and scale tensors whose first dimensions are [layers,] blocks, KV heads.
+struct Blocks {
+  const at::Tensor* t[3];
+  int64_t layers, blocks, bytes[3];
+};
+
+bool blocks(PyObject* const* o, Blocks& b) {
+  for (int i = 0; i < 3; ++i)
+    if (!(b.t[i] = tensor(o[i])) || !b.t[i]->is_cuda() || !b.t[i]->is_contiguous() || b.t[i]->device() != b.t[0]->device()) return false;
+  const int64_t dim = b.t[1]->dim();
+  if ((dim != 4 && dim != 5) || b.t[2]->scalar_type() != at::kFloat) return false;
+  const int lead = (int)dim - 4;
+  b.layers = lead ? b.t[1]->size(0) : 1;
+  b.blocks = b.t[1]->size(lead);
+  if (b.layers <= 0 || b.blocks <= 0 || b.blocks > INT32_MAX || b.layers > INT32_MAX) return false;
+  for (const at::Tensor* t : b.t) {
+    if (t->dim() < lead + 3) return false;
+    for (int i = 0; i < lead + 2; ++i)
+      if (t->size(i) != b.t[1]->size(i)) return false;
+  }
+  for (int i = 0; i < 3; ++i) b.bytes[i] = b.t[i]->numel() / (b.layers * b.blocks) * (int64_t)b.t[i]->element_size();
+  return true;
+}
+
+// copy_blocks(k, v, scales, src, dst, k_to, v_to, scales_to) -> status
+PyObject* copy_blocks(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Blocks from, to;
+  if (!g_copy || n != 8 || !blocks(o, from) || !blocks(o + 5, to) || to.t[0]->device() != from.t[0]->device() || to.layers != from.layers) Py_RETURN_NONE;
+  for (int i = 0; i < 3; ++i) {
+    if (to.t[i]->dim() != from.t[i]->dim() || to.t[i]->scalar_type() != from.t[i]->scalar_type()) Py_RETURN_NONE;
+    const int64_t dim = from.t[1]->dim() - 4;
+    for (int64_t j = dim + 1; j < to.t[i]->dim(); ++j)
+      if (to.t[i]->size(j) != from.t[i]->size(j)) Py_RETURN_NONE;
+  }
+  const c10::Device dev = from.t[0]->device();
+  const at::Tensor* ids = tensor(o[3]);
+  const int32_t *src, *dst;
+  if (!ids || ids->dim() != 1 || ids->size(0) > INT32_MAX || !ints_of(o[3], dev, ids->size(0), src) || !ints_of(o[4], dev, ids->size(0), dst)) Py_RETURN_NONE;
+  if (ids->size(0) == 0) return status(SDV_OK);
+  Launch on(dev);
+  return status(g_copy(from.t[0]->data_ptr(), from.t[1]->data_ptr(), static_cast<const float*>(from.t[2]->data_ptr()), (int32_t)from.blocks,
+                       to.t[0]->data_ptr(), to.t[1]->data_ptr(), static_cast<float*>(to.t[2]->data_ptr()), (int32_t)to.blocks, from.bytes[0],
+                       from.bytes[1], from.bytes[2], (int32_t)from.layers, src, dst, (int32_t)ids->size(0), on.stream));
+  END_HANDLE_TH_ERRORS
+}
+
+// keep(k_pages, v_pages, scales, block_table, cu_kept, kept, starts) -> status
+PyObject* keep(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Blocks b;
+  if (!g_keep || n != 7 || !blocks(o, b)) Py_RETURN_NONE;
+  const at::Tensor &k = *b.t[0], &v = *b.t[1], &s = *b.t[2], *bt = tensor(o[3]), *ids = tensor(o[5]);
+  const c10::Device dev = k.device();
+  const int64_t lead = v.dim() - 4, kv = v.size(lead + 1), d = v.size(lead + 2);
+  if (k.dim() != lead + 6 || s.dim() != lead + 4 || k.scalar_type() != v.scalar_type() ||
+      (k.scalar_type() != at::kFloat8_e4m3fn && k.scalar_type() != at::kChar) || k.size(lead + 2) != 4 || k.size(lead + 3) * 16 != d ||
+      k.size(lead + 4) != 4 || k.size(lead + 5) != 16 || v.size(lead + 3) != 16 || s.size(lead + 2) != 2 || s.size(lead + 3) != 16)
+    Py_RETURN_NONE;
+  if (!bt || bt->dim() != 2 || !fits(*bt, dev, at::kInt) || bt->size(0) > INT32_MAX || bt->size(1) > INT32_MAX || !ids || ids->dim() != 1 ||
+      ids->size(0) > INT32_MAX || kv > INT32_MAX || d > INT32_MAX)
+    Py_RETURN_NONE;
+  const int32_t *cu, *kept, *starts;
+  if (!ints_of(o[4], dev, bt->size(0) + 1, cu) || !ints_of(o[5], dev, ids->size(0), kept) || !ints_of(o[6], dev, bt->size(0), starts)) Py_RETURN_NONE;
+  if (ids->size(0) == 0) return status(SDV_OK);
+  Launch on(dev);
+  return status(g_keep(k.data_ptr(), v.data_ptr(), static_cast<float*>(s.data_ptr()), (int32_t)b.blocks, k.numel() / b.layers,
+                       v.numel() / b.layers, s.numel() / b.layers, (int32_t)b.layers, static_cast<const int32_t*>(bt->data_ptr()),
+                       (int32_t)bt->size(1), cu, kept, (int32_t)ids->size(0), starts, (int32_t)bt->size(0), (int32_t)kv, (int32_t)d, on.stream));
+  END_HANDLE_TH_ERRORS
+}
+
+bool addresses(PyObject* const* o, Py_ssize_t n, void** at) {
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    at[i] = PyLong_AsVoidPtr(o[i]);
+    if (!at[i]) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "a null address");
+      return false;
+    }
+  }
+  return true;
+}
+
+// bind_moves(rope, rope_append, copy_blocks, keep): the same for the operators that move and turn rows
+PyObject* bind_moves(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  void* at[4];
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "bind_moves needs four addresses");
+    return nullptr;
+  }
+  if (!addresses(o, n, at)) return nullptr;
+  g_rope = reinterpret_cast<decltype(g_rope)>(at[0]);
+  g_rope_append = reinterpret_cast<decltype(g_rope_append)>(at[1]);
+  g_copy = reinterpret_cast<decltype(g_copy)>(at[2]);
+  g_keep = reinterpret_cast<decltype(g_keep)>(at[3]);
+  Py_RETURN_NONE;
+}
+
 // bind(append, gather, attention, workspace_size): the addresses of the loaded library's entry points
 PyObject* bind(PyObject*, PyObject* const* o, Py_ssize_t n) {
   void* at[4];
@@ -258,13 +449,7 @@ PyObject* bind(PyObject*, PyObject* const* o, Py_ssize_t n) {
     PyErr_SetString(PyExc_TypeError, "bind needs four addresses");
     return nullptr;
   }
-  for (int i = 0; i < 4; ++i) {
-    at[i] = PyLong_AsVoidPtr(o[i]);
-    if (!at[i]) {
-      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "a null address");
-      return nullptr;
-    }
-  }
+  if (!addresses(o, n, at)) return nullptr;
   g_append = reinterpret_cast<decltype(g_append)>(at[0]);
   g_gather = reinterpret_cast<decltype(g_gather)>(at[1]);
   g_attention = reinterpret_cast<decltype(g_attention)>(at[2]);
@@ -277,6 +462,11 @@ PyMethodDef methods[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(append)), METH_FASTCALL, nullptr},
     {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gather)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attention)), METH_FASTCALL, nullptr},
+    {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rope)), METH_FASTCALL, nullptr},
+    {"rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rope_append)), METH_FASTCALL, nullptr},
+    {"copy_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(copy_blocks)), METH_FASTCALL, nullptr},
+    {"keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(keep)), METH_FASTCALL, nullptr},
+    {"bind_moves", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind_moves)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kv8_binding", nullptr, -1, methods};

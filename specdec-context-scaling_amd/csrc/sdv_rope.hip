@@ -1,0 +1,267 @@
+// Rotary positions of packed rows, and of a step's rows on their way into the kv8 cache (formula: sdv_rope.h).
+#include "sdv_kv8_tile.h"
+#include "sdv_rope.h"
+
+namespace sdv {
+
+// ---------------------------------------------------------------------------- rows of q and k
+struct RopeRows {
+  RopeArgs rope;
+  const int32_t* positions;
+  int rows;
+  const uint16_t* in[2];  // q, k
+  uint16_t* out[2];
+  int64_t in_stride[2], out_stride[2];  // elements between rows
+  int heads[2];
+};
+
+// A lane rotates one unit of a row in HP heads, so that its eight angles serve all of them.
+template <int D, bool IL, int HP>
+__global__ __launch_bounds__(256) void rope_kernel(RopeRows a) {
+  constexpr int U = D / 16;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = e / U;
+  const int u = (int)(e % U), h0 = blockIdx.y * HP, heads = a.heads[0] + a.heads[1];
+  if (row >= a.rows) return;
+  const int d0 = rope_piece<IL>(a.rope, u, 0), d1 = rope_piece<IL>(a.rope, u, 1);
+  uint4 w[HP][2];
+#pragma unroll
+  for (int i = 0; i < HP; ++i) {
+    const int h = min(h0 + i, heads - 1), k = h >= a.heads[0];
+    const uint16_t* src = a.in[k] + row * a.in_stride[k] + (int64_t)(h - (k ? a.heads[0] : 0)) * D;
+    w[i][0] = *reinterpret_cast<const uint4*>(src + d0);
+    w[i][1] = *reinterpret_cast<const uint4*>(src + d1);
+  }
+  const bool turn = u < a.rope.units;
+  float c[8], s[8];
+  if (turn) rope_angles(a.rope, u, a.positions[row], c, s);
+#pragma unroll
+  for (int i = 0; i < HP; ++i) {
+    const int h = h0 + i, k = h >= a.heads[0];
+    if (h >= heads) break;
+    if (turn) {
+      float y[16];
+      rope_rotate<IL>(w[i][0], w[i][1], c, s, y);
+      w[i][0] = rope_pack8(y);
+      w[i][1] = rope_pack8(y + 8);
+    }
+    uint16_t* dst = a.out[k] + row * a.out_stride[k] + (int64_t)(h - (k ? a.heads[0] : 0)) * D;
+    *reinterpret_cast<uint4*>(dst + d0) = w[i][0];
+    *reinterpret_cast<uint4*>(dst + d1) = w[i][1];
+  }
+}
+
+// ---------------------------------------------------------------------------- a step's rows
+struct Kv8RopeArgs {
+  Kv8CacheArgs c;
+  RopeArgs rope;
+  const int32_t* positions;  // per packed row, or nullptr: the row's position in its sequence
+  const uint16_t* q;
+  uint16_t* q_out;
+  int64_t q_stride, out_stride;
+  int q_heads;
+};
+
+constexpr int kRopeHeads = 4;  // query heads of a wavefront
+
+// Workgroups (x, y): x a page block of a sequence, whichever of the call's rows fall in it; y a KV head, whose K and V
+// are quantized and written (as in kv8_append_kernel, but for K's rotation, which is not rounded in between), or
+// kRopeHeads query heads.
+template <int D, int FMT, bool IL>
+__global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
+  constexpr int U = D / 16;      // lanes per row: a unit each
+  constexpr int R = kWave / U;   // rows of a wave-wide load (8 or 16)
+  __shared__ uint4 lds_v[D];
+  const int lane = threadIdx.x, u = lane % U, rr = lane / U;
+  const int d0 = rope_piece<IL>(a.rope, u, 0), d1 = rope_piece<IL>(a.rope, u, 1);
+  const bool turn = u < a.rope.units;
+  Kv8Tile t;
+
+  if ((int)blockIdx.y >= a.c.kv_heads) {  // query heads
+    if (!kv8_tile<true, false>(a.c, (int)blockIdx.x, t)) return;
+    // of R rows, 2^lg are tokens and the others more heads of theirs
+    const int n = t.t1 - t.t0, h0 = ((int)blockIdx.y - a.c.kv_heads) * kRopeHeads;
+    int lg = 0;
+    while ((1 << lg) < min(n, R)) ++lg;
+    const int step = R >> lg, hs = rr >> lg;
+    for (int g = 0; g < n; g += 1 << lg) {
+      const int tok = t.t0 + g + (rr & ((1 << lg) - 1));
+      const int64_t row = t.row + min(tok, t.t1 - 1);
+      const uint16_t* src = a.q + row * a.q_stride;
+      uint4 w[kRopeHeads][2];
+      const auto has = [&](int i) { return i * step + hs < kRopeHeads && h0 + i * step + hs < a.q_heads && tok < t.t1; };
+#pragma unroll
+      for (int i = 0; i < kRopeHeads; ++i) {
+        if (!has(i)) continue;
+        w[i][0] = load_stream16(src + (h0 + i * step + hs) * D + d0);
+        w[i][1] = load_stream16(src + (h0 + i * step + hs) * D + d1);
+      }
+      float c[8], s[8];
+      if (turn) rope_angles(a.rope, u, a.positions ? a.positions[row] : t.block * kBlock + tok, c, s);
+#pragma unroll
+      for (int i = 0; i < kRopeHeads; ++i) {
+        if (!has(i)) continue;
+        if (turn) {
+          float y[16];
+          rope_rotate<IL>(w[i][0], w[i][1], c, s, y);
+          w[i][0] = rope_pack8(y);
+          w[i][1] = rope_pack8(y + 8);
+        }
+        uint16_t* dst = a.q_out + row * a.out_stride + (h0 + i * step + hs) * D;
+        *reinterpret_cast<uint4*>(dst + d0) = w[i][0];
+        *reinterpret_cast<uint4*>(dst + d1) = w[i][1];
+      }
+    }
+    return;
+  }
+
+  if (!kv8_tile<true>(a.c, (int)blockIdx.x, t)) return;  // wave-uniform
+  const int id = kv8_block(a.c.r, t.b, t.block);
+  if (id < 0) return;
+  const int kvh = blockIdx.y;
+  const int64_t page = (int64_t)id * a.c.kv_heads + kvh;
+  uint8_t* kp = a.c.k_pages + page * (kBlock * D);
+  uint8_t* vp = a.c.v_pages + page * (kBlock * D);
+  float* sp = a.c.scales + page * (2 * kBlock);
+
+  // K: lane (rr, u) holds unit u of token j*R + rr; V as kv8_write_v has it.  Tokens that are not the call's re-read a
+  // row that is.
+  constexpr int JK = kBlock / R, LPR = D / 8, JV = kBlock * LPR / kWave;
+  uint4 kw[JK][2], vw[JV];
+  const uint16_t* kin = static_cast<const uint16_t*>(a.c.k) + kvh * D;
+  const uint16_t* vin = static_cast<const uint16_t*>(a.c.v) + kvh * D + 8 * (lane % LPR);
+  int pos[JK];
+#pragma unroll
+  for (int j = 0; j < JK; ++j) {
+    const int tok = min(max(j * R + rr, t.t0), t.t1 - 1);
+    const uint16_t* src = kin + (int64_t)(t.row + tok) * a.c.k_stride;
+    kw[j][0] = load_stream16(src + d0);
+    kw[j][1] = load_stream16(src + d1);
+    pos[j] = a.positions ? a.positions[t.row + tok] : t.block * kBlock + tok;
+  }
+#pragma unroll
+  for (int j = 0; j < JV; ++j) {
+    const int tok = min(max(lane / LPR * JV + j, t.t0), t.t1 - 1);
+    vw[j] = load_stream16(vin + (int64_t)(t.row + tok) * a.c.v_stride);
+  }
+#pragma unroll
+  for (int j = 0; j < JK; ++j) {
+    if (t.t1 <= j * R || t.t0 >= (j + 1) * R) continue;  // none of the call's tokens
+    const int tok = j * R + rr;
+    float y[16];
+    if (turn) {
+      float c[8], s[8];
+      rope_angles(a.rope, u, pos[j], c, s);
+      rope_rotate<IL>(kw[j][0], kw[j][1], c, s, y);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) y[k] = bf16_at(kw[j][k >> 3], k & 7);
+    }
+    uint32_t ab = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) ab = max(ab, __float_as_uint(y[k]) & 0x7FFFFFFFu);
+    ab = unit_max_bits<U>(ab);
+    constexpr float kQ = FMT == kFp8 ? 448.0f : 127.0f;
+    float s = __uint_as_float(ab) / kQ;
+    if (s == 0.0f) s = 1.0f;
+    const bool finite = ab < 0x7F800000u;
+    // the largest quotient passes Q where the scale is below fp32's normal numbers
+#pragma unroll
+    for (int k = 0; k < 16; ++k) y[k] = finite ? fminf(fmaxf(y[k] / s, -kQ), kQ) : 0.0f;
+    if (tok >= t.t0 && tok < t.t1) {
+      uint8_t* dst = kp + (tok >> 2) * (4 * D) + (tok & 3) * 16;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int d = k == 0 ? d0 : d1;
+        *reinterpret_cast<uint2*>(dst + (d >> 4) * 64 + (d & 8)) =
+            make_uint2(kv8_pack4<FMT>(y[8 * k], y[8 * k + 1], y[8 * k + 2], y[8 * k + 3]),
+                       kv8_pack4<FMT>(y[8 * k + 4], y[8 * k + 5], y[8 * k + 6], y[8 * k + 7]));
+      }
+      if (u == 0) sp[tok] = finite ? s : __builtin_nanf("");
+    }
+  }
+  kv8_write_v<D, FMT>(t, vw, vp, sp, lds_v);
+}
+
+}  // namespace sdv
+
+using namespace sdv;
+
+template <int D, bool IL>
+static void rope_launch(const RopeRows& a, hipStream_t st) {
+  const int heads = a.heads[0] + a.heads[1];
+  const int64_t blocks = ((int64_t)a.rows * (D / 16) + 255) / 256;
+  if (blocks * heads <= 1024)
+    hipLaunchKernelGGL((rope_kernel<D, IL, 1>), dim3((unsigned)blocks, (unsigned)heads), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((rope_kernel<D, IL, 4>), dim3((unsigned)blocks, (unsigned)((heads + 3) / 4)), dim3(256), 0, st, a);
+}
+
+extern "C" int sdv_rope(const void* q, int64_t q_stride, int32_t q_heads, const void* k, int64_t k_stride, int32_t k_heads,
+                        const int32_t* positions, const double* inv_freq, int32_t rotary_dim, int32_t interleaved, float scale,
+                        int32_t inverse, int32_t rows, int32_t head_dim, void* q_out, int64_t q_out_stride, void* k_out,
+                        int64_t k_out_stride, void* stream) {
+  if (!q || !q_out || !positions || (k_heads > 0 && (!k || !k_out))) return SDV_ERR_NULL;
+  if (head_dim != 64 && head_dim != 128) return SDV_ERR_UNSUPPORTED;
+  const int st = rope_check(inv_freq, rotary_dim, interleaved, head_dim);
+  if (st != SDV_OK) return st;
+  if (rows < 0 || q_heads <= 0 || k_heads < 0 || q_heads > 32767 || k_heads > 32767 || rows > INT32_MAX / 2 || inverse < 0 || inverse > 1)
+    return SDV_ERR_SHAPE;
+  const int64_t qr = (int64_t)q_heads * head_dim, kr = (int64_t)k_heads * head_dim;
+  if (q_stride < qr || q_out_stride < qr || (k_heads > 0 && (k_stride < kr || k_out_stride < kr))) return SDV_ERR_SHAPE;
+  if (!aligned(q, 16) || !aligned(q_out, 16) || q_stride % 8 || q_out_stride % 8 || !aligned(positions, 4)) return SDV_ERR_ALIGN;
+  if (k_heads > 0 && (!aligned(k, 16) || !aligned(k_out, 16) || k_stride % 8 || k_out_stride % 8)) return SDV_ERR_ALIGN;
+  if (rows == 0) return SDV_OK;
+  const RopeRows a = {{inv_freq, rotary_dim / 16, scale, inverse ? -1.0f : 1.0f}, positions, rows,
+                      {static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k)},
+                      {static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_out)}, {q_stride, k_stride}, {q_out_stride, k_out_stride},
+                      {q_heads, k_heads}};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (head_dim == 128)
+    interleaved ? rope_launch<128, true>(a, s) : rope_launch<128, false>(a, s);
+  else
+    interleaved ? rope_launch<64, true>(a, s) : rope_launch<64, false>(a, s);
+  return hipGetLastError() == hipSuccess ? SDV_OK : SDV_ERR_HIP;
+}
+
+template <int D, int FMT>
+static void kv8_rope_launch(const Kv8RopeArgs& a, bool interleaved, dim3 grid, hipStream_t st) {
+  if (interleaved)
+    hipLaunchKernelGGL((kv8_rope_append_kernel<D, FMT, true>), grid, dim3(kWave), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv8_rope_append_kernel<D, FMT, false>), grid, dim3(kWave), 0, st, a);
+}
+
+extern "C" int sdv_kv8_rope_append(const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int32_t q_heads,
+                                   const void* k_new, const void* v_new, int64_t k_stride, int64_t v_stride, int32_t total_rows,
+                                   void* k_pages, void* v_pages, float* scales, int32_t num_blocks, int32_t format,
+                                   const int32_t* block_table, int32_t max_blocks_per_seq, const int32_t* cu_rows,
+                                   const int32_t* seq_lens, int32_t max_seq_len, int32_t batch, int32_t kv_heads, int32_t head_dim,
+                                   const int32_t* positions, const double* inv_freq, int32_t rotary_dim, int32_t interleaved,
+                                   float scale, void* stream) {
+  if (!q || !q_out) return SDV_ERR_NULL;
+  if (!seq_lens && max_seq_len <= 0) return SDV_ERR_SHAPE;
+  int st = kv8_cache_check(k_new, v_new, k_stride, v_stride, total_rows, k_pages, v_pages, scales, num_blocks, format, block_table,
+                           max_blocks_per_seq, cu_rows, seq_lens, batch, kv_heads, head_dim);
+  if (st != SDV_OK) return st;
+  st = rope_check(inv_freq, rotary_dim, interleaved, head_dim);
+  if (st != SDV_OK) return st;
+  if (q_heads <= 0 || q_heads > 65535 || kv_heads > 32767) return SDV_ERR_SHAPE;
+  const int64_t row = (int64_t)q_heads * head_dim;
+  if (q_stride < row || q_out_stride < row) return SDV_ERR_SHAPE;
+  if (!aligned(q, 16) || !aligned(q_out, 16) || q_stride % 8 || q_out_stride % 8 || !aligned(positions, 4)) return SDV_ERR_ALIGN;
+  if (total_rows == 0) return SDV_OK;
+  const Kv8RopeArgs a = {kv8_cache_args(const_cast<void*>(k_new), const_cast<void*>(v_new), k_stride, v_stride, total_rows, k_pages,
+                                        v_pages, scales, num_blocks, block_table, max_blocks_per_seq, cu_rows, seq_lens, max_seq_len,
+                                        batch, kv_heads),
+                         {inv_freq, rotary_dim / 16, scale, 1.0f}, positions, static_cast<const uint16_t*>(q),
+                         static_cast<uint16_t*>(q_out), q_stride, q_out_stride, q_heads};
+  dim3 grid = kv8_cache_grid(total_rows, batch, kv_heads);
+  grid.y += (unsigned)((q_heads + kRopeHeads - 1) / kRopeHeads);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (head_dim == 128)
+    format == SDV_KV8_FP8 ? kv8_rope_launch<128, kFp8>(a, interleaved, grid, s) : kv8_rope_launch<128, kInt8>(a, interleaved, grid, s);
+  else
+    format == SDV_KV8_FP8 ? kv8_rope_launch<64, kFp8>(a, interleaved, grid, s) : kv8_rope_launch<64, kInt8>(a, interleaved, grid, s);
+  return hipGetLastError() == hipSuccess ? SDV_OK : SDV_ERR_HIP;
+}

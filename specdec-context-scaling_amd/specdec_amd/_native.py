@@ -80,6 +80,14 @@ SIGNATURES = {
                                          _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ, _P, _I64, _P]),
     "sdv_kv8_attention_slot": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I32, _I32,
                                               _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ, _I32, _P, _I64, _P]),
+    "sdv_rope": (ctypes.c_int, [_P, _I64, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, ctypes.c_float, _I32, _I32, _I32,
+                                _P, _I64, _P, _I64, _P]),
+    "sdv_kv8_rope_append": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _P, _P, _I64, _I64, _I32, _P, _P, _P, _I32, _I32,
+                                           _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _P, _P, _I32, _I32, ctypes.c_float,
+                                           _P]),
+    "sdv_copy_blocks": (ctypes.c_int, [_P, _P, _P, _I32, _P, _P, _P, _I32, _I64, _I64, _I64, _I32, _P, _P, _I32, _P]),
+    "sdv_kv8_keep": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I64, _I64, _I32, _P, _I32, _P, _P, _I32, _P, _I32, _I32,
+                                    _I32, _P]),
     "sdv_fp8_encode": (ctypes.c_int, [_P, _P, _I64, _P]),
     "sdv_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "sdv_abi_version": (ctypes.c_int, []),
@@ -139,8 +147,9 @@ def binding():
                 raise SdvError(f"{LIB_PATH.parent / '_kv8_binding.so'} is not built ({e}); run `python -m specdec_amd.build` "
                                f"(or __graft_entry__.build()) on a machine with hipcc") from e
             _BINDING = _kv8_binding
-        _BINDING.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
-                        ("sdv_kv8_append", "sdv_kv8_gather", "sdv_kv8_attention_slot", "sdv_kv8_attention_workspace_size")))
+        at = lambda *names: (ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names)  # noqa: E731
+        _BINDING.bind(*at("sdv_kv8_append", "sdv_kv8_gather", "sdv_kv8_attention_slot", "sdv_kv8_attention_workspace_size"))
+        _BINDING.bind_moves(*at("sdv_rope", "sdv_kv8_rope_append", "sdv_copy_blocks", "sdv_kv8_keep"))
         _BOUND = lib
     return _BINDING
 

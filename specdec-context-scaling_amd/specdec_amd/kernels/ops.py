@@ -19,12 +19,17 @@ Operators
 ``kv8_gather``        the 8-bit cache read back into packed BF16 rows.
 ``kv8_attention``     ragged query rows (single tokens, verify blocks or trees, prompt chunks,
                       or all in one batch) over the 8-bit cache.
+``rope``              rotary positions of packed query and key rows (``rope_frequencies``: what it turns by).
+``kv8_rope_append``   a step's rows in one launch: q rotated, K rotated and quantized, V quantized.
+``copy_blocks``       whole page blocks of every layer copied, within a pool of either cache or to another.
+``kv8_keep``          the 8-bit cache: an accepted path's tokens moved together, in every layer.
 ``fp8_encode``        elementwise fp32 -> E4M3FN on the device.
 """
 from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 import weakref
 
@@ -825,6 +830,227 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     return out
 
 
+# ---------------------------------------------------------------------------- positions and page moves
+def rope_frequencies(head_dim: int, base: float = 1000000.0, *, rotary_dim: int | None = None, scaling: dict | None = None,
+                     device="cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq, scale) for ``rope`` and ``kv8_rope_append``: float64 (rotary_dim / 2,) radians per position, base^(-2i / rotary_dim)
+    for pair i, and what cos and sin are multiplied by.
+
+    scaling stretches a context: {"type": "linear", "factor": f} divides all frequencies by f; {"type": "ntk", "factor": f}
+    raises the base so that the slowest pair's is divided by f and the fastest stays; {"type": "yarn", "factor": f,
+    "original": n, "slow": 1, "fast": 32} (Peng et al., arXiv:2309.00071) divides those that turn less than `slow` times in n
+    positions, leaves those that turn more than `fast` times, goes over between them in proportion to the turns, and has scale
+    0.1 ln f + 1.
+    """
+    r = head_dim if rotary_dim is None else int(rotary_dim)
+    if not 0 < r <= head_dim or r % 16:
+        raise ValueError(f"rotary_dim must be a multiple of 16 up to {head_dim} (got {r})")
+    if base <= 0:
+        raise ValueError(f"base must be positive (got {base})")
+    scaling = dict(scaling or {"type": "none"})
+    kind, factor, scale = scaling.pop("type", None), float(scaling.pop("factor", 1.0)), 1.0
+    if factor < 1:
+        raise ValueError(f"factor must be at least 1 (got {factor})")
+    more = {k: float(scaling.pop(k, v)) for k, v in {"original": 0.0, "slow": 1.0, "fast": 32.0}.items()} if kind == "yarn" else {}
+    if scaling:
+        raise ValueError(f"scaling {kind!r} does not take {sorted(scaling)}")
+    if kind == "ntk":
+        base = base * factor ** (r / (r - 2))
+    inv = base ** (-torch.arange(0, r, 2, dtype=torch.float64) / r)
+    if kind == "linear":
+        inv = inv / factor
+    elif kind == "yarn":
+        if more["original"] <= 0 or not more["slow"] < more["fast"]:
+            raise ValueError("yarn needs the original context length, and slow < fast")
+        turns = more["original"] * inv / (2 * math.pi)
+        stays = ((turns - more["slow"]) / (more["fast"] - more["slow"])).clamp(0, 1)
+        inv = inv / factor * (1 - stays) + inv * stays
+        scale = 0.1 * math.log(factor) + 1
+    elif kind not in ("none", "ntk"):
+        raise ValueError(f"scaling type must be linear, ntk or yarn (got {kind!r})")
+    return inv.to(device), scale
+
+
+def _frequencies(inv_freq, dev, d) -> int:
+    """The rotated dimensions that inv_freq stands for, checked."""
+    _need(inv_freq, "inv_freq", (torch.float64,), dev, (1,))
+    n = 2 * inv_freq.shape[0]
+    if not 0 < n <= d or n % 16:
+        _fail(f"inv_freq {tuple(inv_freq.shape)} stands for {n} dimensions: a multiple of 16 up to {d} is needed")
+    return n
+
+
+def _same_rows(t, n, name):
+    if t.shape[0] != n:
+        _fail(f"{name} {tuple(t.shape)} needs {n} rows")
+    return t
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
+         scale: float = 1.0, inverse: bool = False, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Rotary positions: (q, k) rotated, BF16 (rows, heads, D) each (k may be None), D 64 or 128.
+
+    q and k: rows of any stride that is a multiple of 8 elements (parts of a projection's output as they lie).  positions int32
+    (rows,).  inv_freq float64 (r/2,), scale: see rope_frequencies.  Of a head's first r dimensions pair i is (i, i + r/2), or
+    (2i, 2i + 1) if interleaved: it becomes scale (x cos t - y sin t, x sin t + y cos t), t = position * inv_freq[i], computed
+    in fp32 from an angle in 64 bits and rounded once.  inverse: rotated back (the transpose, as a gradient takes it).  q_out
+    and k_out, which may be q and k themselves (no other overlap): written there.
+    """
+    if q_out is None and k_out is None:
+        got = _native.binding().rope(q, k, positions, inv_freq, interleaved, scale, inverse)
+        if got is not None:
+            if got.__class__ is int:
+                _native.check(got, "sdv_rope")
+            return got
+    if not isinstance(q, torch.Tensor):
+        _fail("q must be a tensor")
+    dev = q.device
+    if dev.type != "cuda":
+        _fail(f"q must be on a HIP device (got {dev})")
+    q, qs = _kv8_rows(q, "q", dev)
+    n, H, d = q.shape
+    if d not in (64, 128):
+        _fail(f"head_dim must be 64 or 128 (got {d})")
+    r = _frequencies(inv_freq, dev, d)
+    pos = _kv8_ints(positions, "positions", dev, n)
+    outs = [torch.empty((n, H, d), dtype=torch.bfloat16, device=dev) if q_out is None else q_out]
+    outs[0], qos = _kv8_rows(_same_rows(outs[0], n, "q_out"), "q_out", dev, H, d, write=True)
+    kp = kop = None
+    ks = kos = kh = 0
+    if k is not None:
+        k, ks = _kv8_rows(k, "k", dev, None, d)
+        kh = _same_rows(k, n, "k").shape[1]
+        outs.append(torch.empty((n, kh, d), dtype=torch.bfloat16, device=dev) if k_out is None else k_out)
+        outs[1], kos = _kv8_rows(_same_rows(outs[1], n, "k_out"), "k_out", dev, kh, d, write=True)
+        kp, kop = k.data_ptr(), outs[1].data_ptr()
+    elif k_out is not None:
+        _fail("k_out without k")
+    else:
+        outs.append(None)
+    if n and H:
+        _kv8_call(_native.load().sdv_rope, "sdv_rope", dev, q.data_ptr(), qs, H, kp, ks, kh, pos, inv_freq.data_ptr(), r,
+                  int(bool(interleaved)), float(scale), int(bool(inverse)), n, d, outs[0].data_ptr(), qos, kop, kos)
+    return tuple(outs)
+
+
+def kv8_rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    scales: torch.Tensor, block_table: torch.Tensor, cu_rows: torch.Tensor, seq_lens: torch.Tensor | None,
+                    max_seq_len: int, inv_freq: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0,
+                    positions: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """A step's rows in one launch: q rotated (returned, BF16 (total, H, D)), k_new rotated and written into the 8-bit cache, v_new written.
+
+    The arguments of kv8_append, and those of rope; positions int32 (total,) where a row's is not the one that it is written
+    at (a tree's nodes), else None.  K is quantized as it is rotated, in fp32: its codes are one rounding nearer to the rotated
+    values than those of rope and then kv8_append.  q_out: written there, which may be q itself; rows behind cu_rows[B] of it are not.
+    """
+    if q_out is None:
+        got = _native.binding().rope_append(q, k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len, inv_freq,
+                                            interleaved, scale, positions)
+        if got is not None:
+            if got.__class__ is int:
+                _native.check(got, "sdv_kv8_rope_append")
+            return got
+    dev = _kv8_device(k_pages)
+    nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
+    q, qs = _kv8_rows(q, "q", dev, None, d)
+    total, H = q.shape[:2]
+    k_new, ks = _kv8_rows(k_new, "k_new", dev, kv, d)
+    v_new, vs = _kv8_rows(v_new, "v_new", dev, kv, d)
+    _same_rows(k_new, total, "k_new")
+    _same_rows(v_new, total, "v_new")
+    if H == 0:
+        _fail(f"q {tuple(q.shape)} has no heads")
+    B, mb = block_table.shape
+    max_seq_len = int(max_seq_len)
+    if seq_lens is None and max_seq_len <= 0:
+        _fail("seq_lens None needs max_seq_len")
+    cu = _kv8_ints(cu_rows, "cu_rows", dev, B + 1)
+    lens = None if seq_lens is None else _kv8_ints(seq_lens, "seq_lens", dev, B)
+    pos = None if positions is None else _kv8_ints(positions, "positions", dev, total)
+    r = _frequencies(inv_freq, dev, d)
+    out = torch.empty((total, H, d), dtype=torch.bfloat16, device=dev) if q_out is None else q_out
+    out, os_ = _kv8_rows(_same_rows(out, total, "q_out"), "q_out", dev, H, d, write=True)
+    if total == 0:
+        return out
+    _kv8_call(_native.load().sdv_kv8_rope_append, "sdv_kv8_rope_append", dev, q.data_ptr(), qs, out.data_ptr(), os_, H, k_new.data_ptr(),
+              v_new.data_ptr(), ks, vs, total, k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), nb, fmt, block_table.data_ptr(),
+              mb, cu, lens, max_seq_len, B, kv, d, pos, inv_freq.data_ptr(), r, int(bool(interleaved)), float(scale))
+    return out
+
+
+def _blocks_of(k, v, s, what, dev=None):
+    """(layers, blocks, bytes of a block of each) of page tensors of either cache, checked."""
+    _need(k, f"{what}k_pages", (torch.bfloat16, torch.float8_e4m3fn, torch.int8), dev)
+    dev = k.device
+    _need(v, f"{what}v_pages", (torch.uint8, torch.float8_e4m3fn, torch.int8), dev, (4, 5))
+    _need(s, f"{what}scales", (torch.float32,), dev)
+    lead = v.dim() - 4
+    front = v.shape[:lead + 2]
+    if k.shape[:lead + 2] != front or s.shape[:lead + 2] != front or min(front) <= 0:
+        _fail(f"{what}pages disagree: k {tuple(k.shape)}, v {tuple(v.shape)}, scales {tuple(s.shape)}")
+    layers, nb = (front[0] if lead else 1), front[lead]
+    return layers, nb, [t.numel() // (layers * nb) * t.element_size() for t in (k, v, s)]
+
+
+def copy_blocks(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *,
+                to: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None) -> None:
+    """Copy whole page blocks, of one layer or of all at once: block src[i] to block dst[i], int32 (n,) each on the device.
+
+    The page tensors of either cache, ([layers,] num_blocks, KV, ...).  to: the page tensors of another pool with the same layers
+    and block shapes, which dst then names the blocks of.  Pairs that name no block are skipped.  No block may be the
+    destination of two pairs, or of one and the source of another.
+    """
+    other = (k_pages, v_pages, scales) if to is None else tuple(to)
+    if len(other) != 3:
+        _fail("`to` needs K pages, V pages and scales")
+    st = _native.binding().copy_blocks(k_pages, v_pages, scales, src, dst, *other)
+    if st is not None:
+        if st:
+            _native.check(st, "sdv_copy_blocks")
+        return
+    layers, nb, size = _blocks_of(k_pages, v_pages, scales, "")
+    dev = k_pages.device
+    layers_to, nb_to, size_to = _blocks_of(*other, "to's ", dev)
+    lead = v_pages.dim() - 4
+    if layers != layers_to or any(x.dtype is not y.dtype or x.dim() != y.dim() or x.shape[lead + 1:] != y.shape[lead + 1:]
+                                  for x, y in zip((k_pages, v_pages, scales), other)):
+        _fail("`to` has other layers, types or block shapes")
+    _need(src, "src", (torch.int32,), dev, (1,))
+    n = src.shape[0]
+    a, b = _kv8_ints(src, "src", dev, n), _kv8_ints(dst, "dst", dev, n)
+    if n:
+        _kv8_call(_native.load().sdv_copy_blocks, "sdv_copy_blocks", dev, k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), nb,
+                  *(t.data_ptr() for t in other), nb_to, *size, layers, a, b, n)
+
+
+def kv8_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, cu_kept: torch.Tensor,
+             kept: torch.Tensor, starts: torch.Tensor) -> None:
+    """Keep some of the 8-bit cache's last tokens and close the gaps between them, in place, in one layer or in all of them.
+
+    The token at position starts[b] + kept[cu_kept[b] + i] of sequence b comes to position starts[b] + i: after the verify of a
+    drafted tree, kept are the accepted path's nodes and starts the contexts before it.  int32 on the device: cu_kept (B + 1,),
+    kept (total,), starts (B,).  Pages as for kv8_append, or with a leading layer dimension.  Up to 64 tokens of a sequence are
+    all read before any is written, whatever their order; of more the entries must ascend.  A token whose source or destination the
+    table does not hold stays.  Sequences whose moved tokens share blocks must not be in one call.
+    """
+    st = _native.binding().keep(k_pages, v_pages, scales, block_table, cu_kept, kept, starts)
+    if st is not None:
+        if st:
+            _native.check(st, "sdv_kv8_keep")
+        return
+    layers, nb, _ = _blocks_of(k_pages, v_pages, scales, "")
+    dev = k_pages.device
+    layered = v_pages.dim() == 5
+    one = [t[0] if layered else t for t in (k_pages, v_pages, scales)]
+    nb, kv, d, _ = _kv8_pages(*one, block_table, dev)
+    B, mb = block_table.shape
+    _need(kept, "kept", (torch.int32,), dev, (1,))
+    cu, first = _kv8_ints(cu_kept, "cu_kept", dev, B + 1), _kv8_ints(starts, "starts", dev, B)
+    if kept.shape[0]:
+        _kv8_call(_native.load().sdv_kv8_keep, "sdv_kv8_keep", dev, k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), nb,
+                  *(t.numel() for t in one), layers, block_table.data_ptr(), mb, cu, kept.data_ptr(), kept.shape[0], first, B, kv, d)
+
+
 # ---------------------------------------------------------------------------- torch.library
 # The ops as torch custom operators (namespace "sdv"), so torch.compile and fake-tensor tracing
 # see them: the real implementations are the functions above (the C ABI through ctypes); the
@@ -914,3 +1140,50 @@ def _lib_kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
 @_lib_kv8_attention.register_fake
 def _(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale=None, tree_mask=None):
     return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("sdv::rope", mutates_args=())
+def _lib_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False,
+              scale: float = 1.0, inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    return rope(q, k, positions, inv_freq, interleaved=interleaved, scale=scale, inverse=inverse)
+
+
+@_lib_rope.register_fake
+def _(q, k, positions, inv_freq, interleaved=False, scale=1.0, inverse=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("sdv::kv8_rope_append", mutates_args=("k_pages", "v_pages", "scales"))
+def _lib_kv8_rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                         scales: torch.Tensor, block_table: torch.Tensor, cu_rows: torch.Tensor, seq_lens: torch.Tensor | None,
+                         max_seq_len: int, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0,
+                         positions: torch.Tensor | None = None) -> torch.Tensor:
+    return kv8_rope_append(q, k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len, inv_freq,
+                           interleaved=interleaved, scale=scale, positions=positions)
+
+
+@_lib_kv8_rope_append.register_fake
+def _(q, k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len, inv_freq, interleaved=False, scale=1.0,
+      positions=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("sdv::copy_blocks", mutates_args=("k_pages", "v_pages", "scales"))
+def _lib_copy_blocks(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    copy_blocks(k_pages, v_pages, scales, src, dst)
+
+
+@_lib_copy_blocks.register_fake
+def _(k_pages, v_pages, scales, src, dst):
+    return None
+
+
+@torch.library.custom_op("sdv::kv8_keep", mutates_args=("k_pages", "v_pages", "scales"))
+def _lib_kv8_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, cu_kept: torch.Tensor,
+                  kept: torch.Tensor, starts: torch.Tensor) -> None:
+    kv8_keep(k_pages, v_pages, scales, block_table, cu_kept, kept, starts)
+
+
+@_lib_kv8_keep.register_fake
+def _(k_pages, v_pages, scales, block_table, cu_kept, kept, starts):
+    return None
