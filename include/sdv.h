@@ -403,6 +403,30 @@ int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const void* k_pages,
                            int32_t max_seq_len, float scale, void* workspace, size_t workspace_bytes, int32_t slot,
                            void* out, int64_t out_stride, void* stream);
 
+/*
+ * sdv_kv8_attention for sequences that begin with the same pages, which are read and computed once for all of them.
+ * Group g is sequences cu_groups[g] .. cu_groups[g+1] - 1 (int32 [groups + 1], must not decrease; sequences may be in no
+ * group).  prefix_lens, int32 [batch], the same for a group's sequences: the first prefix_lens[b] tokens, taken down to
+ * whole blocks (and to max_prefix_len), are the blocks that the table names for the group's first sequence.  Every row
+ * of the group sees all of them, and of its own sequence the keys from there on that sdv_kv8_attention has it see: with
+ * prefixes within the contexts (prefix_lens[b] <= seq_lens[b] - rows) the result is that of sdv_kv8_attention.
+ * A sequence in no group whose prefix_lens is not 0 does not see those keys at all.  groups may be 0.
+ * Tiles have 16 or 32 rows, sums and operands as there.  max_q_len chooses between them (a sequence with more rows is
+ * computed all the same).  The workspace may hold anything and nothing carries over.  max_prefix_len is at most
+ * 16 * max_blocks_per_seq; size limits as for sdv_kv8_attention, with max_prefix_len added to max_seq_len.
+ */
+size_t sdv_kv8_shared_attention_workspace_size(int32_t batch, int32_t groups, int32_t total_rows, int32_t q_heads,
+                                               int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
+                                               int32_t max_seq_len, int32_t max_prefix_len);
+int sdv_kv8_shared_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                             const float* scales, int32_t num_blocks, int32_t format, const int32_t* block_table,
+                             int32_t max_blocks_per_seq, const int32_t* cu_rows, const int32_t* seq_lens,
+                             const uint64_t* tree_mask, const int32_t* cu_groups, const int32_t* prefix_lens,
+                             int32_t batch, int32_t groups, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
+                             int32_t head_dim, int32_t max_q_len, int32_t max_seq_len, int32_t max_prefix_len,
+                             float scale, void* workspace, size_t workspace_bytes, void* out, int64_t out_stride,
+                             void* stream);
+
 /* ------------------------------------------------------------------ positions, page moves
  *
  * Rotary positions.  The first rotary_dim dimensions of a head are pairs (x, y): (i, i + rotary_dim / 2), or

@@ -29,6 +29,8 @@ decltype(&sdv_rope) g_rope;
 decltype(&sdv_kv8_rope_append) g_rope_append;
 decltype(&sdv_copy_blocks) g_copy;
 decltype(&sdv_kv8_keep) g_keep;
+decltype(&sdv_kv8_shared_attention) g_shared;
+decltype(&sdv_kv8_shared_attention_workspace_size) g_shared_size;
 
 // A tensor of no subclass (whose data might not be where it says), or nullptr.
 const at::Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -416,6 +418,56 @@ PyObject* keep(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// shared(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups, prefix_lens,
+//        max_prefix_len, scale, tree_mask, out = None) -> out or status
+PyObject* shared(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages p;
+  int64_t q_row, out_row, max_q, max_len, max_prefix;
+  const int32_t *cu, *lens, *groups, *prefix;
+  if (!g_shared || (n != 14 && n != 15) || !pages(o + 1, p) || !whole(o[7], max_q) || !whole(o[8], max_len) || !whole(o[11], max_prefix)) Py_RETURN_NONE;
+  const at::Tensor *q = rows(o[0], p, 0, q_row), *cg = tensor(o[9]);
+  if (!q || !ints(o[5], p, p.batch + 1, cu) || !lengths(o[6], p, lens) || !cg || cg->dim() != 1 || cg->size(0) < 1 || cg->size(0) > p.batch + 1 ||
+      !ints(o[9], p, cg->size(0), groups) || !ints(o[10], p, p.batch, prefix))
+    Py_RETURN_NONE;
+  const int64_t total = q->size(0), heads = q->size(1);
+  double scale = 1.0 / std::sqrt((double)p.d);
+  if (o[12] != Py_None && !real(o[12], scale)) Py_RETURN_NONE;
+  const uint64_t* tree = nullptr;
+  if (o[13] != Py_None) {
+    const at::Tensor* t = tensor(o[13]);
+    if (!t || max_q > 64 || t->dim() != 1 || t->size(0) != total ||
+        !fits(*t, p.device, t->scalar_type() == at::kUInt64 ? at::kUInt64 : at::kLong))
+      Py_RETURN_NONE;
+    tree = static_cast<const uint64_t*>(t->data_ptr());
+  }
+  const int32_t ng = (int32_t)cg->size(0) - 1;
+  const size_t bytes = g_shared_size(p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix);
+  if (bytes == 0) Py_RETURN_NONE;  // sizes that the general path refuses
+  const at::Tensor* given = nullptr;
+  if (n == 15 && o[14] != Py_None) {
+    given = rows(o[14], p, heads, out_row);
+    if (!given || given->size(0) != total) Py_RETURN_NONE;
+  }
+  Launch on(p);
+  at::Tensor out;
+  if (!given) {
+    out = at::empty({total, heads, p.d}, q->options());
+    out_row = heads * p.d;
+  }
+  const c10::DataPtr ws = c10::hip::HIPCachingAllocator::get()->allocate(bytes);
+  const int st = g_shared(q->data_ptr(), q_row, p.k, p.v, p.s, p.blocks, p.format, p.table, p.max_blocks, cu, lens, tree, groups, prefix,
+                          p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix,
+                          (float)scale, ws.get(), bytes, given ? given->data_ptr() : out.data_ptr(), out_row, on.stream);
+  if (st != SDV_OK) return status(st);
+  if (given) {
+    Py_INCREF(o[14]);
+    return o[14];
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 bool addresses(PyObject* const* o, Py_ssize_t n, void** at) {
   for (Py_ssize_t i = 0; i < n; ++i) {
     at[i] = PyLong_AsVoidPtr(o[i]);
@@ -439,6 +491,19 @@ PyObject* bind_moves(PyObject*, PyObject* const* o, Py_ssize_t n) {
   g_rope_append = reinterpret_cast<decltype(g_rope_append)>(at[1]);
   g_copy = reinterpret_cast<decltype(g_copy)>(at[2]);
   g_keep = reinterpret_cast<decltype(g_keep)>(at[3]);
+  Py_RETURN_NONE;
+}
+
+// bind_shared(shared_attention, its workspace_size)
+PyObject* bind_shared(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  void* at[2];
+  if (n != 2) {
+    PyErr_SetString(PyExc_TypeError, "bind_shared needs two addresses");
+    return nullptr;
+  }
+  if (!addresses(o, n, at)) return nullptr;
+  g_shared = reinterpret_cast<decltype(g_shared)>(at[0]);
+  g_shared_size = reinterpret_cast<decltype(g_shared_size)>(at[1]);
   Py_RETURN_NONE;
 }
 
@@ -467,6 +532,8 @@ PyMethodDef methods[] = {
     {"copy_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(copy_blocks)), METH_FASTCALL, nullptr},
     {"keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(keep)), METH_FASTCALL, nullptr},
     {"bind_moves", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind_moves)), METH_FASTCALL, nullptr},
+    {"shared", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(shared)), METH_FASTCALL, nullptr},
+    {"bind_shared", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind_shared)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kv8_binding", nullptr, -1, methods};

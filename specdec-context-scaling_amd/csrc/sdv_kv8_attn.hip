@@ -8,64 +8,12 @@
 // the second product: e^(..) s^V to 16 bits here, e^(..) and s^V c^V to FP16 in the kernel for many
 // rows.  (With e^(..) s^V as one BF16 operand, 2^-9 of each term, the outputs' error against 64 bits
 // was 2.7e-3, of which BF16 outputs alone make 1.6e-3.)
-#include "sdv_kv8_plan.h"
+#include "sdv_kv8_rows.h"
 
 namespace sdv {
 
-// The value of lane `P` of each group of four lanes.
-template <int P>
-__device__ __forceinline__ float quad_lane(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), P * 0x55, 0xF, 0xF, true));
-}
-
-__device__ __forceinline__ float4 quad_lane4(float4 v, int p) {  // p is a constant after unrolling
-  switch (p) {
-    case 0: return make_float4(quad_lane<0>(v.x), quad_lane<0>(v.y), quad_lane<0>(v.z), quad_lane<0>(v.w));
-    case 1: return make_float4(quad_lane<1>(v.x), quad_lane<1>(v.y), quad_lane<1>(v.z), quad_lane<1>(v.w));
-    case 2: return make_float4(quad_lane<2>(v.x), quad_lane<2>(v.y), quad_lane<2>(v.z), quad_lane<2>(v.w));
-    default: return make_float4(quad_lane<3>(v.x), quad_lane<3>(v.y), quad_lane<3>(v.z), quad_lane<3>(v.w));
-  }
-}
-
-// Bits of a dword's bytes 4w..4w+3 that belong to the first n tokens of a block.
-__device__ __forceinline__ uint32_t kv8_keep(int n, int w) {
-  const int k = n - 4 * w;
-  return k >= 4 ? ~0u : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
-}
-
-// A running maximum is moved only by a score more than 2^8 times its exponential: until then the
-// probabilities are at most 2^8, and BF16 and fp32 hold them as exactly as they hold those below 1.
-constexpr float kKv8Slack = 8.0f;
-
-// Sums of up to 2^30 terms of 2^8 |V| pass fp32's range where V's scales are above 2^81.  From the first
-// scale of 2^64 on a wavefront takes its maxima to be 2^48 times as large: its sums are that much smaller
-// then, and the least probability that counts is 2^-78 (2^-126 otherwise).  Looking for one costs a call
-// over 2048 keys 0.1 us of 7.8.
-constexpr float kKv8LargeScale = 18446744073709551616.0f, kKv8Raise = 48.0f;
-
-constexpr int kKv8Threads = 256;  // of the kernel for few rows
-constexpr int kKv8Grid = 512;     // its workgroups: two per CU
-
 // Counts of finished parts, per slot and range; every call leaves its slot's zero, as the loader does.
 static __device__ uint32_t kv8_counts[SDV_KV8_SLOTS][kKv8Grid];
-
-// The maximum that stands for a row none of whose scores of keys lo .. hi - 1 is above -inf: -inf where
-// it sees none of the keys, the lowest finite number where it does (scores of an infinite q, or NaN).  Both
-// sums are 0 or NaN; over all keys the first is an output of 0 and the second 0 / 0.  Looked for block by
-// block, since it hardly ever comes to this: keys up to the row's own position, or the context and its
-// mask's tokens, in blocks that the table names.  (As a check of each output's sum in kv8_write and the
-// merges the code that this takes made a call over 2048 keys 0.2 us longer, 7.7 to 7.9.)
-__device__ __forceinline__ float kv8_lowest(const Kv8AttnArgs& a, int b, const Kv8Seq& s, int tok, int lo, int hi) {
-  const int last = min(s.tree ? s.ctx - 1 : s.ctx + tok, hi - 1);
-  bool any = false;
-  for (int j = lo / kBlock; !any && j < a.r.max_blocks && j * kBlock <= last; ++j) any = kv8_block(a.r, b, j) >= 0;
-  if (s.tree) {
-    const uint64_t bits = a.tree[s.first + tok];
-    for (int j = max(lo - s.ctx, 0); !any && j < min(min(hi - s.ctx, s.n), 64); ++j)
-      any = ((bits >> j) & 1) != 0 && kv8_block(a.r, b, (s.ctx + j) >> 4) >= 0;
-  }
-  return any ? -3.4028235e38f : -INFINITY;
-}
 
 // ---------------------------------------------------------------------------- shared tiles
 // The parts of a tile that several ranges share: each workgroup leaves its sums in a slot of the
@@ -180,44 +128,16 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttnArgs& a, __amdgpu_buffer_
     if (tid + i * kKv8Threads < t.rows * (D / 4)) kv8_write<D>(a, t, row[i], 4 * (piece[i] % (D / 4)), acc[i], mm[i], ll[i]);
 }
 
-// ---------------------------------------------------------------------------- few rows
-// Tiles of 16 or 32 rows: single tokens and verify blocks.  Each of a workgroup's four wavefronts
-// streams every fourth step of the tile with all of its rows; their sums meet in LDS at its end.
-//
-// A wavefront's step is four page blocks, or two where it has two row tiles (with four their registers
-// do not leave two wavefronts a SIMD: 32 sequences of 2048 to 32768 keys, five rows each, 95 us, so 77).  S^T = K Q^T on
-// v_mfma_f32_16x16x32_bf16: of four blocks, MFMA p takes tokens 4p..4p+3 of each as its 16 key rows, so
-// that lane (n, g) of its result holds row n and tokens 4p + r of block g, and after all four MFMAs every
-// token of block g: with the 16 tokens as its k-slots that is the B operand of O^T = V^T P^T as it stands
-// (A: lane (d, g) the 16 codes of dimension d in block g, one 16-byte load).  Of two blocks, lane group
-// g has tokens 8 (g % 2) + 4p + r of block g / 2.  The matrix cores have time to spare here, so P goes
-// in as two BF16 operands, the rounded value and what the rounding left (16 bits in all), over BF16's
-// whole range of scales.
-//
-// Long batches are bound by memory: single tokens of 32 sequences of 2048 to 32768 keys (293 MB of pages,
-// 2 KV heads of 128) take 55 to 57 us, 5.2 TB/s, a large copy's rate; the matrix cores are busy a tenth of
-// it.  Short calls are bound by latencies, each a microsecond or more: lengths, page ids, the pages,
-// the merge's count, and the parts.  One token over 2048 keys takes 7.5 us, over 32768 18.5.
 template <int D, int FMT, int RT>
 __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a) {
-  constexpr int TR = 16 * RT, KI = D / 64, KS = D / 32, DT = D / 16;
-  constexpr int kWaves = kKv8Threads / kWave, kRow = D + 4, kPart = TR * (D + 4);
-  constexpr int PG = RT == 1 ? 4 : 2;  // page blocks of a wavefront's step, and MFMAs of its q.k^T
-  constexpr int NT = 4 * PG;           // a lane's tokens of them
-  __shared__ __align__(16) float lds_o[kWaves][TR][kRow];
-  __shared__ float lds_m[kWaves][TR], lds_l[kWaves][TR];
-  __shared__ __align__(16) uint16_t lds_q[RT == 1 ? 8 : TR * D];
+  constexpr int TR = 16 * RT, kPart = TR * (D + 4);
+  __shared__ Kv8RowsLds<D, RT> lds;
   __shared__ Kv8PlanLds<kKv8Threads> lds_plan;
-  static_assert(sizeof(lds_o) + sizeof(lds_m) + sizeof(lds_l) + sizeof(lds_q) + sizeof(lds_plan) <= 80 * 1024, "two workgroups per CU");
+  static_assert(sizeof(lds) + sizeof(lds_plan) <= 80 * 1024, "two workgroups per CU");
 
   Kv8Place<TR, kKv8Threads> at;
   if (!at.begin(a, lds_plan, (int)blockIdx.x, (int)gridDim.x)) return;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int n = lane & 15, g = lane >> 4;
-  const int64_t page_bytes = (int64_t)kBlock * D;
-  // the lane's place in a step: block and token of the key row that it loads, of the tokens that it holds
-  const int kblk = PG == 4 ? n >> 2 : n >> 3, vblk = PG == 4 ? g : g >> 1;
-  const int kpart = PG == 4 ? 0 : 2 * (n >> 2 & 1), vtok = PG == 4 ? 0 : 8 * (g & 1);
+  const int tid = threadIdx.x;
   bool first_part = true;
 
   for (;;) {
@@ -228,237 +148,8 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
     if (!at.part(a, s0, s1, steps)) break;  // the range ends within the tile's start
     const int row0 = at.i * TR, rows = min(seq.n * a.G - row0, TR);
 
-    const int32_t* table = a.r.table + (int64_t)b * a.r.max_blocks;
-    // block id of this lane's K and V block in a step; -1: none
-    const auto block_id = [&](int step, int k) {
-      const int j = step * PG + k;
-      const int id = table[min(j, a.r.max_blocks - 1)];
-      return j < a.r.max_blocks && id >= 0 && id < a.r.num_blocks ? id : -1;
-    };
-    int step = s0 * (4 / PG) + wave;
-    const int last = s1 * (4 / PG);
-    int idk = block_id(step, kblk), idv = block_id(step, vblk);
-    int idk_next = block_id(step + kWaves, kblk), idv_next = block_id(step + kWaves, vblk);
-
-    // query operand: lane (n, g), k-step 2i + h: dimensions (4i + g)*16 + 8h .. +7.  One row tile of it
-    // stays in registers; of two tiles it would not leave two wavefronts a SIMD, and lies in LDS.
-    bf16x8 qreg[RT == 1 ? KS : 1];
-    int lim[RT];          // last key that the row sees; with a tree, the context's last
-    uint64_t bits[RT];    // new tokens that it sees (tree)
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = row0 + 16 * rt + n, tok = r / a.G, head = r - tok * a.G;
-      const bool live = 16 * rt + n < rows;
-      const uint16_t* src = a.q + (int64_t)(seq.first + (live ? tok : 0)) * a.q_stride + (int64_t)(kvh * a.G + (live ? head : 0)) * D;
-      if constexpr (RT == 1) {
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk) qreg[kk] = *reinterpret_cast<const bf16x8*>(src + (4 * (kk >> 1) + g) * 16 + 8 * (kk & 1));
-      } else {
-        for (int kk = wave; kk < KS; kk += kWaves)
-          *reinterpret_cast<uint4*>(&lds_q[(rt * KS + kk) * 512 + lane * 8]) =
-              *reinterpret_cast<const uint4*>(src + (4 * (kk >> 1) + g) * 16 + 8 * (kk & 1));
-      }
-      lim[rt] = seq.tree ? seq.ctx - 1 : seq.ctx + (live ? tok : 0);
-      bits[rt] = seq.tree && live ? a.tree[seq.first + tok] : 0;
-    }
-    // keys up to here are seen by every row of the tile
-    const int all = seq.tree ? seq.ctx - 1 : seq.ctx + row0 / a.G;
-
-    f32x4 o[RT][DT];
-    float m[RT], l[RT], raise = 0.0f;  // raise: wave-uniform
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      m[rt] = -INFINITY;
-      l[rt] = 0.0f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    uint4 kw[PG][KI];
-    uint32_t vw[DT][PG];
-    float4 sk, sv, sk_next, sv_next;
-    const auto load_k = [&](int id) {
-      const uint8_t* src = a.k_pages + ((int64_t)max(id, 0) * a.kv_heads + kvh) * page_bytes + kpart * (4 * D) + g * 64 + (n & 3) * 16;
-#pragma unroll
-      for (int p = 0; p < PG; ++p)
-#pragma unroll
-        for (int i = 0; i < KI; ++i) kw[p][i] = load_stream16(src + p * (4 * D) + i * 256);
-    };
-    const auto load_s = [&](int id) {
-      const float* src = a.scales + ((int64_t)max(id, 0) * a.kv_heads + kvh) * (2 * kBlock) + vtok + 4 * (n & (PG - 1));
-      sk_next = *reinterpret_cast<const float4*>(src);
-      sv_next = *reinterpret_cast<const float4*>(src + kBlock);
-    };
-    const auto load_v = [&](int id) {
-      const uint8_t* src = a.v_pages + ((int64_t)max(id, 0) * a.kv_heads + kvh) * page_bytes + n * kBlock + vtok;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        if constexpr (PG == 4) {
-          const uint4 w = load_stream16(src + dt * (16 * kBlock));
-          vw[dt][0] = w.x;
-          vw[dt][1] = w.y;
-          vw[dt][2] = w.z;
-          vw[dt][3] = w.w;
-        } else {
-          const uint64_t w = __builtin_nontemporal_load(reinterpret_cast<const uint64_t*>(src + dt * (16 * kBlock)));
-          vw[dt][0] = (uint32_t)w;
-          vw[dt][1] = (uint32_t)(w >> 32);
-        }
-      }
-    };
-    if (step < last) {
-      load_k(idk);
-      load_s(idv);
-      load_v(idv);
-    }
-    if constexpr (RT > 1) __syncthreads();  // lds_q
-    for (; step < last; step += kWaves) {
-      sk = sk_next;
-      sv = sv_next;
-      f32x4 s[RT][PG];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int p = 0; p < PG; ++p) s[rt][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (RT > 1) asm volatile("" ::: "memory");  // the operand is read again each step
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        bf16x8 qop[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          if constexpr (RT == 1)
-            qop[rt] = qreg[kk];
-          else
-            qop[rt] = *reinterpret_cast<const bf16x8*>(&lds_q[(rt * KS + kk) * 512 + lane * 8]);
-        }
-#pragma unroll
-        for (int p = 0; p < PG; ++p) {
-          const uint4 w = kw[p][kk >> 1];
-          const bf16x8 kop = (kk & 1) ? kv8_bf16x8<FMT>(w.z, w.w) : kv8_bf16x8<FMT>(w.x, w.y);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qop[rt], s[rt][p], 0, 0, 0);
-        }
-      }
-      // The next step's K goes into the registers that are free now; the one after's block ids first, so
-      // that waiting for them later does not wait for the data in between.
-      const int idv_now = idv;
-      const bool more = step + kWaves < last;
-      if (more) {
-        idk = idk_next;
-        idv = idv_next;
-        idk_next = block_id(step + 2 * kWaves, kblk);
-        idv_next = block_id(step + 2 * kWaves, vblk);
-        load_k(idk);
-        load_s(idv);
-      }
-
-      const bool masked = (step + 1) * (PG * kBlock) - 1 > all || __any(idv_now < 0);
-      const int key0 = step * (PG * kBlock) + vblk * kBlock + vtok;  // this lane's first token
-      // which of this lane's tokens each of its rows sees
-      uint32_t vis[RT];
-      if (masked) {
-        const auto first = [](int k) { return (1u << min(max(k, 0), NT)) - 1u; };
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          vis[rt] = first(lim[rt] + 1 - key0);
-          const int sh = key0 - seq.ctx;  // the token behind bit 0 of the mask, from this lane's first
-          if (seq.tree && sh > -NT && sh < 64) vis[rt] |= (uint32_t)(sh >= 0 ? bits[rt] >> sh : bits[rt] << -sh) & first(seq.T - key0);
-          if (idv_now < 0) vis[rt] = 0;
-        }
-      }
-      const auto seen = [&](int rt, int t) { return ((vis[rt] >> t) & 1) != 0; };
-      if (masked) {  // codes behind the sequence's end, or of no block, may decode to NaN
-        const int valid = idv_now < 0 ? 0 : seq.T - key0;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-          for (int p = 0; p < PG; ++p) vw[dt][p] &= kv8_keep(valid, p);
-        }
-      }
-      const float raised = raise;
-      if (__any(fmaxf(fmaxf(sv.x, sv.y), fmaxf(sv.z, sv.w)) >= kKv8LargeScale)) raise = kKv8Raise;
-      constexpr int NH = PG / 2;  // p.V products per dimension tile, 32 tokens each
-      bf16x8 hi[RT][NH], lo[RT][NH];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float y[NT];
-#pragma unroll
-        for (int p = 0; p < PG; ++p) {
-          const float4 k4 = quad_lane4(sk, p);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) y[4 * p + r] = s[rt][p][r] * ((&k4.x)[r] * a.c);
-        }
-        if (masked) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) y[t] = seen(rt, t) ? y[t] : -INFINITY;
-        }
-        float mx = y[0];
-#pragma unroll
-        for (int t = 1; t < NT; ++t) mx = fmaxf(mx, y[t]);
-        if (__any(mx > m[rt] + kKv8Slack) || raise != raised) {
-          float2 pr = lane_pair<16>(mx);
-          mx = fmaxf(pr.x, pr.y);
-          pr = lane_pair<32>(mx);
-          mx = fmaxf(fmaxf(pr.x, pr.y), m[rt]);
-          const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mx + (raised - raise));
-          l[rt] *= f;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
-          m[rt] = mx;
-        }
-        const float ms = m[rt] == -INFINITY ? 0.0f : m[rt] + raise;
-        uint32_t wh[2 * PG], wl[2 * PG];
-#pragma unroll
-        for (int p = 0; p < PG; ++p) {
-          const float4 v4 = quad_lane4(sv, p);
-          float e[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float x = __builtin_amdgcn_exp2f(y[4 * p + r] - ms);
-            l[rt] += x;
-            e[r] = x * (&v4.x)[r];
-            // the scale of a token that the row does not see may be anything
-            if (masked) e[r] = seen(rt, 4 * p + r) ? e[r] : 0.0f;
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t w = pack_bf16x2(e[2 * h], e[2 * h + 1]);
-            wh[2 * p + h] = w;
-            wl[2 * p + h] = pack_bf16x2(e[2 * h] - bf16_lo(w), e[2 * h + 1] - bf16_hi(w));
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          hi[rt][h] = __builtin_bit_cast(bf16x8, make_uint4(wh[4 * h], wh[4 * h + 1], wh[4 * h + 2], wh[4 * h + 3]));
-          lo[rt][h] = __builtin_bit_cast(bf16x8, make_uint4(wl[4 * h], wl[4 * h + 1], wl[4 * h + 2], wl[4 * h + 3]));
-        }
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          const bf16x8 v = kv8_bf16x8<FMT>(vw[dt][2 * h], vw[dt][2 * h + 1]);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi[rt][h], o[rt][dt], 0, 0, 0);
-            o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo[rt][h], o[rt][dt], 0, 0, 0);
-          }
-        }
-      if (more) load_v(idv);
-    }
-
-    // the wavefronts' sums: lane (n, g) holds row n, dimensions 16 dt + 4g + i
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float2 pr = lane_pair<16>(l[rt]);
-      pr = lane_pair<32>(pr.x + pr.y);
-      if (g == 0) {
-        lds_m[wave][16 * rt + n] = m[rt] + raise;
-        lds_l[wave][16 * rt + n] = pr.x + pr.y;
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(&lds_o[wave][16 * rt + n][16 * dt + 4 * g]) = o[rt][dt];
-    }
+    const Kv8View view = {a.r.table + (int64_t)b * a.r.max_blocks, a.r.max_blocks, a.r.num_blocks, a.tree};
+    kv8_rows_tile<D, FMT, RT>(a, view, seq, kvh, row0, rows, s0, s1, lds);
     __syncthreads();
     const bool whole = s0 == 0 && s1 == steps;
     const int slot = 2 * at.w + (first_part ? 0 : 1);
@@ -466,18 +157,9 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
     const int part = slot * kPart * 4;  // byte offsets: at most 1024 parts of 32 rows
     for (int e = tid; e < rows * (D / 4); e += kKv8Threads) {
       const int r = e / (D / 4), d = 4 * (e % (D / 4));
-      float mm = lds_m[0][r];
-#pragma unroll
-      for (int k = 1; k < kWaves; ++k) mm = fmaxf(mm, lds_m[k][r]);
-      float ll = 0.0f;
-      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < kWaves; ++k) {
-        const float f = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(lds_m[k][r] - mm);
-        ll += lds_l[k][r] * f;
-        acc += *reinterpret_cast<const f32x4*>(&lds_o[k][r][d]) * f;
-      }
-      if (__builtin_expect(mm == -INFINITY, 0)) mm = kv8_lowest(a, b, seq, (row0 + r) / a.G, s0 * kKv8Step, s1 * kKv8Step);
+      float mm, ll;
+      const f32x4 acc = kv8_rows_sum<D, RT>(lds, r, d, mm, ll);
+      if (__builtin_expect(mm == -INFINITY, 0)) mm = kv8_lowest(a.tree, view.max_blocks, seq, (row0 + r) / a.G, s0 * kKv8Step, s1 * kKv8Step, [&](int j) { return view.named(j); });
       if (whole) {
         kv8_write<D>(a, {row0, rows, seq.first, kvh}, r, d, acc, mm, ll);
       } else {
@@ -490,7 +172,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_rows_kernel(Kv8AttnArgs a)
       uint32_t* done = a.done ? a.done : kv8_counts[a.slot];
       if (kv8_last(done + w0, parts, lds_plan.T)) {
         kv8_merge<D, TR>(a, parts_mem, w0, at.second_part(a), parts, {row0, rows, seq.first, kvh},
-                         reinterpret_cast<float2*>(&lds_o[0][0][0]));
+                         reinterpret_cast<float2*>(&lds.o[0][0][0]));
       }
     }
     first_part = false;

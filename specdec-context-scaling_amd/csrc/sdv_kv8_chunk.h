@@ -548,7 +548,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2
     const float unit = __builtin_amdgcn_ldexpf(1.0f, e_acc - (FMT == kFp8 ? 5 : 7));
     const float2 pr = lane_pair<32>(l);
     l = pr.x + pr.y;
-    if (__builtin_expect(rv && m == -INFINITY, 0)) m = kv8_lowest(a, b, seq, tok, slo * kKv8Step, shi * kKv8Step);
+    if (__builtin_expect(rv && m == -INFINITY, 0)) m = kv8_lowest(a.tree, a.r.max_blocks, seq, tok, slo * kKv8Step, shi * kKv8Step, [&](int j) { return kv8_block(a.r, b, j) >= 0; });
     const bool whole = slo == 0 && shi == steps;
     // a row that sees nothing: 0; a part without exponentials has no weight
     const float inv = m == -INFINITY || (!whole && l == 0.0f) ? 0.0f : unit / l;

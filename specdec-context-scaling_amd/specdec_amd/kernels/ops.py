@@ -19,6 +19,7 @@ Operators
 ``kv8_gather``        the 8-bit cache read back into packed BF16 rows.
 ``kv8_attention``     ragged query rows (single tokens, verify blocks or trees, prompt chunks,
                       or all in one batch) over the 8-bit cache.
+``kv8_shared_attention``  the same for sequences that begin with the same pages, read once for all.
 ``rope``              rotary positions of packed query and key rows (``rope_frequencies``: what it turns by).
 ``kv8_rope_append``   a step's rows in one launch: q rotated, K rotated and quantized, V quantized.
 ``copy_blocks``       whole page blocks of every layer copied, within a pool of either cache or to another.
@@ -830,6 +831,64 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     return out
 
 
+def kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                         cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_q_len: int, max_seq_len: int, cu_groups: torch.Tensor,
+                         prefix_lens: torch.Tensor, max_prefix_len: int, *, scale: float | None = None,
+                         tree_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """kv8_attention for sequences that begin with the same pages, whose shared keys are read and computed once for each group of them.
+
+    cu_groups int32 (groups + 1,): group g is sequences cu_groups[g] .. cu_groups[g+1] - 1; a sequence may be in none.  prefix_lens
+    int32 (B,), the same for all of a group and at most each one's context before its new tokens (0 for a sequence in no group): as
+    many first tokens, taken down to whole blocks, are the blocks that the table names for the group's first sequence.  Every row
+    of the group sees them all, then its own sequence's keys from there on.  max_prefix_len bounds them.  The other arguments, and the
+    result, are kv8_attention's, to the order of the sums.  For few new tokens a sequence: tiles hold 32 rows of a group.
+    """
+    got = _native.binding().shared(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups,
+                                   prefix_lens, max_prefix_len, scale, tree_mask, out)
+    if got is not None:
+        if got.__class__ is int:
+            _native.check(got, "sdv_kv8_shared_attention")
+        return got
+    dev = _kv8_device(k_pages)
+    nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
+    q, q_row = _kv8_rows(q, "q", dev, None, d)
+    total, H = q.shape[:2]
+    if H == 0 or H % kv:
+        _fail(f"q {tuple(q.shape)} does not match pages (KV={kv}, D={d})")
+    B, mb = block_table.shape
+    max_q_len, max_seq_len, max_prefix_len = int(max_q_len), int(max_seq_len), int(max_prefix_len)
+    cu = _kv8_ints(cu_rows, "cu_rows", dev, B + 1)
+    lens = None if seq_lens is None else _kv8_ints(seq_lens, "seq_lens", dev, B)
+    _need(cu_groups, "cu_groups", (torch.int32,), dev, (1,))
+    groups = cu_groups.shape[0] - 1
+    if not 0 <= groups <= B:
+        _fail(f"cu_groups {tuple(cu_groups.shape)} needs 1 to {B + 1} entries")
+    prefix = _kv8_ints(prefix_lens, "prefix_lens", dev, B)
+    tree = None
+    if tree_mask is not None:
+        if max_q_len > 64:
+            _fail(f"a tree mask holds 64 tokens (max_q_len {max_q_len})")
+        tree = _kv8_ints(tree_mask, "tree_mask", dev, total, torch.uint64 if tree_mask.dtype is torch.uint64 else torch.int64)
+    if out is None:
+        out = torch.empty((total, H, d), dtype=torch.bfloat16, device=dev)
+        out_row = H * d
+    else:
+        out, out_row = _kv8_rows(_same_rows(out, total, "out"), "out", dev, H, d, write=True)
+    lib = _native.load()
+    nbytes = lib.sdv_kv8_shared_attention_workspace_size(B, groups, total, H, kv, d, max_q_len, max_seq_len, max_prefix_len)
+    if nbytes == 0 or max_prefix_len > mb * BLOCK:
+        _fail(f"unsupported sizes B={B} groups={groups} rows={total} H={H} KV={kv} D={d} max_q_len={max_q_len} "
+              f"max_seq_len={max_seq_len} max_prefix_len={max_prefix_len}")
+    if total == 0:
+        return out
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _kv8_call(lib.sdv_kv8_shared_attention, "sdv_kv8_shared_attention", dev, q.data_ptr(), q_row, k_pages.data_ptr(), v_pages.data_ptr(),
+              scales.data_ptr(), nb, fmt, block_table.data_ptr(), mb, cu, lens, tree, cu_groups.data_ptr(), prefix, B, groups, total, H, kv,
+              d, max_q_len, max_seq_len, max_prefix_len, d ** -0.5 if scale is None else float(scale), ws.data_ptr(), nbytes,
+              out.data_ptr(), out_row)
+    return out
+
+
 # ---------------------------------------------------------------------------- positions and page moves
 def rope_frequencies(head_dim: int, base: float = 1000000.0, *, rotary_dim: int | None = None, scaling: dict | None = None,
                      device="cuda") -> tuple[torch.Tensor, float]:
@@ -1139,6 +1198,21 @@ def _lib_kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
 
 @_lib_kv8_attention.register_fake
 def _(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale=None, tree_mask=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("sdv::kv8_shared_attention", mutates_args=())
+def _lib_kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
+                              block_table: torch.Tensor, cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_q_len: int,
+                              max_seq_len: int, cu_groups: torch.Tensor, prefix_lens: torch.Tensor, max_prefix_len: int,
+                              scale: float | None = None, tree_mask: torch.Tensor | None = None) -> torch.Tensor:
+    return kv8_shared_attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups, prefix_lens,
+                                max_prefix_len, scale=scale, tree_mask=tree_mask)
+
+
+@_lib_kv8_shared_attention.register_fake
+def _(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups, prefix_lens, max_prefix_len,
+      scale=None, tree_mask=None):
     return q.new_empty(q.shape)
 
 
