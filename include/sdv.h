@@ -411,21 +411,28 @@ int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const void* k_pages,
  * of the group sees all of them, and of its own sequence the keys from there on that sdv_kv8_attention has it see: with
  * prefixes within the contexts (prefix_lens[b] <= seq_lens[b] - rows) the result is that of sdv_kv8_attention.
  * A sequence in no group whose prefix_lens is not 0 does not see those keys at all.  groups may be 0.
- * Tiles have 16 or 32 rows, sums and operands as there.  max_q_len chooses between them (a sequence with more rows is
- * computed all the same).  The workspace may hold anything and nothing carries over.  max_prefix_len is at most
- * 16 * max_blocks_per_seq; size limits as for sdv_kv8_attention, with max_prefix_len added to max_seq_len.
+ * tile_rows: rows of a prefix's tile, 32 (operands and sums as in sdv_kv8_attention's tiles of 32) or 128 (as in its
+ * tiles of 256, but that an item, up to 1/512 of the call, whose V scales lie more than 2^18 apart is computed as with 32); a
+ * sequence's own tiles have 16 or 32, by max_q_len (a sequence with more rows is computed all the same).
+ * sdv_kv8_shared_attention_tile_rows says which of them is faster for these sizes, or 0 where sdv_kv8_attention is faster than
+ * both (short prefixes or few sequences; more than 64 rows a sequence and KV head; sizes that are refused).
+ * The workspace may hold anything and nothing carries over.  max_prefix_len is at most 16 * max_blocks_per_seq; size
+ * limits as for sdv_kv8_attention, with max_prefix_len added to max_seq_len.
  */
+int32_t sdv_kv8_shared_attention_tile_rows(int32_t batch, int32_t groups, int32_t total_rows, int32_t q_heads,
+                                           int32_t kv_heads, int32_t head_dim, int32_t max_q_len, int32_t max_seq_len,
+                                           int32_t max_prefix_len);
 size_t sdv_kv8_shared_attention_workspace_size(int32_t batch, int32_t groups, int32_t total_rows, int32_t q_heads,
                                                int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
-                                               int32_t max_seq_len, int32_t max_prefix_len);
+                                               int32_t max_seq_len, int32_t max_prefix_len, int32_t tile_rows);
 int sdv_kv8_shared_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                              const float* scales, int32_t num_blocks, int32_t format, const int32_t* block_table,
                              int32_t max_blocks_per_seq, const int32_t* cu_rows, const int32_t* seq_lens,
                              const uint64_t* tree_mask, const int32_t* cu_groups, const int32_t* prefix_lens,
                              int32_t batch, int32_t groups, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
                              int32_t head_dim, int32_t max_q_len, int32_t max_seq_len, int32_t max_prefix_len,
-                             float scale, void* workspace, size_t workspace_bytes, void* out, int64_t out_stride,
-                             void* stream);
+                             int32_t tile_rows, float scale, void* workspace, size_t workspace_bytes, void* out,
+                             int64_t out_stride, void* stream);
 
 /* ------------------------------------------------------------------ positions, page moves
  *

@@ -31,6 +31,7 @@ decltype(&sdv_copy_blocks) g_copy;
 decltype(&sdv_kv8_keep) g_keep;
 decltype(&sdv_kv8_shared_attention) g_shared;
 decltype(&sdv_kv8_shared_attention_workspace_size) g_shared_size;
+decltype(&sdv_kv8_shared_attention_tile_rows) g_shared_rows;
 
 // A tensor of no subclass (whose data might not be where it says), or nullptr.
 const at::Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -419,13 +420,15 @@ PyObject* keep(PyObject*, PyObject* const* o, Py_ssize_t n) {
 }
 
 // shared(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups, prefix_lens,
-//        max_prefix_len, scale, tree_mask, out = None) -> out or status
+//        max_prefix_len, scale, tree_mask, tile_rows, out = None) -> out or status
 PyObject* shared(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Pages p;
-  int64_t q_row, out_row, max_q, max_len, max_prefix;
+  int64_t q_row, out_row, max_q, max_len, max_prefix, tile;
   const int32_t *cu, *lens, *groups, *prefix;
-  if (!g_shared || (n != 14 && n != 15) || !pages(o + 1, p) || !whole(o[7], max_q) || !whole(o[8], max_len) || !whole(o[11], max_prefix)) Py_RETURN_NONE;
+  if (!g_shared || (n != 15 && n != 16) || !pages(o + 1, p) || !whole(o[7], max_q) || !whole(o[8], max_len) || !whole(o[11], max_prefix) ||
+      !whole(o[14], tile))
+    Py_RETURN_NONE;
   const at::Tensor *q = rows(o[0], p, 0, q_row), *cg = tensor(o[9]);
   if (!q || !ints(o[5], p, p.batch + 1, cu) || !lengths(o[6], p, lens) || !cg || cg->dim() != 1 || cg->size(0) < 1 || cg->size(0) > p.batch + 1 ||
       !ints(o[9], p, cg->size(0), groups) || !ints(o[10], p, p.batch, prefix))
@@ -442,11 +445,22 @@ PyObject* shared(PyObject*, PyObject* const* o, Py_ssize_t n) {
     tree = static_cast<const uint64_t*>(t->data_ptr());
   }
   const int32_t ng = (int32_t)cg->size(0) - 1;
-  const size_t bytes = g_shared_size(p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix);
+  if (tile == 0) {
+    tile = g_shared_rows(p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix);
+    if (tile == 0) {  // as every sequence by itself, or sizes that the general path refuses
+      if (max_prefix > (int64_t)p.max_blocks * 16 ||
+          g_shared_size(p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix, 32) == 0)
+        Py_RETURN_NONE;
+      PyObject* const plain[12] = {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], o[8], o[12], o[13], n == 16 ? o[15] : Py_None};
+      return attention(nullptr, plain, 12);
+    }
+  }
+  const size_t bytes = g_shared_size(p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix,
+                                     (int32_t)tile);
   if (bytes == 0) Py_RETURN_NONE;  // sizes that the general path refuses
   const at::Tensor* given = nullptr;
-  if (n == 15 && o[14] != Py_None) {
-    given = rows(o[14], p, heads, out_row);
+  if (n == 16 && o[15] != Py_None) {
+    given = rows(o[15], p, heads, out_row);
     if (!given || given->size(0) != total) Py_RETURN_NONE;
   }
   Launch on(p);
@@ -458,11 +472,11 @@ PyObject* shared(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const c10::DataPtr ws = c10::hip::HIPCachingAllocator::get()->allocate(bytes);
   const int st = g_shared(q->data_ptr(), q_row, p.k, p.v, p.s, p.blocks, p.format, p.table, p.max_blocks, cu, lens, tree, groups, prefix,
                           p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix,
-                          (float)scale, ws.get(), bytes, given ? given->data_ptr() : out.data_ptr(), out_row, on.stream);
+                          (int32_t)tile, (float)scale, ws.get(), bytes, given ? given->data_ptr() : out.data_ptr(), out_row, on.stream);
   if (st != SDV_OK) return status(st);
   if (given) {
-    Py_INCREF(o[14]);
-    return o[14];
+    Py_INCREF(o[15]);
+    return o[15];
   }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -494,16 +508,17 @@ PyObject* bind_moves(PyObject*, PyObject* const* o, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// bind_shared(shared_attention, its workspace_size)
+// bind_shared(shared_attention, its workspace_size, its tile_rows)
 PyObject* bind_shared(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  void* at[2];
-  if (n != 2) {
-    PyErr_SetString(PyExc_TypeError, "bind_shared needs two addresses");
+  void* at[3];
+  if (n != 3) {
+    PyErr_SetString(PyExc_TypeError, "bind_shared needs three addresses");
     return nullptr;
   }
   if (!addresses(o, n, at)) return nullptr;
   g_shared = reinterpret_cast<decltype(g_shared)>(at[0]);
   g_shared_size = reinterpret_cast<decltype(g_shared_size)>(at[1]);
+  g_shared_rows = reinterpret_cast<decltype(g_shared_rows)>(at[2]);
   Py_RETURN_NONE;
 }
 

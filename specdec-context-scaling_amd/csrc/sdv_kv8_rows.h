@@ -94,7 +94,8 @@ struct Kv8RowsLds {
 
 // Steps s0 .. s1 - 1 of the tile that begins with row row0 of the sequence and has `rows` of them; each wavefront's sums
 // to lds.
-template <int D, int FMT, int RT>
+// AGAIN: the pages are read by other tiles as well, and by way of the caches.
+template <int D, int FMT, int RT, bool AGAIN = false>
 __device__ __forceinline__ void kv8_rows_tile(const Kv8AttnArgs& a, const Kv8View& w, const Kv8Seq& seq, int kvh, int row0, int rows,
                                               int s0, int s1, Kv8RowsLds<D, RT>& lds) {
   constexpr int KI = D / 64, KS = D / 32, DT = D / 16, kWaves = kKv8Threads / kWave;
@@ -152,6 +153,7 @@ __device__ __forceinline__ void kv8_rows_tile(const Kv8AttnArgs& a, const Kv8Vie
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
+  const auto load16 = [](const uint8_t* p) { return AGAIN ? *reinterpret_cast<const uint4*>(p) : load_stream16(p); };
   uint4 kw[PG][KI];
   uint32_t vw[DT][PG];
   float4 sk, sv, sk_next, sv_next;
@@ -160,7 +162,7 @@ __device__ __forceinline__ void kv8_rows_tile(const Kv8AttnArgs& a, const Kv8Vie
 #pragma unroll
     for (int p = 0; p < PG; ++p)
 #pragma unroll
-      for (int i = 0; i < KI; ++i) kw[p][i] = load_stream16(src + p * (4 * D) + i * 256);
+      for (int i = 0; i < KI; ++i) kw[p][i] = load16(src + p * (4 * D) + i * 256);
   };
   const auto load_s = [&](int id) {
     const float* src = a.scales + ((int64_t)max(id, 0) * a.kv_heads + kvh) * (2 * kBlock) + vtok + 4 * (n & (PG - 1));
@@ -172,13 +174,14 @@ __device__ __forceinline__ void kv8_rows_tile(const Kv8AttnArgs& a, const Kv8Vie
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       if constexpr (PG == 4) {
-        const uint4 x = load_stream16(src + dt * (16 * kBlock));
+        const uint4 x = load16(src + dt * (16 * kBlock));
         vw[dt][0] = x.x;
         vw[dt][1] = x.y;
         vw[dt][2] = x.z;
         vw[dt][3] = x.w;
       } else {
-        const uint64_t w = __builtin_nontemporal_load(reinterpret_cast<const uint64_t*>(src + dt * (16 * kBlock)));
+        const uint64_t* at = reinterpret_cast<const uint64_t*>(src + dt * (16 * kBlock));
+          const uint64_t w = AGAIN ? *at : __builtin_nontemporal_load(at);
         vw[dt][0] = (uint32_t)w;
         vw[dt][1] = (uint32_t)(w >> 32);
       }

@@ -2,238 +2,325 @@
 //
 // A group is consecutive sequences whose first P tokens (whole blocks) are the same pages.  Its rows lie together in the
 // packed tensors, so a group's prefix is one more sequence: all of its rows, each of which sees all P keys.  A sequence's
-// own part is the sequence it was with its first P keys left out.  Every tile of either leaves its sums with their
-// maximum and their sum of exponentials; a second launch adds those up for each row:
+// own part is the sequence it was with its first P keys left out.  Tiles of 32 rows of a prefix, and of 16 or 32 of a
+// sequence, are cut along their keys into items, one a workgroup where there is one for each, and computed by
+// kv8_rows_tile.  Every item leaves its sums with their maximum and their sum of exponentials; a second launch adds
+// those up for each row:
 //
 //   M = max_k m_k,   out = sum_k e^(m_k - M) acc_k / sum_k e^(m_k - M) l_k
 //
-// Tiles of 32 rows of a prefix, and of 16 or 32 of a sequence, are cut into ranges as in kv8_rows_kernel, and computed
-// by its code; a prefix's pages are read once per 32 rows of the group, from memory once.
-#include "sdv_kv8_rows.h"
+// The items of one stretch of a prefix's keys, one for each of its tiles, stand one after another and go to the
+// workgroups of one XCD, whose L2 then serves all of them but the first.
+#include "sdv_kv8_wide.h"
 
 namespace sdv {
-
-// What one launch leaves for the next, of a prefix or a sequence: units of its tiles, and which parts are theirs.
-struct Kv8SharedTiles {
-  uint32_t unit0;  // units before it, of one KV head
-  uint32_t tile0;  // tiles before it, likewise
-  uint32_t units;  // of each of its tiles, those of its start among them; 0: no tiles
-  int first, n;    // its packed rows
-  int pad[3];
-};
-struct Kv8SharedPlan {
-  uint32_t per_head, tiles;  // units and tiles of a KV head
-  uint32_t share, rest;      // every range has `share` units, the first `rest` one more
-  int start;
-  int pad[3];
-};
 
 struct Kv8SharedArgs {
   Kv8AttnArgs a;
   const int32_t* cu_groups;
   const int32_t* prefix;
   int groups, max_prefix;
-  uint32_t parts;  // that the workspace holds: more than tables whose entries do not decrease ever need
-  Kv8SharedPlan* plan;
-  Kv8SharedTiles* of;  // per prefix, then per sequence
+  bool wide;          // tiles of a prefix have kWideRows rows, else 32
+  uint32_t parts[2];  // that the workspace holds, of prefixes and of sequences: no fewer than tables need whose entries do not decrease
+  float* part[2];
+  struct Kv8SharedRow* rows;  // per packed token
 };
 
-constexpr int kSharedModes = 4;   // units of 4, 8, 16 and 32 steps, one a workgroup where there is one for each
-constexpr int kSharedStart = 5;   // else single steps, and so many that stand for a tile's start
+// Where the parts of a packed token's rows lie: of the prefix (k = 0) and of the sequence.  Row r = row0[k] + head of KV
+// head h: part base[k] + h * per_head[k] + c * tiles[k] + r / tile for each of the chunks c < chunks[k].
+struct Kv8SharedRow {
+  uint32_t base[2], per_head[2];
+  int tiles[2], chunks[2], row0[2];
+  int pad[6];
+};
+
+constexpr int kSharedStart = 5;   // steps that starting an item costs, about
+constexpr int kSharedWide = 4;    // steps that one of kWideRows rows costs, about
+constexpr int kSharedShort = 4;   // steps of those that an item has at least: its part costs as much
+constexpr int kSharedLengths = 4;  // of items, in steps, that are tried: 1, 5/4, 3/2 and 2 times a workgroup's even share
 
 // Prefix v, or sequence v - groups: its rows, keys and blocks.
 struct Kv8SharedSeq {
-  Kv8Seq seq;
-  int skip;   // blocks of the table in front of its first key
-  int table;  // whose table
-  int steps;  // of 64 keys, of each tile
+  int first, n;  // packed rows
+  int T;         // keys; of a sequence those behind the prefix
+  int table;     // whose table
+  int skip;      // blocks of the table in front of the first key
+  int tiles;
+  __device__ __forceinline__ uint32_t steps() const { return (uint32_t)(max(T, 0) + kKv8Step - 1) >> kKv8StepBits; }
 };
 
-template <int TP, int TS>
-__device__ __forceinline__ Kv8SharedSeq kv8_shared_seq(const Kv8SharedArgs& s, int v) {
-  const Kv8AttnArgs& a = s.a;
+// From the tables' entries: rows first .. end - 1, a prefix of P tokens, and of a sequence its length.
+template <int TS>
+__device__ __forceinline__ Kv8SharedSeq kv8_shared_prefix(const Kv8SharedArgs& s, int b0, int b1, int first, int end, int P) {
   Kv8SharedSeq x;
+  x.table = min(b0, s.a.r.batch - 1);
   x.skip = 0;
-  if (v < s.groups) {
-    const int b0 = min(max(s.cu_groups[v], 0), a.r.batch), b1 = min(max(s.cu_groups[v + 1], b0), a.r.batch);
-    x.table = min(b0, a.r.batch - 1);
-    const int first = min(max(a.r.cu[b0], 0), a.r.total), end = min(max(a.r.cu[b1], 0), a.r.total);
-    const int P = b0 < b1 ? min(max(s.prefix[x.table], 0), s.max_prefix) & ~(kBlock - 1) : 0;
-    x.seq.first = first;
-    x.seq.n = P > 0 ? max(end - first, 0) : 0;
-    x.seq.T = x.seq.ctx = P;
-    x.seq.tiles = (x.seq.n * a.G + TP - 1) / TP;
-    x.seq.tree = true;  // of no visible new tokens
-  } else {
-    const int b = v - s.groups;
-    int first, n;
-    kv8_rows(a.r, b, first, n);
-    const int P = min(max(s.prefix[b], 0), s.max_prefix) & ~(kBlock - 1);
-    const int T = (a.lens ? min(max(a.lens[b], 0), a.max_len) : a.max_len) - P;
-    x.table = b;
-    x.skip = P / kBlock;
-    x.seq = kv8_seq_of<TS>(a, first, T > 0 ? n : 0, T);
-    x.seq.ctx = T - n;
-  }
-  x.steps = (max(x.seq.T, 0) + kKv8Step - 1) >> kKv8StepBits;
+  x.first = min(max(first, 0), s.a.r.total);
+  x.T = b0 < b1 ? min(max(P, 0), s.max_prefix) & ~(kBlock - 1) : 0;
+  x.n = x.T > 0 ? max(min(max(end, 0), s.a.r.total) - x.first, 0) : 0;
+  x.tiles = s.wide ? (x.n * s.a.G + kWideRows - 1) / kWideRows : (x.n * s.a.G + 31) / 32;
+  return x;
+}
+template <int TS>
+__device__ __forceinline__ Kv8SharedSeq kv8_shared_own(const Kv8SharedArgs& s, int b, int first, int end, int P, int len) {
+  Kv8SharedSeq x;
+  P = min(max(P, 0), s.max_prefix) & ~(kBlock - 1);
+  x.table = b;
+  x.skip = P / kBlock;
+  x.first = min(max(first, 0), s.a.r.total);
+  x.T = (s.a.lens ? min(max(len, 0), s.a.max_len) : s.a.max_len) - P;
+  x.n = x.T > 0 ? max(min(max(end, 0), s.a.r.total) - x.first, 0) : 0;  // none: nothing behind the prefix
+  x.tiles = (x.n * s.a.G + TS - 1) / TS;
   return x;
 }
 
-__device__ __forceinline__ uint32_t kv8_shared_units(const Kv8SharedSeq& x, int unit) {
-  return (uint32_t)(x.steps + (1 << unit) - 1) >> unit;
+template <int TS>
+__device__ __forceinline__ Kv8SharedSeq kv8_shared_seq(const Kv8SharedArgs& s, int v) {
+  const Kv8AttnArgs& a = s.a;
+  if (v < s.groups) {
+    const int b0 = min(max(s.cu_groups[v], 0), a.r.batch), b1 = min(max(s.cu_groups[v + 1], b0), a.r.batch);
+    return kv8_shared_prefix<TS>(s, b0, b1, a.r.cu[b0], a.r.cu[b1], s.prefix[min(b0, a.r.batch - 1)]);
+  }
+  const int b = v - s.groups;
+  return kv8_shared_own<TS>(s, b, a.r.cu[b], a.r.cu[b + 1], s.prefix[b], a.lens ? a.lens[b] : 0);
 }
 
-struct Kv8SharedLds {
-  uint4 run[kKv8Threads];  // units and tiles of the wavefront's runs up to and with this one, units and tiles of this one
-  uint32_t total[kKv8Threads / kWave][kSharedModes + 2];
+// The tables in LDS, where a workgroup has a thread for each prefix and sequence: all of them in one load each, where a
+// prefix's rows would be a second one after its sequences.
+struct Kv8SharedTables {
+  int cu[kKv8Threads + 1], prefix[kKv8Threads];
 };
 
-// A workgroup's place among the units: as Kv8Place, over prefixes and sequences.
-template <int TP, int TS>
-struct Kv8SharedPlace {
-  uint32_t per_head, tiles, share, rest;
-  int unit, start;
-  int ranges;
-  uint32_t u, end;
-  int kvh, v, i;
-  Kv8SharedSeq x;
-  uint32_t tile0, units_of;  // the tile's first unit and its units
-  uint32_t ordinal;          // tiles before it, of all KV heads
+struct Kv8SharedLds {
+  uint32_t sum[kKv8Threads / kWave][2 * kSharedLengths + 1];
+  uint2 run[kKv8Threads];  // items of prefixes, and of sequences, of the wavefront's runs up to and with this one
+};
 
-  __device__ __forceinline__ bool begin(const Kv8SharedArgs& s, Kv8SharedLds& lds, int w, int grid) {
+// A call's items, in this order: (prefixes, then sequences) x (KV head) x (v) x (chunk of its keys) x (tile).
+template <int TS>
+struct Kv8SharedItems {
+  int count, per_run;       // prefixes and sequences; of a thread's run
+  uint32_t length[2];       // steps of an item of a prefix, and of a sequence, at most
+  uint32_t per_head[2];     // items of a KV head
+  uint32_t items;
+
+  // The item that is being computed.
+  Kv8SharedSeq x;
+  int kvh, tile, chunk, v;
+  uint32_t chunks;
+
+  __device__ __forceinline__ uint32_t chunks_of(int i, uint32_t steps) const { return (steps + length[i] - 1) / length[i]; }
+
+  // seqs: a run's last prefix or sequence, its only one where the runs hold one each.
+  __device__ __forceinline__ void begin(const Kv8SharedArgs& s, Kv8SharedLds& lds, Kv8SharedSeq* seqs, uint32_t grid) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int count = s.groups + s.a.r.batch, per_run = (count + kKv8Threads - 1) / kKv8Threads;
-    uint32_t mine[kSharedModes + 2] = {};  // units at each size, at single steps, tiles
-    for (int k = 0; k < per_run; ++k) {
-      const int y = tid * per_run + k;
-      if (y >= count) break;
-      const Kv8SharedSeq q = kv8_shared_seq<TP, TS>(s, y);
-#pragma unroll
-      for (int m = 0; m < kSharedModes; ++m) mine[m] += (uint32_t)q.seq.tiles * kv8_shared_units(q, m + 2);
-      mine[kSharedModes] += (uint32_t)q.seq.tiles * (uint32_t)(q.steps + kSharedStart);
-      mine[kSharedModes + 1] += (uint32_t)q.seq.tiles;
-    }
-    uint32_t scan[kSharedModes + 2];
-#pragma unroll
-    for (int m = 0; m < kSharedModes + 2; ++m) {
-      scan[m] = kv8_lane_scan(mine[m]);
-      if (lane == kWave - 1) lds.total[wave][m] = scan[m];
-    }
-    __syncthreads();
-    uint32_t total[kSharedModes + 2];
-#pragma unroll
-    for (int m = 0; m < kSharedModes + 2; ++m) {
-      total[m] = 0;
-#pragma unroll
-      for (int k = 0; k < kKv8Threads / kWave; ++k) total[m] += lds.total[k][m];
-      total[m] = __builtin_amdgcn_readfirstlane(total[m]);
-    }
-    tiles = total[kSharedModes + 1];
-    int mode = kSharedModes;
-#pragma unroll
-    for (int m = kSharedModes - 1; m >= 0; --m)
-      if (total[m] * (uint32_t)s.a.kv_heads <= (uint32_t)grid) mode = m;
-    unit = mode == kSharedModes ? 0 : mode + 2;
-    start = mode == kSharedModes ? kSharedStart : 0;
-    uint32_t upto = scan[kSharedModes], of_run = mine[kSharedModes];
-    per_head = total[kSharedModes];
-#pragma unroll
-    for (int m = 0; m < kSharedModes; ++m)
-      if (m == mode) {
-        upto = scan[m];
-        of_run = mine[m];
-        per_head = total[m];
+    const uint32_t heads = (uint32_t)s.a.kv_heads, weight = s.wide ? kSharedWide : 1;
+    count = s.groups + s.a.r.batch;
+    per_run = (count + kKv8Threads - 1) / kKv8Threads;
+    uint32_t mine = 0;  // steps, and those of the tiles' starts
+    const auto count_in = [&](int y, const Kv8SharedSeq& q) {
+      mine += (uint32_t)q.tiles * (q.steps() * (y < s.groups ? weight : 1) + kSharedStart);
+      seqs[tid] = q;
+    };
+    if (per_run == 1) {
+      Kv8SharedTables& tables = *reinterpret_cast<Kv8SharedTables*>(seqs + kKv8Threads);
+      const int b = tid - s.groups;
+      const bool own = b >= 0 && tid < count;
+      int g0 = 0, g1 = 0, len = 0;
+      if (tid < s.groups) {
+        g0 = s.cu_groups[tid];
+        g1 = s.cu_groups[tid + 1];
       }
-    lds.run[tid] = make_uint4(upto, scan[kSharedModes + 1], of_run, mine[kSharedModes + 1]);
-    const uint32_t units = per_head * (uint32_t)s.a.kv_heads;
-    ranges = (int)min((uint32_t)grid, units);
-    share = ranges > 0 ? units / (uint32_t)ranges : 0;
-    rest = units - share * (uint32_t)ranges;
-    __syncthreads();
-    if (w == 0) {  // what the second launch needs
-      uint32_t u0 = 0, t0 = 0;
-      for (int k = 0; k < wave; ++k) {
-        u0 += lds.run[k * kWave + kWave - 1].x;
-        t0 += lds.run[k * kWave + kWave - 1].y;
+      if (own) {
+        const int first = s.a.r.cu[b], P = s.prefix[b];
+        if (s.a.lens) len = s.a.lens[b];
+        tables.cu[b] = first;
+        tables.prefix[b] = P;
       }
-      u0 += upto - of_run;
-      t0 += scan[kSharedModes + 1] - mine[kSharedModes + 1];
+      if (tid == 0) tables.cu[s.a.r.batch] = s.a.r.cu[s.a.r.batch];
+      __syncthreads();
+      if (tid < s.groups) {
+        const int b0 = min(max(g0, 0), s.a.r.batch), b1 = min(max(g1, b0), s.a.r.batch);
+        count_in(tid, kv8_shared_prefix<TS>(s, b0, b1, tables.cu[b0], tables.cu[b1], tables.prefix[min(b0, s.a.r.batch - 1)]));
+      } else if (own) {
+        count_in(tid, kv8_shared_own<TS>(s, b, tables.cu[b], tables.cu[b + 1], tables.prefix[b], len));
+      }
+    } else {
       for (int k = 0; k < per_run; ++k) {
         const int y = tid * per_run + k;
         if (y >= count) break;
-        const Kv8SharedSeq q = kv8_shared_seq<TP, TS>(s, y);
-        const uint32_t each = q.seq.tiles > 0 ? kv8_shared_units(q, unit) + (uint32_t)start : 0;
-        s.of[y] = {u0, t0, each, q.seq.first, q.seq.n, {0, 0, 0}};
-        u0 += (uint32_t)q.seq.tiles * each;
-        t0 += (uint32_t)q.seq.tiles;
+        count_in(y, kv8_shared_seq<TS>(s, y));
       }
-      if (tid == 0) *s.plan = {per_head, tiles, share, rest, start, {0, 0, 0}};
     }
-    if (w >= ranges) return false;
-    u = (uint32_t)w * share + min((uint32_t)w, rest);
-    end = u + share + ((uint32_t)w < rest ? 1 : 0);
-    kvh = (int)(u / per_head);
-    uint32_t rem = u - (uint32_t)kvh * per_head;
-    tile0 = (uint32_t)kvh * per_head;
-    ordinal = (uint32_t)kvh * tiles;
-    // the wavefront whose runs hold the unit, then the run: the first that ends behind it
+    mine = kv8_lane_scan(mine);
+    if (lane == kWave - 1) lds.sum[wave][2 * kSharedLengths] = mine;
+    __syncthreads();
+    uint32_t total = 0;
+#pragma unroll
+    for (int k = 0; k < kKv8Threads / kWave; ++k) total += lds.sum[k][2 * kSharedLengths];
+    total = __builtin_amdgcn_readfirstlane(total) * heads;
+    const uint32_t even = (total + grid - 1) / grid;
+    const uint32_t tried[kSharedLengths] = {(even + 3) & ~3u, (even + even / 4 + 3) & ~3u, (even + even / 2 + 3) & ~3u, (2 * even + 3) & ~3u};
+    const auto length_of = [&](int i, int m) {
+      uint32_t x = 4;
+#pragma unroll
+      for (int k = 0; k < kSharedLengths; ++k)
+        if (k == m) x = max(tried[k], 4u);
+      return i == 0 && s.wide ? max(x / kSharedWide, (uint32_t)kSharedShort) : x;
+    };
+    uint32_t of[2][kSharedLengths] = {};
+    for (int k = 0; k < per_run; ++k) {
+      const int y = tid * per_run + k;
+      if (y >= count) break;
+      const Kv8SharedSeq q = per_run == 1 ? seqs[tid] : kv8_shared_seq<TS>(s, y);
+#pragma unroll
+      for (int m = 0; m < kSharedLengths; ++m) {
+        const uint32_t each = length_of(y < s.groups ? 0 : 1, m);
+        const uint32_t n = (uint32_t)q.tiles * ((q.steps() + each - 1) / each);
+        if (y < s.groups)
+          of[0][m] += n;
+        else
+          of[1][m] += n;
+      }
+    }
+    uint32_t scan[2][kSharedLengths];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int m = 0; m < kSharedLengths; ++m) {
+        scan[i][m] = kv8_lane_scan(of[i][m]);
+        if (lane == kWave - 1) lds.sum[wave][i * kSharedLengths + m] = scan[i][m];
+      }
+    __syncthreads();
+    uint32_t all[2][kSharedLengths];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int m = 0; m < kSharedLengths; ++m) {
+        all[i][m] = 0;
+#pragma unroll
+        for (int k = 0; k < kKv8Threads / kWave; ++k) all[i][m] += lds.sum[k][i * kSharedLengths + m];
+        all[i][m] = __builtin_amdgcn_readfirstlane(all[i][m]);
+      }
+    // the shortest with an item a workgroup, else with a prefix's item a workgroup, else an even share
+    int best = -1, next = 0;
+#pragma unroll
+    for (int m = kSharedLengths - 1; m >= 0; --m) {
+      if (all[0][m] * heads <= grid) next = m;
+      if ((all[0][m] + all[1][m]) * heads <= grid) best = m;
+    }
+    if (best < 0) best = next;
+#pragma unroll
+    for (int m = 0; m < kSharedLengths; ++m)
+      if (m == best) {
+        length[0] = length_of(0, m);
+        length[1] = length_of(1, m);
+        per_head[0] = all[0][m];
+        per_head[1] = all[1][m];
+        lds.run[tid] = make_uint2(scan[0][m], scan[1][m]);
+      }
+    items = (per_head[0] + per_head[1]) * heads;
+    __syncthreads();
+  }
+
+  // Items before those of prefix or sequence y (of one KV head and its kind).
+  __device__ __forceinline__ uint32_t before(const Kv8SharedArgs& s, const Kv8SharedLds& lds, int y) const {
+    const int i = y < s.groups ? 0 : 1, run = y / per_run;
+    uint32_t n = run % kWave ? (&lds.run[run - 1].x)[i] : 0;
+    for (int k = 0; k < run / kWave; ++k) n += (&lds.run[k * kWave + kWave - 1].x)[i];
+    for (int k = run * per_run; k < y; ++k) {
+      if ((k < s.groups ? 0 : 1) != i) continue;
+      const Kv8SharedSeq q = kv8_shared_seq<TS>(s, k);
+      n += (uint32_t)q.tiles * chunks_of(i, q.steps());
+    }
+    return n;
+  }
+
+  // The item of this number (< items); seqs: as begin left them, or nullptr.
+  __device__ __forceinline__ bool find(const Kv8SharedArgs& s, const Kv8SharedLds& lds, const Kv8SharedSeq* seqs, uint32_t item) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const uint32_t prefixes = per_head[0] * (uint32_t)s.a.kv_heads;
+    const int i = item < prefixes ? 0 : 1;
+    uint32_t rem = item - (i ? prefixes : 0);
+    kvh = (int)(rem / per_head[i]);
+    rem -= (uint32_t)kvh * per_head[i];
+    // the wavefront whose runs hold the item, then the run: the first that ends behind it
     int wv = 0;
 #pragma unroll
     for (int k = 0; k < kKv8Threads / kWave - 1; ++k) {
-      const uint4 r = lds.run[k * kWave + kWave - 1];
-      if (wv == k && rem >= r.x) {
-        rem -= r.x;
-        tile0 += r.x;
-        ordinal += r.y;
+      const uint32_t n = (&lds.run[k * kWave + kWave - 1].x)[i];
+      if (wv == k && rem >= n) {
+        rem -= n;
         wv = k + 1;
       }
     }
     wv = __builtin_amdgcn_readfirstlane(wv);
     rem = __builtin_amdgcn_readfirstlane(rem);
-    const uint4 run = lds.run[wv * kWave + lane];
-    const int at = min(__popcll(__ballot(run.x <= rem)), kWave - 1);
-    const uint32_t before = __builtin_amdgcn_readlane(run.x, at) - __builtin_amdgcn_readlane(run.z, at);
-    rem -= before;
-    tile0 += before;
-    ordinal += __builtin_amdgcn_readlane(run.y, at) - __builtin_amdgcn_readlane(run.w, at);
-    for (v = (wv * kWave + at) * per_run;; ++v) {
-      if (v >= count) return false;  // not reached: the runs hold the unit
-      x = kv8_shared_seq<TP, TS>(s, v);
-      units_of = kv8_shared_units(x, unit) + (uint32_t)start;
-      const uint32_t all = (uint32_t)x.seq.tiles * units_of;
-      if (rem < all) break;
-      rem -= all;
-      tile0 += all;
-      ordinal += (uint32_t)x.seq.tiles;
+    const uint32_t upto = (&lds.run[wv * kWave + lane].x)[i];
+    const int at = min(__popcll(__ballot(upto <= rem)), kWave - 1);
+    if (at > 0) rem -= __builtin_amdgcn_readlane(upto, at - 1);
+    v = (wv * kWave + at) * per_run;
+    if (per_run == 1) {
+      x = seqs ? seqs[v] : kv8_shared_seq<TS>(s, v);
+    } else {
+      for (;; ++v) {
+        if (v >= count) return false;  // not reached: the runs hold the item
+        if ((v < s.groups ? 0 : 1) != i) continue;
+        x = kv8_shared_seq<TS>(s, v);
+        const uint32_t n = (uint32_t)x.tiles * chunks_of(i, x.steps());
+        if (rem < n) break;
+        rem -= n;
+      }
     }
-    i = (int)(rem / units_of);
-    tile0 += (uint32_t)i * units_of;
-    ordinal += (uint32_t)i;
+    x.first = __builtin_amdgcn_readfirstlane(x.first);
+    x.n = __builtin_amdgcn_readfirstlane(x.n);
+    x.T = __builtin_amdgcn_readfirstlane(x.T);
+    x.table = __builtin_amdgcn_readfirstlane(x.table);
+    x.skip = __builtin_amdgcn_readfirstlane(x.skip);
+    x.tiles = __builtin_amdgcn_readfirstlane(x.tiles);
+    if (x.tiles <= 0) return false;  // not reached
+    chunks = chunks_of(i, x.steps());
+    chunk = (int)(rem / (uint32_t)x.tiles);
+    tile = (int)(rem - (uint32_t)chunk * (uint32_t)x.tiles);
     return true;
   }
 
-  // The tile after this one; false past the last (not reached while u < end).
-  __device__ __forceinline__ bool next(const Kv8SharedArgs& s) {
-    tile0 += units_of;
-    ++ordinal;
-    if (++i < x.seq.tiles) return true;
-    i = 0;
-    do {
-      if (++v >= s.groups + s.a.r.batch) {
-        v = 0;
-        if (++kvh >= s.a.kv_heads) return false;
-      }
-      x = kv8_shared_seq<TP, TS>(s, v);
-    } while (x.seq.tiles == 0);
-    units_of = kv8_shared_units(x, unit) + (uint32_t)start;
-    return true;
+  // The row table's entry of a packed token.
+  __device__ __forceinline__ void describe(const Kv8SharedArgs& s, const Kv8SharedLds& lds, int token) const {
+    const Kv8AttnArgs& a = s.a;
+    Kv8SharedRow row = {};
+    // the sequence: as many end at or before the token; its group: as many end at or before it
+    int b = 0, g = 0;
+    for (int hi = a.r.batch; b < hi;) {
+      const int mid = (b + hi) / 2;
+      if (min(max(a.r.cu[mid + 1], 0), a.r.total) <= token) b = mid + 1; else hi = mid;
+    }
+    for (int hi = s.groups; g < hi;) {
+      const int mid = (g + hi) / 2;
+      if (s.cu_groups[mid + 1] <= b) g = mid + 1; else hi = mid;
+    }
+    const int of[2] = {g < s.groups && s.cu_groups[g] <= b ? g : -1, b < a.r.batch ? s.groups + b : -1};
+    // in no sequence
+    row.row0[0] = b < a.r.batch && token >= min(max(a.r.cu[b], 0), a.r.total) ? 0 : -1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (row.row0[0] < 0 || of[k] < 0) continue;
+      const Kv8SharedSeq q = kv8_shared_seq<TS>(s, of[k]);
+      if (token < q.first || token - q.first >= q.n) continue;
+      row.row0[k] = (token - q.first) * a.G;
+      row.tiles[k] = q.tiles;
+      row.chunks[k] = (int)chunks_of(k, q.steps());
+      row.per_head[k] = per_head[k];
+      row.base[k] = before(s, lds, of[k]);
+    }
+    s.rows[token] = row;
   }
 };
 
-// A part: [32][D] sums, then [32] (maximum, sum of exponentials).
+// A part of a tile of TR rows: [TR][D] sums, then [TR] (maximum, sum of exponentials).
 template <int D>
-constexpr int shared_part() {
-  return 32 * (D + 2);
+constexpr int shared_part(int TR) {
+  return TR * (D + 2);
 }
 
 // RS: row tiles of 16 of a sequence's tile.
@@ -242,116 +329,174 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_shared_kernel(Kv8SharedArg
   constexpr int RP = 2;
   __shared__ Kv8RowsLds<D, RP> lds;
   __shared__ Kv8SharedLds lds_plan;
-  static_assert(sizeof(Kv8RowsLds<D, RS>) <= sizeof(lds), "a sequence's tile uses the same memory");
+  static_assert(sizeof(Kv8RowsLds<D, RS>) <= sizeof(lds) && sizeof(Kv8WideLds<D>) <= sizeof(lds), "every kind of tile uses the same memory");
   const Kv8AttnArgs& a = s.a;
-  Kv8SharedPlace<16 * RP, 16 * RS> at;
-  const int w = (int)blockIdx.x;
-  if (!at.begin(s, lds_plan, w, (int)gridDim.x)) return;
-  for (;;) {
-    const uint32_t last_unit = min(at.units_of, at.end - at.tile0);
-    const int lo = max((int)(at.u - at.tile0) - at.start, 0), hi = (int)last_unit - at.start;
-    if (lo >= hi) break;  // the range ends within the tile's start
-    const bool prefix = at.v < s.groups;
-    const int TR = prefix ? 16 * RP : 16 * RS;
-    const Kv8Seq seq = at.x.seq;
-    const int row0 = at.i * TR, rows = min(seq.n * a.G - row0, TR);
+  Kv8SharedItems<16 * RS> at;
+  const uint32_t grid = gridDim.x, w = blockIdx.x;
+  static_assert(sizeof(lds.o) >= kKv8Threads * sizeof(Kv8SharedSeq) + sizeof(Kv8SharedTables), "room for the plan until the first sums");
+  static_assert(sizeof(lds) + sizeof(lds_plan) <= 80 * 1024, "two workgroups per CU");
+  const Kv8SharedSeq* seqs = reinterpret_cast<Kv8SharedSeq*>(&lds.o);
+  at.begin(s, lds_plan, reinterpret_cast<Kv8SharedSeq*>(&lds.o), grid);
+  // Workgroups w, w + 8, ... share an XCD: an eighth of the prefixes' items, one after another, and of the sequences' are
+  // theirs.
+  const uint32_t prefixes = at.per_head[0] * (uint32_t)a.kv_heads, mine_p = (prefixes + 7) / 8, mine_s = (at.items - prefixes + 7) / 8;
+  for (uint32_t j = w >> 3; j < mine_p + mine_s; j += grid >> 3) {
+    const uint32_t item = j < mine_p ? (w & 7) * mine_p + j : prefixes + (w & 7) * mine_s + (j - mine_p);
+    if (item >= (j < mine_p ? prefixes : at.items)) continue;
+    if (!at.find(s, lds_plan, seqs, item)) break;
+    __syncthreads();
+    seqs = nullptr;
+    const bool prefix = at.v < s.groups, wide = prefix && s.wide;
+    const uint32_t slot = prefix ? item : item - prefixes;
+    if (slot >= s.parts[prefix ? 0 : 1]) break;
+    const int TR = wide ? kWideRows : prefix ? 16 * RP : 16 * RS;
+    const Kv8SharedSeq x = at.x;
+    const int row0 = at.tile * TR, rows = min(x.n * a.G - row0, TR);
+    Kv8Seq seq;
+    seq.first = x.first;
+    seq.n = x.n;
+    seq.T = x.T;
+    seq.ctx = prefix ? x.T : x.T - x.n;
+    seq.tiles = x.tiles;
+    seq.tree = prefix || a.tree != nullptr;  // of a prefix every row sees all keys: a tree's context
+    int steps = (int)x.steps();
+    int each = (steps + (int)at.chunks - 1) / (int)at.chunks;
+    if (!wide) each = (each + 3) & ~3;
     // a tile of early rows sees fewer keys than its sequence's last
-    int steps = at.x.steps;
     if (!seq.tree) steps = min(steps, max(seq.ctx + (row0 + rows - 1) / a.G + kKv8Step, 0) >> kKv8StepBits);
-    const int s0 = min(lo << at.unit, steps), s1 = min(hi << at.unit, steps);
-    const Kv8View view = {a.r.table + (int64_t)at.x.table * a.r.max_blocks + at.x.skip, a.r.max_blocks - at.x.skip, a.r.num_blocks,
+    const int s0 = min(at.chunk * each, steps), s1 = min(s0 + each, steps);
+    const Kv8View view = {a.r.table + (int64_t)x.table * a.r.max_blocks + x.skip, a.r.max_blocks - x.skip, a.r.num_blocks,
                           prefix ? nullptr : a.tree};
-    const uint32_t slot = at.ordinal + (uint32_t)w;  // each part's own: from one to the next the tile or the range is another
-    if (slot >= s.parts) break;
-    float* part = a.part + (int64_t)slot * shared_part<D>();
-    const auto leave = [&](const auto& sums) {
+    float* part = s.part[prefix ? 0 : 1] + (int64_t)slot * shared_part<D>(TR);
+    const auto lowest = [&](int r) {
+      Kv8Seq c = seq;
+      c.tree = !prefix && seq.tree;
+      const int until = prefix ? min(s1 * kKv8Step, seq.T) : s1 * kKv8Step;
+      return kv8_lowest(a.tree, view.max_blocks, c, (row0 + r) / a.G, s0 * kKv8Step, until, [&](int j) { return view.named(j); });
+    };
+    const auto leave = [&](const auto& sums, int at_row, int count) {  // of a tile of few rows, from row at_row of the part on
       __syncthreads();
-      for (int e = threadIdx.x; e < rows * (D / 4); e += kKv8Threads) {
+      for (int e = threadIdx.x; e < count * (D / 4); e += kKv8Threads) {
         const int r = e / (D / 4), d = 4 * (e % (D / 4));
         float mm, ll;
         const f32x4 acc = kv8_rows_sum(sums, r, d, mm, ll);
-        if (__builtin_expect(mm == -INFINITY, 0)) {
-          Kv8Seq c = seq;
-          c.tree = !prefix && seq.tree;
-          const int until = prefix ? min(s1 * kKv8Step, seq.T) : s1 * kKv8Step;
-          mm = kv8_lowest(a.tree, view.max_blocks, c, (row0 + r) / a.G, s0 * kKv8Step, until, [&](int j) { return view.named(j); });
-        }
-        *reinterpret_cast<f32x4*>(part + r * D + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(part + 32 * D + 2 * r) = make_float2(mm, ll);
+        if (__builtin_expect(mm == -INFINITY, 0)) mm = lowest(at_row + r);
+        *reinterpret_cast<f32x4*>(part + (at_row + r) * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(part + TR * D + 2 * (at_row + r)) = make_float2(mm, ll);
       }
     };
-    if (RS == RP || prefix) {
-      kv8_rows_tile<D, FMT, RP>(a, view, seq, at.kvh, row0, rows, s0, s1, lds);
-      leave(lds);
+    Kv8WideLds<D>& lds_wide = reinterpret_cast<Kv8WideLds<D>&>(lds);
+    int E = 0;
+    f32x16 acc[D / 32];
+    float m, l;
+    if (wide && kv8_wide_tile<D, FMT>(a, view, x.first, x.T, at.kvh, row0, rows, s0, s1, E, lds_wide, acc, m, l)) {
+      // in units of 1; where V is large enough for the sums of 2^30 keys to pass fp32's range, as of a maximum 2^48 times as large
+      const float raise = E >= 64 ? kKv8Raise : 0.0f;
+      const float unit = __builtin_amdgcn_ldexpf(1.0f, E - (FMT == kFp8 ? 5 : 7) - (int)(kWideBits + raise));
+      const int lane = threadIdx.x & (kWave - 1), g = lane >> 5, r = (int)threadIdx.x / kWave * 32 + (lane & 31);
+      const float2 pr = lane_pair<32>(l);
+      if (r < rows) {
+        m = __builtin_expect(m == -INFINITY, 0) ? lowest(r) : m + raise;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<f32x4*>(part + r * D + 32 * dt + 8 * j + 4 * g) =
+                f32x4{acc[dt][4 * j] * unit, acc[dt][4 * j + 1] * unit, acc[dt][4 * j + 2] * unit, acc[dt][4 * j + 3] * unit};
+        if (g == 0) *reinterpret_cast<float2*>(part + TR * D + 2 * r) = make_float2(m, __builtin_amdgcn_ldexpf(pr.x + pr.y, -(int)(kWideBits + raise)));
+      }
+    } else if (prefix) {
+      for (int k = 0; k < rows; k += 16 * RP) {  // a tile of kWideRows as several of few rows
+        const int count = min(rows - k, 16 * RP);
+        __syncthreads();
+        kv8_rows_tile<D, FMT, RP, true>(a, view, seq, at.kvh, row0 + k, count, s0, s1, lds);
+        leave(lds, k, count);
+      }
     } else {
       auto& few = reinterpret_cast<Kv8RowsLds<D, RS>&>(lds);
       kv8_rows_tile<D, FMT, RS>(a, view, seq, at.kvh, row0, rows, s0, s1, few);
-      leave(few);
+      leave(few, 0, rows);
     }
-    at.u = at.tile0 + last_unit;
-    if (at.u >= at.end || !at.next(s)) break;
     __syncthreads();
   }
+  // the row table, from the last workgroups on, which have the least to do
+  for (uint32_t token = (grid - 1 - w) * kKv8Threads + threadIdx.x; token < (uint32_t)a.r.total; token += grid * kKv8Threads)
+    at.describe(s, lds_plan, (int)token);
 }
 
-// The rows of a packed token and KV head: the parts of the prefix's tile and of the sequence's that hold them, added up.
-constexpr int kSharedMergeThreads = 256;
+// The rows of a packed token and KV head: their parts added up, four dimensions a thread, the parts of a row by as many
+// groups of threads as have kSharedMergeBatch of them in flight each (at most eight groups).
+constexpr int kSharedMergeThreads = 512, kSharedMergeBatch = 8;
 
 template <int D, int TS>
 __global__ __launch_bounds__(kSharedMergeThreads) void kv8_shared_merge_kernel(Kv8SharedArgs s) {
+  constexpr int LN = D / 4, GR = kSharedMergeThreads / LN;
+  __shared__ f32x4 lds_acc[GR][LN];
+  __shared__ float2 lds_ml[GR];
   const Kv8AttnArgs& a = s.a;
-  __shared__ int found[2];
   const int tid = threadIdx.x, token = blockIdx.x, kvh = blockIdx.y;
-  if (tid < 2) found[tid] = 0;
-  __syncthreads();
-  // the sequence: as many end at or before the token; the group: as many end at or before the sequence
-  for (int x = tid; x < a.r.batch; x += kSharedMergeThreads) {
-    const uint64_t before = __ballot(min(max(a.r.cu[x + 1], 0), a.r.total) <= token);
-    if ((tid & (kWave - 1)) == 0) atomicAdd(&found[0], __popcll(before));
-  }
-  __syncthreads();
-  const int b = found[0];
-  if (b >= a.r.batch || token < min(max(a.r.cu[b], 0), a.r.total)) return;  // behind the last sequence
-  for (int x = tid; x < s.groups; x += kSharedMergeThreads) {
-    const uint64_t before = __ballot(s.cu_groups[x + 1] <= b);
-    if ((tid & (kWave - 1)) == 0) atomicAdd(&found[1], __popcll(before));
-  }
-  __syncthreads();
-  const int g = found[1];
-  const Kv8SharedPlan plan = *s.plan;
-  const bool grouped = g < s.groups && s.cu_groups[g] <= b;
-  Kv8SharedTiles of[2] = {s.of[grouped ? g : 0], s.of[s.groups + b]};
-  if (!grouped) of[0].units = 0;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (token < of[k].first || token - of[k].first >= of[k].n) of[k].units = 0;
-  const auto owner = [&](uint32_t x) {
-    const uint32_t split = plan.rest * (plan.share + 1);
-    return x < split ? x / (plan.share + 1) : plan.rest + (x - split) / plan.share;
-  };
-  for (int e = tid; e < a.G * (D / 4); e += kSharedMergeThreads) {
-    const int head = e / (D / 4), d = 4 * (e % (D / 4));
+  const Kv8SharedRow row = s.rows[token];
+  if (row.row0[0] < 0) return;  // in no sequence
+  const int n0 = row.chunks[0], n = n0 + row.chunks[1], TP = s.wide ? kWideRows : 32;
+  int lg = 0;
+  while (lg < 3 && (kSharedMergeBatch << lg) < n) ++lg;
+  const int group = tid / LN, ln = tid % LN, d = 4 * ln;
+  for (int h0 = 0; h0 < a.G; h0 += GR >> lg) {
+    const int head = h0 + (group >> lg);
+    const bool live = head < a.G;
+    const int r0 = row.row0[0] + min(head, a.G - 1), r1 = row.row0[1] + min(head, a.G - 1);
+    const uint32_t base0 = row.base[0] + (uint32_t)kvh * row.per_head[0] + (uint32_t)(r0 / TP);
+    const uint32_t base1 = row.base[1] + (uint32_t)kvh * row.per_head[1] + (uint32_t)(r1 / TS);
+    const float* const own = s.part[1] + (r1 % TS) * D + d;
+    const float* const prefix = s.part[0] + (r0 % TP) * D + d;
     float m = -INFINITY, l = 0.0f;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = group & ((1 << lg) - 1); live && k0 < n; k0 += kSharedMergeBatch << lg) {
+      float2 st[kSharedMergeBatch];
+      f32x4 y[kSharedMergeBatch];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (of[k].units == 0) continue;
-      const int TR = k == 0 ? 32 : TS;
-      const int row = (token - of[k].first) * a.G + head, i = row / TR, r = row - i * TR;
-      const uint32_t t0 = (uint32_t)kvh * plan.per_head + of[k].unit0 + (uint32_t)i * of[k].units;
-      const uint32_t first = owner(t0 + (uint32_t)plan.start), last = owner(t0 + of[k].units - 1);
-      const uint32_t slot = (uint32_t)kvh * plan.tiles + of[k].tile0 + (uint32_t)i + first;
-      const float* part = a.part + (int64_t)slot * shared_part<D>();
-      for (uint32_t j = 0; j <= last - first && slot + j < s.parts; ++j, part += shared_part<D>()) {
-        const float2 st = *reinterpret_cast<const float2*>(part + 32 * D + 2 * r);
-        const f32x4 y = *reinterpret_cast<const f32x4*>(part + r * D + d);
-        const float mx = fmaxf(m, st.x);
-        const float f0 = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx), f1 = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.x - mx);
-        l = l * f0 + st.y * f1;
-        acc = acc * f0 + y * f1;
-        m = mx;
+      for (int k = 0; k < kSharedMergeBatch; ++k) {  // past the last part that again, not counted
+        const int c = min(k0 + (k << lg), n - 1);
+        const uint32_t x0 = min(base0 + (uint32_t)(c * row.tiles[0]), s.parts[0] - 1), x1 = min(base1 + (uint32_t)((c - n0) * row.tiles[1]), s.parts[1] - 1);
+        const float* const part = c < n0 ? prefix + (int64_t)x0 * shared_part<D>(TP) : own + (int64_t)x1 * shared_part<D>(TS);
+        const int stats = c < n0 ? (TP - r0 % TP) * D + 2 * (r0 % TP) - d : (TS - r1 % TS) * D + 2 * (r1 % TS) - d;
+        st[k] = *reinterpret_cast<const float2*>(part + stats);
+        y[k] = *reinterpret_cast<const f32x4*>(part);
+      }
+      float mx = m;
+#pragma unroll
+      for (int k = 0; k < kSharedMergeBatch; ++k) mx = fmaxf(mx, st[k].x);
+      const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+      l *= f;
+      acc *= f;
+      m = mx;
+#pragma unroll
+      for (int k = 0; k < kSharedMergeBatch; ++k) {
+        const float w = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st[k].x - mx);
+        if (k0 + (k << lg) < n) {
+          l += st[k].y * w;
+          acc += y[k] * w;
+        }
       }
     }
+    if (lg > 0) {  // the groups' sums
+      __syncthreads();
+      lds_acc[group][ln] = acc;
+      if (ln == 0) lds_ml[group] = make_float2(m, l);
+      __syncthreads();
+      const int g0 = group & ~((1 << lg) - 1);
+      m = -INFINITY;
+      for (int k = 0; k < 1 << lg; ++k) m = fmaxf(m, lds_ml[g0 + k].x);
+      l = 0.0f;
+      acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int k = 0; k < 1 << lg; ++k) {
+        const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(lds_ml[g0 + k].x - m);
+        l += lds_ml[g0 + k].y * w;
+        acc += lds_acc[g0 + k][ln] * w;
+      }
+      if (group != g0) continue;
+    }
+    if (!live) continue;
     const float inv = m == -INFINITY ? 0.0f : 1.0f / l;  // a row that sees nothing: 0
     *reinterpret_cast<uint2*>(a.out + (int64_t)token * a.out_stride + (int64_t)(kvh * a.G + head) * D + d) =
         make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
@@ -362,47 +507,72 @@ __global__ __launch_bounds__(kSharedMergeThreads) void kv8_shared_merge_kernel(K
 
 using namespace sdv;
 
-// Most tiles of one KV head.
-static int64_t shared_tiles(int32_t batch, int32_t groups, int32_t total, int32_t G, int tile) {
-  const int64_t rows = (int64_t)total * G, own = rows / tile + batch, prefix = rows / 32 + groups;
-  return (own < rows ? own : rows) + (prefix < rows ? prefix : rows);
+static int shared_tile(int32_t G, int32_t max_q_len) { return (int64_t)G * max_q_len <= 16 ? 16 : 32; }
+
+// Rows of a prefix's tile, or 0 where a call takes longer here than in sdv_kv8_attention, which reads the prefix again for
+// every sequence, from the caches: it has one launch, and long tiles of a sequence's own rows.
+constexpr int64_t kSharedKeys = 1 << 18, kSharedWideKeys = 15 << 20;
+static int shared_rows(int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
+                       int32_t max_prefix) {
+  const int64_t own = (int64_t)G * max_q_len, saved = (int64_t)(batch - groups) * max_prefix * kv_heads;
+  if (groups <= 0 || own > 64 || saved < (own <= 16 ? 2 * kSharedKeys : kSharedKeys / 2)) return 0;
+  const int64_t keys = (int64_t)total * G / groups * max_prefix * kv_heads / 2;
+  return keys >= (head_dim == 128 ? kSharedWideKeys : kSharedWideKeys / 3) ? kWideRows : 32;
 }
 
-static int shared_tile(int32_t G, int32_t max_q_len) { return (int64_t)G * max_q_len <= 16 ? 16 : 32; }
+// Most tiles of all KV heads' prefixes (k = 0) and sequences.
+static int64_t shared_tiles(int k, bool wide, int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t max_q_len) {
+  const int64_t rows = (int64_t)total * G;
+  const int64_t cut = k == 0 ? rows / (wide ? kWideRows : 32) + groups : rows / shared_tile(G, max_q_len) + batch;
+  return (cut < rows ? cut : rows) * kv_heads;
+}
 
 // The plan's sums are 32 bits wide, and a part's number a 31-bit one.
 static int shared_sizes(int32_t batch, int32_t groups, int32_t total, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
                         int32_t max_len, int32_t max_prefix) {
-  if (batch <= 0 || groups < 0 || groups > batch || total < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || kv_heads > 65535 ||
+  if (batch <= 0 || groups < 0 || groups > batch || total < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 65535 ||
       max_q_len <= 0 || max_len <= 0 || max_prefix < 0)
     return SDV_ERR_SHAPE;
   if (head_dim != 64 && head_dim != 128) return SDV_ERR_UNSUPPORTED;
   if (batch > INT32_MAX / 4 || total > INT32_MAX / 2) return SDV_ERR_SHAPE;
   const int32_t G = q_heads / kv_heads;
   if (((int64_t)max_len + max_prefix + total) * G > (1 << 30)) return SDV_ERR_SHAPE;
-  const int64_t tiles = shared_tiles(batch, groups, total, G, shared_tile(G, max_q_len)) * kv_heads;
-  const int64_t longest = max_len > max_prefix ? max_len : max_prefix;
-  return tiles > INT32_MAX / 8 || tiles * (longest / kKv8Step + 1 + kSharedStart) > INT32_MAX ? SDV_ERR_SHAPE : SDV_OK;
+  const int64_t prefixes = shared_tiles(0, false, batch, groups, total, G, kv_heads, max_q_len), own = shared_tiles(1, false, batch, groups, total, G, kv_heads, max_q_len);
+  if (prefixes + own > INT32_MAX / 8) return SDV_ERR_SHAPE;
+  const int64_t steps = prefixes * (max_prefix / kKv8Step + 1) * kSharedWide + own * (max_len / kKv8Step + 1) + (prefixes + own) * kSharedStart;
+  return steps > INT32_MAX / 4 ? SDV_ERR_SHAPE : SDV_OK;
 }
 
-static size_t shared_tables(int32_t batch, int32_t groups) {
-  return round_up(sizeof(Kv8SharedPlan) + ((size_t)batch + groups) * sizeof(Kv8SharedTiles), 256);
+static size_t shared_tables(int32_t total) { return round_up((size_t)total * sizeof(Kv8SharedRow), 256); }
+
+// Parts of prefixes and of sequences: a chunk has an even share of all steps at least.
+static int64_t shared_parts(int k, bool wide, int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t max_q_len) {
+  return shared_tiles(k, wide, batch, groups, total, G, kv_heads, max_q_len) + kKv8Grid;
+}
+static size_t shared_part_bytes(int k, bool wide, int32_t G, int32_t head_dim, int32_t max_q_len) {
+  const int rows = k == 1 ? shared_tile(G, max_q_len) : wide ? kWideRows : 32;
+  return sizeof(float) * (head_dim == 128 ? shared_part<128>(rows) : shared_part<64>(rows));
 }
 
-static int64_t shared_parts(int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t max_q_len) {
-  return shared_tiles(batch, groups, total, G, shared_tile(G, max_q_len)) * kv_heads + kKv8Grid;
+static size_t shared_workspace(bool wide, int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t head_dim, int32_t max_q_len) {
+  size_t bytes = shared_tables(total);
+  for (int k = 0; k < 2; ++k)
+    bytes += (size_t)shared_parts(k, wide, batch, groups, total, G, kv_heads, max_q_len) * shared_part_bytes(k, wide, G, head_dim, max_q_len);
+  return bytes;
 }
 
-static size_t shared_workspace(int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t head_dim, int32_t max_q_len) {
-  return shared_tables(batch, groups) +
-         (size_t)shared_parts(batch, groups, total, G, kv_heads, max_q_len) * sizeof(float) * (head_dim == 128 ? shared_part<128>() : shared_part<64>());
+extern "C" int32_t sdv_kv8_shared_attention_tile_rows(int32_t batch, int32_t groups, int32_t total_rows, int32_t q_heads, int32_t kv_heads,
+                                                      int32_t head_dim, int32_t max_q_len, int32_t max_seq_len, int32_t max_prefix_len) {
+  if (shared_sizes(batch, groups, total_rows, q_heads, kv_heads, head_dim, max_q_len, max_seq_len, max_prefix_len) != SDV_OK) return 0;
+  return shared_rows(batch, groups, total_rows, q_heads / kv_heads, kv_heads, head_dim, max_q_len, max_prefix_len);
 }
 
 extern "C" size_t sdv_kv8_shared_attention_workspace_size(int32_t batch, int32_t groups, int32_t total_rows, int32_t q_heads,
                                                           int32_t kv_heads, int32_t head_dim, int32_t max_q_len, int32_t max_seq_len,
-                                                          int32_t max_prefix_len) {
+                                                          int32_t max_prefix_len, int32_t tile_rows) {
   if (shared_sizes(batch, groups, total_rows, q_heads, kv_heads, head_dim, max_q_len, max_seq_len, max_prefix_len) != SDV_OK) return 0;
-  return shared_workspace(batch, groups, total_rows, q_heads / kv_heads, kv_heads, head_dim, max_q_len);
+  if (tile_rows != 32 && tile_rows != kWideRows) return 0;
+  return shared_workspace(tile_rows != 32, batch, groups, total_rows, q_heads / kv_heads, kv_heads, head_dim, max_q_len);
 }
 
 template <int D, int FMT>
@@ -422,7 +592,7 @@ extern "C" int sdv_kv8_shared_attention(const void* q, int64_t q_stride, const v
                                         const int32_t* cu_rows, const int32_t* seq_lens, const uint64_t* tree_mask,
                                         const int32_t* cu_groups, const int32_t* prefix_lens, int32_t batch, int32_t groups,
                                         int32_t total_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
-                                        int32_t max_seq_len, int32_t max_prefix_len, float scale, void* workspace,
+                                        int32_t max_seq_len, int32_t max_prefix_len, int32_t tile_rows, float scale, void* workspace,
                                         size_t workspace_bytes, void* out, int64_t out_stride, void* stream) {
   if (!q || !k_pages || !v_pages || !scales || !block_table || !cu_rows || !cu_groups || !prefix_lens || !out) return SDV_ERR_NULL;
   const int sizes = shared_sizes(batch, groups, total_rows, q_heads, kv_heads, head_dim, max_q_len, max_seq_len, max_prefix_len);
@@ -431,6 +601,7 @@ extern "C" int sdv_kv8_shared_attention(const void* q, int64_t q_stride, const v
   if (max_prefix_len > (int64_t)max_blocks_per_seq * kBlock) return SDV_ERR_SHAPE;
   if (format != SDV_KV8_FP8 && format != SDV_KV8_INT8) return SDV_ERR_UNSUPPORTED;
   if (tree_mask && max_q_len > 64) return SDV_ERR_UNSUPPORTED;
+  if (tile_rows != 32 && tile_rows != kWideRows) return SDV_ERR_UNSUPPORTED;
   const int64_t row = (int64_t)q_heads * head_dim;
   if (q_stride < row || out_stride < row) return SDV_ERR_SHAPE;
   if (!aligned(q, 16) || !aligned(out, 16) || q_stride % 8 || out_stride % 8 || !aligned(k_pages, 16) || !aligned(v_pages, 16) ||
@@ -438,7 +609,7 @@ extern "C" int sdv_kv8_shared_attention(const void* q, int64_t q_stride, const v
       !aligned(cu_groups, 4) || !aligned(prefix_lens, 4))
     return SDV_ERR_ALIGN;
   const int G = q_heads / kv_heads;
-  if (!workspace || !aligned(workspace, 256) || workspace_bytes < shared_workspace(batch, groups, total_rows, G, kv_heads, head_dim, max_q_len))
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < shared_workspace(tile_rows != 32, batch, groups, total_rows, G, kv_heads, head_dim, max_q_len))
     return SDV_ERR_WORKSPACE;
   if (total_rows == 0) return SDV_OK;
 
@@ -466,10 +637,13 @@ extern "C" int sdv_kv8_shared_attention(const void* q, int64_t q_stride, const v
   s.prefix = prefix_lens;
   s.groups = groups;
   s.max_prefix = max_prefix_len;
-  s.parts = (uint32_t)shared_parts(batch, groups, total_rows, G, kv_heads, max_q_len);
-  s.plan = static_cast<Kv8SharedPlan*>(workspace);
-  s.of = reinterpret_cast<Kv8SharedTiles*>(s.plan + 1);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + shared_tables(batch, groups));
+  s.wide = tile_rows != 32;
+  for (int k = 0; k < 2; ++k) s.parts[k] = (uint32_t)shared_parts(k, s.wide, batch, groups, total_rows, G, kv_heads, max_q_len);
+  s.rows = static_cast<Kv8SharedRow*>(workspace);
+  a.part = nullptr;
+  char* const parts = static_cast<char*>(workspace) + shared_tables(total_rows);
+  s.part[0] = reinterpret_cast<float*>(parts);
+  s.part[1] = reinterpret_cast<float*>(parts + s.parts[0] * shared_part_bytes(0, s.wide, G, head_dim, max_q_len));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int tile = shared_tile(G, max_q_len);
   if (head_dim == 128)

@@ -80,10 +80,11 @@ SIGNATURES = {
                                          _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ, _P, _I64, _P]),
     "sdv_kv8_attention_slot": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I32, _I32,
                                               _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ, _I32, _P, _I64, _P]),
-    "sdv_kv8_shared_attention_workspace_size": (_SZ, [_I32] * 9),
+    "sdv_kv8_shared_attention_tile_rows": (_I32, [_I32] * 9),
+    "sdv_kv8_shared_attention_workspace_size": (_SZ, [_I32] * 10),
     "sdv_kv8_shared_attention": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _P, _P, _I32, _I32,
-                                                _I32, _I32, _I32, _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ, _P,
-                                                _I64, _P]),
+                                                _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, ctypes.c_float, _P, _SZ,
+                                                _P, _I64, _P]),
     "sdv_rope": (ctypes.c_int, [_P, _I64, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, ctypes.c_float, _I32, _I32, _I32,
                                 _P, _I64, _P, _I64, _P]),
     "sdv_kv8_rope_append": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _P, _P, _I64, _I64, _I32, _P, _P, _P, _I32, _I32,
@@ -154,7 +155,8 @@ def binding():
         at = lambda *names: (ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names)  # noqa: E731
         _BINDING.bind(*at("sdv_kv8_append", "sdv_kv8_gather", "sdv_kv8_attention_slot", "sdv_kv8_attention_workspace_size"))
         _BINDING.bind_moves(*at("sdv_rope", "sdv_kv8_rope_append", "sdv_copy_blocks", "sdv_kv8_keep"))
-        _BINDING.bind_shared(*at("sdv_kv8_shared_attention", "sdv_kv8_shared_attention_workspace_size"))
+        _BINDING.bind_shared(*at("sdv_kv8_shared_attention", "sdv_kv8_shared_attention_workspace_size",
+                                  "sdv_kv8_shared_attention_tile_rows"))
         _BOUND = lib
     return _BINDING
 

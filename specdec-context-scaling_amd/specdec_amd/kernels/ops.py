@@ -834,7 +834,7 @@ def kv8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 def kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
                          cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_q_len: int, max_seq_len: int, cu_groups: torch.Tensor,
                          prefix_lens: torch.Tensor, max_prefix_len: int, *, scale: float | None = None,
-                         tree_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                         tree_mask: torch.Tensor | None = None, tile_rows: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
     """kv8_attention for sequences that begin with the same pages, whose shared keys are read and computed once for each group of them.
 
     cu_groups int32 (groups + 1,): group g is sequences cu_groups[g] .. cu_groups[g+1] - 1; a sequence may be in none.  prefix_lens
@@ -844,11 +844,13 @@ def kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     result, are kv8_attention's, to the order of the sums.  For few new tokens a sequence: tiles hold 32 rows of a group.
     """
     got = _native.binding().shared(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups,
-                                   prefix_lens, max_prefix_len, scale, tree_mask, out)
+                                   prefix_lens, max_prefix_len, scale, tree_mask, tile_rows, out)
     if got is not None:
         if got.__class__ is int:
             _native.check(got, "sdv_kv8_shared_attention")
         return got
+    if tile_rows not in (0, 32, 128):
+        raise ValueError(f"tile_rows must be 0, 32 or 128 (got {tile_rows})")
     dev = _kv8_device(k_pages)
     nb, kv, d, fmt = _kv8_pages(k_pages, v_pages, scales, block_table, dev)
     q, q_row = _kv8_rows(q, "q", dev, None, d)
@@ -875,16 +877,21 @@ def kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     else:
         out, out_row = _kv8_rows(_same_rows(out, total, "out"), "out", dev, H, d, write=True)
     lib = _native.load()
-    nbytes = lib.sdv_kv8_shared_attention_workspace_size(B, groups, total, H, kv, d, max_q_len, max_seq_len, max_prefix_len)
+    sizes = (B, groups, total, H, kv, d, max_q_len, max_seq_len, max_prefix_len)
+    tile = tile_rows or lib.sdv_kv8_shared_attention_tile_rows(*sizes)
+    nbytes = lib.sdv_kv8_shared_attention_workspace_size(*sizes, tile or 32)
     if nbytes == 0 or max_prefix_len > mb * BLOCK:
         _fail(f"unsupported sizes B={B} groups={groups} rows={total} H={H} KV={kv} D={d} max_q_len={max_q_len} "
               f"max_seq_len={max_seq_len} max_prefix_len={max_prefix_len}")
     if total == 0:
         return out
+    if tile == 0:
+        return kv8_attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale=scale,
+                             tree_mask=tree_mask, out=out)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _kv8_call(lib.sdv_kv8_shared_attention, "sdv_kv8_shared_attention", dev, q.data_ptr(), q_row, k_pages.data_ptr(), v_pages.data_ptr(),
               scales.data_ptr(), nb, fmt, block_table.data_ptr(), mb, cu, lens, tree, cu_groups.data_ptr(), prefix, B, groups, total, H, kv,
-              d, max_q_len, max_seq_len, max_prefix_len, d ** -0.5 if scale is None else float(scale), ws.data_ptr(), nbytes,
+              d, max_q_len, max_seq_len, max_prefix_len, tile, d ** -0.5 if scale is None else float(scale), ws.data_ptr(), nbytes,
               out.data_ptr(), out_row)
     return out
 
@@ -1205,14 +1212,14 @@ def _(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, ma
 def _lib_kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
                               block_table: torch.Tensor, cu_rows: torch.Tensor, seq_lens: torch.Tensor | None, max_q_len: int,
                               max_seq_len: int, cu_groups: torch.Tensor, prefix_lens: torch.Tensor, max_prefix_len: int,
-                              scale: float | None = None, tree_mask: torch.Tensor | None = None) -> torch.Tensor:
+                              scale: float | None = None, tree_mask: torch.Tensor | None = None, tile_rows: int = 0) -> torch.Tensor:
     return kv8_shared_attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups, prefix_lens,
-                                max_prefix_len, scale=scale, tree_mask=tree_mask)
+                                max_prefix_len, scale=scale, tree_mask=tree_mask, tile_rows=tile_rows)
 
 
 @_lib_kv8_shared_attention.register_fake
 def _(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups, prefix_lens, max_prefix_len,
-      scale=None, tree_mask=None):
+      scale=None, tree_mask=None, tile_rows=0):
     return q.new_empty(q.shape)
 
 

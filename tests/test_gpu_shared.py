@@ -102,43 +102,51 @@ CASES = {
 }
 
 
+TILES = pytest.mark.parametrize("tile", [32, 128])
+
+
 @pytest.mark.parametrize("fmt", ["fp8", "int8"])
 @pytest.mark.parametrize("heads", list(HEADS))
 @pytest.mark.parametrize("name", list(CASES))
 def test_shared(cuda_device, name, heads, fmt):
-    announce(f"shared {name} {heads} {fmt}")
     case = Case(heads, fmt, CASES[name])
-    ref.within(case.run(cuda_device), *case.want())
+    want = case.want()
+    for tile in (0, 32, 128):
+        announce(f"shared {name} {heads} {fmt} {tile}")
+        ref.within(case.run(cuda_device, tile_rows=tile), *want)
 
 
+@TILES
 @pytest.mark.parametrize("heads", ["target", "draft"])
 @pytest.mark.parametrize("name", ["verify", "ragged", "rows", "groups"])
-def test_trees(cuda_device, name, heads):
-    announce(f"shared trees {name} {heads}")
+def test_trees(cuda_device, name, heads, tile):
+    announce(f"shared trees {name} {heads} {tile}")
     case = Case(heads, "fp8", CASES[name])
     rng, words = random.Random(3), []
     for n in case.new:
         for i in range(n):
             words.append((words[len(words) - 1 - rng.randrange(min(i, 4))] if i else 0) | 1 << i)
     tree = torch.tensor([w - (1 << 64) if w >> 63 else w for w in words], dtype=torch.int64)
-    ref.within(case.run(cuda_device, tree_mask=tree.to(cuda_device)), *case.want(tree=tree))
+    ref.within(case.run(cuda_device, tree_mask=tree.to(cuda_device), tile_rows=tile), *case.want(tree=tree))
 
 
-def test_one_length_a_scale_and_a_given_output(cuda_device):
+@TILES
+def test_one_length_a_scale_and_a_given_output(cuda_device, tile):
     case = Case("draft", "int8", [(10, [(37, 3)] * 3)])
     dev = cuda_device
     wide = torch.full((9 + 2, 20, 64), 7.0, dtype=torch.bfloat16, device=dev)
     q = torch.cat((case.q, case.q[:2])).to(dev)  # two rows behind the last sequence
-    got = ops.kv8_shared_attention(q, *case.args(dev, lens=False), scale=0.05, out=wide[:, 3:17])
+    got = ops.kv8_shared_attention(q, *case.args(dev, lens=False), tile_rows=tile, scale=0.05, out=wide[:, 3:17])
     assert got.data_ptr() == wide[:, 3:17].data_ptr()
     ref.within(got[:9], *case.want(scale=0.05))
     assert bool((wide[9:] == 7.0).all()) and bool((wide[:, :3] == 7.0).all()) and bool((wide[:, 17:] == 7.0).all())
     odd = torch.empty((11, 14 * 64 + 3), dtype=torch.bfloat16, device=dev)[:, 3:].view(11, 14, 64).copy_(q)  # copied
-    assert torch.equal(ops.kv8_shared_attention(odd, *case.args(dev), scale=0.05)[:9], got[:9])
-    assert ops.kv8_shared_attention(q[:0], *case.args(dev)).shape == (0, 14, 64)
+    assert torch.equal(ops.kv8_shared_attention(odd, *case.args(dev), tile_rows=tile, scale=0.05)[:9], got[:9])
+    assert ops.kv8_shared_attention(q[:0], *case.args(dev), tile_rows=tile).shape == (0, 14, 64)
 
 
-def test_prefixes_are_whole_blocks(cuda_device):
+@TILES
+def test_prefixes_are_whole_blocks(cuda_device, tile):
     """A length inside a block counts down to its start; a bound below the lengths cuts them: the rest is read through each table."""
     case = Case("target", "fp8", CASES["verify"])
     case.table, dev = case.table.clone(), cuda_device
@@ -149,25 +157,27 @@ def test_prefixes_are_whole_blocks(cuda_device):
         announce(f"shared prefixes {prefix} {most}")
         if most > 16 * case.table.shape[1]:
             most = args[-1] = 16 * case.table.shape[1]
-        ref.within(ops.kv8_shared_attention(case.q.to(dev), *args), *want)
+        ref.within(ops.kv8_shared_attention(case.q.to(dev), *args, tile_rows=tile), *want)
     args[-3] = _ints([0], dev)  # no groups, no prefixes
-    ref.within(ops.kv8_shared_attention(case.q.to(dev), *args), *want)
+    ref.within(ops.kv8_shared_attention(case.q.to(dev), *args, tile_rows=tile), *want)
 
 
-def test_every_row_sees_the_whole_prefix(cuda_device):
+@TILES
+def test_every_row_sees_the_whole_prefix(cuda_device, tile):
     """A prefix that reaches past a context: as documented, its keys for every row, then what is left of the sequence's own."""
     case, dev = Case("mha", "fp8", [(4, [(2, 2), (20, 9)])]), cuda_device
     args = list(case.args(dev))
     args[5] = _ints([60, 84], dev)  # the first sequence ends within the prefix
     announce("shared prefix past a context")
-    got = ops.kv8_shared_attention(case.q.to(dev), *args)
+    got = ops.kv8_shared_attention(case.q.to(dev), *args, tile_rows=tile)
     want, bound = ref.attention(case.q[:2], case.pages, case.table[:1], [2], [64], tree=torch.tensor([3, 3]))
     ref.within(got[:2], want, bound)
     ref.within(got[2:], *(x[2:] for x in case.want()))
 
 
+@TILES
 @pytest.mark.parametrize("heads", ["target", "draft"])
-def test_what_is_not_seen_or_not_finite(cuda_device, heads):
+def test_what_is_not_seen_or_not_finite(cuda_device, heads, tile):
     """NaN scales where a sequence ends and in unnamed blocks; NaN and infinities in the prefix reach its group alone; infinite
     queries; sequences of length 0 and tables without blocks."""
     dev = cuda_device
@@ -178,7 +188,7 @@ def test_what_is_not_seen_or_not_finite(cuda_device, heads):
     case.table[5, 0], case.table[5, 2] = 10 ** 6, -5
     case.q[4, 0] = math.inf
     announce(f"shared not finite {heads}")
-    got = case.run(dev)
+    got = case.run(dev, tile_rows=tile)
     want, bound = case.want()
     bad = torch.isnan(want)
     assert bool(torch.isnan(got.cpu())[bad].all())
@@ -190,43 +200,82 @@ def test_what_is_not_seen_or_not_finite(cuda_device, heads):
         assert bool(torch.isnan(got[:3, :h]).all())
 
 
-def test_rows_that_see_nothing(cuda_device):
+@TILES
+def test_rows_that_see_nothing(cuda_device, tile):
     dev = cuda_device
     case = Case("target", "int8", [(2, [(3, 2), (20, 5)])])
     case.table[:] = -1
-    assert bool((case.run(dev) == 0).all())
+    assert bool((case.run(dev, tile_rows=tile) == 0).all())
     case = Case("target", "int8", [(None, [(0, 0), (6, 2)])])
     args = list(case.args(dev))
     args[5] = _ints([0, 1], dev)  # two rows of a sequence of one token
-    got = ops.kv8_shared_attention(case.q.to(dev), *args)
+    got = ops.kv8_shared_attention(case.q.to(dev), *args, tile_rows=tile)
     assert bool((got[0] == 0).all()) and bool((got[1] != 0).any())
     # scores of -inf alone are NaN, as in kv8_attention: a query of -inf over keys of one sign
     case = Case("mha", "int8", [(2, [(3, 1), (20, 1)])])
     case.pages.k.view(torch.int8).fill_(3)
     case.q.fill_(-math.inf)
-    assert bool(torch.isnan(case.run(dev)).all())
+    assert bool(torch.isnan(case.run(dev, tile_rows=tile)).all())
 
 
-def test_large_scales_stay_finite(cuda_device):
+@TILES
+def test_large_scales_stay_finite(cuda_device, tile):
     case = Case("target", "fp8", [(12, [(9, 2), (30, 2), (60, 2)])])
     case.pages.s[:, :, 1] *= 2.0 ** 118
-    got = case.run(cuda_device)
+    got = case.run(cuda_device, tile_rows=tile)
     want, bound = case.want()
     assert bool(torch.isfinite(got).all())
     ref.within(got, want, bound)
 
 
-def test_recorded_calls_follow_their_inputs(cuda_device):
+@pytest.mark.parametrize("heads,fmt", [("target", "fp8"), ("draft", "int8")])
+def test_scales_that_lie_far_apart(cuda_device, heads, fmt):
+    """V of some of a prefix's tokens 2^-30 of the others': tiles of 128 rows go over to narrow ones where they meet both, and
+    what those tokens give is as exact as ever for the rows that see hardly anything else."""
+    case = Case(heads, fmt, [(24, [(9, 3), (30, 3), (60, 3), (2, 1), (5, 2)])])
+    small = case.table[0, 3:7].long()
+    case.pages.s[small, :, 1] *= 2.0 ** -30
+    case.pages.s[case.table[0, 12].long(), :, 1, 5] = 0.0  # a scale of 0, as no writer leaves it, is no scale
+    # keys of the others far below those: their scores are -60 and less
+    case.pages.s[:, :, 0] *= 1e-3
+    for tile in (32, 128):
+        ref.within(case.run(cuda_device, tile_rows=tile), *case.want())
+
+
+@pytest.mark.parametrize("heads,groups,rows", [
+    ("target", [(16, [(9, 1)] * 3)], 0),                      # short
+    ("target", [(4096 // 16, [(20, 1)] * 70)], 32),           # single tokens
+    ("draft", [(8192 // 16, [(40, 5)] * 20)], 128),           # verify blocks
+    ("target", [(8192 // 16, [(40, 20)] * 20)], 0)])          # 120 rows a sequence and KV head
+def test_the_faster_way_is_chosen(cuda_device, heads, groups, rows):
+    from specdec_amd import _native
+
+    announce(f"shared choice {heads} {rows}")
+    case = Case(heads, "fp8", groups)
+    got = _native.load().sdv_kv8_shared_attention_tile_rows(len(case.new), len(case.groups) - 1, sum(case.new), case.h, case.kv, case.d, max(case.new),
+                                                            max(case.lens), max(case.prefix))
+    assert got == rows
+    args, q = case.args(cuda_device), case.q.to(cuda_device)
+    out = ops.kv8_shared_attention(q, *args)
+    same = ops.kv8_shared_attention(q, *args, tile_rows=rows) if rows else ops.kv8_attention(q, *args[:8])
+    assert torch.equal(out, same)
+    at = case.new[0]  # the first sequence's rows, in 64 bits
+    want, bound = ref.attention(case.q[:at], case.pages, case.table[:1], case.new[:1], case.lens[:1])
+    ref.within(out[:at], want, bound)
+
+
+@TILES
+def test_recorded_calls_follow_their_inputs(cuda_device, tile):
     """Two graphs of the same call and eager calls between them: lengths, rows and pages as they are at each replay."""
     dev = cuda_device
     case = Case("draft", "fp8", [(40, [(60, 2)] * 5)])
     args, q = case.args(dev), case.q.to(dev)
-    ops.kv8_shared_attention(q, *args)
+    ops.kv8_shared_attention(q, *args, tile_rows=tile)
     graphs = []
     for _ in range(2):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            got = ops.kv8_shared_attention(q, *args)
+            got = ops.kv8_shared_attention(q, *args, tile_rows=tile)
         graphs.append((graph, got))
     for step in range(6):
         lens = [640 + 60 - (step * 7 + b) % 50 for b in range(5)]
@@ -235,29 +284,31 @@ def test_recorded_calls_follow_their_inputs(cuda_device):
         for graph, got in graphs:
             graph.replay()
             torch.cuda.synchronize()
-            eager = ops.kv8_shared_attention(q, *args)
+            eager = ops.kv8_shared_attention(q, *args, tile_rows=tile)
             assert torch.equal(got, eager)
         ref.within(eager, *ref.attention(q.cpu(), case.pages, case.table, case.new, lens))
 
 
-def test_streams_and_repeats(cuda_device):
+@TILES
+def test_streams_and_repeats(cuda_device, tile):
     """Calls that overlap on two streams, and the same call again, give the same bits."""
     dev = cuda_device
     a, b = Case("target", "fp8", CASES["eight"]), Case("target", "int8", CASES["many"], seed=5)
     xa, xb, qa, qb = a.args(dev), b.args(dev), a.q.to(dev), b.q.to(dev)
-    want = ops.kv8_shared_attention(qa, *xa), ops.kv8_shared_attention(qb, *xb)
+    want = ops.kv8_shared_attention(qa, *xa, tile_rows=tile), ops.kv8_shared_attention(qb, *xb, tile_rows=tile)
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
     got = []
     for _ in range(10):
-        got.append((ops.kv8_shared_attention(qa, *xa), want[0]))
+        got.append((ops.kv8_shared_attention(qa, *xa, tile_rows=tile), want[0]))
         with torch.cuda.stream(side):
-            got.append((ops.kv8_shared_attention(qb, *xb), want[1]))
+            got.append((ops.kv8_shared_attention(qb, *xb, tile_rows=tile), want[1]))
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in got)
 
 
-def test_tables_that_decrease_stay_in_bounds(cuda_device):
+@TILES
+def test_tables_that_decrease_stay_in_bounds(cuda_device, tile):
     """Bad row and group tables, negative and huge lengths: whatever comes out, nothing else is written."""
     dev = cuda_device
     case = Case("target", "fp8", CASES["groups"])
@@ -270,7 +321,7 @@ def test_tables_that_decrease_stay_in_bounds(cuda_device):
         for lens, prefix in ((case.lens, case.prefix), ([2 ** 31 - 1, -1, 0, -(2 ** 31), 5, 10 ** 6], [2 ** 31 - 1, -9, 48, 10 ** 9, 7, 16])):
             args[4], args[8], args[5], args[9] = _ints(cu, dev), _ints(groups, dev), _ints(lens, dev), _ints(prefix, dev)
             announce(f"shared bad tables {cu} {groups} {lens} {prefix}")
-            ops.kv8_shared_attention(q, *args, out=guard[2:-2])
+            ops.kv8_shared_attention(q, *args, tile_rows=tile, out=guard[2:-2])
             torch.cuda.synchronize()
             assert bool((guard[:2] == 7.0).all()) and bool((guard[-2:] == 7.0).all())
 
@@ -286,6 +337,9 @@ def test_refusals(cuda_device):
                 dict(prefix_lens=good["prefix_lens"][:2]), dict(prefix_lens=good["prefix_lens"].cpu()), dict(max_prefix_len=-1),
                 dict(max_prefix_len=10 ** 6), dict(max_seq_len=0), dict(max_q_len=0), dict(q=good["q"][:, :7]), dict(q=good["q"].float()),
                 dict(cu_rows=good["cu_rows"][:3]), dict(out=torch.empty_like(good["q"])[:2]), dict(tree_mask=tree[:3]),
-                dict(tree_mask=tree, max_q_len=65), dict(max_seq_len=2 ** 31 - 1)):
+                dict(tree_mask=tree, max_q_len=65), dict(max_seq_len=2 ** 31 - 1), dict(tile_rows=128, max_prefix_len=10 ** 6),
+                dict(tile_rows=32, max_seq_len=2 ** 31 - 1)):
         with pytest.raises(SdvError):
             ops.kv8_shared_attention(**{**good, **bad})
+    with pytest.raises(ValueError):
+        ops.kv8_shared_attention(**good, tile_rows=64)
