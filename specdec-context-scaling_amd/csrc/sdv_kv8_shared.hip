@@ -37,7 +37,6 @@ struct Kv8SharedRow {
 constexpr int kSharedStart = 5;   // steps that starting an item costs, about
 constexpr int kSharedWide = 4;    // steps that one of kWideRows rows costs, about
 constexpr int kSharedShort = 4;   // steps of those that an item has at least: its part costs as much
-constexpr int kSharedLengths = 4;  // of items, in steps, that are tried: 1, 5/4, 3/2 and 2 times a workgroup's even share
 
 // Prefix v, or sequence v - groups: its rows, keys and blocks.
 struct Kv8SharedSeq {
@@ -92,7 +91,7 @@ struct Kv8SharedTables {
 };
 
 struct Kv8SharedLds {
-  uint32_t sum[kKv8Threads / kWave][2 * kSharedLengths + 1];
+  uint32_t sum[kKv8Threads / kWave][2];  // steps (those of a wide tile by kSharedWide) and tiles
   uint2 run[kKv8Threads];  // items of prefixes, and of sequences, of the wavefront's runs up to and with this one
 };
 
@@ -117,9 +116,10 @@ struct Kv8SharedItems {
     const uint32_t heads = (uint32_t)s.a.kv_heads, weight = s.wide ? kSharedWide : 1;
     count = s.groups + s.a.r.batch;
     per_run = (count + kKv8Threads - 1) / kKv8Threads;
-    uint32_t mine = 0;  // steps, and those of the tiles' starts
+    uint32_t steps = 0, tiles = 0;
     const auto count_in = [&](int y, const Kv8SharedSeq& q) {
-      mine += (uint32_t)q.tiles * (q.steps() * (y < s.groups ? weight : 1) + kSharedStart);
+      steps += (uint32_t)q.tiles * q.steps() * (y < s.groups ? weight : 1);
+      tiles += (uint32_t)q.tiles;
       seqs[tid] = q;
     };
     if (per_run == 1) {
@@ -152,75 +152,47 @@ struct Kv8SharedItems {
         count_in(y, kv8_shared_seq<TS>(s, y));
       }
     }
-    mine = kv8_lane_scan(mine);
-    if (lane == kWave - 1) lds.sum[wave][2 * kSharedLengths] = mine;
+    steps = kv8_lane_scan(steps);
+    tiles = kv8_lane_scan(tiles);
+    if (lane == kWave - 1) {
+      lds.sum[wave][0] = steps;
+      lds.sum[wave][1] = tiles;
+    }
     __syncthreads();
-    uint32_t total = 0;
+    steps = tiles = 0;
 #pragma unroll
-    for (int k = 0; k < kKv8Threads / kWave; ++k) total += lds.sum[k][2 * kSharedLengths];
-    total = __builtin_amdgcn_readfirstlane(total) * heads;
-    const uint32_t even = (total + grid - 1) / grid;
-    const uint32_t tried[kSharedLengths] = {(even + 3) & ~3u, (even + even / 4 + 3) & ~3u, (even + even / 2 + 3) & ~3u, (2 * even + 3) & ~3u};
-    const auto length_of = [&](int i, int m) {
-      uint32_t x = 4;
-#pragma unroll
-      for (int k = 0; k < kSharedLengths; ++k)
-        if (k == m) x = max(tried[k], 4u);
-      return i == 0 && s.wide ? max(x / kSharedWide, (uint32_t)kSharedShort) : x;
-    };
-    uint32_t of[2][kSharedLengths] = {};
+    for (int k = 0; k < kKv8Threads / kWave; ++k) {
+      steps += lds.sum[k][0];
+      tiles += lds.sum[k][1];
+    }
+    steps = __builtin_amdgcn_readfirstlane(steps) * heads;
+    tiles = __builtin_amdgcn_readfirstlane(tiles) * heads;
+    // A tile of n steps has at most n / length + 1 chunks, so this length leaves an item for every workgroup; where the tiles
+    // alone are too many for that, an even share of the steps and starts.
+    uint32_t each = 2 * tiles <= grid ? steps / (grid - tiles) + 1 : (steps + kSharedStart * tiles) / grid + 1;
+    each = (each + 3) & ~3u;
+    length[1] = each;
+    length[0] = s.wide ? max(each / kSharedWide, (uint32_t)kSharedShort) : each;
+    uint2 mine = make_uint2(0, 0);
     for (int k = 0; k < per_run; ++k) {
       const int y = tid * per_run + k;
       if (y >= count) break;
       const Kv8SharedSeq q = per_run == 1 ? seqs[tid] : kv8_shared_seq<TS>(s, y);
-#pragma unroll
-      for (int m = 0; m < kSharedLengths; ++m) {
-        const uint32_t each = length_of(y < s.groups ? 0 : 1, m);
-        const uint32_t n = (uint32_t)q.tiles * ((q.steps() + each - 1) / each);
-        if (y < s.groups)
-          of[0][m] += n;
-        else
-          of[1][m] += n;
-      }
+      const uint32_t n = (uint32_t)q.tiles * chunks_of(y < s.groups ? 0 : 1, q.steps());
+      mine.x += y < s.groups ? n : 0;
+      mine.y += y < s.groups ? 0 : n;
     }
-    uint32_t scan[2][kSharedLengths];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int m = 0; m < kSharedLengths; ++m) {
-        scan[i][m] = kv8_lane_scan(of[i][m]);
-        if (lane == kWave - 1) lds.sum[wave][i * kSharedLengths + m] = scan[i][m];
-      }
+    lds.run[tid] = make_uint2(kv8_lane_scan(mine.x), kv8_lane_scan(mine.y));
     __syncthreads();
-    uint32_t all[2][kSharedLengths];
+    per_head[0] = per_head[1] = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int m = 0; m < kSharedLengths; ++m) {
-        all[i][m] = 0;
-#pragma unroll
-        for (int k = 0; k < kKv8Threads / kWave; ++k) all[i][m] += lds.sum[k][i * kSharedLengths + m];
-        all[i][m] = __builtin_amdgcn_readfirstlane(all[i][m]);
-      }
-    // the shortest with an item a workgroup, else with a prefix's item a workgroup, else an even share
-    int best = -1, next = 0;
-#pragma unroll
-    for (int m = kSharedLengths - 1; m >= 0; --m) {
-      if (all[0][m] * heads <= grid) next = m;
-      if ((all[0][m] + all[1][m]) * heads <= grid) best = m;
+    for (int k = 0; k < kKv8Threads / kWave; ++k) {
+      per_head[0] += lds.run[k * kWave + kWave - 1].x;
+      per_head[1] += lds.run[k * kWave + kWave - 1].y;
     }
-    if (best < 0) best = next;
-#pragma unroll
-    for (int m = 0; m < kSharedLengths; ++m)
-      if (m == best) {
-        length[0] = length_of(0, m);
-        length[1] = length_of(1, m);
-        per_head[0] = all[0][m];
-        per_head[1] = all[1][m];
-        lds.run[tid] = make_uint2(scan[0][m], scan[1][m]);
-      }
+    per_head[0] = __builtin_amdgcn_readfirstlane(per_head[0]);
+    per_head[1] = __builtin_amdgcn_readfirstlane(per_head[1]);
     items = (per_head[0] + per_head[1]) * heads;
-    __syncthreads();
   }
 
   // Items before those of prefix or sequence y (of one KV head and its kind).
@@ -426,7 +398,7 @@ __global__ __launch_bounds__(kKv8Threads, 2) void kv8_shared_kernel(Kv8SharedArg
 
 // The rows of a packed token and KV head: their parts added up, four dimensions a thread, the parts of a row by as many
 // groups of threads as have kSharedMergeBatch of them in flight each (at most eight groups).
-constexpr int kSharedMergeThreads = 512, kSharedMergeBatch = 8;
+constexpr int kSharedMergeThreads = 512, kSharedMergeBatch = 8, kSharedMergeHeads = 4;  // heads of a workgroup
 
 template <int D, int TS>
 __global__ __launch_bounds__(kSharedMergeThreads) void kv8_shared_merge_kernel(Kv8SharedArgs s) {
@@ -441,9 +413,10 @@ __global__ __launch_bounds__(kSharedMergeThreads) void kv8_shared_merge_kernel(K
   int lg = 0;
   while (lg < 3 && (kSharedMergeBatch << lg) < n) ++lg;
   const int group = tid / LN, ln = tid % LN, d = 4 * ln;
-  for (int h0 = 0; h0 < a.G; h0 += GR >> lg) {
+  const int first = (int)blockIdx.z * kSharedMergeHeads, end = min(first + kSharedMergeHeads, a.G);
+  for (int h0 = first; h0 < end; h0 += GR >> lg) {
     const int head = h0 + (group >> lg);
-    const bool live = head < a.G;
+    const bool live = head < end;
     const int r0 = row.row0[0] + min(head, a.G - 1), r1 = row.row0[1] + min(head, a.G - 1);
     const uint32_t base0 = row.base[0] + (uint32_t)kvh * row.per_head[0] + (uint32_t)(r0 / TP);
     const uint32_t base1 = row.base[1] + (uint32_t)kvh * row.per_head[1] + (uint32_t)(r1 / TS);
@@ -510,12 +483,22 @@ using namespace sdv;
 static int shared_tile(int32_t G, int32_t max_q_len) { return (int64_t)G * max_q_len <= 16 ? 16 : 32; }
 
 // Rows of a prefix's tile, or 0 where a call takes longer here than in sdv_kv8_attention, which reads the prefix again for
-// every sequence, from the caches: it has one launch, and long tiles of a sequence's own rows.
-constexpr int64_t kSharedKeys = 1 << 18, kSharedWideKeys = 15 << 20;
+// every sequence, from the caches: it has one launch, and tiles of 256 of a sequence's own rows.  From 204 sizes of one group
+// (2 to 64 sequences, 1, 5 and 24 rows each, prefixes of 256 to 32768, heads 12/2/128 and 14/2/64), GPU time in us, sdv_kv8_attention
+// first, then tiles of 32 and of 128 rows, 12/2/128:
+//   up to 16 rows a sequence and KV head, by the keys not read again: 16 x 1 over 8192 18 19 25, 32 x 1 over 4096 17 17 23, 8 x 1 over
+//     32768 30 26 32, 32 x 1 over 8192 24 20 28, 64 x 1 over 8192 38 28 33;
+//   up to 64, by the prefix: 2 x 5 over 1024 13 14 19 and over 4096 18 15 21, 16 x 5 over 1024 14 16 22 and over 4096 25 24 26;
+//   more: 8 x 24 over 4096 31 34 40, 32 x 24 over 8192 85 133 93;
+//   and of the two kinds of tiles, by a group's rows times its prefix: 8 x 5 over 32768 49 40 42, 32 x 5 over 8192 42 43 42, 64 x 1 over
+//     32768 124 59 49, 32 x 5 over 32768 111 107 75, 64 x 5 over 32768 215 205 125; with heads of 64 from a third of that on (32 x 1 over
+//     16384 26 23 22, 64 x 1 over 4096 18 16 18).
+constexpr int64_t kSharedKeys = 1 << 18, kSharedPrefix = 1 << 12, kSharedWideKeys = 8 << 20;
 static int shared_rows(int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
                        int32_t max_prefix) {
-  const int64_t own = (int64_t)G * max_q_len, saved = (int64_t)(batch - groups) * max_prefix * kv_heads;
-  if (groups <= 0 || own > 64 || saved < (own <= 16 ? 2 * kSharedKeys : kSharedKeys / 2)) return 0;
+  const int64_t own = (int64_t)G * max_q_len;
+  if (groups <= 0 || batch == groups || own > 64) return 0;
+  if (own <= 16 ? (int64_t)(batch - groups) * max_prefix * kv_heads < kSharedKeys * 15 / 16 : max_prefix < kSharedPrefix) return 0;
   const int64_t keys = (int64_t)total * G / groups * max_prefix * kv_heads / 2;
   return keys >= (head_dim == 128 ? kSharedWideKeys : kSharedWideKeys / 3) ? kWideRows : 32;
 }
@@ -577,7 +560,7 @@ extern "C" size_t sdv_kv8_shared_attention_workspace_size(int32_t batch, int32_t
 
 template <int D, int FMT>
 static void shared_launch(const Kv8SharedArgs& s, int tile, hipStream_t st) {
-  const dim3 grid(kKv8Grid), merge((unsigned)s.a.r.total, (unsigned)s.a.kv_heads);
+  const dim3 grid(kKv8Grid), merge((unsigned)s.a.r.total, (unsigned)s.a.kv_heads, (unsigned)((s.a.G + kSharedMergeHeads - 1) / kSharedMergeHeads));
   if (tile == 16) {
     hipLaunchKernelGGL((kv8_shared_kernel<D, FMT, 1>), grid, dim3(kKv8Threads), 0, st, s);
     hipLaunchKernelGGL((kv8_shared_merge_kernel<D, 16>), merge, dim3(kSharedMergeThreads), 0, st, s);

@@ -245,6 +245,7 @@ def test_scales_that_lie_far_apart(cuda_device, heads, fmt):
 @pytest.mark.parametrize("heads,groups,rows", [
     ("target", [(16, [(9, 1)] * 3)], 0),                      # short
     ("target", [(4096 // 16, [(20, 1)] * 70)], 32),           # single tokens
+    ("mha", [(4096 // 16, [(20, 17)] * 2)], 32),              # more rows than one tile of 16 holds
     ("draft", [(8192 // 16, [(40, 5)] * 20)], 128),           # verify blocks
     ("target", [(8192 // 16, [(40, 20)] * 20)], 0)])          # 120 rows a sequence and KV head
 def test_the_faster_way_is_chosen(cuda_device, heads, groups, rows):
