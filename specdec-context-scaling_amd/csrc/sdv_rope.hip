@@ -64,102 +64,111 @@ struct Kv8RopeArgs {
 
 constexpr int kRopeHeads = 4;  // query heads of a wavefront
 
-// Workgroups (x, y): x a page block of a sequence, whichever of the call's rows fall in it; y a KV head, whose K and V
-// are quantized and written (as in kv8_append_kernel, but for K's rotation, which is not rounded in between), or
-// kRopeHeads query heads.
+// Workgroups (x, y) of one wavefront: x a page block of a sequence, whichever of the call's rows fall in it; y a KV head, whose K
+// is rotated, quantized and written, or one whose V is written (as by kv8_append_kernel), or kRopeHeads query heads of as
+// many of its tokens as a load has rows.  So many wavefronts share the angles of no more than four heads, but each is little
+// more than its loads one after another (lengths, rows, pages), which are what a call takes: a chunk of 2048 tokens with K, V
+// and all tokens' heads in one wavefront each took 8.9 us in a graph, 7.0 like this; 32 tokens 5.4 and 4.2.
 template <int D, int FMT, bool IL>
 __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
   constexpr int U = D / 16;      // lanes per row: a unit each
   constexpr int R = kWave / U;   // rows of a wave-wide load (8 or 16)
+  constexpr int P = kBlock / R;  // loads of a block
   __shared__ uint4 lds_v[D];
-  const int lane = threadIdx.x, u = lane % U, rr = lane / U;
+  const int lane = threadIdx.x, u = lane % U, rr = lane / U, y = blockIdx.y;
   const int d0 = rope_piece<IL>(a.rope, u, 0), d1 = rope_piece<IL>(a.rope, u, 1);
   const bool turn = u < a.rope.units;
   Kv8Tile t;
 
-  if ((int)blockIdx.y >= a.c.kv_heads) {  // query heads
+  if (y >= 2 * a.c.kv_heads) {  // query heads
     if (!kv8_tile<true, false>(a.c, (int)blockIdx.x, t)) return;
+    const int part = (y - 2 * a.c.kv_heads) % P, h0 = (y - 2 * a.c.kv_heads) / P * kRopeHeads;
+    const int first = max(t.t0, part * R), n = min(t.t1, (part + 1) * R) - first;
+    if (n <= 0) return;
     // of R rows, 2^lg are tokens and the others more heads of theirs
-    const int n = t.t1 - t.t0, h0 = ((int)blockIdx.y - a.c.kv_heads) * kRopeHeads;
     int lg = 0;
-    while ((1 << lg) < min(n, R)) ++lg;
-    const int step = R >> lg, hs = rr >> lg;
-    for (int g = 0; g < n; g += 1 << lg) {
-      const int tok = t.t0 + g + (rr & ((1 << lg) - 1));
-      const int64_t row = t.row + min(tok, t.t1 - 1);
-      const uint16_t* src = a.q + row * a.q_stride;
-      uint4 w[kRopeHeads][2];
-      const auto has = [&](int i) { return i * step + hs < kRopeHeads && h0 + i * step + hs < a.q_heads && tok < t.t1; };
+    while ((1 << lg) < n) ++lg;
+    const int step = R >> lg, hs = rr >> lg, tok = first + (rr & ((1 << lg) - 1));
+    const int64_t row = t.row + min(tok, t.t1 - 1);
+    const uint16_t* src = a.q + row * a.q_stride;
+    const auto has = [&](int i) { return i * step + hs < kRopeHeads && h0 + i * step + hs < a.q_heads && tok < first + n; };
+    uint4 w[kRopeHeads][2];
 #pragma unroll
-      for (int i = 0; i < kRopeHeads; ++i) {
-        if (!has(i)) continue;
-        w[i][0] = load_stream16(src + (h0 + i * step + hs) * D + d0);
-        w[i][1] = load_stream16(src + (h0 + i * step + hs) * D + d1);
-      }
-      float c[8], s[8];
-      if (turn) rope_angles(a.rope, u, a.positions ? a.positions[row] : t.block * kBlock + tok, c, s);
+    for (int i = 0; i < kRopeHeads; ++i) {
+      if (!has(i)) continue;
+      w[i][0] = load_stream16(src + (h0 + i * step + hs) * D + d0);
+      w[i][1] = load_stream16(src + (h0 + i * step + hs) * D + d1);
+    }
+    float c[8], s[8];
+    if (turn) rope_angles(a.rope, u, a.positions ? a.positions[row] : t.block * kBlock + tok, c, s);
 #pragma unroll
-      for (int i = 0; i < kRopeHeads; ++i) {
-        if (!has(i)) continue;
-        if (turn) {
-          float y[16];
-          rope_rotate<IL>(w[i][0], w[i][1], c, s, y);
-          w[i][0] = rope_pack8(y);
-          w[i][1] = rope_pack8(y + 8);
-        }
-        uint16_t* dst = a.q_out + row * a.out_stride + (h0 + i * step + hs) * D;
-        *reinterpret_cast<uint4*>(dst + d0) = w[i][0];
-        *reinterpret_cast<uint4*>(dst + d1) = w[i][1];
+    for (int i = 0; i < kRopeHeads; ++i) {
+      if (!has(i)) continue;
+      if (turn) {
+        float z[16];
+        rope_rotate<IL>(w[i][0], w[i][1], c, s, z);
+        w[i][0] = rope_pack8(z);
+        w[i][1] = rope_pack8(z + 8);
       }
+      uint16_t* dst = a.q_out + row * a.out_stride + (h0 + i * step + hs) * D;
+      *reinterpret_cast<uint4*>(dst + d0) = w[i][0];
+      *reinterpret_cast<uint4*>(dst + d1) = w[i][1];
     }
     return;
   }
 
+  // Tokens that are not the call's re-read a row that is; rows are loaded before it is known whether they have a block.
   if (!kv8_tile<true>(a.c, (int)blockIdx.x, t)) return;  // wave-uniform
-  const int id = kv8_block(a.c.r, t.b, t.block);
-  if (id < 0) return;
-  const int kvh = blockIdx.y;
-  const int64_t page = (int64_t)id * a.c.kv_heads + kvh;
-  uint8_t* kp = a.c.k_pages + page * (kBlock * D);
-  uint8_t* vp = a.c.v_pages + page * (kBlock * D);
-  float* sp = a.c.scales + page * (2 * kBlock);
-
-  // K: lane (rr, u) holds unit u of token j*R + rr; V as kv8_write_v has it.  Tokens that are not the call's re-read a
-  // row that is.
-  constexpr int JK = kBlock / R, LPR = D / 8, JV = kBlock * LPR / kWave;
-  uint4 kw[JK][2], vw[JV];
-  const uint16_t* kin = static_cast<const uint16_t*>(a.c.k) + kvh * D;
-  const uint16_t* vin = static_cast<const uint16_t*>(a.c.v) + kvh * D + 8 * (lane % LPR);
-  int pos[JK];
+  const int kvh = y % a.c.kv_heads;
+  if (y >= a.c.kv_heads) {  // V, as kv8_write_v has it
+    constexpr int LPR = D / 8, JV = kBlock * LPR / kWave;
+    const uint16_t* vin = static_cast<const uint16_t*>(a.c.v) + kvh * D + 8 * (lane % LPR);
+    uint4 vw[JV];
 #pragma unroll
-  for (int j = 0; j < JK; ++j) {
+    for (int j = 0; j < JV; ++j) {
+      const int tok = min(max(lane / LPR * JV + j, t.t0), t.t1 - 1);
+      vw[j] = load_stream16(vin + (int64_t)(t.row + tok) * a.c.v_stride);
+    }
+    const int id = kv8_block(a.c.r, t.b, t.block);
+    if (id < 0) return;
+    const int64_t page = (int64_t)id * a.c.kv_heads + kvh;
+    kv8_write_v<D, FMT>(t, vw, a.c.v_pages + page * (kBlock * D), a.c.scales + page * (2 * kBlock), lds_v);
+    return;
+  }
+
+  // K: lane (rr, u) holds unit u of token j*R + rr
+  uint4 kw[P][2];
+  const uint16_t* kin = static_cast<const uint16_t*>(a.c.k) + kvh * D;
+  int pos[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
     const int tok = min(max(j * R + rr, t.t0), t.t1 - 1);
     const uint16_t* src = kin + (int64_t)(t.row + tok) * a.c.k_stride;
     kw[j][0] = load_stream16(src + d0);
     kw[j][1] = load_stream16(src + d1);
     pos[j] = a.positions ? a.positions[t.row + tok] : t.block * kBlock + tok;
   }
+  const int id = kv8_block(a.c.r, t.b, t.block);
+  if (id < 0) return;
+  const int64_t page = (int64_t)id * a.c.kv_heads + kvh;
+  uint8_t* kp = a.c.k_pages + page * (kBlock * D);
+  float* sp = a.c.scales + page * (2 * kBlock);
 #pragma unroll
-  for (int j = 0; j < JV; ++j) {
-    const int tok = min(max(lane / LPR * JV + j, t.t0), t.t1 - 1);
-    vw[j] = load_stream16(vin + (int64_t)(t.row + tok) * a.c.v_stride);
-  }
-#pragma unroll
-  for (int j = 0; j < JK; ++j) {
+  for (int j = 0; j < P; ++j) {
     if (t.t1 <= j * R || t.t0 >= (j + 1) * R) continue;  // none of the call's tokens
     const int tok = j * R + rr;
-    float y[16];
+    float z[16];
     if (turn) {
       float c[8], s[8];
       rope_angles(a.rope, u, pos[j], c, s);
-      rope_rotate<IL>(kw[j][0], kw[j][1], c, s, y);
+      rope_rotate<IL>(kw[j][0], kw[j][1], c, s, z);
     } else {
 #pragma unroll
-      for (int k = 0; k < 16; ++k) y[k] = bf16_at(kw[j][k >> 3], k & 7);
+      for (int k = 0; k < 16; ++k) z[k] = bf16_at(kw[j][k >> 3], k & 7);
     }
     uint32_t ab = 0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) ab = max(ab, __float_as_uint(y[k]) & 0x7FFFFFFFu);
+    for (int k = 0; k < 16; ++k) ab = max(ab, __float_as_uint(z[k]) & 0x7FFFFFFFu);
     ab = unit_max_bits<U>(ab);
     constexpr float kQ = FMT == kFp8 ? 448.0f : 127.0f;
     float s = __uint_as_float(ab) / kQ;
@@ -167,20 +176,19 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
     const bool finite = ab < 0x7F800000u;
     // the largest quotient passes Q where the scale is below fp32's normal numbers
 #pragma unroll
-    for (int k = 0; k < 16; ++k) y[k] = finite ? fminf(fmaxf(y[k] / s, -kQ), kQ) : 0.0f;
+    for (int k = 0; k < 16; ++k) z[k] = finite ? fminf(fmaxf(z[k] / s, -kQ), kQ) : 0.0f;
     if (tok >= t.t0 && tok < t.t1) {
       uint8_t* dst = kp + (tok >> 2) * (4 * D) + (tok & 3) * 16;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int d = k == 0 ? d0 : d1;
         *reinterpret_cast<uint2*>(dst + (d >> 4) * 64 + (d & 8)) =
-            make_uint2(kv8_pack4<FMT>(y[8 * k], y[8 * k + 1], y[8 * k + 2], y[8 * k + 3]),
-                       kv8_pack4<FMT>(y[8 * k + 4], y[8 * k + 5], y[8 * k + 6], y[8 * k + 7]));
+            make_uint2(kv8_pack4<FMT>(z[8 * k], z[8 * k + 1], z[8 * k + 2], z[8 * k + 3]),
+                       kv8_pack4<FMT>(z[8 * k + 4], z[8 * k + 5], z[8 * k + 6], z[8 * k + 7]));
       }
       if (u == 0) sp[tok] = finite ? s : __builtin_nanf("");
     }
   }
-  kv8_write_v<D, FMT>(t, vw, vp, sp, lds_v);
 }
 
 }  // namespace sdv
@@ -246,7 +254,7 @@ extern "C" int sdv_kv8_rope_append(const void* q, int64_t q_stride, void* q_out,
   if (st != SDV_OK) return st;
   st = rope_check(inv_freq, rotary_dim, interleaved, head_dim);
   if (st != SDV_OK) return st;
-  if (q_heads <= 0 || q_heads > 65535 || kv_heads > 32767) return SDV_ERR_SHAPE;
+  if (q_heads <= 0 || q_heads > 65535 || kv_heads > 16383) return SDV_ERR_SHAPE;
   const int64_t row = (int64_t)q_heads * head_dim;
   if (q_stride < row || q_out_stride < row) return SDV_ERR_SHAPE;
   if (!aligned(q, 16) || !aligned(q_out, 16) || q_stride % 8 || q_out_stride % 8 || !aligned(positions, 4)) return SDV_ERR_ALIGN;
@@ -257,7 +265,7 @@ extern "C" int sdv_kv8_rope_append(const void* q, int64_t q_stride, void* q_out,
                          {inv_freq, rotary_dim / 16, scale, 1.0f}, positions, static_cast<const uint16_t*>(q),
                          static_cast<uint16_t*>(q_out), q_stride, q_out_stride, q_heads};
   dim3 grid = kv8_cache_grid(total_rows, batch, kv_heads);
-  grid.y += (unsigned)((q_heads + kRopeHeads - 1) / kRopeHeads);
+  grid.y = (unsigned)(2 * kv_heads + (q_heads + kRopeHeads - 1) / kRopeHeads * (head_dim / 64));  // a part per load of a block
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 128)
     format == SDV_KV8_FP8 ? kv8_rope_launch<128, kFp8>(a, interleaved, grid, s) : kv8_rope_launch<128, kInt8>(a, interleaved, grid, s);
