@@ -22,15 +22,17 @@ struct RopeArgs {
   float sign;              // -1: the inverse rotation (the transpose)
 };
 
+// Cosine and sine of frequency i at `pos`, with the scale and the sign.
+__device__ __forceinline__ void rope_angle(const RopeArgs& r, int i, int pos, float& c, float& s) {
+  const double p = (double)pos * 0.15915494309189535, f = r.inv_freq[i];  // 1 / (2 pi)
+  sincospif(2.0f * (float)__builtin_fma(p, f, -rint(p * f)), &s, &c);
+  c *= r.scale;
+  s *= r.scale * r.sign;
+}
+
 __device__ __forceinline__ void rope_angles(const RopeArgs& r, int u, int pos, float (&c)[8], float (&s)[8]) {
-  const double p = (double)pos * 0.15915494309189535;  // 1 / (2 pi)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const double f = r.inv_freq[8 * u + i];
-    sincospif(2.0f * (float)__builtin_fma(p, f, -rint(p * f)), &s[i], &c[i]);
-    c[i] *= r.scale;
-    s[i] *= r.scale * r.sign;
-  }
+  for (int i = 0; i < 8; ++i) rope_angle(r, 8 * u + i, pos, c[i], s[i]);
 }
 
 // First dimension of a unit's two pieces.
@@ -42,7 +44,7 @@ __device__ __forceinline__ int rope_piece(const RopeArgs& r, int u, int which) {
 
 // A unit's 16 values, rotated, in fp32.
 template <bool IL>
-__device__ __forceinline__ void rope_rotate(uint4 w0, uint4 w1, const float (&c)[8], const float (&s)[8], float (&y)[16]) {
+__device__ __forceinline__ void rope_rotate(uint4 w0, uint4 w1, const float* c, const float* s, float (&y)[16]) {
   const auto at = [&](int k) {
     const uint32_t w = k < 8 ? (&w0.x)[k >> 1] : (&w1.x)[(k & 7) >> 1];
     return (k & 1) ? bf16_hi(w) : bf16_lo(w);

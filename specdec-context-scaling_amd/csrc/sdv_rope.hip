@@ -15,40 +15,37 @@ struct RopeRows {
   int heads[2];
 };
 
-// A lane rotates one unit of a row in HP heads, so that its eight angles serve all of them.
-template <int D, bool IL, int HP>
-__global__ __launch_bounds__(256) void rope_kernel(RopeRows a) {
-  constexpr int U = D / 16;
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = e / U;
-  const int u = (int)(e % U), h0 = blockIdx.y * HP, heads = a.heads[0] + a.heads[1];
-  if (row >= a.rows) return;
+constexpr int kRopeThreads = 256, kRopeGroup = 8;  // threads and heads of a workgroup
+
+// A workgroup has kRopeGroup heads of as many rows as it has threads for.  A thread loads one unit and, meanwhile, works out one
+// of the rows' angles for all heads of the workgroup: with each lane's eight angles its own the calls waited for the sines.
+template <int D, bool IL>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeRows a) {
+  constexpr int U = D / 16, A = D / 2, RB = kRopeThreads / A;  // units and angles of a row; rows
+  __shared__ __align__(16) float cs[2][RB][A];
+  const int tid = threadIdx.x, r = tid / A, u = tid % U, heads = a.heads[0] + a.heads[1];
+  const int64_t row = (int64_t)blockIdx.x * RB + r;
+  const int h = blockIdx.y * kRopeGroup + tid % A / U, k = h >= a.heads[0];
+  const bool has = row < a.rows && h < heads, turn = u < a.rope.units;
   const int d0 = rope_piece<IL>(a.rope, u, 0), d1 = rope_piece<IL>(a.rope, u, 1);
-  uint4 w[HP][2];
-#pragma unroll
-  for (int i = 0; i < HP; ++i) {
-    const int h = min(h0 + i, heads - 1), k = h >= a.heads[0];
-    const uint16_t* src = a.in[k] + row * a.in_stride[k] + (int64_t)(h - (k ? a.heads[0] : 0)) * D;
-    w[i][0] = *reinterpret_cast<const uint4*>(src + d0);
-    w[i][1] = *reinterpret_cast<const uint4*>(src + d1);
+  const int64_t at = (int64_t)(h - (k ? a.heads[0] : 0)) * D;
+  uint4 w[2];
+  if (has) {
+    w[0] = *reinterpret_cast<const uint4*>(a.in[k] + row * a.in_stride[k] + at + d0);
+    w[1] = *reinterpret_cast<const uint4*>(a.in[k] + row * a.in_stride[k] + at + d1);
   }
-  const bool turn = u < a.rope.units;
-  float c[8], s[8];
-  if (turn) rope_angles(a.rope, u, a.positions[row], c, s);
-#pragma unroll
-  for (int i = 0; i < HP; ++i) {
-    const int h = h0 + i, k = h >= a.heads[0];
-    if (h >= heads) break;
-    if (turn) {
-      float y[16];
-      rope_rotate<IL>(w[i][0], w[i][1], c, s, y);
-      w[i][0] = rope_pack8(y);
-      w[i][1] = rope_pack8(y + 8);
-    }
-    uint16_t* dst = a.out[k] + row * a.out_stride[k] + (int64_t)(h - (k ? a.heads[0] : 0)) * D;
-    *reinterpret_cast<uint4*>(dst + d0) = w[i][0];
-    *reinterpret_cast<uint4*>(dst + d1) = w[i][1];
+  if (row < a.rows && tid % A < 8 * a.rope.units) rope_angle(a.rope, tid % A, a.positions[row], cs[0][r][tid % A], cs[1][r][tid % A]);
+  __syncthreads();
+  if (!has) return;
+  if (turn) {
+    float y[16];
+    rope_rotate<IL>(w[0], w[1], &cs[0][r][8 * u], &cs[1][r][8 * u], y);
+    w[0] = rope_pack8(y);
+    w[1] = rope_pack8(y + 8);
   }
+  uint16_t* dst = a.out[k] + row * a.out_stride[k] + at;
+  *reinterpret_cast<uint4*>(dst + d0) = w[0];
+  *reinterpret_cast<uint4*>(dst + d1) = w[1];
 }
 
 // ---------------------------------------------------------------------------- a step's rows
@@ -197,12 +194,9 @@ using namespace sdv;
 
 template <int D, bool IL>
 static void rope_launch(const RopeRows& a, hipStream_t st) {
-  const int heads = a.heads[0] + a.heads[1];
-  const int64_t blocks = ((int64_t)a.rows * (D / 16) + 255) / 256;
-  if (blocks * heads <= 1024)
-    hipLaunchKernelGGL((rope_kernel<D, IL, 1>), dim3((unsigned)blocks, (unsigned)heads), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((rope_kernel<D, IL, 4>), dim3((unsigned)blocks, (unsigned)((heads + 3) / 4)), dim3(256), 0, st, a);
+  constexpr int rows = kRopeThreads / (D / 2);
+  const dim3 grid((unsigned)((a.rows + rows - 1) / rows), (unsigned)((a.heads[0] + a.heads[1] + kRopeGroup - 1) / kRopeGroup));
+  hipLaunchKernelGGL((rope_kernel<D, IL>), grid, dim3(kRopeThreads), 0, st, a);
 }
 
 extern "C" int sdv_rope(const void* q, int64_t q_stride, int32_t q_heads, const void* k, int64_t k_stride, int32_t k_heads,
