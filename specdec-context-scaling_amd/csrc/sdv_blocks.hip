@@ -14,7 +14,7 @@ struct CopyArgs {
 };
 
 // A wavefront copies one block of one layer, its three parts as one run of 16-byte pieces, kCopyBatch of them a lane in
-// flight.
+// flight.  Bound by the memory: 3001 blocks of 18 layers (627 MB both ways) 102 us, 6.1 TB/s; 32 of them 4.5 us.
 constexpr int kCopyWaves = 4, kCopyBatch = 8;
 
 __global__ __launch_bounds__(kCopyWaves * kWave) void copy_blocks_kernel(CopyArgs a) {
@@ -59,6 +59,10 @@ constexpr int kKeepTokens = 64, kKeepThreads = 256;
 // A workgroup moves the tokens of one sequence, KV head and layer: 64 at a time, all of them read before the first is
 // written.  Destinations lie in order, so that with ascending entries (each at least its own index) a later batch reads
 // nothing that an earlier one has written.
+//
+// A token's V is one byte of every row of its page, so that it moves D / 4 times its bytes (whole cache lines) and a call
+// is bound by those and by its chain of loads (entries, pages, codes): the paths of 8 trees of 24 4.2 us in a graph, of 48 trees
+// of 64 in 8 KV heads 7.8.  With the loads of tokens that stay done too, so that eight are under way without a condition: 4.9, 10.8.
 template <int D>
 __global__ __launch_bounds__(kKeepThreads) void kv8_keep_kernel(KeepArgs a) {
   __shared__ __align__(16) uint8_t lds_k[kKeepTokens][D], lds_v[kKeepTokens][D];

@@ -30,11 +30,6 @@ __device__ __forceinline__ void rope_angle(const RopeArgs& r, int i, int pos, fl
   s *= r.scale * r.sign;
 }
 
-__device__ __forceinline__ void rope_angles(const RopeArgs& r, int u, int pos, float (&c)[8], float (&s)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) rope_angle(r, 8 * u + i, pos, c[i], s[i]);
-}
-
 // First dimension of a unit's two pieces.
 template <bool IL>
 __device__ __forceinline__ int rope_piece(const RopeArgs& r, int u, int which) {

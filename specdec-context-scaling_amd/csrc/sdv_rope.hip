@@ -18,7 +18,10 @@ struct RopeRows {
 constexpr int kRopeThreads = 256, kRopeGroup = 8;  // threads and heads of a workgroup
 
 // A workgroup has kRopeGroup heads of as many rows as it has threads for.  A thread loads one unit and, meanwhile, works out one
-// of the rows' angles for all heads of the workgroup: with each lane's eight angles its own the calls waited for the sines.
+// of the rows' angles for all heads of the workgroup.  32 rows of 14 heads of 128: 2.5 us in a graph (2.9 with each lane's eight
+// angles its own), of which an empty launch takes 2.1; 8191 rows of 16 heads of 64 7.4 us (8.1), 4.5 TB/s.  Those move what
+// a copy moves in 4.5 us: the rest is the start and some 190 vector instructions a thread, whose loads, sines and stores follow
+// one another in every thread at the same time.
 template <int D, bool IL>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeRows a) {
   constexpr int U = D / 16, A = D / 2, RB = kRopeThreads / A;  // units and angles of a row; rows
@@ -61,17 +64,44 @@ struct Kv8RopeArgs {
 
 constexpr int kRopeHeads = 4;  // query heads of a wavefront
 
+// A lane's eight angles of token `tok`, one of first .. first + n of a page block.  Of up to kRopeFew tokens the lanes work out
+// the angles in turns and share them: a lane's own eight, one after another, kept a step of one token a sequence waiting (32
+// of them 4.2 us in a graph, 3.7 like this), where a full block has work for every lane either way (2048 tokens 7.3 us, 9.1 with
+// their angles shared).
+constexpr int kRopeFew = 2;
+
+template <int D>
+__device__ __forceinline__ void rope_token(const Kv8RopeArgs& a, const Kv8Tile& t, int first, int n, int tok, int u, bool turn,
+                                           float (&cs)[2][kRopeFew][D / 2], float (&c)[8], float (&s)[8]) {
+  constexpr int A = D / 2;
+  const auto pos = [&](int tok) { return a.positions ? a.positions[t.row + tok] : t.block * kBlock + tok; };
+  if (n <= kRopeFew) {  // wave-uniform
+    for (int e = threadIdx.x; e < n * A; e += kWave)
+      if (e % A < 8 * a.rope.units) rope_angle(a.rope, e % A, pos(first + e / A), cs[0][e / A][e % A], cs[1][e / A][e % A]);
+    __syncthreads();  // of one wavefront
+    const int i = min(max(tok - first, 0), n - 1);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = cs[0][i][8 * u + k], s[k] = cs[1][i][8 * u + k];
+  } else if (turn) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) rope_angle(a.rope, 8 * u + k, pos(min(max(tok, first), first + n - 1)), c[k], s[k]);
+  }
+}
+
 // Workgroups (x, y) of one wavefront: x a page block of a sequence, whichever of the call's rows fall in it; y a KV head, whose K
 // is rotated, quantized and written, or one whose V is written (as by kv8_append_kernel), or kRopeHeads query heads of as
 // many of its tokens as a load has rows.  So many wavefronts share the angles of no more than four heads, but each is little
-// more than its loads one after another (lengths, rows, pages), which are what a call takes: a chunk of 2048 tokens with K, V
-// and all tokens' heads in one wavefront each took 8.9 us in a graph, 7.0 like this; 32 tokens 5.4 and 4.2.
+// more than its loads one after another (lengths, rows, pages), which are what a call takes: with K, V and all tokens of the
+// heads in one wavefront each a step of 2048 tokens took 8.9 us in a graph, 7.0 like this (7.3 with rope_token).
 template <int D, int FMT, bool IL>
 __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
   constexpr int U = D / 16;      // lanes per row: a unit each
   constexpr int R = kWave / U;   // rows of a wave-wide load (8 or 16)
   constexpr int P = kBlock / R;  // loads of a block
-  __shared__ uint4 lds_v[D];
+  __shared__ union {
+    uint4 v[D];
+    float cs[2][kRopeFew][D / 2];
+  } lds;
   const int lane = threadIdx.x, u = lane % U, rr = lane / U, y = blockIdx.y;
   const int d0 = rope_piece<IL>(a.rope, u, 0), d1 = rope_piece<IL>(a.rope, u, 1);
   const bool turn = u < a.rope.units;
@@ -97,7 +127,7 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
       w[i][1] = load_stream16(src + (h0 + i * step + hs) * D + d1);
     }
     float c[8], s[8];
-    if (turn) rope_angles(a.rope, u, a.positions ? a.positions[row] : t.block * kBlock + tok, c, s);
+    rope_token<D>(a, t, first, n, tok, u, turn, lds.cs, c, s);
 #pragma unroll
     for (int i = 0; i < kRopeHeads; ++i) {
       if (!has(i)) continue;
@@ -129,21 +159,19 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
     const int id = kv8_block(a.c.r, t.b, t.block);
     if (id < 0) return;
     const int64_t page = (int64_t)id * a.c.kv_heads + kvh;
-    kv8_write_v<D, FMT>(t, vw, a.c.v_pages + page * (kBlock * D), a.c.scales + page * (2 * kBlock), lds_v);
+    kv8_write_v<D, FMT>(t, vw, a.c.v_pages + page * (kBlock * D), a.c.scales + page * (2 * kBlock), lds.v);
     return;
   }
 
   // K: lane (rr, u) holds unit u of token j*R + rr
   uint4 kw[P][2];
   const uint16_t* kin = static_cast<const uint16_t*>(a.c.k) + kvh * D;
-  int pos[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) {
     const int tok = min(max(j * R + rr, t.t0), t.t1 - 1);
     const uint16_t* src = kin + (int64_t)(t.row + tok) * a.c.k_stride;
     kw[j][0] = load_stream16(src + d0);
     kw[j][1] = load_stream16(src + d1);
-    pos[j] = a.positions ? a.positions[t.row + tok] : t.block * kBlock + tok;
   }
   const int id = kv8_block(a.c.r, t.b, t.block);
   if (id < 0) return;
@@ -154,10 +182,9 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
   for (int j = 0; j < P; ++j) {
     if (t.t1 <= j * R || t.t0 >= (j + 1) * R) continue;  // none of the call's tokens
     const int tok = j * R + rr;
-    float z[16];
+    float z[16], c[8], s[8];
+    rope_token<D>(a, t, t.t0, t.t1 - t.t0, tok, u, turn, lds.cs, c, s);
     if (turn) {
-      float c[8], s[8];
-      rope_angles(a.rope, u, pos[j], c, s);
       rope_rotate<IL>(kw[j][0], kw[j][1], c, s, z);
     } else {
 #pragma unroll
@@ -168,12 +195,12 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
     for (int k = 0; k < 16; ++k) ab = max(ab, __float_as_uint(z[k]) & 0x7FFFFFFFu);
     ab = unit_max_bits<U>(ab);
     constexpr float kQ = FMT == kFp8 ? 448.0f : 127.0f;
-    float s = __uint_as_float(ab) / kQ;
-    if (s == 0.0f) s = 1.0f;
+    float scale = __uint_as_float(ab) / kQ;
+    if (scale == 0.0f) scale = 1.0f;
     const bool finite = ab < 0x7F800000u;
     // the largest quotient passes Q where the scale is below fp32's normal numbers
 #pragma unroll
-    for (int k = 0; k < 16; ++k) z[k] = finite ? fminf(fmaxf(z[k] / s, -kQ), kQ) : 0.0f;
+    for (int k = 0; k < 16; ++k) z[k] = finite ? fminf(fmaxf(z[k] / scale, -kQ), kQ) : 0.0f;
     if (tok >= t.t0 && tok < t.t1) {
       uint8_t* dst = kp + (tok >> 2) * (4 * D) + (tok & 3) * 16;
 #pragma unroll
@@ -183,7 +210,7 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
             make_uint2(kv8_pack4<FMT>(z[8 * k], z[8 * k + 1], z[8 * k + 2], z[8 * k + 3]),
                        kv8_pack4<FMT>(z[8 * k + 4], z[8 * k + 5], z[8 * k + 6], z[8 * k + 7]));
       }
-      if (u == 0) sp[tok] = finite ? s : __builtin_nanf("");
+      if (u == 0) sp[tok] = finite ? scale : __builtin_nanf("");
     }
   }
 }
