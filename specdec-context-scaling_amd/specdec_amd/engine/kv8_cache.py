@@ -14,6 +14,10 @@ Every call may give each sequence its own number of rows (``counts``): a step th
 sequences, verifies drafted blocks or trees of others and takes a chunk of a third one's prompt is
 one write and one attention per layer.
 
+``rope_write`` and ``append_attend(rope=...)`` give a step's q and K their rotary positions on the way (``ops.kv8_rope_append``),
+``keep`` leaves the accepted path of each verified tree (``ops.kv8_keep``), and ``attend`` reads the blocks that neighbouring
+sequences share (``fork``) once for them all (``ops.kv8_shared_attention``): a fork's sequences are best given numbers in a row.
+
 Recording into a HIP graph: with equal counts and lengths a recorded ``append_attend`` reads nothing
 from the host but the row table, which an earlier call with the same counts has made; what it cannot
 do inside a recording (add blocks, grow the pool, new tables) raises.  Pages and tables that a recording
@@ -45,6 +49,8 @@ class KV8Cache(PagedKVCache):
                          capacity_tokens=capacity_tokens, device=device, seed=seed, growable=growable)
         self._cu: tuple | None = None     # ((counts, stream), device row table) of the last call
         self._lens: tuple | None = None   # ((lengths, stream), device array) of the last call
+        self._prefixes: tuple | None = None  # ((groups and prefixes, stream), device array) of the last call
+        self._grouped: tuple | None = None   # (block table, whole blocks of context, group bounds, prefixes, what _find_groups kept)
         self._served = (None, None)       # block table and K pages that _streams stands for
         self._streams: set = set()        # streams that the allocator knows to use them
 
@@ -62,6 +68,14 @@ class KV8Cache(PagedKVCache):
         super()._grow(min_blocks)
         self._served = (None, None)
 
+    def _copy(self, src: list[int], dst: list[int], to=None) -> None:
+        self._note_stream()
+        super()._copy(src, dst, to)
+
+    def compact(self, num_blocks: int | None = None) -> None:
+        super().compact(num_blocks)
+        self._served, self._grouped = (None, None), None
+
     @property
     def scales(self) -> torch.Tensor:
         return self.v_scales  # the pool's third page tensor: here K's scales as well
@@ -72,6 +86,8 @@ class KV8Cache(PagedKVCache):
         its own, and a recording's is made with it."""
         for b in range(self.batch):
             self.reserve(b, n_tokens)
+        if self.alloc.shared:
+            self._own(self.lengths, [n_tokens] * self.batch)
         self.block_table()
 
     # ------------------------------------------------------------------ tables
@@ -106,6 +122,48 @@ class KV8Cache(PagedKVCache):
         self._lens = self._table("sequence lengths", self._lens, tuple(lengths), lambda: list(lengths))
         return self._hold(self._lens[1]), longest
 
+    def _groups(self, counts, lengths):
+        """(device group bounds, device prefix lengths, longest prefix) for ops.kv8_shared_attention, or None where no
+        neighbouring sequences begin with the same blocks.
+
+        A group goes on while the next sequence shares half of what its sequences share so far, so that one with a short
+        common beginning ends it.  Only what every row of the group sees counts: the prefix ends with the shortest
+        context before its new tokens."""
+        whole = [max(0, n - c) // BLOCK for n, c in zip(lengths, counts)]
+        table = self.block_table()
+        if self._grouped is None or self._grouped[0] is not table or self._grouped[1] != whole:
+            self._grouped = (table, whole, *self._find_groups(whole, {} if self._grouped is None or self._grouped[0] is not table
+                                                              else self._grouped[4]))
+        bounds, prefix = self._grouped[2:4]
+        longest = max(prefix)
+        if longest == 0:
+            return None
+        self._prefixes = self._table("shared prefixes", self._prefixes, (bounds, prefix), lambda: bounds + prefix)
+        on_device = self._hold(self._prefixes[1])
+        return on_device[:len(bounds)], on_device[len(bounds):], longest
+
+    def _find_groups(self, whole, same: dict):
+        """(group bounds, prefix lengths, `same`): sequence b's context is whole[b] whole blocks; `same` keeps how many first
+        blocks two sequences both hold."""
+        bounds, prefix, first, common = [0], [0] * self.batch, 0, None
+        for b in range(1, self.batch + 1):
+            now = 0
+            if b < self.batch:
+                if (first, b) not in same:
+                    x, y = self.blocks[first], self.blocks[b]
+                    same[first, b] = next((j for j, (i, k) in enumerate(zip(x, y)) if i != k), min(len(x), len(y)))
+                now = min(same[first, b], whole[first], whole[b], *(() if common is None else (common,)))
+            if now > 0 and (common is None or 2 * now >= common):
+                common = now
+                continue
+            if common is None and first > 0 and prefix[first - 1] == 0:
+                bounds[-1] = b  # one more that shares nothing
+            else:
+                bounds.append(b)
+                prefix[first:b] = [(common or 0) * BLOCK] * (b - first)
+            first, common = b, None
+        return tuple(bounds), tuple(prefix), same
+
     def _note_stream(self) -> None:
         """The block table and the pages are one for all streams, and go back to the memory of the stream
         that made them when they are replaced.  The allocator is told of every other stream that uses them,
@@ -137,6 +195,14 @@ class KV8Cache(PagedKVCache):
         """Append counts[b] tokens to each sequence of one layer: k_new/v_new BF16 (sum(counts), KV, D),
         sequence after sequence.  Positions start at ``starts`` (default: the current lengths); the
         lengths become start + count."""
+        cu, ends = self._room(k_new, counts, starts)
+        if max(ends) > 0:
+            lens, longest = self._lengths(ends)
+            ops.kv8_append(k_new, v_new, *self._operands(layer), cu, lens, longest)
+        self.lengths[:] = ends
+
+    def _room(self, k_new: torch.Tensor, counts, starts):
+        """(device row table, lengths afterwards) of a write, with the blocks that it needs."""
         starts = list(self.lengths) if starts is None else [int(s) for s in starts]
         counts, cu = self._rows(counts)
         ends = [s + c for s, c in zip(starts, counts)]
@@ -146,9 +212,49 @@ class KV8Cache(PagedKVCache):
             raise SdvError(f"k_new {tuple(k_new.shape)} does not hold {sum(counts)} rows")
         for b in range(self.batch):
             self.reserve(b, ends[b])
+        if self.alloc.shared:
+            self._own(starts, ends)
+        return cu, ends
+
+    def rope_write(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, counts, inv_freq: torch.Tensor, starts=None, *,
+                   interleaved: bool = False, rope_scale: float = 1.0, positions: torch.Tensor | None = None) -> torch.Tensor:
+        """write() of rows whose q and k have no positions yet: in one launch k_new is rotated and written, and q BF16
+        (sum(counts), H, D) rotated and returned.  inv_freq and rope_scale: ops.rope_frequencies.  positions (int32, one a row): those of
+        rows that do not stand where they are written, a tree's nodes (the context and the node's depth)."""
+        cu, ends = self._room(k_new, counts, starts)
         if max(ends) > 0:
             lens, longest = self._lengths(ends)
-            ops.kv8_append(k_new, v_new, *self._operands(layer), cu, lens, longest)
+            q = ops.kv8_rope_append(q, k_new, v_new, *self._operands(layer), cu, lens, longest, inv_freq, interleaved=interleaved,
+                                    scale=rope_scale, positions=positions)
+        self.lengths[:] = ends
+        return q
+
+    def keep(self, paths, starts) -> None:
+        """After the verify of drafted trees: of the tokens from position starts[b] on (its tree's nodes) sequence b keeps
+        those numbered paths[b], ascending, moved together in all layers; its length becomes starts[b] + len(paths[b]).  A sequence
+        stays as it is with no path and its length as the start."""
+        paths, starts = [[int(i) for i in p] for p in paths], [int(s) for s in starts]
+        if len(paths) != self.batch or len(starts) != self.batch:
+            raise ValueError(f"{len(paths)} paths and {len(starts)} starts for a batch of {self.batch}")
+        for p, s, n in zip(paths, starts, self.lengths):
+            if not 0 <= s <= n or any(y <= x for x, y in zip([-1] + p, p + [n - s])):
+                raise ValueError(f"path {p} from position {s} of a sequence of {n} tokens")
+        _no_recording(self.device, "a path would be copied from the host")
+        ends = [s + len(p) for p, s in zip(paths, starts)]
+        # those before the first gap are where they belong
+        gaps = [next((i for i, x in enumerate(p) if x != i), len(p)) for p in paths]
+        if self.alloc.shared:
+            self._own([s + g for s, g in zip(starts, gaps)], ends)
+        cu, flat = [0], []
+        for p, g in zip(paths, gaps):
+            flat += [x - g for x in p[g:]]
+            cu.append(len(flat))
+        if flat:
+            table = torch.tensor(cu + [s + g for s, g in zip(starts, gaps)] + flat, dtype=torch.int32).to(self.device)
+            bt = self.block_table()
+            self._note_stream()
+            B = self.batch
+            ops.kv8_keep(self.k_pages, self.v_pages, self.scales, bt, table[:B + 1], table[2 * B + 1:], table[B + 1:2 * B + 1])
         self.lengths[:] = ends
 
     def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, starts: list[int] | None = None):
@@ -166,20 +272,14 @@ class KV8Cache(PagedKVCache):
 
     def attend(self, layer: int, q: torch.Tensor, *, counts=None, q_token_major: bool = False, lengths=None,
                scale: float | None = None, tree_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-        """Attention of every sequence's last tokens over this layer's pages at the current lengths.
+        """Attention of every sequence's last tokens over this layer's pages at the current lengths.  The blocks that
+        neighbouring sequences both hold from their first on (fork) are read once for them all.
 
         q BF16 (sum(counts), H, D) with ``counts`` rows per sequence; without counts (B, H, S, D), or
         (B, S, H, D) with q_token_major, S rows of every sequence.  Returns out shaped like q.
         tree_mask (int64, one word a row): see ops.kv8_attention."""
         lengths = list(self.lengths) if lengths is None else [int(n) for n in lengths]
-        rows, shape = q, None
-        if counts is None:
-            if q.dim() != 4 or q.shape[0] != self.batch:
-                raise SdvError(f"q {tuple(q.shape)} is not (B = {self.batch}, H, S, D); with rows of different counts pass counts")
-            rows = q if q_token_major else q.transpose(1, 2)
-            shape = rows.shape
-            counts = (shape[1],) * self.batch
-            rows = rows.reshape(-1, *shape[2:])
+        rows, shape, counts = self._packed(q, counts, q_token_major)
         counts, cu = self._rows(counts)
         if rows.dim() != 3 or rows.shape[0] != sum(counts):
             raise SdvError(f"q {tuple(q.shape)} does not hold {sum(counts)} rows")
@@ -187,8 +287,26 @@ class KV8Cache(PagedKVCache):
             raise SdvError(f"out {tuple(out.shape)} != q {tuple(q.shape)}")
         direct = out if shape is None else None
         lens, longest = self._lengths(lengths)
-        got = ops.kv8_attention(rows, *self._operands(layer), cu, lens, max(1, *counts), max(1, longest), scale=scale,
-                                tree_mask=tree_mask, out=direct)
+        groups = self._groups(counts, lengths) if self.alloc.shared else None
+        if groups is None:
+            got = ops.kv8_attention(rows, *self._operands(layer), cu, lens, max(1, *counts), max(1, longest), scale=scale,
+                                    tree_mask=tree_mask, out=direct)
+        else:
+            got = ops.kv8_shared_attention(rows, *self._operands(layer), cu, lens, max(1, *counts), max(1, longest), *groups, scale=scale,
+                                           tree_mask=tree_mask, out=direct)
+        return self._unpacked(got, shape, q_token_major, out)
+
+    def _packed(self, q: torch.Tensor, counts, q_token_major: bool):
+        """(q's rows sequence after sequence, its shape token-major or None where it came like that, counts)."""
+        if counts is not None:
+            return q, None, counts
+        if q.dim() != 4 or q.shape[0] != self.batch:
+            raise SdvError(f"q {tuple(q.shape)} is not (B = {self.batch}, H, S, D); with rows of different counts pass counts")
+        rows = q if q_token_major else q.transpose(1, 2)
+        return rows.reshape(-1, *rows.shape[2:]), rows.shape, (rows.shape[1],) * self.batch
+
+    @staticmethod
+    def _unpacked(got: torch.Tensor, shape, q_token_major: bool, out):
         if shape is not None:
             got = got.view(shape)
             got = got if q_token_major else got.transpose(1, 2).contiguous()
@@ -198,14 +316,32 @@ class KV8Cache(PagedKVCache):
 
     def append_attend(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, starts: list[int] | None = None, *,
                       counts=None, q_token_major: bool = False, scale: float | None = None, tree_mask: torch.Tensor | None = None,
-                      out: torch.Tensor | None = None) -> torch.Tensor:
+                      out: torch.Tensor | None = None, rope: torch.Tensor | None = None, interleaved: bool = False, rope_scale: float = 1.0,
+                      positions: torch.Tensor | None = None) -> torch.Tensor:
         """The layer's new tokens written, then attention over the context that includes them: k_new and
-        v_new as for write() with ``counts``, else (B, S, KV, D); q as for attend()."""
+        v_new as for write() with ``counts``, else (B, S, KV, D); q as for attend().
+
+        rope (float64 frequencies of ops.rope_frequencies): q and k_new have no positions yet and get them on the way, as in
+        rope_write(), which takes the three arguments behind it (positions: one a row, sequence after sequence)."""
+        if rope is None:
+            if interleaved or rope_scale != 1.0 or positions is not None:
+                raise ValueError("interleaved, rope_scale and positions go with rope")
+            if counts is None:
+                self.append(layer, k_new, v_new, starts)
+            else:
+                self.write(layer, k_new, v_new, counts, starts)
+            return self.attend(layer, q, counts=counts, q_token_major=q_token_major, scale=scale, tree_mask=tree_mask, out=out)
+        rows, shape, per_seq = self._packed(q, counts, q_token_major)
+        if out is not None and out.shape != q.shape:
+            raise SdvError(f"out {tuple(out.shape)} != q {tuple(q.shape)}")
         if counts is None:
-            self.append(layer, k_new, v_new, starts)
-        else:
-            self.write(layer, k_new, v_new, counts, starts)
-        return self.attend(layer, q, counts=counts, q_token_major=q_token_major, scale=scale, tree_mask=tree_mask, out=out)
+            if k_new.shape[:2] != shape[:2]:
+                raise SdvError(f"k_new {tuple(k_new.shape)} does not hold the tokens of q {tuple(q.shape)}")
+            k_new, v_new = (t.reshape(-1, self.kv_heads, self.head_dim) for t in (k_new, v_new))
+        rows = self.rope_write(layer, rows, k_new, v_new, per_seq, rope, starts, interleaved=interleaved, rope_scale=rope_scale,
+                               positions=positions)
+        got = self.attend(layer, rows, counts=per_seq, scale=scale, tree_mask=tree_mask, out=out if shape is None else None)
+        return self._unpacked(got, shape, q_token_major, out)
 
     def read(self, layer: int, counts, starts=None):
         """(k, v) BF16 (sum(counts), KV, D): counts[b] tokens of each sequence from position starts[b]

@@ -25,6 +25,12 @@ recording read stay alive as long as the pool.  A graph goes on with those it wa
 once the pool has grown, what it writes does not reach the new pages, and it has to be
 recorded again.
 
+Sharing: ``fork`` gives a sequence the first tokens of another without copying them -- whole page blocks
+are held by both, the last one, if it is not full, is copied -- so a prompt that many sequences continue
+is stored (and, by KV8Cache.attend, read) once.  A sequence that would write into a block others hold, which
+it can only after a trim below the fork, gets its own copy of it first.  ``compact`` moves the blocks in use
+into page tensors of their number.  Both copy every layer in one launch (``ops.copy_blocks``).
+
 Ownership rule (the reference's trim returns views and its appends build new tensors, so an
 untrimmed handle keeps its data; here appends write pages in place): after
 ``trim``/``set_length`` to n tokens, the next append overwrites slots n.. of that sequence,
@@ -61,6 +67,7 @@ class BlockAllocator:
         self.seed = seed
         self._rng = random.Random(seed) if seed is not None else None
         self.free: list[int] = []
+        self.shared: dict[int, int] = {}  # blocks that several sequences hold: how many beyond the first
         self.grow(num_blocks)
 
     def grow(self, new_total: int) -> None:
@@ -76,8 +83,27 @@ class BlockAllocator:
             raise RuntimeError(f"block pool exhausted: need {n}, {len(self.free)} free of {self.num_blocks}")
         return [self.free.pop() for _ in range(n)]
 
+    def share(self, blocks) -> None:
+        """One more holder of each of `blocks`."""
+        for b in blocks:
+            self.shared[b] = self.shared.get(b, 0) + 1
+
     def release(self, blocks) -> None:
-        self.free.extend(reversed(list(blocks)))
+        """One holder less of each of `blocks`; those that no one holds any more are free."""
+        blocks = list(blocks)
+        if self.shared:
+            blocks = [b for b in blocks if not self._still_held(b)]
+        self.free.extend(reversed(blocks))
+
+    def _still_held(self, b: int) -> bool:
+        more = self.shared.get(b)
+        if more is None:
+            return False
+        if more == 1:
+            del self.shared[b]
+        else:
+            self.shared[b] = more - 1
+        return True
 
 
 class PagedKVCache:
@@ -160,11 +186,85 @@ class PagedKVCache:
         if need <= 0:
             return
         _no_recording(self.device, f"sequence {seq} needs {need} more page blocks")
-        if need > len(self.alloc.free):
+        self.blocks[seq].extend(self._take(need))
+        self._bt = None
+
+    def _take(self, n: int) -> list[int]:
+        if n > len(self.alloc.free):
             if not self.growable:
                 raise RuntimeError(f"block pool exhausted ({self.alloc.num_blocks} blocks) and growable=False")
-            self._grow(self.alloc.num_blocks + need)
-        self.blocks[seq].extend(self.alloc.alloc(need))
+            self._grow(self.alloc.num_blocks + n)
+        return self.alloc.alloc(n)
+
+    def _copy(self, src: list[int], dst: list[int], to=None) -> None:
+        """Blocks src to dst (of the page tensors `to`), all layers in one launch."""
+        pairs = torch.tensor([src, dst], dtype=torch.int32).to(self.device)
+        ops.copy_blocks(self.k_pages, self.v_pages, self.v_scales, pairs[0], pairs[1], to=to)
+
+    def _own(self, starts, ends) -> bool:
+        """Before positions starts[b] .. ends[b] - 1 are written: each of their blocks that another sequence
+        holds too is replaced by a copy.  Whether there was one."""
+        at = [(b, j) for b, (s, e) in enumerate(zip(starts, ends)) if e > s
+              for j in range(s // BLOCK, min(-(-e // BLOCK), len(self.blocks[b]))) if self.blocks[b][j] in self.alloc.shared]
+        if not at:
+            return False
+        _no_recording(self.device, "a shared page block would be copied")
+        fresh = self._take(len(at))
+        old = [self.blocks[b][j] for b, j in at]
+        self._copy(old, fresh)
+        for (b, j), new in zip(at, fresh):
+            self.blocks[b][j] = new
+        self.alloc.release(old)
+        self._bt = None
+        return True
+
+    def fork(self, src: int, dst, n_tokens: int | None = None) -> None:
+        """Sequence `dst`, or each of several, becomes the first n_tokens tokens (default: all) of `src`, in all layers.
+        What it held before is freed.
+
+        Whole blocks are shared, the last one, if it is not full, copied: what either sequence writes from there on is
+        its own.  A recorded step of `dst` has to be recorded again, one of `src` goes on as it was."""
+        to = [int(d) for d in dst] if hasattr(dst, "__iter__") else [int(dst)]
+        if not 0 <= src < self.batch or any(not 0 <= d < self.batch for d in to) or src in to or len(set(to)) != len(to):
+            raise ValueError(f"cannot fork sequence {src} into {to} in a batch of {self.batch}")
+        n = self.lengths[src] if n_tokens is None else int(n_tokens)
+        if not 0 <= n <= self.lengths[src]:
+            raise ValueError(f"sequence {src} has {self.lengths[src]} tokens, {n} asked for")
+        _no_recording(self.device, "the block table would be rebuilt")
+        for d in to:
+            self.free_sequence(d)
+        full, rest = divmod(n, BLOCK)
+        whole, last = self.blocks[src][:full], []
+        if rest and to:
+            last = self._take(len(to))
+            self._copy([self.blocks[src][full]] * len(to), last)
+        for i, d in enumerate(to):
+            self.alloc.share(whole)
+            self.blocks[d] = whole + last[i:i + 1]
+            self.lengths[d] = n
+        self._bt = None
+
+    def compact(self, num_blocks: int | None = None) -> None:
+        """Page tensors of num_blocks blocks (default: as many as are in use), with the blocks in use moved together in
+        the sequences' order.  Slots handed out before name other tokens' places then, and recorded steps have to be
+        recorded again."""
+        moved: dict[int, int] = {}
+        for blocks in self.blocks:
+            for b in blocks:
+                moved.setdefault(b, len(moved))
+        n = max(1, len(moved)) if num_blocks is None else int(num_blocks)
+        if n < max(1, len(moved)):
+            raise ValueError(f"{len(moved)} blocks are in use, {n} asked for")
+        _no_recording(self.device, "the page pool would be replaced")
+        pages = self._new_pages(n)
+        if moved:
+            self._copy(list(moved), list(moved.values()), to=pages)
+        self.k_pages, self.v_pages, self.v_scales = pages
+        shared = {moved[b]: more for b, more in self.alloc.shared.items()}
+        self.alloc = BlockAllocator(n, self.alloc.seed)
+        self.alloc.free = [b for b in self.alloc.free if b >= len(moved)]
+        self.alloc.shared = shared
+        self.blocks = [[moved[b] for b in blocks] for blocks in self.blocks]
         self._bt = None
 
     def reserve_all(self, n_tokens: int, q_heads: int | None = None, q_len: int | None = None) -> None:
@@ -175,6 +275,8 @@ class PagedKVCache:
         served and none given, the workspace is sized by the first call)."""
         for b in range(self.batch):
             self.reserve(b, n_tokens)
+        if self.alloc.shared:
+            self._own(self.lengths, [n_tokens] * self.batch)
         self.block_table()
         heads = q_heads or self._q_heads
         rows = max(q_len or 0, self._q_len, 1)
@@ -248,6 +350,8 @@ class PagedKVCache:
         starts = list(self.lengths) if starts is None else list(starts)
         for b in range(B):
             self.reserve(b, starts[b] + S)
+        if self.alloc.shared:
+            self._own(starts[:B], [n + S for n in starts[:B]])
         slots = self.slot_mapping(starts, S)
         kp, vp, vs = self.layer(layer)
         ops.quant_append(v_new.reshape(B * S, self.kv_heads, self.head_dim), slots, kp, vp, vs,
@@ -269,6 +373,8 @@ class PagedKVCache:
         starts = list(self.lengths) if starts is None else list(starts)
         for b in range(B):
             self.reserve(b, starts[b] + S)
+        if self.alloc.shared:
+            self._own(starts[:B], [n + S for n in starts[:B]])
         for b in range(B):
             self.lengths[b] = starts[b] + S
         tmax = max(self.lengths)
@@ -348,6 +454,9 @@ class PagedKVCache:
         for b, n in enumerate(lengths):
             if n > len(self.blocks[b]) * BLOCK:
                 self.reserve(b, n)
+        if self.alloc.shared and self._own([0] * self.batch, lengths) and slots is not None:
+            raise SdvError("some of these sequences' blocks were another's too and have been replaced: the slots given name the "
+                           "old ones (pass none)")
         on_device = self.device.type == "cuda"
         key = (tuple(lengths), ops._stream(self.k_pages.device) if on_device else 0)
         stale = self._tiles is None or self._tiles[:2] != key
