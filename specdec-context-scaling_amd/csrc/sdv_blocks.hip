@@ -54,17 +54,22 @@ struct KeepArgs {
   int kv_heads;
 };
 
-constexpr int kKeepTokens = 64, kKeepThreads = 256;
+constexpr int kKeepTokens = 64;
+template <int D>
+constexpr int kKeepThreads = 2 * D;
 
 // A workgroup moves the tokens of one sequence, KV head and layer: 64 at a time, all of them read before the first is
 // written.  Destinations lie in order, so that with ascending entries (each at least its own index) a later batch reads
 // nothing that an earlier one has written.
 //
 // A token's V is one byte of every row of its page, so that it moves D / 4 times its bytes (whole cache lines) and a call
-// is bound by those and by its chain of loads (entries, pages, codes): the paths of 8 trees of 24 4.2 us in a graph, of 48 trees
-// of 64 in 8 KV heads 7.8.  With the loads of tokens that stay done too, so that eight are under way without a condition: 4.9, 10.8.
+// is bound by those and by its chain of loads (entries, pages, codes): the paths of 8 trees of 24 (2 KV heads of 128, 28 layers)
+// 4.3 us in a graph, of 48 trees of 64 (2 of 64, 24 layers) 7.3.  Two tokens' V at a time: with 256 threads for 64 dimensions
+// too the latter take 7.8, with 128 for 128 the former 4.9.  With the loads of tokens that stay done too, so that eight are under
+// way without a condition: 4.9, 10.8.
 template <int D>
-__global__ __launch_bounds__(kKeepThreads) void kv8_keep_kernel(KeepArgs a) {
+__global__ __launch_bounds__(kKeepThreads<D>) void kv8_keep_kernel(KeepArgs a) {
+  constexpr int T = kKeepThreads<D>;
   __shared__ __align__(16) uint8_t lds_k[kKeepTokens][D], lds_v[kKeepTokens][D];
   __shared__ float lds_s[kKeepTokens][2];
   __shared__ int from[kKeepTokens], to[kKeepTokens];  // slots, -1: none
@@ -93,35 +98,35 @@ __global__ __launch_bounds__(kKeepThreads) void kv8_keep_kernel(KeepArgs a) {
     }
     __syncthreads();
 #pragma unroll 2
-    for (int e = tid; e < m * (D / 16); e += kKeepThreads) {
+    for (int e = tid; e < m * (D / 16); e += T) {
       const int i = e / (D / 16), c = e % (D / 16), x = from[i];
       if (x >= 0)
         *reinterpret_cast<uint4*>(&lds_k[i][16 * c]) = *reinterpret_cast<const uint4*>(k + page(x) * (kBlock * D) + (x >> 2 & 3) * (4 * D) + c * 64 + (x & 3) * 16);
     }
 #pragma unroll 4
-    for (int e = tid; e < m * D; e += kKeepThreads) {
+    for (int e = tid; e < m * D; e += T) {
       const int i = e / D, d = e % D, x = from[i];
       if (x >= 0) lds_v[i][d] = v[page(x) * (kBlock * D) + d * kBlock + (x & 15)];
     }
-    if (tid < 2 * m && from[tid >> 1] >= 0) {
-      const int x = from[tid >> 1];
-      lds_s[tid >> 1][tid & 1] = s[page(x) * (2 * kBlock) + (tid & 1) * kBlock + (x & 15)];
+    for (int e = tid; e < 2 * m; e += T) {
+      const int x = from[e >> 1];
+      if (x >= 0) lds_s[e >> 1][e & 1] = s[page(x) * (2 * kBlock) + (e & 1) * kBlock + (x & 15)];
     }
     __syncthreads();
 #pragma unroll 2
-    for (int e = tid; e < m * (D / 16); e += kKeepThreads) {
+    for (int e = tid; e < m * (D / 16); e += T) {
       const int i = e / (D / 16), c = e % (D / 16), y = to[i];
       if (y >= 0)
         *reinterpret_cast<uint4*>(k + page(y) * (kBlock * D) + (y >> 2 & 3) * (4 * D) + c * 64 + (y & 3) * 16) = *reinterpret_cast<const uint4*>(&lds_k[i][16 * c]);
     }
 #pragma unroll 4
-    for (int e = tid; e < m * D; e += kKeepThreads) {
+    for (int e = tid; e < m * D; e += T) {
       const int i = e / D, d = e % D, y = to[i];
       if (y >= 0) v[page(y) * (kBlock * D) + d * kBlock + (y & 15)] = lds_v[i][d];
     }
-    if (tid < 2 * m && to[tid >> 1] >= 0) {
-      const int y = to[tid >> 1];
-      s[page(y) * (2 * kBlock) + (tid & 1) * kBlock + (y & 15)] = lds_s[tid >> 1][tid & 1];
+    for (int e = tid; e < 2 * m; e += T) {
+      const int y = to[e >> 1];
+      if (y >= 0) s[page(y) * (2 * kBlock) + (e & 1) * kBlock + (y & 15)] = lds_s[e >> 1][e & 1];
     }
     __syncthreads();  // the LDS arrays; and a later batch's reads stand behind this one's writes
   }
@@ -170,8 +175,8 @@ extern "C" int sdv_kv8_keep(void* k_pages, void* v_pages, float* scales, int32_t
   const dim3 grid((unsigned)batch, (unsigned)kv_heads, (unsigned)num_layers);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 128)
-    hipLaunchKernelGGL((kv8_keep_kernel<128>), grid, dim3(kKeepThreads), 0, s, a);
+    hipLaunchKernelGGL((kv8_keep_kernel<128>), grid, dim3(kKeepThreads<128>), 0, s, a);
   else
-    hipLaunchKernelGGL((kv8_keep_kernel<64>), grid, dim3(kKeepThreads), 0, s, a);
+    hipLaunchKernelGGL((kv8_keep_kernel<64>), grid, dim3(kKeepThreads<64>), 0, s, a);
   return hipGetLastError() == hipSuccess ? SDV_OK : SDV_ERR_HIP;
 }
