@@ -409,7 +409,8 @@ int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const void* k_pages,
  * group).  prefix_lens, int32 [batch], the same for a group's sequences: the first prefix_lens[b] tokens, taken down to
  * whole blocks (and to max_prefix_len), are the blocks that the table names for the group's first sequence.  Every row
  * of the group sees all of them, and of its own sequence the keys from there on that sdv_kv8_attention has it see: with
- * prefixes within the contexts (prefix_lens[b] <= seq_lens[b] - rows) the result is that of sdv_kv8_attention.
+ * prefixes within the contexts (prefix_lens[b] <= seq_lens[b] - rows) and a table that names the same blocks for all of
+ * a group the result is that of sdv_kv8_attention.
  * A sequence in no group whose prefix_lens is not 0 does not see those keys at all.  groups may be 0.
  * tile_rows: rows of a prefix's tile, 32 (operands and sums as in sdv_kv8_attention's tiles of 32) or 128 (as in its
  * tiles of 256, but that an item, up to 1/512 of the call, whose V scales lie more than 2^18 apart is computed as with 32); a

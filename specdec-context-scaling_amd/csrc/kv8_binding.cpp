@@ -451,10 +451,8 @@ PyObject* shared(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const int32_t ng = (int32_t)cg->size(0) - 1;
   if (tile == 0) {
     tile = g_shared_rows(p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix);
-    if (tile == 0) {  // as every sequence by itself, or sizes that the general path refuses
-      if (max_prefix > (int64_t)p.max_blocks * 16 ||
-          g_shared_size(p.batch, ng, (int32_t)total, (int32_t)heads, p.kv, p.d, (int32_t)max_q, (int32_t)max_len, (int32_t)max_prefix, 32) == 0)
-        Py_RETURN_NONE;
+    if (tile == 0) {  // every sequence by itself
+      if (max_prefix > (int64_t)p.max_blocks * 16) Py_RETURN_NONE;
       PyObject* const plain[12] = {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], o[8], o[12], o[13], n == 16 ? o[15] : Py_None};
       return attention(nullptr, plain, 12);
     }

@@ -838,10 +838,13 @@ def kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     """kv8_attention for sequences that begin with the same pages, whose shared keys are read and computed once for each group of them.
 
     cu_groups int32 (groups + 1,): group g is sequences cu_groups[g] .. cu_groups[g+1] - 1; a sequence may be in none.  prefix_lens
-    int32 (B,), the same for all of a group and at most each one's context before its new tokens (0 for a sequence in no group): as
-    many first tokens, taken down to whole blocks, are the blocks that the table names for the group's first sequence.  Every row
-    of the group sees them all, then its own sequence's keys from there on.  max_prefix_len bounds them.  The other arguments, and the
-    result, are kv8_attention's, to the order of the sums.  For few new tokens a sequence: tiles hold 32 rows of a group.
+    int32 (B,), the same for all of a group and at most each one's context before its new tokens (0 for a sequence in no group): so
+    many first tokens, taken down to whole blocks, are blocks that the table names alike for all of the group.  Every row of the group
+    sees them all, then its own sequence's keys from there on.  max_prefix_len bounds them.  The other arguments, and the result, are
+    kv8_attention's, to the order of the sums.
+
+    tile_rows: rows of the group that a workgroup has at a time, 32 or 128; 0: whichever is faster for these sizes, or kv8_attention where
+    that is faster than both (short prefixes, few sequences, more than 64 rows of a sequence and KV head).
     """
     got = _native.binding().shared(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups,
                                    prefix_lens, max_prefix_len, scale, tree_mask, tile_rows, out)
@@ -876,18 +879,20 @@ def kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
         out_row = H * d
     else:
         out, out_row = _kv8_rows(_same_rows(out, total, "out"), "out", dev, H, d, write=True)
+    if not 0 <= max_prefix_len <= mb * BLOCK:
+        _fail(f"max_prefix_len {max_prefix_len} outside the table's {mb} blocks")
     lib = _native.load()
     sizes = (B, groups, total, H, kv, d, max_q_len, max_seq_len, max_prefix_len)
     tile = tile_rows or lib.sdv_kv8_shared_attention_tile_rows(*sizes)
-    nbytes = lib.sdv_kv8_shared_attention_workspace_size(*sizes, tile or 32)
-    if nbytes == 0 or max_prefix_len > mb * BLOCK:
+    if tile == 0:
+        return kv8_attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale=scale,
+                             tree_mask=tree_mask, out=out)
+    nbytes = lib.sdv_kv8_shared_attention_workspace_size(*sizes, tile)
+    if nbytes == 0:
         _fail(f"unsupported sizes B={B} groups={groups} rows={total} H={H} KV={kv} D={d} max_q_len={max_q_len} "
               f"max_seq_len={max_seq_len} max_prefix_len={max_prefix_len}")
     if total == 0:
         return out
-    if tile == 0:
-        return kv8_attention(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, scale=scale,
-                             tree_mask=tree_mask, out=out)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _kv8_call(lib.sdv_kv8_shared_attention, "sdv_kv8_shared_attention", dev, q.data_ptr(), q_row, k_pages.data_ptr(), v_pages.data_ptr(),
               scales.data_ptr(), nb, fmt, block_table.data_ptr(), mb, cu, lens, tree, cu_groups.data_ptr(), prefix, B, groups, total, H, kv,
@@ -977,6 +982,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
     n, H, d = q.shape
     if d not in (64, 128):
         _fail(f"head_dim must be 64 or 128 (got {d})")
+    if H == 0:
+        _fail(f"q {tuple(q.shape)} has no heads")
     r = _frequencies(inv_freq, dev, d)
     pos = _kv8_ints(positions, "positions", dev, n)
     outs = [torch.empty((n, H, d), dtype=torch.bfloat16, device=dev) if q_out is None else q_out]
@@ -993,7 +1000,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
         _fail("k_out without k")
     else:
         outs.append(None)
-    if n and H:
+    if n:
         _kv8_call(_native.load().sdv_rope, "sdv_rope", dev, q.data_ptr(), qs, H, kp, ks, kh, pos, inv_freq.data_ptr(), r,
                   int(bool(interleaved)), float(scale), int(bool(inverse)), n, d, outs[0].data_ptr(), qos, kop, kos)
     return tuple(outs)

@@ -307,7 +307,7 @@ def test_refusals(cuda_device):
     x, pos, inv = _rows((6, h + kv, d), 3).to(dev), _ints(list(range(6)), dev), ops.rope_frequencies(d, device=dev)[0]
     q, k = x[:, :h], x[:, h:]
     for bad in (dict(q=q.float()), dict(k=k[:5]), dict(positions=pos.long()), dict(positions=pos[:5]), dict(positions=pos.cpu()),
-                dict(inv_freq=inv.float()), dict(inv_freq=inv[:5]), dict(inv_freq=torch.cat((inv, inv))), dict(inv_freq=inv[:0]), dict(q=q[..., :32]),
+                dict(q=q[:, :0]), dict(inv_freq=inv.float()), dict(inv_freq=inv[:5]), dict(inv_freq=torch.cat((inv, inv))), dict(inv_freq=inv[:0]), dict(q=q[..., :32]),
                 dict(q_out=q[:5]), dict(k=None, k_out=k.clone()), dict(q_out=torch.empty((6, h, d + 1), dtype=torch.bfloat16, device=dev)[..., :d])):
         args = dict(q=q, k=k, positions=pos, inv_freq=inv)
         args.update(bad)

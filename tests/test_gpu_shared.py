@@ -344,3 +344,17 @@ def test_refusals(cuda_device):
             ops.kv8_shared_attention(**{**good, **bad})
     with pytest.raises(ValueError):
         ops.kv8_shared_attention(**good, tile_rows=64)
+
+
+def test_sizes_that_only_plain_attention_takes(cuda_device):
+    """Bounds of the lengths and the prefix that are too large together for shared attention's plan: sequence by sequence."""
+    dev = cuda_device
+    case = Case("target", "fp8", CASES["pair"])
+    args = list(case.args(dev))
+    wide = torch.full((2, 5_000_000), -1, dtype=torch.int32, device=dev)
+    wide[:, :case.table.shape[1]] = args[3]
+    args[3], args[7], args[10] = wide, 100_000_000, 80_000_000
+    announce("shared with bounds of 100 and 80 million tokens")
+    ref.within(ops.kv8_shared_attention(case.q.to(dev), *args), *case.want())
+    with pytest.raises(SdvError, match="unsupported sizes"):
+        ops.kv8_shared_attention(case.q.to(dev), *args, tile_rows=32)
