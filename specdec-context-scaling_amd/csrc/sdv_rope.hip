@@ -31,7 +31,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeRows a) {
   const int h = blockIdx.y * kRopeGroup + tid % A / U, k = h >= a.heads[0];
   const bool has = row < a.rows && h < heads, turn = u < a.rope.units;
   const int d0 = rope_piece<IL>(a.rope, u, 0), d1 = rope_piece<IL>(a.rope, u, 1);
-  const int64_t at = (int64_t)(h - (k ? a.heads[0] : 0)) * D;
+  const int at = (h - (k ? a.heads[0] : 0)) * D;
   uint4 w[2];
   if (has) {
     w[0] = *reinterpret_cast<const uint4*>(a.in[k] + row * a.in_stride[k] + at + d0);
@@ -123,8 +123,8 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
 #pragma unroll
     for (int i = 0; i < kRopeHeads; ++i) {
       if (!has(i)) continue;
-      w[i][0] = load_stream16(src + (h0 + i * step + hs) * D + d0);
-      w[i][1] = load_stream16(src + (h0 + i * step + hs) * D + d1);
+      w[i][0] = *reinterpret_cast<const uint4*>(src + (h0 + i * step + hs) * D + d0);
+      w[i][1] = *reinterpret_cast<const uint4*>(src + (h0 + i * step + hs) * D + d1);
     }
     float c[8], s[8];
     rope_token<D>(a, t, first, n, tok, u, turn, lds.cs, c, s);
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
 #pragma unroll
     for (int j = 0; j < JV; ++j) {
       const int tok = min(max(lane / LPR * JV + j, t.t0), t.t1 - 1);
-      vw[j] = load_stream16(vin + (int64_t)(t.row + tok) * a.c.v_stride);
+      vw[j] = *reinterpret_cast<const uint4*>(vin + (int64_t)(t.row + tok) * a.c.v_stride);
     }
     const int id = kv8_block(a.c.r, t.b, t.block);
     if (id < 0) return;
@@ -170,8 +170,8 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
   for (int j = 0; j < P; ++j) {
     const int tok = min(max(j * R + rr, t.t0), t.t1 - 1);
     const uint16_t* src = kin + (int64_t)(t.row + tok) * a.c.k_stride;
-    kw[j][0] = load_stream16(src + d0);
-    kw[j][1] = load_stream16(src + d1);
+    kw[j][0] = *reinterpret_cast<const uint4*>(src + d0);
+    kw[j][1] = *reinterpret_cast<const uint4*>(src + d1);
   }
   const int id = kv8_block(a.c.r, t.b, t.block);
   if (id < 0) return;
