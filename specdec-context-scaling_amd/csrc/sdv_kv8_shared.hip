@@ -35,7 +35,7 @@ struct Kv8SharedRow {
 };
 
 constexpr int kSharedStart = 5;   // steps that starting an item costs, about
-constexpr int kSharedWide = 4;    // steps that one of kWideRows rows costs, about
+constexpr int kSharedWide = 3;    // a step's time with kWideRows rows; with tiles of 16 rows of a sequence it is 1, of 32 2, about
 constexpr int kSharedShort = 4;   // steps of those that an item has at least: its part costs as much
 
 // Prefix v, or sequence v - groups: its rows, keys and blocks.
@@ -91,7 +91,8 @@ struct Kv8SharedTables {
 };
 
 struct Kv8SharedLds {
-  uint32_t sum[kKv8Threads / kWave][2];  // steps (those of a wide tile by kSharedWide) and tiles
+  uint32_t sum[kKv8Threads / kWave][2];  // steps, by the time that they take, and tiles
+  uint32_t less[kKv8Threads / kWave];  // items of all prefixes and sequences, of fewer steps
   uint2 run[kKv8Threads];  // items of prefixes, and of sequences, of the wavefront's runs up to and with this one
 };
 
@@ -99,7 +100,7 @@ struct Kv8SharedLds {
 template <int TS>
 struct Kv8SharedItems {
   int count, per_run;       // prefixes and sequences; of a thread's run
-  uint32_t length[2];       // steps of an item of a prefix, and of a sequence, at most
+  uint32_t length[2];       // steps of an item of a prefix, and of a sequence, at most: they take as long
   uint32_t per_head[2];     // items of a KV head
   uint32_t items;
 
@@ -113,25 +114,25 @@ struct Kv8SharedItems {
   // seqs: a run's last prefix or sequence, its only one where the runs hold one each.
   __device__ __forceinline__ void begin(const Kv8SharedArgs& s, Kv8SharedLds& lds, Kv8SharedSeq* seqs, uint32_t grid) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const uint32_t heads = (uint32_t)s.a.kv_heads, weight = s.wide ? kSharedWide : 1;
+    const uint32_t heads = (uint32_t)s.a.kv_heads, weight = s.wide ? kSharedWide : 1, own = s.wide ? TS / 16 : 1;
     count = s.groups + s.a.r.batch;
     per_run = (count + kKv8Threads - 1) / kKv8Threads;
     uint32_t steps = 0, tiles = 0;
     const auto count_in = [&](int y, const Kv8SharedSeq& q) {
-      steps += (uint32_t)q.tiles * q.steps() * (y < s.groups ? weight : 1);
+      steps += (uint32_t)q.tiles * q.steps() * (y < s.groups ? weight : own);
       tiles += (uint32_t)q.tiles;
       seqs[tid] = q;
     };
     if (per_run == 1) {
       Kv8SharedTables& tables = *reinterpret_cast<Kv8SharedTables*>(seqs + kKv8Threads);
       const int b = tid - s.groups;
-      const bool own = b >= 0 && tid < count;
+      const bool has = b >= 0 && tid < count;
       int g0 = 0, g1 = 0, len = 0;
       if (tid < s.groups) {
         g0 = s.cu_groups[tid];
         g1 = s.cu_groups[tid + 1];
       }
-      if (own) {
+      if (has) {
         const int first = s.a.r.cu[b], P = s.prefix[b];
         if (s.a.lens) len = s.a.lens[b];
         tables.cu[b] = first;
@@ -142,7 +143,7 @@ struct Kv8SharedItems {
       if (tid < s.groups) {
         const int b0 = min(max(g0, 0), s.a.r.batch), b1 = min(max(g1, b0), s.a.r.batch);
         count_in(tid, kv8_shared_prefix<TS>(s, b0, b1, tables.cu[b0], tables.cu[b1], tables.prefix[min(b0, s.a.r.batch - 1)]));
-      } else if (own) {
+      } else if (has) {
         count_in(tid, kv8_shared_own<TS>(s, b, tables.cu[b], tables.cu[b + 1], tables.prefix[b], len));
       }
     } else {
@@ -167,21 +168,39 @@ struct Kv8SharedItems {
     }
     steps = __builtin_amdgcn_readfirstlane(steps) * heads;
     tiles = __builtin_amdgcn_readfirstlane(tiles) * heads;
-    // A tile of n steps has at most n / length + 1 chunks, so this length leaves an item for every workgroup; where the tiles
-    // alone are too many for that, an even share of the steps and starts.
-    uint32_t each = 2 * tiles <= grid ? steps / (grid - tiles) + 1 : (steps + kSharedStart * tiles) / grid + 1;
-    each = (each + 3) & ~3u;
-    length[1] = each;
-    length[0] = s.wide ? max(each / kSharedWide, (uint32_t)kSharedShort) : each;
-    uint2 mine = make_uint2(0, 0);
+    // A tile of n steps has at most n / length + 1 chunks, so `most` steps leave an item for every workgroup, whatever the
+    // tiles.  They are as many as that takes where every tile is cut short, and `less`, half way to where none is, do too as a
+    // rule: then they are taken.  Where the tiles alone are too many for that, an even share of the steps and starts.
+    const bool fits = 2 * tiles <= grid;
+    const uint32_t most = fits ? steps / (grid - tiles) + 1 : (steps + kSharedStart * tiles) / grid + 1;
+    const uint32_t less = fits ? (most + steps / grid + 1) / 2 : most;
+    const auto share = [&](uint32_t each, int i) -> uint32_t {
+      if (i == 1 || !s.wide) return ((each + own - 1) / own + 3) & ~3u;
+      return max((each + kSharedWide - 1) / kSharedWide, (uint32_t)kSharedShort);
+    };
+    uint32_t n_of[2][2] = {{0, 0}, {0, 0}};  // by share and kind
     for (int k = 0; k < per_run; ++k) {
       const int y = tid * per_run + k;
       if (y >= count) break;
       const Kv8SharedSeq q = per_run == 1 ? seqs[tid] : kv8_shared_seq<TS>(s, y);
-      const uint32_t n = (uint32_t)q.tiles * chunks_of(y < s.groups ? 0 : 1, q.steps());
-      mine.x += y < s.groups ? n : 0;
-      mine.y += y < s.groups ? 0 : n;
+      const int i = y < s.groups ? 0 : 1;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t len = share(t ? less : most, i), n = (uint32_t)q.tiles * ((q.steps() + len - 1) / len);
+        n_of[t][0] += i == 0 ? n : 0;
+        n_of[t][1] += i == 1 ? n : 0;
+      }
     }
+    const uint32_t with_less = kv8_lane_scan(n_of[1][0] + n_of[1][1]);
+    if (lane == kWave - 1) lds.less[wave] = with_less;
+    __syncthreads();
+    uint32_t n_less = 0;
+#pragma unroll
+    for (int k = 0; k < kKv8Threads / kWave; ++k) n_less += lds.less[k];
+    const bool take = fits && __builtin_amdgcn_readfirstlane(n_less) * heads <= grid;
+    length[0] = share(take ? less : most, 0);
+    length[1] = share(take ? less : most, 1);
+    const uint2 mine = take ? make_uint2(n_of[1][0], n_of[1][1]) : make_uint2(n_of[0][0], n_of[0][1]);
     lds.run[tid] = make_uint2(kv8_lane_scan(mine.x), kv8_lane_scan(mine.y));
     __syncthreads();
     per_head[0] = per_head[1] = 0;
@@ -522,7 +541,7 @@ static int shared_sizes(int32_t batch, int32_t groups, int32_t total, int32_t q_
   if (((int64_t)max_len + max_prefix + total) * G > (1 << 30)) return SDV_ERR_SHAPE;
   const int64_t prefixes = shared_tiles(0, false, batch, groups, total, G, kv_heads, max_q_len), own = shared_tiles(1, false, batch, groups, total, G, kv_heads, max_q_len);
   if (prefixes + own > INT32_MAX / 8) return SDV_ERR_SHAPE;
-  const int64_t steps = prefixes * (max_prefix / kKv8Step + 1) * kSharedWide + own * (max_len / kKv8Step + 1) + (prefixes + own) * kSharedStart;
+  const int64_t steps = prefixes * (max_prefix / kKv8Step + 1) * kSharedWide + own * 2 * (max_len / kKv8Step + 1) + (prefixes + own) * kSharedStart;
   return steps > INT32_MAX / 4 ? SDV_ERR_SHAPE : SDV_OK;
 }
 
