@@ -168,39 +168,50 @@ struct Kv8SharedItems {
     }
     steps = __builtin_amdgcn_readfirstlane(steps) * heads;
     tiles = __builtin_amdgcn_readfirstlane(tiles) * heads;
-    // A tile of n steps has at most n / length + 1 chunks, so `most` steps leave an item for every workgroup, whatever the
-    // tiles.  They are as many as that takes where every tile is cut short, and `less`, half way to where none is, do too as a
-    // rule: then they are taken.  Where the tiles alone are too many for that, an even share of the steps and starts.
-    const bool fits = 2 * tiles <= grid;
-    const uint32_t most = fits ? steps / (grid - tiles) + 1 : (steps + kSharedStart * tiles) / grid + 1;
-    const uint32_t less = fits ? (most + steps / grid + 1) / 2 : most;
-    const auto share = [&](uint32_t each, int i) -> uint32_t {
-      if (i == 1 || !s.wide) return ((each + own - 1) / own + 3) & ~3u;
-      return max((each + kSharedWide - 1) / kSharedWide, (uint32_t)kSharedShort);
+    // A tile of n steps has at most n / length + 1 chunks, so with an even share of the steps over the workgroups that the tiles
+    // leave (and two for each XCD, which takes an eighth of either kind's items, rounded up) there is a workgroup for every
+    // item.  Where the tiles alone are too many for that: an even share of the steps and starts.
+    const bool fits = 2 * tiles <= grid - 16;
+    uint32_t each = fits ? steps / (grid - 16 - tiles) + 1 : (steps + kSharedStart * tiles) / grid + 1;
+    const auto share = [&](uint32_t each) {
+      length[1] = ((each + own - 1) / own + 3) & ~3u;
+      length[0] = s.wide ? max((each + kSharedWide - 1) / kSharedWide, (uint32_t)kSharedShort) : length[1];
     };
-    uint32_t n_of[2][2] = {{0, 0}, {0, 0}};  // by share and kind
-    for (int k = 0; k < per_run; ++k) {
-      const int y = tid * per_run + k;
-      if (y >= count) break;
-      const Kv8SharedSeq q = per_run == 1 ? seqs[tid] : kv8_shared_seq<TS>(s, y);
-      const int i = y < s.groups ? 0 : 1;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint32_t len = share(t ? less : most, i), n = (uint32_t)q.tiles * ((q.steps() + len - 1) / len);
-        n_of[t][0] += i == 0 ? n : 0;
-        n_of[t][1] += i == 1 ? n : 0;
+    const auto items_of = [&]() {
+      uint2 n = make_uint2(0, 0);
+      for (int k = 0; k < per_run; ++k) {
+        const int y = tid * per_run + k;
+        if (y >= count) break;
+        const Kv8SharedSeq q = per_run == 1 ? seqs[tid] : kv8_shared_seq<TS>(s, y);
+        const uint32_t c = (uint32_t)q.tiles * chunks_of(y < s.groups ? 0 : 1, q.steps());
+        n.x += y < s.groups ? c : 0;
+        n.y += y < s.groups ? 0 : c;
       }
-    }
-    const uint32_t with_less = kv8_lane_scan(n_of[1][0] + n_of[1][1]);
-    if (lane == kWave - 1) lds.less[wave] = with_less;
-    __syncthreads();
-    uint32_t n_less = 0;
+      return n;
+    };
+    uint2 mine;
+    bool taken = false;
+    // That is what it takes where every tile ends in a short item.  As a rule there is a workgroup for each with items half way to
+    // where none does: then they are taken, with tiles of kWideRows (32 x 5 rows over 32768 tokens 76.2 -> 72.9 us; with
+    // tiles of 32, whose steps are short, the more parts take longer: 32 x 1 over 8192 20.3 -> 24.3).
+    if (s.wide && fits) {
+      share((each + steps / grid + 1) / 2);
+      mine = items_of();
+      const uint32_t n = kv8_lane_scan(min(mine.x, 1023u) | min(mine.y, 1023u) << 16);  // more do not fit anyway
+      if (lane == kWave - 1) lds.less[wave] = n;
+      __syncthreads();
+      uint32_t p = 0, q = 0;
 #pragma unroll
-    for (int k = 0; k < kKv8Threads / kWave; ++k) n_less += lds.less[k];
-    const bool take = fits && __builtin_amdgcn_readfirstlane(n_less) * heads <= grid;
-    length[0] = share(take ? less : most, 0);
-    length[1] = share(take ? less : most, 1);
-    const uint2 mine = take ? make_uint2(n_of[1][0], n_of[1][1]) : make_uint2(n_of[0][0], n_of[0][1]);
+      for (int k = 0; k < kKv8Threads / kWave; ++k) {
+        p += lds.less[k] & 0xFFFF;
+        q += lds.less[k] >> 16;
+      }
+      taken = (__builtin_amdgcn_readfirstlane(p) * heads + 7) / 8 + (__builtin_amdgcn_readfirstlane(q) * heads + 7) / 8 <= grid / 8;
+    }
+    if (!taken) {
+      share(each);
+      mine = items_of();
+    }
     lds.run[tid] = make_uint2(kv8_lane_scan(mine.x), kv8_lane_scan(mine.y));
     __syncthreads();
     per_head[0] = per_head[1] = 0;
