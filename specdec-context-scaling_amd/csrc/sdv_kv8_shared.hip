@@ -516,13 +516,14 @@ static int shared_tile(int32_t G, int32_t max_q_len) { return (int64_t)G * max_q
 // every sequence, from the caches: it has one launch, and tiles of 256 of a sequence's own rows.  From 204 sizes of one group
 // (2 to 64 sequences, 1, 5 and 24 rows each, prefixes of 256 to 32768, heads 12/2/128 and 14/2/64), GPU time in us, sdv_kv8_attention
 // first, then tiles of 32 and of 128 rows, 12/2/128:
-//   up to 16 rows a sequence and KV head, by the keys not read again: 16 x 1 over 8192 18 19 25, 32 x 1 over 4096 17 17 23, 8 x 1 over
-//     32768 30 26 32, 32 x 1 over 8192 24 20 28, 64 x 1 over 8192 38 28 33;
-//   up to 64, by the prefix: 2 x 5 over 1024 13 14 19 and over 4096 18 15 21, 16 x 5 over 1024 14 16 22 and over 4096 25 24 26;
-//   more: 8 x 24 over 4096 31 34 40, 32 x 24 over 8192 85 133 93;
-//   and of the two kinds of tiles, by a group's rows times its prefix: 8 x 5 over 32768 49 40 42, 32 x 5 over 8192 42 43 42, 64 x 1 over
-//     32768 124 59 49, 32 x 5 over 32768 111 107 75, 64 x 5 over 32768 215 205 125; with heads of 64 from a third of that on (32 x 1 over
-//     16384 26 23 22, 64 x 1 over 4096 18 16 18).
+//   up to 16 rows a sequence and KV head, by the keys not read again: 16 x 1 over 8192 19 19 26, 32 x 1 over 4096 17 17 23, 8 x 1 over
+//     32768 30 26 33, 32 x 1 over 8192 24 20 28, 64 x 1 over 8192 38 29 34;
+//   up to 64, by the prefix: 2 x 5 over 1024 13 14 19 and over 4096 18 15 21, 16 x 5 over 1024 14 16 22 and over 4096 25 24 27;
+//   more: 8 x 24 over 4096 31 34 39, 32 x 24 over 8192 81 134 88;
+//   and of the two kinds of tiles, by a group's rows times its prefix: 8 x 5 over 32768 50 41 42, 32 x 5 over 8192 43 44 42, 64 x 1 over
+//     32768 126 65 50, 32 x 5 over 32768 112 109 71, 64 x 5 over 32768 217 206 131; with heads of 64 from a third of that on (32 x 1 over
+//     16384 27 23 23, 64 x 1 over 4096 18 17 19).
+// Over all of the sizes this takes 1.2% longer than the fastest of the three for each.
 constexpr int64_t kSharedKeys = 1 << 18, kSharedPrefix = 1 << 12, kSharedWideKeys = 8 << 20;
 static int shared_rows(int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
                        int32_t max_prefix) {
