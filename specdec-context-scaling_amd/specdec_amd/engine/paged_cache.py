@@ -201,6 +201,16 @@ class PagedKVCache:
         pairs = torch.tensor([src, dst], dtype=torch.int32).to(self.device)
         ops.copy_blocks(self.k_pages, self.v_pages, self.v_scales, pairs[0], pairs[1], to=to)
 
+    def _copies(self, src: list[int]) -> list[int]:
+        """New blocks that hold what `src` do."""
+        fresh = self._take(len(src))
+        try:
+            self._copy(src, fresh)
+        except BaseException:
+            self.alloc.release(fresh)
+            raise
+        return fresh
+
     def _own(self, starts, ends) -> bool:
         """Before positions starts[b] .. ends[b] - 1 are written: each of their blocks that another sequence
         holds too is replaced by a copy.  Whether there was one."""
@@ -209,9 +219,8 @@ class PagedKVCache:
         if not at:
             return False
         _no_recording(self.device, "a shared page block would be copied")
-        fresh = self._take(len(at))
         old = [self.blocks[b][j] for b, j in at]
-        self._copy(old, fresh)
+        fresh = self._copies(old)
         for (b, j), new in zip(at, fresh):
             self.blocks[b][j] = new
         self.alloc.release(old)
@@ -236,8 +245,7 @@ class PagedKVCache:
         full, rest = divmod(n, BLOCK)
         whole, last = self.blocks[src][:full], []
         if rest and to:
-            last = self._take(len(to))
-            self._copy([self.blocks[src][full]] * len(to), last)
+            last = self._copies([self.blocks[src][full]] * len(to))
         for i, d in enumerate(to):
             self.alloc.share(whole)
             self.blocks[d] = whole + last[i:i + 1]

@@ -185,6 +185,22 @@ def test_refusals(kind):
 
 @KINDS
 @pytest.mark.parametrize("call", ["fork", "compact", "write"])
+def test_a_copy_that_fails_loses_no_blocks(kind, call, monkeypatch):
+    m = Model(kind, 3, 12)
+    m.write(0, 40)
+    m.fork(0, 1)
+    m.trim(1, 20)
+
+    def fails(*a, **kw):
+        raise SdvError("no copy")
+    monkeypatch.setattr(paged_cache.ops, "copy_blocks", fails)
+    with pytest.raises(SdvError, match="no copy"):
+        {"fork": lambda: m.pool.fork(0, 2), "compact": m.pool.compact, "write": lambda: m.write(1, 1)}[call]()
+    m.check()
+
+
+@KINDS
+@pytest.mark.parametrize("call", ["fork", "compact", "write"])
 def test_a_recording_is_refused(kind, call, monkeypatch):
     m = Model(kind, 3, 12)
     m.write(0, 40)
