@@ -50,7 +50,7 @@ class KV8Cache(PagedKVCache):
         self._cu: tuple | None = None     # ((counts, stream), device row table) of the last call
         self._lens: tuple | None = None   # ((lengths, stream), device array) of the last call
         self._prefixes: tuple | None = None  # ((groups and prefixes, stream), device array) of the last call
-        self._grouped: tuple | None = None   # (block table, whole blocks of context, group bounds, prefixes, what _find_groups kept)
+        self._grouped: tuple | None = None   # (block table, counts, lengths, what _find_groups kept, group bounds, prefixes)
         self._served = (None, None)       # block table and K pages that _streams stands for
         self._streams: set = set()        # streams that the allocator knows to use them
 
@@ -129,12 +129,12 @@ class KV8Cache(PagedKVCache):
         A group goes on while the next sequence shares half of what its sequences share so far, so that one with a short
         common beginning ends it.  Only what every row of the group sees counts: the prefix ends with the shortest
         context before its new tokens."""
-        whole = [max(0, n - c) // BLOCK for n, c in zip(lengths, counts)]
-        table = self.block_table()
-        if self._grouped is None or self._grouped[0] is not table or self._grouped[1] != whole:
-            self._grouped = (table, whole, *self._find_groups(whole, {} if self._grouped is None or self._grouped[0] is not table
-                                                              else self._grouped[4]))
-        bounds, prefix = self._grouped[2:4]
+        table, kept = self.block_table(), self._grouped
+        if kept is None or kept[0] is not table or kept[1] != counts or kept[2] != lengths:  # once for a step's layers
+            same = {} if kept is None or kept[0] is not table else kept[3]
+            whole = [max(0, n - c) // BLOCK for n, c in zip(lengths, counts)]
+            kept = self._grouped = (table, counts, list(lengths), same, *self._find_groups(whole, same))
+        bounds, prefix = kept[4:]
         longest = max(prefix)
         if longest == 0:
             return None
@@ -143,8 +143,8 @@ class KV8Cache(PagedKVCache):
         return on_device[:len(bounds)], on_device[len(bounds):], longest
 
     def _find_groups(self, whole, same: dict):
-        """(group bounds, prefix lengths, `same`): sequence b's context is whole[b] whole blocks; `same` keeps how many first
-        blocks two sequences both hold."""
+        """(group bounds, prefix lengths): sequence b's context is whole[b] whole blocks; `same` keeps how many first blocks two
+        sequences both hold."""
         bounds, prefix, first, common = [0], [0] * self.batch, 0, None
         for b in range(1, self.batch + 1):
             now = 0
@@ -162,7 +162,7 @@ class KV8Cache(PagedKVCache):
                 bounds.append(b)
                 prefix[first:b] = [(common or 0) * BLOCK] * (b - first)
             first, common = b, None
-        return tuple(bounds), tuple(prefix), same
+        return tuple(bounds), tuple(prefix)
 
     def _note_stream(self) -> None:
         """The block table and the pages are one for all streams, and go back to the memory of the stream
