@@ -95,6 +95,13 @@ class BlockAllocator:
             blocks = [b for b in blocks if not self._still_held(b)]
         self.free.extend(reversed(blocks))
 
+    def take_back(self, blocks) -> None:
+        """What release(blocks) has given back, held again."""
+        free = set(self.free)
+        self.share(b for b in blocks if b not in free)
+        again = free.intersection(blocks)
+        self.free = [b for b in self.free if b not in again]
+
     def _still_held(self, b: int) -> bool:
         more = self.shared.get(b)
         if more is None:
@@ -229,7 +236,7 @@ class PagedKVCache:
 
     def fork(self, src: int, dst, n_tokens: int | None = None) -> None:
         """Sequence `dst`, or each of several, becomes the first n_tokens tokens (default: all) of `src`, in all layers.
-        What it held before is freed.
+        What it held before is freed; if there is no room for the copies, or they fail, every sequence stays as it was.
 
         Whole blocks are shared, the last one, if it is not full, copied: what either sequence writes from there on is
         its own.  A recorded step of `dst` has to be recorded again, one of `src` goes on as it was."""
@@ -240,12 +247,22 @@ class PagedKVCache:
         if not 0 <= n <= self.lengths[src]:
             raise ValueError(f"sequence {src} has {self.lengths[src]} tokens, {n} asked for")
         _no_recording(self.device, "the block table would be rebuilt")
-        for d in to:
-            self.free_sequence(d)
         full, rest = divmod(n, BLOCK)
-        whole, last = self.blocks[src][:full], []
-        if rest and to:
-            last = self._copies([self.blocks[src][full]] * len(to))
+        whole, copied = self.blocks[src][:full], self.blocks[src][full:full + 1] * len(to) if rest else []
+        held = [self.blocks[d] for d in to]
+        if len(copied) <= len(self.alloc.free):
+            last = self._copies(copied) if copied else []
+            for blocks in held:
+                self.alloc.release(blocks)
+        else:  # it takes what the destinations give back
+            for blocks in held:
+                self.alloc.release(blocks)
+            try:
+                last = self._copies(copied)
+            except BaseException:
+                for blocks in reversed(held):
+                    self.alloc.take_back(blocks)
+                raise
         for i, d in enumerate(to):
             self.alloc.share(whole)
             self.blocks[d] = whole + last[i:i + 1]
