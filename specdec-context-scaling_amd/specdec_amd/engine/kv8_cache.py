@@ -180,12 +180,13 @@ class KV8Cache(PagedKVCache):
                 if t is not None:
                     t.record_stream(on)
 
-    def _operands(self, layer: int):
-        """(K pages, V pages, scales, block table) of a call on the current stream."""
+    def _operands(self, layer: int, starts=(), ends=()):
+        """(K pages, V pages, scales, block table) of a call on the current stream that writes positions starts[b] .. ends[b] - 1."""
         table = self.block_table()
         if _recording(self.device):
             self._hold(table)
             self._hold_pages()
+            self._hold_writes(starts, ends)
         else:
             self._note_stream()
         return (*self.layer(layer), table)
@@ -195,14 +196,14 @@ class KV8Cache(PagedKVCache):
         """Append counts[b] tokens to each sequence of one layer: k_new/v_new BF16 (sum(counts), KV, D),
         sequence after sequence.  Positions start at ``starts`` (default: the current lengths); the
         lengths become start + count."""
-        cu, ends = self._room(k_new, counts, starts)
+        cu, starts, ends = self._room(k_new, counts, starts)
         if max(ends) > 0:
             lens, longest = self._lengths(ends)
-            ops.kv8_append(k_new, v_new, *self._operands(layer), cu, lens, longest)
+            ops.kv8_append(k_new, v_new, *self._operands(layer, starts, ends), cu, lens, longest)
         self.lengths[:] = ends
 
     def _room(self, k_new: torch.Tensor, counts, starts):
-        """(device row table, lengths afterwards) of a write, with the blocks that it needs."""
+        """(device row table, lengths before and afterwards) of a write, with the blocks that it needs."""
         starts = list(self.lengths) if starts is None else [int(s) for s in starts]
         counts, cu = self._rows(counts)
         ends = [s + c for s, c in zip(starts, counts)]
@@ -214,17 +215,17 @@ class KV8Cache(PagedKVCache):
             self.reserve(b, ends[b])
         if self.alloc.shared:
             self._own(starts, ends)
-        return cu, ends
+        return cu, starts, ends
 
     def rope_write(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, counts, inv_freq: torch.Tensor, starts=None, *,
                    interleaved: bool = False, rope_scale: float = 1.0, positions: torch.Tensor | None = None) -> torch.Tensor:
         """write() of rows whose q and k have no positions yet: in one launch k_new is rotated and written, and q BF16
         (sum(counts), H, D) rotated and returned.  inv_freq and rope_scale: ops.rope_frequencies.  positions (int32, one a row): those of
         rows that do not stand where they are written, a tree's nodes (the context and the node's depth)."""
-        cu, ends = self._room(k_new, counts, starts)
+        cu, starts, ends = self._room(k_new, counts, starts)
         if max(ends) > 0:
             lens, longest = self._lengths(ends)
-            q = ops.kv8_rope_append(q, k_new, v_new, *self._operands(layer), cu, lens, longest, inv_freq, interleaved=interleaved,
+            q = ops.kv8_rope_append(q, k_new, v_new, *self._operands(layer, starts, ends), cu, lens, longest, inv_freq, interleaved=interleaved,
                                     scale=rope_scale, positions=positions)
         self.lengths[:] = ends
         return q

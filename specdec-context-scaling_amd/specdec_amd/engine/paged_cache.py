@@ -28,8 +28,10 @@ recorded again.
 Sharing: ``fork`` gives a sequence the first tokens of another without copying them -- whole page blocks
 are held by both, the last one, if it is not full, is copied -- so a prompt that many sequences continue
 is stored (and, by KV8Cache.attend, read) once.  A sequence that would write into a block others hold, which
-it can only after a trim below the fork, gets its own copy of it first.  ``compact`` moves the blocks in use
-into page tensors of their number.  Both copy every layer in one launch (``ops.copy_blocks``).
+it can only after a trim below the fork, gets its own copy of it first (a step recorded before then still reads
+the other and has to be recorded again).  A recorded step writes its blocks at every replay, past that check, so
+``fork`` copies these too.  ``compact`` moves the blocks in use into page tensors of their number.  Both copy
+every layer in one launch (``ops.copy_blocks``).
 
 Ownership rule (the reference's trim returns views and its appends build new tensors, so an
 untrimmed handle keeps its data; here appends write pages in place): after
@@ -68,6 +70,7 @@ class BlockAllocator:
         self._rng = random.Random(seed) if seed is not None else None
         self.free: list[int] = []
         self.shared: dict[int, int] = {}  # blocks that several sequences hold: how many beyond the first
+        self.recorded: set[int] = set()  # blocks that a recorded graph writes, until they are given out again: never shared
         self.grow(num_blocks)
 
     def grow(self, new_total: int) -> None:
@@ -81,7 +84,10 @@ class BlockAllocator:
     def alloc(self, n: int) -> list[int]:
         if n > len(self.free):
             raise RuntimeError(f"block pool exhausted: need {n}, {len(self.free)} free of {self.num_blocks}")
-        return [self.free.pop() for _ in range(n)]
+        out = [self.free.pop() for _ in range(n)]
+        if self.recorded:
+            self.recorded.difference_update(out)
+        return out
 
     def share(self, blocks) -> None:
         """One more holder of each of `blocks`."""
@@ -164,6 +170,7 @@ class PagedKVCache:
         v[:, :old].copy_(self.v_pages)
         s[:, :old].copy_(self.v_scales)
         self.k_pages, self.v_pages, self.v_scales = k, v, s
+        self.alloc.recorded.clear()  # their graphs write the old pages
         self.alloc.grow(new)
 
     def _layer_pointers(self, i: int, device: torch.device):
@@ -239,7 +246,8 @@ class PagedKVCache:
         What it held before is freed; if there is no room for the copies, or they fail, every sequence stays as it was.
 
         Whole blocks are shared, the last one, if it is not full, copied: what either sequence writes from there on is
-        its own.  A recorded step of `dst` has to be recorded again, one of `src` goes on as it was."""
+        its own.  Blocks that a recorded step of `src` writes are copied as well, so that it goes on as it was (its replays come to
+        no _own()); a recorded step that has rows of `dst` has to be recorded again."""
         to = [int(d) for d in dst] if hasattr(dst, "__iter__") else [int(dst)]
         if not 0 <= src < self.batch or any(not 0 <= d < self.batch for d in to) or src in to or len(set(to)) != len(to):
             raise ValueError(f"cannot fork sequence {src} into {to} in a batch of {self.batch}")
@@ -248,13 +256,16 @@ class PagedKVCache:
             raise ValueError(f"sequence {src} has {self.lengths[src]} tokens, {n} asked for")
         _no_recording(self.device, "the block table would be rebuilt")
         full, rest = divmod(n, BLOCK)
-        whole, copied = self.blocks[src][:full], self.blocks[src][full:full + 1] * len(to) if rest else []
+        mine = self.blocks[src][:full + (rest > 0)]
+        own = [j for j, x in enumerate(mine) if j == full or x in self.alloc.recorded]
+        whole, copied = [x for j, x in enumerate(mine) if j not in own], [mine[j] for j in own] * len(to)
         held = [self.blocks[d] for d in to]
         if len(copied) <= len(self.alloc.free):
             last = self._copies(copied) if copied else []
             for blocks in held:
                 self.alloc.release(blocks)
         else:  # it takes what the destinations give back
+            recorded = set(self.alloc.recorded)
             for blocks in held:
                 self.alloc.release(blocks)
             try:
@@ -262,10 +273,13 @@ class PagedKVCache:
             except BaseException:
                 for blocks in reversed(held):
                     self.alloc.take_back(blocks)
+                self.alloc.recorded = recorded
                 raise
         for i, d in enumerate(to):
             self.alloc.share(whole)
-            self.blocks[d] = whole + last[i:i + 1]
+            self.blocks[d] = list(mine)
+            for j, x in zip(own, last[i * len(own):]):
+                self.blocks[d][j] = x
             self.lengths[d] = n
         self._bt = None
 
@@ -344,6 +358,13 @@ class PagedKVCache:
             for t in (self.k_pages, self.v_pages, self.v_scales):
                 self._hold(t)
 
+    def _hold_writes(self, starts, ends) -> None:
+        """The blocks of positions starts[b] .. ends[b] - 1, which a call that is being recorded writes, are never shared:
+        every replay writes them, whoever holds them by then."""
+        for blocks, s, e in zip(self.blocks, starts, ends):
+            if e > s:
+                self.alloc.recorded.update(blocks[s // BLOCK:-(-e // BLOCK)])
+
     def max_blocks(self) -> int:
         return max(1, max(len(b) for b in self.blocks))
 
@@ -410,6 +431,7 @@ class PagedKVCache:
         if _recording(self.device):
             self._hold_pages()
             self._hold(self.block_table())
+            self._hold_writes(starts, self.lengths[:B])
         if uniform and out is None:
             # the engine's per-layer call: its host cost is part of every token, so what the
             # general path checks one helper call at a time is tested here in one expression, and
@@ -494,6 +516,7 @@ class PagedKVCache:
                                            "slots that it returns)")
             table = self._recorded.setdefault(key[0], self._tiles[2])
             self._hold_pages()
+            self._hold_writes([0] * self.batch, lengths)
         elif on_device:
             if slots is None or stale:
                 fresh, table = self._varlen(lengths)
