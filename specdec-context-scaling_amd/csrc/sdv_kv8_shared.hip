@@ -589,16 +589,23 @@ extern "C" size_t sdv_kv8_shared_attention_workspace_size(int32_t batch, int32_t
   return shared_workspace(tile_rows != 32, batch, groups, total_rows, q_heads / kv_heads, kv_heads, head_dim, max_q_len);
 }
 
+template <int D, int FMT, int RS>
+static void shared_launch(const Kv8SharedArgs& s, hipStream_t st) {
+  hipLaunchKernelGGL((kv8_shared_kernel<D, FMT, RS>), dim3(kKv8Grid), dim3(kKv8Threads), 0, st, s);
+  constexpr int most = 1 << 22;  // tokens of a launch, which has fewer than 2^32 threads along x
+  for (int first = 0; first < s.a.r.total; first += most) {
+    Kv8SharedArgs x = s;
+    x.rows += first;
+    x.a.out += first * x.a.out_stride;
+    const int n = s.a.r.total - first < most ? s.a.r.total - first : most;
+    const dim3 merge((unsigned)n, (unsigned)s.a.kv_heads, (unsigned)((s.a.G + kSharedMergeHeads - 1) / kSharedMergeHeads));
+    hipLaunchKernelGGL((kv8_shared_merge_kernel<D, 16 * RS>), merge, dim3(kSharedMergeThreads), 0, st, x);
+  }
+}
+
 template <int D, int FMT>
 static void shared_launch(const Kv8SharedArgs& s, int tile, hipStream_t st) {
-  const dim3 grid(kKv8Grid), merge((unsigned)s.a.r.total, (unsigned)s.a.kv_heads, (unsigned)((s.a.G + kSharedMergeHeads - 1) / kSharedMergeHeads));
-  if (tile == 16) {
-    hipLaunchKernelGGL((kv8_shared_kernel<D, FMT, 1>), grid, dim3(kKv8Threads), 0, st, s);
-    hipLaunchKernelGGL((kv8_shared_merge_kernel<D, 16>), merge, dim3(kSharedMergeThreads), 0, st, s);
-  } else {
-    hipLaunchKernelGGL((kv8_shared_kernel<D, FMT, 2>), grid, dim3(kKv8Threads), 0, st, s);
-    hipLaunchKernelGGL((kv8_shared_merge_kernel<D, 32>), merge, dim3(kSharedMergeThreads), 0, st, s);
-  }
+  tile == 16 ? shared_launch<D, FMT, 1>(s, st) : shared_launch<D, FMT, 2>(s, st);
 }
 
 extern "C" int sdv_kv8_shared_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, const float* scales,

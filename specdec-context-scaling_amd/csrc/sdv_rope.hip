@@ -220,11 +220,22 @@ __global__ __launch_bounds__(64) void kv8_rope_append_kernel(Kv8RopeArgs a) {
 
 using namespace sdv;
 
+// A launch has fewer than 2^32 threads along x: of more rows (2^25 of 128 dimensions, 2^26 of 64) one for each so many.
 template <int D, bool IL>
 static void rope_launch(const RopeRows& a, hipStream_t st) {
-  constexpr int rows = kRopeThreads / (D / 2);
-  const dim3 grid((unsigned)((a.rows + rows - 1) / rows), (unsigned)((a.heads[0] + a.heads[1] + kRopeGroup - 1) / kRopeGroup));
-  hipLaunchKernelGGL((rope_kernel<D, IL>), grid, dim3(kRopeThreads), 0, st, a);
+  constexpr int rows = kRopeThreads / (D / 2), most = (1 << 23) * rows;
+  const unsigned groups = (unsigned)((a.heads[0] + a.heads[1] + kRopeGroup - 1) / kRopeGroup);
+  for (int first = 0; first < a.rows; first += most) {
+    RopeRows x = a;
+    x.rows = a.rows - first < most ? a.rows - first : most;
+    x.positions += first;
+    for (int k = 0; k < 2; ++k) {
+      if (x.heads[k] == 0) continue;
+      x.in[k] += first * x.in_stride[k];
+      x.out[k] += first * x.out_stride[k];
+    }
+    hipLaunchKernelGGL((rope_kernel<D, IL>), dim3((unsigned)((x.rows + rows - 1) / rows), groups), dim3(kRopeThreads), 0, st, x);
+  }
 }
 
 extern "C" int sdv_rope(const void* q, int64_t q_stride, int32_t q_heads, const void* k, int64_t k_stride, int32_t k_heads,
