@@ -10,6 +10,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/Exceptions.h>
@@ -302,6 +303,7 @@ PyObject* rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const at::Tensor *q = rows_of(o[0], dev, d, 0, qs), *k = nullptr;
   if (!q || (o[1] != Py_None && !(k = rows_of(o[1], dev, d, 0, ks))) || !ints_of(o[2], dev, q->size(0), positions)) Py_RETURN_NONE;
   if (k && k->size(0) != q->size(0)) Py_RETURN_NONE;
+  if (c10::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()))) Py_RETURN_NONE;
   const int32_t rotary = frequencies(o[3], dev, d, inv_freq);
   if (rotary == 0) Py_RETURN_NONE;
   Launch on(dev);

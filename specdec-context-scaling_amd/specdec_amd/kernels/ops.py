@@ -964,8 +964,9 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
     q and k: rows of any stride that is a multiple of 8 elements (parts of a projection's output as they lie).  positions int32
     (rows,).  inv_freq float64 (r/2,), scale: see rope_frequencies.  Of a head's first r dimensions pair i is (i, i + r/2), or
     (2i, 2i + 1) if interleaved: it becomes scale (x cos t - y sin t, x sin t + y cos t), t = position * inv_freq[i], computed
-    in fp32 from an angle in 64 bits and rounded once.  inverse: rotated back (the transpose, as a gradient takes it).  q_out
-    and k_out, which may be q and k themselves (no other overlap): written there.
+    in fp32 from an angle in 64 bits and rounded once.  inverse: rotated back (the transpose).  Gradients of q and k are those
+    of the results rotated back by the same angles, BF16 like them.  q_out and k_out, which may be q and k themselves (no other
+    overlap): written there, outside autograd.
     """
     if q_out is None and k_out is None:
         got = _native.binding().rope(q, k, positions, inv_freq, interleaved, scale, inverse)
@@ -975,6 +976,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
             return got
     if not isinstance(q, torch.Tensor):
         _fail("q must be a tensor")
+    if q_out is None and k_out is None and torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k)):
+        return _Rope.apply(q, k, positions, inv_freq, interleaved, scale, inverse)
     dev = q.device
     if dev.type != "cuda":
         _fail(f"q must be on a HIP device (got {dev})")
@@ -1006,6 +1009,26 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
     return tuple(outs)
 
 
+class _Rope(torch.autograd.Function):
+    """rope of rows that require grad: a linear map, s times a rotation, whose transpose is s times the inverse rotation."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = dict(interleaved=interleaved, scale=scale, inverse=not inverse)
+        ctx.set_materialize_grads(False)
+        return rope(q, k, positions, inv_freq, interleaved=interleaved, scale=scale, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        grads = [g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad)]
+        given = [g for g in grads if g is not None]
+        if given:
+            back = iter(rope(given[0], given[1] if len(given) > 1 else None, *ctx.saved_tensors, **ctx.how))
+            grads = [None if g is None else next(back) for g in grads]
+        return (*grads, None, None, None, None, None)
+
+
 def kv8_rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     scales: torch.Tensor, block_table: torch.Tensor, cu_rows: torch.Tensor, seq_lens: torch.Tensor | None,
                     max_seq_len: int, inv_freq: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0,
@@ -1015,6 +1038,7 @@ def kv8_rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k
     The arguments of kv8_append, and those of rope; positions int32 (total,) where a row's is not the one that it is written
     at (a tree's nodes), else None.  K is quantized as it is rotated, in fp32: its codes are one rounding nearer to the rotated
     values than those of rope and then kv8_append.  q_out: written there, which may be q itself; rows behind cu_rows[B] of it are not.
+    Like the cache's other operators outside autograd.
     """
     if q_out is None:
         got = _native.binding().rope_append(q, k_new, v_new, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_seq_len, inv_freq,
@@ -1239,6 +1263,19 @@ def _lib_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
 @_lib_rope.register_fake
 def _(q, k, positions, inv_freq, interleaved=False, scale=1.0, inverse=False):
     return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+def _rope_keep(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[2:4])
+    ctx.how = inputs[4:]
+
+
+def _rope_back(ctx, gq, gk):
+    interleaved, scale, inverse = ctx.how
+    return (*torch.ops.sdv.rope(gq, gk, *ctx.saved_tensors, interleaved, scale, not inverse), None, None, None, None, None)
+
+
+_lib_rope.register_autograd(_rope_back, setup_context=_rope_keep)
 
 
 @torch.library.custom_op("sdv::kv8_rope_append", mutates_args=("k_pages", "v_pages", "scales"))
