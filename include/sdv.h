@@ -327,7 +327,8 @@ int sdv_pack_contiguous(const void* k, const void* v_codes, const float* v_scale
  * [total_rows][heads][head_dim] whose tokens lie `*_stride` elements apart (a multiple of 8, at
  * least heads * head_dim), so that the q, k and v parts of one projection's output can be passed
  * as they lie.  block_table int32 [batch][max_blocks_per_seq]; an entry outside [0, num_blocks), or a
- * position past the table, is never dereferenced.
+ * position past the table, is never dereferenced.  A call that writes or reads back rows has
+ * min(total_rows, total_rows / 16 + 2 batch) < 2^26.
  * Alignment: packed tensors, pages and scales 16 B, int32 arrays 4 B, tree_mask 8 B, workspace 256 B. */
 #define SDV_KV8_FP8 0
 #define SDV_KV8_INT8 1

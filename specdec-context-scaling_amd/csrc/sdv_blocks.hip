@@ -146,11 +146,17 @@ extern "C" int sdv_copy_blocks(const void* k_from, const void* v_from, const flo
       !aligned(k_to, 16) || !aligned(v_to, 16) || !aligned(s_to, 16) || !aligned(src, 4) || !aligned(dst, 4))
     return SDV_ERR_ALIGN;
   if (n == 0) return SDV_OK;
-  const CopyArgs a = {{static_cast<const uint8_t*>(k_from), static_cast<const uint8_t*>(v_from), reinterpret_cast<const uint8_t*>(s_from)},
-                      {static_cast<uint8_t*>(k_to), static_cast<uint8_t*>(v_to), reinterpret_cast<uint8_t*>(s_to)},
-                      {(int)k_bytes, (int)v_bytes, (int)s_bytes}, from_blocks, to_blocks, src, dst, n};
-  hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)((n + (int64_t)kCopyWaves - 1) / kCopyWaves), (unsigned)num_layers),
-                     dim3(kCopyWaves * kWave), 0, static_cast<hipStream_t>(stream), a);
+  CopyArgs a = {{static_cast<const uint8_t*>(k_from), static_cast<const uint8_t*>(v_from), reinterpret_cast<const uint8_t*>(s_from)},
+                {static_cast<uint8_t*>(k_to), static_cast<uint8_t*>(v_to), reinterpret_cast<uint8_t*>(s_to)},
+                {(int)k_bytes, (int)v_bytes, (int)s_bytes}, from_blocks, to_blocks, src, dst, n};
+  constexpr int most = 1 << 25;  // pairs of a launch, which has fewer than 2^32 threads along x
+  for (int64_t first = 0; first < n; first += most) {
+    a.src = src + first;
+    a.dst = dst + first;
+    a.n = (int)(n - first < most ? n - first : most);
+    hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)((a.n + kCopyWaves - 1) / kCopyWaves), (unsigned)num_layers),
+                       dim3(kCopyWaves * kWave), 0, static_cast<hipStream_t>(stream), a);
+  }
   return hipGetLastError() == hipSuccess ? SDV_OK : SDV_ERR_HIP;
 }
 
@@ -169,14 +175,21 @@ extern "C" int sdv_kv8_keep(void* k_pages, void* v_pages, float* scales, int32_t
       s_layer_stride % 4 || !aligned(block_table, 4) || !aligned(cu_kept, 4) || !aligned(kept, 4) || !aligned(starts, 4))
     return SDV_ERR_ALIGN;
   if (total_kept == 0) return SDV_OK;
-  const KeepArgs a = {{cu_kept, block_table, max_blocks_per_seq, num_blocks, batch, total_kept}, kept, starts,
-                      static_cast<uint8_t*>(k_pages), static_cast<uint8_t*>(v_pages), scales, k_layer_stride, v_layer_stride,
-                      s_layer_stride, kv_heads};
-  const dim3 grid((unsigned)batch, (unsigned)kv_heads, (unsigned)num_layers);
+  KeepArgs a = {{cu_kept, block_table, max_blocks_per_seq, num_blocks, batch, total_kept}, kept, starts,
+                static_cast<uint8_t*>(k_pages), static_cast<uint8_t*>(v_pages), scales, k_layer_stride, v_layer_stride,
+                s_layer_stride, kv_heads};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (head_dim == 128)
-    hipLaunchKernelGGL((kv8_keep_kernel<128>), grid, dim3(kKeepThreads<128>), 0, s, a);
-  else
-    hipLaunchKernelGGL((kv8_keep_kernel<64>), grid, dim3(kKeepThreads<64>), 0, s, a);
+  constexpr int most = 1 << 23;  // sequences of a launch, which has fewer than 2^32 threads along x
+  for (int64_t first = 0; first < batch; first += most) {
+    a.r.cu = cu_kept + first;
+    a.r.table = block_table + first * max_blocks_per_seq;
+    a.r.batch = (int)(batch - first < most ? batch - first : most);
+    a.starts = starts + first;
+    const dim3 grid((unsigned)a.r.batch, (unsigned)kv_heads, (unsigned)num_layers);
+    if (head_dim == 128)
+      hipLaunchKernelGGL((kv8_keep_kernel<128>), grid, dim3(kKeepThreads<128>), 0, s, a);
+    else
+      hipLaunchKernelGGL((kv8_keep_kernel<64>), grid, dim3(kKeepThreads<64>), 0, s, a);
+  }
   return hipGetLastError() == hipSuccess ? SDV_OK : SDV_ERR_HIP;
 }

@@ -170,7 +170,12 @@ __device__ __forceinline__ void kv8_write_v(const Kv8Tile& t, const uint4 (&vw)[
 
 // ---------------------------------------------------------------------------- host
 // Checks and grid that the entry points share.  Every sequence's rows touch at most
-// min(n, (n + 30) / 16) blocks.
+// min(n, (n + 30) / 16) blocks, a wavefront each; a launch has fewer than 2^32 threads along x.
+inline int64_t kv8_cache_tiles(int32_t total, int32_t batch) {
+  const int64_t tiles = (int64_t)total / kBlock + 2 * (int64_t)batch;
+  return tiles < total ? tiles : total;
+}
+
 inline int kv8_cache_check(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int32_t total,
                            const void* k_pages, const void* v_pages, const float* scales, int32_t num_blocks,
                            int32_t format, const int32_t* table, int32_t max_blocks, const int32_t* cu,
@@ -178,6 +183,7 @@ inline int kv8_cache_check(const void* k, const void* v, int64_t k_stride, int64
   if (!k || !v || !k_pages || !v_pages || !scales || !table || !cu) return SDV_ERR_NULL;
   if (total < 0 || num_blocks <= 0 || max_blocks <= 0 || batch <= 0 || kv_heads <= 0 || kv_heads > 65535) return SDV_ERR_SHAPE;
   if (max_blocks > INT32_MAX / kBlock || total > INT32_MAX / 2 || batch > INT32_MAX / 4) return SDV_ERR_SHAPE;
+  if (kv8_cache_tiles(total, batch) >= (1LL << 32) / kWave) return SDV_ERR_SHAPE;
   if (head_dim != 64 && head_dim != 128) return SDV_ERR_UNSUPPORTED;
   if (format != SDV_KV8_FP8 && format != SDV_KV8_INT8) return SDV_ERR_UNSUPPORTED;
   const int64_t row = (int64_t)kv_heads * head_dim;
@@ -197,8 +203,7 @@ inline Kv8CacheArgs kv8_cache_args(void* k, void* v, int64_t k_stride, int64_t v
 }
 
 inline dim3 kv8_cache_grid(int32_t total, int32_t batch, int32_t kv_heads) {
-  const int64_t tiles = (int64_t)total / kBlock + 2 * (int64_t)batch;
-  return dim3((unsigned)(tiles < total ? tiles : total), (unsigned)kv_heads);
+  return dim3((unsigned)kv8_cache_tiles(total, batch), (unsigned)kv_heads);
 }
 
 }  // namespace sdv
