@@ -98,6 +98,7 @@ int sdv_quant_append(const void* v_new, const void* k_new, const int32_t* slot_m
  * (its prefill writes one 2048-token chunk of one sequence): for the batched varlen prefill of
  * the paged engine, whose sequences start anywhere in the packed input -- tiles that begin at
  * each sequence's first row let whole page blocks take the 16-byte stores instead of bytes.
+ * A call has fewer than 2^26 tiles (sdv_quant_append: ceil(n_tokens / 16)).
  */
 int sdv_quant_append_tiles(const void* v_new, const void* k_new, const int32_t* slot_mapping,
                            int32_t n_tokens, int32_t kv_heads, int32_t head_dim, int32_t group_size,
@@ -301,7 +302,7 @@ int sdv_paged_attention_noalloc(const void* q, const void* k_pages, const void* 
  * the same shape, v_scales fp32 [batch][kv_heads][seq_len].  k_pages / v_pages / page_scales hold
  * batch * ceil(seq_len/16) pages in the layout above, block b*ceil(seq_len/16) + j being tokens
  * 16j.. of sequence b, and block_table int32 [batch][ceil(seq_len/16)] receives those block ids.
- * Tokens past seq_len in a last block get K 0, code 0 and scale 1.  Alignment: k/k_pages 16 B,
+ * Tokens past seq_len in a last block get K 0, code 0 and scale 1.  kv_heads * pages < 2^26.  Alignment: k/k_pages 16 B,
  * the rest 4 B.  For callers that hold the reference's cache tensors (model_self.py:778-800) and
  * call its op over them (specdec/kernels/ops.py:67-76); no counterpart of its own.
  */

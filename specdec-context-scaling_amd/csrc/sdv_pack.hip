@@ -85,7 +85,7 @@ extern "C" int sdv_pack_contiguous(const void* k, const void* v_codes, const flo
   if (batch <= 0 || kv_heads <= 0 || seq_len <= 0 || seq_len > INT32_MAX - kBlock) return SDV_ERR_SHAPE;
   if (head_dim != 64 && head_dim != 128) return SDV_ERR_UNSUPPORTED;
   const int64_t nbps = (seq_len + kBlock - 1) / kBlock, pages = batch * nbps;
-  if (pages > INT32_MAX / kv_heads) return SDV_ERR_SHAPE;
+  if (pages * kv_heads >= 1 << 26) return SDV_ERR_SHAPE;  // a launch has fewer than 2^32 threads along x
   if (!aligned(k, 16) || !aligned(v_codes, 4) || !aligned(v_scales, 4) || !aligned(k_pages, 16) || !aligned(v_pages, 4) ||
       !aligned(page_scales, 4) || !aligned(block_table, 4))
     return SDV_ERR_ALIGN;

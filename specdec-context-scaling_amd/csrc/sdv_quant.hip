@@ -346,6 +346,7 @@ static int quant_append(const void* v_new, const void* k_new, const int32_t* slo
 
   const int64_t n_waves = tiles ? n_tiles : (n_tokens + kBlock - 1) / kBlock;
   if (n_waves == 0) return SDV_OK;
+  if (n_waves >= 1 << 26) return SDV_ERR_SHAPE;  // a launch has fewer than 2^32 threads along x
   dim3 grid((unsigned)((n_waves + kQuantWaves - 1) / kQuantWaves), kv_heads, num_layers);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 block(64 * kQuantWaves);
