@@ -417,8 +417,9 @@ int sdv_kv8_attention_slot(const void* q, int64_t q_stride, const void* k_pages,
  * tile_rows: rows of a prefix's tile, 32 (operands and sums as in sdv_kv8_attention's tiles of 32) or 128 (as in its
  * tiles of 256, but that an item, up to 1/512 of the call, whose V scales lie more than 2^18 apart is computed as with 32); a
  * sequence's own tiles have 16 or 32, by max_q_len (a sequence with more rows is computed all the same).
- * sdv_kv8_shared_attention_tile_rows says which of them is faster for these sizes, or 0 where sdv_kv8_attention is faster than
- * both (short prefixes or few sequences; more than 64 rows a sequence and KV head; sizes that are refused).
+ * sdv_kv8_shared_attention_tile_rows says which of them is faster for one group of these sizes, or 0 where sdv_kv8_attention is
+ * faster than both (short prefixes or few sequences; more than 64 rows a sequence and KV head; sizes that are refused).  It takes all
+ * sequences to share max_prefix_len: with few that do, sdv_kv8_attention may be faster than its choice.
  * The workspace may hold anything and nothing carries over.  max_prefix_len is at most 16 * max_blocks_per_seq; size
  * limits as for sdv_kv8_attention, with max_prefix_len added to max_seq_len.
  */

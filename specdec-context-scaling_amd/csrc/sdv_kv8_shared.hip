@@ -516,20 +516,26 @@ static int shared_tile(int32_t G, int32_t max_q_len) { return (int64_t)G * max_q
 // every sequence, from the caches: it has one launch, and tiles of 256 of a sequence's own rows.  From 204 sizes of one group
 // (2 to 64 sequences, 1, 5 and 24 rows each, prefixes of 256 to 32768, heads 12/2/128 and 14/2/64), GPU time in us, sdv_kv8_attention
 // first, then tiles of 32 and of 128 rows, 12/2/128:
-//   up to 16 rows a sequence and KV head, by the keys not read again: 16 x 1 over 8192 19 19 26, 32 x 1 over 4096 17 17 23, 8 x 1 over
-//     32768 30 26 33, 32 x 1 over 8192 24 20 28, 64 x 1 over 8192 38 29 34;
+//   up to 16 rows a sequence and KV head, by the keys not read again: the ways meet between 200 and 250 thousand (4 x 1 over 32768
+//     26 24 30, 8 x 1 over 16384 21 22 27, 16 x 1 over 8192 19 19 26, 32 x 1 over 4096 17 17 23; with heads of 64 19 17 20, 15 16 19,
+//     15 15 18, 14 14 17), and twice as many are worth the other launch: 8 x 1 over 32768 30 26 33, 32 x 1 over 8192 24 20 28,
+//     64 x 1 over 8192 38 29 34;
 //   up to 64, by the prefix: 2 x 5 over 1024 13 14 19 and over 4096 18 15 21, 16 x 5 over 1024 14 16 22 and over 4096 25 24 27;
 //   more: 8 x 24 over 4096 31 34 39, 32 x 24 over 8192 81 134 88;
 //   and of the two kinds of tiles, by a group's rows times its prefix: 8 x 5 over 32768 50 41 42, 32 x 5 over 8192 43 44 42, 64 x 1 over
 //     32768 126 65 50, 32 x 5 over 32768 112 109 71, 64 x 5 over 32768 217 206 131; with heads of 64 from a third of that on (32 x 1 over
 //     16384 27 23 23, 64 x 1 over 4096 18 17 19).
-// Over all of the sizes this takes 1.2% longer than the fastest of the three for each.
+// Over all of the sizes this takes 1.2% longer than the fastest of the three for each.  It has no more than the counts and the
+// longest prefix, and is that of batches of one group: sequences that share nothing count as if they did, and one with many rows
+// keeps all from sharing.  kv8_attention would be faster for 62 single tokens over 8392 tokens of their own and a pair that shares 8192
+// (57 74 70, taken: 74), for 56 such and 8 that share (55 71 61), for 16 pairs (27 30 38) and for 56 blocks of 5 rows over 4000
+// and 8 that share 4096 (45 58 50); with 32 that share and 32 that do not it is 49 51 46.
 constexpr int64_t kSharedKeys = 1 << 18, kSharedPrefix = 1 << 12, kSharedWideKeys = 8 << 20;
 static int shared_rows(int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
                        int32_t max_prefix) {
   const int64_t own = (int64_t)G * max_q_len;
   if (groups <= 0 || batch == groups || own > 64) return 0;
-  if (own <= 16 ? (int64_t)(batch - groups) * max_prefix * kv_heads < kSharedKeys * 15 / 16 : max_prefix < kSharedPrefix) return 0;
+  if (own <= 16 ? (int64_t)(batch - groups) * max_prefix * kv_heads < kSharedKeys : max_prefix < kSharedPrefix) return 0;
   const int64_t keys = (int64_t)total * G / groups * max_prefix * kv_heads / 2;
   return keys >= (head_dim == 128 ? kSharedWideKeys : kSharedWideKeys / 3) ? kWideRows : 32;
 }

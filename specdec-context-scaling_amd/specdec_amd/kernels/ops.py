@@ -841,10 +841,12 @@ def kv8_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     int32 (B,), the same for all of a group and at most each one's context before its new tokens (0 for a sequence in no group): so
     many first tokens, taken down to whole blocks, are blocks that the table names alike for all of the group.  Every row of the group
     sees them all, then its own sequence's keys from there on.  max_prefix_len bounds them.  The other arguments, and the result, are
-    kv8_attention's, to the order of the sums.
+    kv8_attention's, to its roundings: tiles of 32 rows hold the exponentials in 16 bits and the codes exactly, as it does for few rows,
+    those of 128 hold the exponentials, and V with its scale, in FP16, as it does for many.
 
-    tile_rows: rows of the group that a workgroup has at a time, 32 or 128; 0: whichever is faster for these sizes, or kv8_attention where
-    that is faster than both (short prefixes, few sequences, more than 64 rows of a sequence and KV head).
+    tile_rows: rows of the group that a workgroup has at a time, 32 or 128; 0: whichever is faster for one group of these sizes, or
+    kv8_attention where that is faster than both (short prefixes, few sequences, more than 64 rows of a sequence and KV head).  With
+    few sequences in groups, or prefixes of very different lengths, kv8_attention may be faster than that choice.
     """
     got = _native.binding().shared(q, k_pages, v_pages, scales, block_table, cu_rows, seq_lens, max_q_len, max_seq_len, cu_groups,
                                    prefix_lens, max_prefix_len, scale, tree_mask, tile_rows, out)
