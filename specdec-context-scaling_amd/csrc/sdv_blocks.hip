@@ -14,7 +14,7 @@ struct CopyArgs {
 };
 
 // A wavefront copies one block of one layer, its three parts as one run of 16-byte pieces, kCopyBatch of them a lane in
-// flight.  Bound by the memory: 3001 blocks of 18 layers (627 MB both ways) 102 us, 6.1 TB/s; 32 of them 4.5 us.
+// flight.  Bound by the memory: 3001 blocks of 24 layers (627 MB both ways) 102 us, 6.1 TB/s; 32 of them 4.5 us.
 constexpr int kCopyWaves = 4, kCopyBatch = 8;
 
 __global__ __launch_bounds__(kCopyWaves * kWave) void copy_blocks_kernel(CopyArgs a) {

@@ -181,7 +181,7 @@ __device__ __forceinline__ void kv8_rows_tile(const Kv8AttnArgs& a, const Kv8Vie
         vw[dt][3] = x.w;
       } else {
         const uint64_t* at = reinterpret_cast<const uint64_t*>(src + dt * (16 * kBlock));
-          const uint64_t w = AGAIN ? *at : __builtin_nontemporal_load(at);
+        const uint64_t w = AGAIN ? *at : __builtin_nontemporal_load(at);
         vw[dt][0] = (uint32_t)w;
         vw[dt][1] = (uint32_t)(w >> 32);
       }

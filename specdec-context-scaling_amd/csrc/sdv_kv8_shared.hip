@@ -2,9 +2,9 @@
 //
 // A group is consecutive sequences whose first P tokens (whole blocks) are the same pages.  Its rows lie together in the
 // packed tensors, so a group's prefix is one more sequence: all of its rows, each of which sees all P keys.  A sequence's
-// own part is the sequence it was with its first P keys left out.  Tiles of 32 rows of a prefix, and of 16 or 32 of a
-// sequence, are cut along their keys into items, one a workgroup where there is one for each, and computed by
-// kv8_rows_tile.  Every item leaves its sums with their maximum and their sum of exponentials; a second launch adds
+// own part is the sequence it was with its first P keys left out.  Tiles of 32 or 128 rows of a prefix, and of 16 or 32 of
+// a sequence, are cut along their keys into items, one a workgroup where there is one for each, and computed by
+// kv8_rows_tile, those of 128 rows by kv8_wide_tile.  Every item leaves its sums with their maximum and their sum of exponentials; a second launch adds
 // those up for each row:
 //
 //   M = max_k m_k,   out = sum_k e^(m_k - M) acc_k / sum_k e^(m_k - M) l_k
@@ -49,7 +49,6 @@ struct Kv8SharedSeq {
 };
 
 // From the tables' entries: rows first .. end - 1, a prefix of P tokens, and of a sequence its length.
-template <int TS>
 __device__ __forceinline__ Kv8SharedSeq kv8_shared_prefix(const Kv8SharedArgs& s, int b0, int b1, int first, int end, int P) {
   Kv8SharedSeq x;
   x.table = min(b0, s.a.r.batch - 1);
@@ -78,7 +77,7 @@ __device__ __forceinline__ Kv8SharedSeq kv8_shared_seq(const Kv8SharedArgs& s, i
   const Kv8AttnArgs& a = s.a;
   if (v < s.groups) {
     const int b0 = min(max(s.cu_groups[v], 0), a.r.batch), b1 = min(max(s.cu_groups[v + 1], b0), a.r.batch);
-    return kv8_shared_prefix<TS>(s, b0, b1, a.r.cu[b0], a.r.cu[b1], s.prefix[min(b0, a.r.batch - 1)]);
+    return kv8_shared_prefix(s, b0, b1, a.r.cu[b0], a.r.cu[b1], s.prefix[min(b0, a.r.batch - 1)]);
   }
   const int b = v - s.groups;
   return kv8_shared_own<TS>(s, b, a.r.cu[b], a.r.cu[b + 1], s.prefix[b], a.lens ? a.lens[b] : 0);
@@ -142,7 +141,7 @@ struct Kv8SharedItems {
       __syncthreads();
       if (tid < s.groups) {
         const int b0 = min(max(g0, 0), s.a.r.batch), b1 = min(max(g1, b0), s.a.r.batch);
-        count_in(tid, kv8_shared_prefix<TS>(s, b0, b1, tables.cu[b0], tables.cu[b1], tables.prefix[min(b0, s.a.r.batch - 1)]));
+        count_in(tid, kv8_shared_prefix(s, b0, b1, tables.cu[b0], tables.cu[b1], tables.prefix[min(b0, s.a.r.batch - 1)]));
       } else if (has) {
         count_in(tid, kv8_shared_own<TS>(s, b, tables.cu[b], tables.cu[b + 1], tables.prefix[b], len));
       }

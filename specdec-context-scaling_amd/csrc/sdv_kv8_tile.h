@@ -1,4 +1,4 @@
-// What the kernels that move rows into and out of the kv8 cache share (sdv_kv8_cache.hip, sdv_kv8_rope.hip): which
+// What the kernels that move rows into and out of the kv8 cache share (sdv_kv8_cache.hip, sdv_rope.hip): which
 // page block a wavefront has, the quantization of a row, and the writing of a block's V.
 #pragma once
 

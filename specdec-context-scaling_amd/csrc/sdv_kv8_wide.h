@@ -276,8 +276,8 @@ __device__ __forceinline__ bool kv8_wide_tile(const Kv8AttnArgs& a, const Kv8Vie
   const auto operand = [&](int h) { return __builtin_bit_cast(f16x8, make_uint4(pw[4 * h], pw[4 * h + 1], pw[4 * h + 2], pw[4 * h + 3])); };
 
   // Of two workgroups of a CU the older one's wavefronts go first, and it is done a quarter earlier; then the other has the CU to
-  // itself, which it does not fill.  By turns of four stages they end together: 75.1 -> 73.3 us for 32 x 5 rows over 32768 tokens,
-  // 80.2 -> 77.3 for 64 x 5 over 16384.
+  // itself, which it does not fill.  By turns of four stages they end together: 75.3 -> 73.0 us, with the merge, for 32 x 5
+  // rows over 32768 tokens, 79.5 -> 76.8 for 64 x 5 over 16384 (in a graph of 20 calls).
   const int older = blockIdx.x < gridDim.x / 2 ? 1 : 0;
   for (int s = s0; s < s1; ++s) {
     if (((s - s0) >> 2 & 1) == older)
