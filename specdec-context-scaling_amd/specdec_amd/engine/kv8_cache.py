@@ -274,7 +274,8 @@ class KV8Cache(PagedKVCache):
     def attend(self, layer: int, q: torch.Tensor, *, counts=None, q_token_major: bool = False, lengths=None,
                scale: float | None = None, tree_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of every sequence's last tokens over this layer's pages at the current lengths.  The blocks that
-        neighbouring sequences both hold from their first on (fork) are read once for them all.
+        neighbouring sequences both hold from their first on (fork) are read once for them all, as ops.kv8_shared_attention
+        chooses and rounds.
 
         q BF16 (sum(counts), H, D) with ``counts`` rows per sequence; without counts (B, H, S, D), or
         (B, S, H, D) with q_token_major, S rows of every sequence.  Returns out shaped like q.

@@ -913,7 +913,8 @@ def rope_frequencies(head_dim: int, base: float = 1000000.0, *, rotary_dim: int 
     raises the base so that the slowest pair's is divided by f and the fastest stays; {"type": "yarn", "factor": f,
     "original": n, "slow": 1, "fast": 32} (Peng et al., arXiv:2309.00071) divides those that turn less than `slow` times in n
     positions, leaves those that turn more than `fast` times, goes over between them in proportion to the turns, and has scale
-    0.1 ln f + 1.
+    0.1 ln f + 1.  That is the paper's ramp; models that go over in proportion to the pair's number, between rounded bounds, have other
+    frequencies in between.  Any float64 tensor will do: those of a model's own configuration serve as they are.
     """
     r = head_dim if rotary_dim is None else int(rotary_dim)
     if not 0 < r <= head_dim or r % 16:
