@@ -526,9 +526,9 @@ static int shared_tile(int32_t G, int32_t max_q_len) { return (int64_t)G * max_q
 //     16384 27 23 23, 64 x 1 over 4096 18 17 19).
 // Over all of the sizes this takes 1.2% longer than the fastest of the three for each.  It has no more than the counts and the
 // longest prefix, and is that of batches of one group: sequences that share nothing count as if they did, and one with many rows
-// keeps all from sharing.  kv8_attention would be faster for 62 single tokens over 8392 tokens of their own and a pair that shares 8192
-// (57 74 70, taken: 74; with 2000 of their own 22 31 29), for 56 such and 8 that share (55 71 61), for 16 pairs (27 30 38) and for 56 blocks of 5 rows over 4000
-// and 8 that share 4096 (45 58 50); with 32 that share and 32 that do not it is 49 51 46.
+// keeps all from sharing.  kv8_attention would be faster for 62 single tokens over 8392 tokens of their own and a pair that shares
+// 8192 (57 74 70, taken: 74; with 2000 of their own 22 31 29), for 56 such and 8 that share (55 71 61), for 16 pairs (27 30 38)
+// and for 56 blocks of 5 rows over 4000 and 8 that share 4096 (45 58 50); with 32 that share and 32 that do not it is 49 51 46.
 constexpr int64_t kSharedKeys = 1 << 18, kSharedPrefix = 1 << 12, kSharedWideKeys = 8 << 20;
 static int shared_rows(int32_t batch, int32_t groups, int32_t total, int32_t G, int32_t kv_heads, int32_t head_dim, int32_t max_q_len,
                        int32_t max_prefix) {

@@ -23,7 +23,8 @@ from the host), grow the pool (new page tensors), grow the workspace -- raises i
 ``reserve_all`` and ``workspace`` before recording make room.  The pages and tables that a
 recording read stay alive as long as the pool.  A graph goes on with those it was recorded with:
 once the pool has grown, what it writes does not reach the new pages, and it has to be
-recorded again.
+recorded again.  Nor may a step be replayed that has rows of a sequence freed, or forked into, since:
+its blocks may be another's by then.
 
 Sharing: ``fork`` gives a sequence the first tokens of another without copying them -- whole page blocks
 are held by both, the last one, if it is not full, is copied -- so a prompt that many sequences continue
