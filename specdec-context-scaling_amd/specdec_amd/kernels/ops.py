@@ -968,7 +968,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
     (rows,).  inv_freq float64 (r/2,), scale: see rope_frequencies.  Of a head's first r dimensions pair i is (i, i + r/2), or
     (2i, 2i + 1) if interleaved: it becomes scale (x cos t - y sin t, x sin t + y cos t), t = position * inv_freq[i], computed
     in fp32 from an angle in 64 bits and rounded once.  inverse: rotated back (the transpose).  Gradients of q and k are those
-    of the results rotated back by the same angles, BF16 like them.  q_out and k_out, which may be q and k themselves (no other
+    of the results rotated back by the same angles, BF16 like them (recorded into a HIP graph only of tensors that the recording
+    makes, not of leaves).  q_out and k_out, which may be q and k themselves (no other
     overlap): written there, outside autograd.
     """
     if q_out is None and k_out is None:
@@ -1012,18 +1013,31 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
     return tuple(outs)
 
 
+def _rope_recorded(ctx) -> None:
+    # a leaf's gradient is added up on the stream where the leaf was first used; one that an eager graph still holds would draw
+    # that stream into the recording, which torch ends the process over
+    if ctx.leaf and torch.cuda.is_current_stream_capturing():
+        raise SdvError("the gradient of rope's q or k is being recorded into a HIP graph while they are leaves: record the "
+                       "operation that makes them as well (a clone will do)")
+
+
+def _leaf(*tensors) -> bool:
+    return any(t is not None and t.requires_grad and t.is_leaf for t in tensors)
+
+
 class _Rope(torch.autograd.Function):
     """rope of rows that require grad: a linear map, s times a rotation, whose transpose is s times the inverse rotation."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.how = dict(interleaved=interleaved, scale=scale, inverse=not inverse)
+        ctx.how, ctx.leaf = dict(interleaved=interleaved, scale=scale, inverse=not inverse), _leaf(q, k)
         ctx.set_materialize_grads(False)
         return rope(q, k, positions, inv_freq, interleaved=interleaved, scale=scale, inverse=inverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
+        _rope_recorded(ctx)
         grads = [g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad)]
         given = [g for g in grads if g is not None]
         if given:
@@ -1270,10 +1284,11 @@ def _(q, k, positions, inv_freq, interleaved=False, scale=1.0, inverse=False):
 
 def _rope_keep(ctx, inputs, output):
     ctx.save_for_backward(*inputs[2:4])
-    ctx.how = inputs[4:]
+    ctx.how, ctx.leaf = inputs[4:], _leaf(*inputs[:2])
 
 
 def _rope_back(ctx, gq, gk):
+    _rope_recorded(ctx)
     interleaved, scale, inverse = ctx.how
     return (*torch.ops.sdv.rope(gq, gk, *ctx.saved_tensors, interleaved, scale, not inverse), None, None, None, None, None)
 

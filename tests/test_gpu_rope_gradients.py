@@ -7,6 +7,7 @@ import torch
 
 import kv8_reference as ref
 from conftest import announce
+from specdec_amd._native import SdvError
 from specdec_amd.kernels import ops
 from test_gpu_rope import FP32, HEADS, _check, _ints, _rows, _turned
 
@@ -122,3 +123,55 @@ def test_the_torch_operator(cuda_device, compiled):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
     if not compiled:
         torch.library.opcheck(torch.ops.sdv.rope.default, (q, k, pos, inv, True, 0.5))
+
+
+@pytest.mark.parametrize("library", [False, True])
+def test_a_recorded_gradient(cuda_device, library):
+    """Of rows that the recording makes: every replay gives the eager gradients of the inputs of the time."""
+    dev = cuda_device
+    (x, y), inv = _leaves("target", 33, dev)
+    pos = _ints(list(range(33)), dev)
+    up = [_rows(t.shape, 11 + i).to(dev) for i, t in enumerate((x, y))]
+    turn = (lambda q, k: torch.ops.sdv.rope(q, k, pos, inv, False, 2.0)) if library else (lambda q, k: ops.rope(q, k, pos, inv, scale=2.0))
+
+    def step(x, y):
+        q, k = x * 2, y * 2
+        a, b = turn(q, k)
+        return [a, b, *torch.autograd.grad((a, b), (q, k), up)]
+    fresh = lambda: [t.detach().clone().requires_grad_() for t in (x, y)]  # noqa: E731
+    announce(f"rope's gradient: warm-up {library}")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*fresh())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = [t.detach() for t in step(x, y)]
+    for turn_ in range(4):
+        with torch.no_grad():
+            for i, t in enumerate((x, y, *up)):
+                t.copy_(_rows(t.shape, 30 + 5 * turn_ + i))
+            pos.add_(100)
+        announce(f"rope's gradient: replay {turn_} {library}")
+        graph.replay()
+        want = step(*fresh())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("library", [False, True])
+def test_a_leafs_gradient_is_not_recorded(cuda_device, library):
+    dev = cuda_device
+    (q, k), inv = _leaves("draft", 5, dev)
+    pos = _ints([3, 1, 4, 1, 5], dev)
+    turn = torch.ops.sdv.rope if library else ops.rope
+    up = [torch.ones_like(q), torch.ones_like(k)]
+    announce(f"a leaf's gradient in a recording {library}")
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(SdvError, match="leaves"):
+        with torch.cuda.graph(graph):
+            outs = turn(q, k, pos, inv)
+            torch.autograd.grad(outs, (q, k), up)
+    got = torch.autograd.grad(turn(q, k, pos, inv), (q, k), up)
+    assert torch.equal(got[0], ops.rope(up[0], None, pos, inv, inverse=True)[0])
